@@ -259,9 +259,10 @@ def _plain_plan(st):
     room[torch.where(back.flatten(), at, free.numel())] = tables.flatten()
     free = room[:-1]
     n_free = st["n_free"] + back.sum(dtype=torch.int32)
-    need = torch.where(ends, 0, (lens + more + page - 1) // page - held)
+    fits = ~ends & (lens + more <= tables.shape[1] * page)
+    need = torch.where(fits, (lens + more + page - 1) // page - held, 0)
     upto = torch.cumsum(need, 0, dtype=torch.int32)
-    granted = ~ends & ((need == 0) | (upto <= n_free)) & (lens + more <= tables.shape[1] * page)
+    granted = fits & ((need == 0) | (upto <= n_free))
     need = torch.where(granted, need, 0)
     idx = col - held.unsqueeze(1)
     new = (idx >= 0) & (idx < need.unsqueeze(1))
