@@ -20,7 +20,7 @@ extern "C" {
 #endif
 
 /* ggml type ids (gguf_loader.rs:24-42) */
-enum { SPX_F32 = 0, SPX_F16 = 1, SPX_Q5_0 = 6, SPX_Q8_0 = 8, SPX_Q4_K = 12, SPX_Q6_K = 14 };
+enum { SPX_F32 = 0, SPX_F16 = 1, SPX_Q5_0 = 6, SPX_Q8_0 = 8, SPX_Q4_K = 12, SPX_Q6_K = 14, SPX_BF16 = 30 };
 
 typedef struct spx_ctx spx_ctx;
 typedef struct spx_tensor spx_tensor;
@@ -106,6 +106,91 @@ int spx_moe(spx_ctx *ctx, const spx_tensor *gate, const spx_tensor *up, const sp
  * The same bits as spx_moe for the same routing. */
 int spx_moe_dev(spx_ctx *ctx, const spx_tensor *gate, const spx_tensor *up, const spx_tensor *down, const float *x,
                 int64_t ld_x, int m, int k, const int32_t *chosen, const float *weights, float *y, int64_t ld_y);
+
+/* ------------------------------------------------------------------ batches of sequences */
+/* Operators for a host that runs a batch of sequences layer by layer: pages and slots planned on
+ * the device, a paged key / value cache in 4 bits, attention over it, and a report on the logits.
+ * No counterpart in the reference, which keeps one sequence's f16 cache. None of these calls
+ * allocates, waits on the host or copies to it, so a step of them can be captured into a graph;
+ * scratch memory is the caller's (the *_ws functions say how much), and calls that may run at the
+ * same time need scratch of their own. Activations are SPX_F32, SPX_F16 or SPX_BF16 (`type`), with
+ * rows `ld` elements apart; every rounding to 16 bits is to nearest even. */
+
+/* One step's bookkeeping for n_seq <= 4096 sequences with block tables [n_seq][table_cols] of page
+ * ids, pages of page_tokens (a power of two, 16..256) tokens. Sequence s holds lens[s] tokens in
+ * its first ceil(lens[s] / page_tokens) pages. In this order:
+ *   add[s] < 0: the sequence ends; its pages go onto the free list (after the n_free[0] entries
+ *     there, by sequence and place), its new length is 0;
+ *   add[s] >= 0: add[s] tokens follow. Sequences take the pages they lack in order, the k-th page
+ *     taken being the (k + 1)-th last of the free list, as long as what they and all before them
+ *     need is there; a sequence that needs pages after that, whose table is too short, or whose
+ *     rows end behind `rows`, is refused: status[s] = 1, its length stays and its rows get no slot.
+ * Outputs: lens_out[n_seq], n_free_out[1] (either may be its input), tables and free_list[n_pages]
+ * updated in place, q_start[n_seq + 1] (the first row of each sequence: add's running sum, refused
+ * ones counted; at most `rows`), and for each of `rows` <= 262144 rows its slot
+ * (page id * page_tokens + place in the page) and its position, -1 where a row has none (refused
+ * sequences, rows behind the last one). n_seq * table_cols and n_pages * page_tokens are < 2^31. */
+int spx_pages_plan(spx_ctx *ctx, int n_seq, int page_tokens, int table_cols, int n_pages, int rows, const int32_t *lens,
+                   const int32_t *add, const int32_t *n_free, int32_t *tables, int32_t *free_list, int32_t *lens_out,
+                   int32_t *n_free_out, int32_t *q_start, int32_t *slots, int32_t *positions, int32_t *status);
+
+/* The 4-bit cache of one layer: a pool of n_pages pages. Groups of 32 channels of a token's key or
+ * value head share a scale: with m the value of largest magnitude (the first of them), d = -m / 8
+ * rounded to bf16, then to f16, at most 8160 in magnitude (zero is +0); a value is held as the integer nearest
+ * to value / d (half to even) in -8..7 and stands for integer * d, which is exact in f16. A group
+ * that holds a NaN or an infinity stands for NaN throughout.
+ * Layout, all little endian: [n_pages][n_kv][page_tokens / 16] tiles of 16 tokens, 18 * head_dim
+ * bytes each (G = head_dim / 32; codes are integer + 8):
+ *   key codes    [4][16 tokens][G][4 bytes]: word (h, t, g) holds channels 32g + 8h + 0..7 of token
+ *                t, its nibbles in the order 0, 2, 4, 6, 1, 3, 5, 7
+ *   value codes  [4][16][4 tokens][G bytes]: (a, l, b) holds channels l * head_dim / 16 .. of token
+ *                4a + b, low nibble first
+ *   key scales   f16 [16 tokens][G]
+ *   value scales f16 [G][16 tokens] */
+typedef struct {
+  int n_kv, head_dim;  /* key / value heads; 64 or 128 */
+  int page_tokens;     /* a power of two, 16..256 */
+  int n_pages;
+} spx_kv4_shape;
+int64_t spx_kv4_bytes(const spx_kv4_shape *shape); /* the pool's bytes; 0 when the shape is not one of these */
+
+/* Rows k, v [rows][n_kv][head_dim] into the pool's slots. A slot outside the pool (-1) is passed
+ * over; slots of one call are distinct. The pool's address is a multiple of 16. */
+int spx_kv4_append(spx_ctx *ctx, const spx_kv4_shape *shape, void *pool, int type, const void *k, int64_t ld_k, const void *v,
+                   int64_t ld_v, int rows, const int32_t *slots);
+/* The values that the pool's slots stand for; zeros for a slot outside the pool. */
+int spx_kv4_read(spx_ctx *ctx, const spx_kv4_shape *shape, const void *pool, int type, int rows, const int32_t *slots, void *k,
+                 int64_t ld_k, void *v, int64_t ld_v);
+
+/* Attention over the pool: rows q_start[s] .. q_start[s + 1] - 1 of q [rows][n_heads][head_dim] are
+ * the last tokens of sequence s, whose kv_lens[s] tokens (its new ones among them) lie in the pages
+ * of tables[s][0 ..]. Row i of its n sits at position p = kv_lens[s] - n + i and sees positions
+ * 0 .. p (window > 0: the last `window` of them); out gets softmax(scale * q.k) v of each head
+ * (query head h reads key head h / (n_heads / n_kv)), scale <= 0 meaning 1 / sqrt(head_dim). A row
+ * that sees nothing gets zeros; rows behind q_start[n_seq] are left as they were. A page id outside
+ * the pool makes its tokens unseen; lengths beyond the table and row numbers beyond `rows` are cut
+ * there. max_kv says how long sequences are at most: it steers how the work is split, results do
+ * not depend on its being right. Sums, maxima and probabilities are held in 32 bits; SPX_F32 rows
+ * meet the cache as two f16 parts (22 bits), SPX_F16 and SPX_BF16 rows as they are.
+ * ws: spx_kv4_attention_ws bytes, a multiple of 16 in address. n_heads <= 1024. */
+int64_t spx_kv4_attention_ws(const spx_kv4_shape *shape, int n_heads, int rows, int n_seq, int max_kv);
+int spx_kv4_attention(spx_ctx *ctx, const spx_kv4_shape *shape, const void *pool, int type, const void *q, int64_t ld_q,
+                      int n_heads, int rows, int n_seq, const int32_t *q_start, const int32_t *kv_lens, const int32_t *tables,
+                      int table_cols, float scale, int window, int max_kv, void *out, int64_t ld_out, void *ws,
+                      int64_t ws_bytes);
+
+/* For each row of logits [rows][vocab] (over logit_scale, as spx_sample takes them): the log
+ * probability of targets[row] (NULL: not asked for; NaN for an id out of range), the entropy of the
+ * row's distribution in nats, and its top_n <= 32 most likely tokens with their log probabilities,
+ * larger first, equal logits by ascending id. -inf logits have probability zero and are no
+ * alternatives (missing ones: id -1, -inf); a row of nothing but -inf has log probabilities -inf
+ * and entropy 0; a row that holds a NaN or +inf has NaN log probabilities and entropy and ids -1.
+ * logp, entropy: [rows] or NULL; top_ids, top_logp: [rows][top_n], not used when top_n is 0.
+ * ws: spx_logprobs_ws bytes, a multiple of 16 in address. */
+int64_t spx_logprobs_ws(int rows, int vocab, int top_n);
+int spx_logprobs(spx_ctx *ctx, int type, const void *logits, int64_t ld, int rows, int vocab, float logit_scale,
+                 const int32_t *targets, int top_n, float *logp, float *entropy, int32_t *top_ids, float *top_logp, void *ws,
+                 int64_t ws_bytes);
 
 /* ------------------------------------------------------------------ synthetic weights */
 /* Seeded synthetic tensor in GGUF block layout (n_expert slabs of rows x cols). kind 0:

@@ -31,6 +31,15 @@ SIGNATURES = {
     "spx_matvec_noalloc": (C.c_int, [P, P, C.c_int, P, I64, C.c_int, P, I64]),
     "spx_moe": (C.c_int, [P, P, P, P, P, I64, C.c_int, C.c_int, P, P, P, I64]),
     "spx_moe_dev": (C.c_int, [P, P, P, P, P, I64, C.c_int, C.c_int, P, P, P, I64]),
+    "spx_pages_plan": (C.c_int, [P] + [C.c_int] * 5 + [P] * 11),
+    "spx_kv4_bytes": (I64, [P]),
+    "spx_kv4_append": (C.c_int, [P, P, P, C.c_int, P, I64, P, I64, C.c_int, P]),
+    "spx_kv4_read": (C.c_int, [P, P, P, C.c_int, C.c_int, P, P, I64, P, I64]),
+    "spx_kv4_attention_ws": (I64, [P, C.c_int, C.c_int, C.c_int, C.c_int]),
+    "spx_kv4_attention": (C.c_int, [P, P, P, C.c_int, P, I64, C.c_int, C.c_int, C.c_int, P, P, P, C.c_int, C.c_float, C.c_int, C.c_int,
+                                    P, I64, P, I64]),
+    "spx_logprobs_ws": (I64, [C.c_int, C.c_int, C.c_int]),
+    "spx_logprobs": (C.c_int, [P, C.c_int, P, I64, C.c_int, C.c_int, C.c_float, P, C.c_int, P, P, P, P, P, I64]),
     "spx_synth_tensor": (C.c_int, [C.c_int, I64, I64, C.c_int, C.c_uint64, C.c_float, C.c_int, P]),
     "spx_engine_create": (C.c_int, [P, P, C.POINTER(P)]),
     "spx_engine_set_tensor": (C.c_int, [P, C.c_char_p, C.c_int, I64, I64, C.c_int, P]),

@@ -16,7 +16,7 @@ try:  # device buffers of the operator functions below are torch tensors; a cont
 except ImportError:  # pragma: no cover - torch is part of this image
     torch = None
 
-F32, F16, Q5_0, Q8_0, Q4K, Q6K = 0, 1, 6, 8, 12, 14
+F32, F16, Q5_0, Q8_0, Q4K, Q6K, BF16 = 0, 1, 6, 8, 12, 14, 30
 
 
 class Context:
@@ -29,6 +29,7 @@ class Context:
         h = P()
         check(lib.spx_create(device, C.byref(h)))  # fails (SpxError) without a visible GPU
         self.h = h
+        self._stream = None
         self._children = weakref.WeakSet()   # engines / tensors to release before the context
 
     def adopt(self, obj):
@@ -36,6 +37,13 @@ class Context:
 
     def sync(self):
         check(lib.spx_sync(self.h))
+
+    def torch_stream(self):
+        """The context's stream as a torch stream: a program that makes it torch's current one
+        (torch.cuda.set_stream) orders its own work and the operators' on one stream."""
+        if self._stream is None:
+            self._stream = torch.cuda.ExternalStream(lib.spx_get_stream(self.h), device=self.device)
+        return self._stream
 
     def close(self):
         if self.h:
@@ -178,6 +186,164 @@ def moe_dev(ctx, gate, up, down, x, chosen, weights):
     check(lib.spx_moe_dev(ctx.h, gate.h, up.h, down.h, _p(x), x.stride(0), m, k, _p(chosen), _p(weights), _p(y), y.stride(0)))
     ctx.sync()
     return y
+
+
+# ------------------------------------------------------------------ batches of sequences
+# These wait for nothing on the host: a call's work is ordered after what torch's current stream
+# holds, and that stream's later work after the call's (no cost where the two are one stream, see
+# Context.torch_stream). Inside a captured graph they record their launches.
+class _Ordered:
+    def __init__(self, ctx, *tensors):
+        for t in tensors:
+            if t is not None and (not t.is_cuda or t.device.index != ctx.device):
+                raise ValueError(f"expected tensors on cuda:{ctx.device}")
+        self.ours = ctx.torch_stream()
+        self.theirs = torch.cuda.current_stream(ctx.device)
+        self.same = self.ours.cuda_stream == self.theirs.cuda_stream
+
+    def __enter__(self):
+        if not self.same:
+            self.ours.wait_stream(self.theirs)
+
+    def __exit__(self, *exc):
+        if not self.same:
+            self.theirs.wait_stream(self.ours)
+
+
+def _row_type(t):
+    try:
+        return {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}[t.dtype if hasattr(t, "dtype") else t]
+    except KeyError:
+        raise ValueError(f"expected float32, float16 or bfloat16, got {t.dtype if hasattr(t, 'dtype') else t}") from None
+
+
+def _i32(t, *shape):
+    if t.dtype != torch.int32 or not t.is_contiguous() or tuple(t.shape) != shape:
+        raise ValueError(f"expected a contiguous int32 tensor {shape}, got {t.dtype} {tuple(t.shape)}")
+    return t
+
+
+def _rows3(t, heads, hd, name):
+    """A [rows, heads, hd] tensor whose rows are dense; the distance between rows."""
+    if t.dim() != 3 or t.shape[1] != heads or t.shape[2] != hd or t.stride(2) != 1 or (heads > 1 and t.stride(1) != hd):
+        raise ValueError(f"{name}: expected [rows, {heads}, {hd}] with dense rows, got {tuple(t.shape)}, strides {t.stride()}")
+    return t.stride(0) if t.shape[0] > 1 else heads * hd
+
+
+class PagesPlan:
+    """What pages_plan leaves: lens, n_free, q_start, slots, positions, status (int32 tensors)."""
+    __slots__ = ("lens", "n_free", "q_start", "slots", "positions", "status")
+
+
+def pages_plan(ctx, lens, add, tables, free_list, n_free, page_tokens, rows):
+    """One step's pages, slots and positions (spx_pages_plan): lens, add [n_seq], tables [n_seq,
+    table_cols], free_list [n_pages] and n_free [1] are int32 cuda tensors; tables and free_list are
+    updated in place, the rest comes back new (pass the plan's lens and n_free to the next step).
+    rows: how many rows the step has room for, at least the sum of the positive adds."""
+    n = lens.numel()
+    _i32(lens, n), _i32(add, n), _i32(tables, n, tables.shape[1] if tables.dim() == 2 else 0), _i32(n_free, 1), _i32(free_list, free_list.numel())
+    p = PagesPlan()
+    buf = torch.empty(3 * n + 2 + 2 * rows, dtype=torch.int32, device=lens.device)
+    p.lens, p.status, p.q_start, p.n_free, p.slots, p.positions = buf.split((n, n, n + 1, 1, rows, rows))
+    with _Ordered(ctx, lens, add, tables, free_list, n_free):
+        check(lib.spx_pages_plan(ctx.h, n, page_tokens, tables.shape[1], free_list.numel(), rows, _p(lens), _p(add), _p(n_free), _p(tables),
+                                 _p(free_list), _p(p.lens), _p(p.n_free), _p(p.q_start), _p(p.slots), _p(p.positions), _p(p.status)))
+    return p
+
+
+class Kv4Shape(C.Structure):
+    """spx_kv4_shape: the shape of a layer's 4-bit key / value pool."""
+    _fields_ = [("n_kv", C.c_int), ("head_dim", C.c_int), ("page_tokens", C.c_int), ("n_pages", C.c_int)]
+
+    @property
+    def nbytes(self):
+        n = lib.spx_kv4_bytes(C.byref(self))
+        if n <= 0:
+            raise ValueError("not a shape of a 4-bit cache: head_dim 64 or 128, page_tokens a power of two in 16..256, n_kv and n_pages positive")
+        return n
+
+    def pool(self, device="cuda"):
+        """A layer's pool for this shape (a uint8 tensor of zeros)."""
+        return torch.zeros(self.nbytes, dtype=torch.uint8, device=device)
+
+
+def _pool(shape, pool):
+    if pool.dtype != torch.uint8 or not pool.is_contiguous() or pool.numel() < shape.nbytes:
+        raise ValueError(f"the pool must be a contiguous uint8 tensor of {shape.nbytes} bytes")
+    return _p(pool)
+
+
+def kv4_append(ctx, shape, pool, k, v, slots):
+    """Puts rows k, v [rows, n_kv, head_dim] into the pool's slots [rows] (spx_kv4_append)."""
+    t, n = _row_type(k), slots.numel()
+    if v.dtype != k.dtype or k.shape[0] != n or v.shape[0] != n:
+        raise ValueError("k and v must have one type and a row for each slot")
+    ld_k, ld_v = _rows3(k, shape.n_kv, shape.head_dim, "k"), _rows3(v, shape.n_kv, shape.head_dim, "v")
+    with _Ordered(ctx, pool, k, v, slots):
+        check(lib.spx_kv4_append(ctx.h, C.byref(shape), _pool(shape, pool), t, _p(k), ld_k, _p(v), ld_v, n, _p(_i32(slots, n))))
+
+
+def kv4_read(ctx, shape, pool, slots, dtype=None):
+    """(k, v) [rows, n_kv, head_dim]: the values that the pool's slots [rows] stand for (spx_kv4_read)."""
+    dtype = dtype or torch.float32
+    t, n, w = _row_type(dtype), slots.numel(), shape.n_kv * shape.head_dim
+    k, v = torch.empty((2, n, shape.n_kv, shape.head_dim), dtype=dtype, device=pool.device).unbind(0)
+    with _Ordered(ctx, pool, slots):
+        check(lib.spx_kv4_read(ctx.h, C.byref(shape), _pool(shape, pool), t, n, _p(_i32(slots, n)), _p(k), w, _p(v), w))
+    return k, v
+
+
+def kv4_attention(ctx, shape, pool, q, q_start, kv_lens, tables, scale=0.0, window=0, max_kv=None, out=None, ws=None):
+    """Attention of q [rows, n_heads, head_dim] over the pool (spx_kv4_attention): q_start [n_seq + 1],
+    kv_lens [n_seq] and tables [n_seq, table_cols] int32. out: [rows, n_heads, head_dim] of q's type
+    (rows behind the last sequence stay as they are there). ws: scratch, a uint8 tensor; without one
+    the call takes its own from torch's allocator."""
+    t, n = _row_type(q), kv_lens.numel()
+    rows, heads, hd = q.shape
+    ld_q = _rows3(q, heads, shape.head_dim, "q")
+    if out is None:
+        out = torch.empty((rows, heads, hd), dtype=q.dtype, device=q.device)
+    elif out.dtype != q.dtype or out.shape != q.shape:
+        raise ValueError("out must have q's type and shape")
+    ld_out = _rows3(out, heads, hd, "out")
+    cols = tables.shape[1] if tables.dim() == 2 else 0
+    max_kv = cols * shape.page_tokens if max_kv is None else max_kv
+    need = lib.spx_kv4_attention_ws(C.byref(shape), heads, rows, n, max_kv)
+    if ws is None and need > 0:
+        ws = torch.empty(need, dtype=torch.uint8, device=q.device)
+    with _Ordered(ctx, pool, q, q_start, kv_lens, tables, out, ws):
+        check(lib.spx_kv4_attention(ctx.h, C.byref(shape), _pool(shape, pool), t, _p(q), ld_q, heads, rows, n, _p(_i32(q_start, n + 1)),
+                                    _p(_i32(kv_lens, n)), _p(_i32(tables, n, cols)), cols, scale, window, max_kv, _p(out), ld_out,
+                                    _p(ws) if ws is not None else None, ws.numel() if ws is not None else 0))
+    return out
+
+
+class Logprobs:
+    """What logprobs leaves: logp [rows] (None without targets), entropy [rows], top_ids and
+    top_logp [rows, top]."""
+    __slots__ = ("logp", "entropy", "top_ids", "top_logp")
+
+
+def logprobs(ctx, logits, targets=None, top=0, logit_scale=1.0, ws=None):
+    """Log probabilities of targets [rows] (int32), the entropy and the `top` most likely tokens of
+    each row of logits [rows, vocab] (spx_logprobs). ws as in kv4_attention."""
+    t = _row_type(logits)
+    if logits.dim() != 2 or logits.stride(1) != 1:
+        raise ValueError("logits must be [rows, vocab] with dense rows")
+    rows, vocab = logits.shape
+    r = Logprobs()
+    r.logp = torch.empty(rows, dtype=torch.float32, device=logits.device) if targets is not None else None
+    r.entropy = torch.empty(rows, dtype=torch.float32, device=logits.device)
+    r.top_ids = torch.empty((rows, top), dtype=torch.int32, device=logits.device)
+    r.top_logp = torch.empty((rows, top), dtype=torch.float32, device=logits.device)
+    need = lib.spx_logprobs_ws(rows, vocab, top)
+    if ws is None and need > 0:
+        ws = torch.empty(need, dtype=torch.uint8, device=logits.device)
+    with _Ordered(ctx, logits, targets, ws):
+        check(lib.spx_logprobs(ctx.h, t, _p(logits), logits.stride(0) if rows > 1 else vocab, rows, vocab, logit_scale,
+                               _p(_i32(targets, rows)) if targets is not None else None, top, _p(r.logp) if targets is not None else None,
+                               _p(r.entropy), _p(r.top_ids), _p(r.top_logp), _p(ws) if ws is not None else None, ws.numel() if ws is not None else 0))
+    return r
 
 
 class SamplerParams(C.Structure):
