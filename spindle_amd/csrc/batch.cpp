@@ -177,8 +177,9 @@ int spx_kv4_attention(spx_ctx *ctx, const spx_kv4_shape *shape, const void *pool
 }
 
 int64_t spx_logprobs_ws(int rows, int vocab, int top_n) {
-  (void)rows; (void)vocab; (void)top_n;
-  return 0;
+  if (rows < 1 || rows > 1 << 18 || vocab < 1 || vocab > 1 << 24 || top_n < 0 || top_n > 32) return 0;
+  const int64_t parts = logprobs_parts(rows, vocab);
+  return parts > 1 ? rows * parts * (16 + 8 * (int64_t)top_n) : 0;
 }
 
 int spx_logprobs(spx_ctx *ctx, int type, const void *logits, int64_t ld, int rows, int vocab, float logit_scale,
@@ -201,7 +202,7 @@ int spx_logprobs(spx_ctx *ctx, int type, const void *logits, int64_t ld, int row
     if (rows == 0) return 0;
     OnDevice dev(ctx->device);
     if (dev.err != hipSuccess) return hip_fail(dev.err, "spx_logprobs");
-    LogprobArgs a{logits, ld, rows, vocab, top_n, logit_scale, targets, logp, entropy, top_logp, top_ids};
+    LogprobArgs a{logits, ld, rows, vocab, top_n, logit_scale, targets, logp, entropy, top_logp, top_ids, ws};
     SPX_HIP(launch_logprobs(a, type, ctx->stream));
     return 0;
   });

@@ -46,7 +46,9 @@ struct LogprobArgs {
   const int32_t *targets;
   float *logp, *entropy, *top_logp;
   int32_t *top_ids;
+  void *ws;
 };
+int logprobs_parts(int rows, int vocab);
 hipError_t launch_logprobs(const LogprobArgs &a, int type, hipStream_t s);
 
 }  // namespace spx
