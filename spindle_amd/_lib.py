@@ -123,7 +123,9 @@ def load():
 
 class _Lazy:
     def __getattr__(self, name):
-        return getattr(load(), name)
+        f = getattr(load(), name)
+        setattr(self, name, f)  # found here the next time
+        return f
 
 
 lib = _Lazy()

@@ -191,43 +191,48 @@ def moe_dev(ctx, gate, up, down, x, chosen, weights):
 # ------------------------------------------------------------------ batches of sequences
 # These wait for nothing on the host: a call's work is ordered after what torch's current stream
 # holds, and that stream's later work after the call's (no cost where the two are one stream, see
-# Context.torch_stream). Inside a captured graph they record their launches.
-class _Ordered:
-    def __init__(self, ctx, *tensors):
-        for t in tensors:
-            if t is not None and (not t.is_cuda or t.device.index != ctx.device):
-                raise ValueError(f"expected tensors on cuda:{ctx.device}")
-        self.ours = ctx.torch_stream()
-        self.theirs = torch.cuda.current_stream(ctx.device)
-        self.same = self.ours.cuda_stream == self.theirs.cuda_stream
-
-    def __enter__(self):
-        if not self.same:
-            self.ours.wait_stream(self.theirs)
-
-    def __exit__(self, *exc):
-        if not self.same:
-            self.theirs.wait_stream(self.ours)
+# Context.torch_stream). Inside a captured graph they record their launches. Calls this small are
+# bound by the host, so arguments are checked with as few steps as it takes.
+_ROW_TYPES = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16} if torch is not None else {}
 
 
-def _row_type(t):
+def _run(ctx, tensors, call, *args):
+    """call(ctx.h, *args) in order with torch's current stream."""
+    for t in tensors:
+        if t.get_device() != ctx.device:
+            raise ValueError(f"expected tensors on cuda:{ctx.device}, got {t.device}")
+    theirs = torch.cuda.current_stream(ctx.device)
+    ours = ctx.torch_stream()
+    if theirs == ours:
+        check(call(ctx.h, *args))
+        return
+    ours.wait_stream(theirs)
     try:
-        return {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}[t.dtype if hasattr(t, "dtype") else t]
-    except KeyError:
-        raise ValueError(f"expected float32, float16 or bfloat16, got {t.dtype if hasattr(t, 'dtype') else t}") from None
+        check(call(ctx.h, *args))
+    finally:
+        theirs.wait_stream(ours)
 
 
-def _i32(t, *shape):
-    if t.dtype != torch.int32 or not t.is_contiguous() or tuple(t.shape) != shape:
-        raise ValueError(f"expected a contiguous int32 tensor {shape}, got {t.dtype} {tuple(t.shape)}")
+def _row_type(dtype):
+    t = _ROW_TYPES.get(dtype)
+    if t is None:
+        raise ValueError(f"expected float32, float16 or bfloat16, got {dtype}")
     return t
 
 
+def _i32(t, *shape):
+    """The address of a dense int32 tensor of this shape."""
+    if t.dtype is not torch.int32 or t.shape != shape or not t.is_contiguous():
+        raise ValueError(f"expected a contiguous int32 tensor {shape}, got {t.dtype} {tuple(t.shape)}")
+    return t.data_ptr()
+
+
 def _rows3(t, heads, hd, name):
-    """A [rows, heads, hd] tensor whose rows are dense; the distance between rows."""
-    if t.dim() != 3 or t.shape[1] != heads or t.shape[2] != hd or t.stride(2) != 1 or (heads > 1 and t.stride(1) != hd):
+    """The distance between the rows of a [rows, heads, hd] tensor whose rows are dense."""
+    n, w = t.shape[0], heads * hd
+    if t.shape != (n, heads, hd) or not (t.is_contiguous() or (t.stride(2) == 1 and (heads == 1 or t.stride(1) == hd))):
         raise ValueError(f"{name}: expected [rows, {heads}, {hd}] with dense rows, got {tuple(t.shape)}, strides {t.stride()}")
-    return t.stride(0) if t.shape[0] > 1 else heads * hd
+    return t.stride(0) if n > 1 else w
 
 
 class PagesPlan:
@@ -240,14 +245,14 @@ def pages_plan(ctx, lens, add, tables, free_list, n_free, page_tokens, rows):
     table_cols], free_list [n_pages] and n_free [1] are int32 cuda tensors; tables and free_list are
     updated in place, the rest comes back new (pass the plan's lens and n_free to the next step).
     rows: how many rows the step has room for, at least the sum of the positive adds."""
-    n = lens.numel()
-    _i32(lens, n), _i32(add, n), _i32(tables, n, tables.shape[1] if tables.dim() == 2 else 0), _i32(n_free, 1), _i32(free_list, free_list.numel())
-    p = PagesPlan()
+    n, cols, pages = lens.numel(), tables.shape[1] if tables.dim() == 2 else 0, free_list.numel()
+    ins = _i32(lens, n), _i32(add, n), _i32(n_free, 1), _i32(tables, n, cols), _i32(free_list, pages)
+    p, rows = PagesPlan(), max(rows, 0)
     buf = torch.empty(3 * n + 2 + 2 * rows, dtype=torch.int32, device=lens.device)
     p.lens, p.status, p.q_start, p.n_free, p.slots, p.positions = buf.split((n, n, n + 1, 1, rows, rows))
-    with _Ordered(ctx, lens, add, tables, free_list, n_free):
-        check(lib.spx_pages_plan(ctx.h, n, page_tokens, tables.shape[1], free_list.numel(), rows, _p(lens), _p(add), _p(n_free), _p(tables),
-                                 _p(free_list), _p(p.lens), _p(p.n_free), _p(p.q_start), _p(p.slots), _p(p.positions), _p(p.status)))
+    at = buf.data_ptr()  # (the parts in this order)
+    _run(ctx, (lens, add, tables, free_list, n_free), lib.spx_pages_plan, n, page_tokens, cols, pages, rows, *ins, at, at + 4 * (3 * n + 1),
+         at + 8 * n, at + 4 * (3 * n + 2), at + 4 * (3 * n + 2 + rows), at + 4 * n)
     return p
 
 
@@ -268,29 +273,38 @@ class Kv4Shape(C.Structure):
 
 
 def _pool(shape, pool):
-    if pool.dtype != torch.uint8 or not pool.is_contiguous() or pool.numel() < shape.nbytes:
+    if pool.dtype is not torch.uint8 or not pool.is_contiguous() or pool.numel() < shape.nbytes:
         raise ValueError(f"the pool must be a contiguous uint8 tensor of {shape.nbytes} bytes")
-    return _p(pool)
+    return pool.data_ptr()
 
 
 def kv4_append(ctx, shape, pool, k, v, slots):
     """Puts rows k, v [rows, n_kv, head_dim] into the pool's slots [rows] (spx_kv4_append)."""
-    t, n = _row_type(k), slots.numel()
-    if v.dtype != k.dtype or k.shape[0] != n or v.shape[0] != n:
+    t, n, kv, hd = _row_type(k.dtype), slots.numel(), shape.n_kv, shape.head_dim
+    if v.dtype is not k.dtype or k.shape[0] != n or v.shape[0] != n:
         raise ValueError("k and v must have one type and a row for each slot")
-    ld_k, ld_v = _rows3(k, shape.n_kv, shape.head_dim, "k"), _rows3(v, shape.n_kv, shape.head_dim, "v")
-    with _Ordered(ctx, pool, k, v, slots):
-        check(lib.spx_kv4_append(ctx.h, C.byref(shape), _pool(shape, pool), t, _p(k), ld_k, _p(v), ld_v, n, _p(_i32(slots, n))))
+    _run(ctx, (pool, k, v, slots), lib.spx_kv4_append, C.byref(shape), _pool(shape, pool), t, k.data_ptr(), _rows3(k, kv, hd, "k"), v.data_ptr(),
+         _rows3(v, kv, hd, "v"), n, _i32(slots, n))
 
 
 def kv4_read(ctx, shape, pool, slots, dtype=None):
     """(k, v) [rows, n_kv, head_dim]: the values that the pool's slots [rows] stand for (spx_kv4_read)."""
     dtype = dtype or torch.float32
     t, n, w = _row_type(dtype), slots.numel(), shape.n_kv * shape.head_dim
-    k, v = torch.empty((2, n, shape.n_kv, shape.head_dim), dtype=dtype, device=pool.device).unbind(0)
-    with _Ordered(ctx, pool, slots):
-        check(lib.spx_kv4_read(ctx.h, C.byref(shape), _pool(shape, pool), t, n, _p(_i32(slots, n)), _p(k), w, _p(v), w))
+    both = torch.empty((2, n, shape.n_kv, shape.head_dim), dtype=dtype, device=pool.device)
+    k, v = both.unbind(0)
+    at = both.data_ptr()
+    _run(ctx, (pool, slots), lib.spx_kv4_read, C.byref(shape), _pool(shape, pool), t, n, _i32(slots, n), at, w, at + n * w * dtype.itemsize, w)
     return k, v
+
+
+def _scratch(need, ws, like):
+    """(address, bytes) of a call's scratch, and the tensor that keeps it."""
+    if ws is None:
+        if need <= 0:
+            return None, 0, like
+        ws = torch.empty(need, dtype=torch.uint8, device=like.device)
+    return ws.data_ptr(), ws.numel() * ws.element_size(), ws
 
 
 def kv4_attention(ctx, shape, pool, q, q_start, kv_lens, tables, scale=0.0, window=0, max_kv=None, out=None, ws=None):
@@ -298,23 +312,21 @@ def kv4_attention(ctx, shape, pool, q, q_start, kv_lens, tables, scale=0.0, wind
     kv_lens [n_seq] and tables [n_seq, table_cols] int32. out: [rows, n_heads, head_dim] of q's type
     (rows behind the last sequence stay as they are there). ws: scratch, a uint8 tensor; without one
     the call takes its own from torch's allocator."""
-    t, n = _row_type(q), kv_lens.numel()
-    rows, heads, hd = q.shape
-    ld_q = _rows3(q, heads, shape.head_dim, "q")
+    t, n, hd = _row_type(q.dtype), kv_lens.numel(), shape.head_dim
+    rows, heads = q.shape[0], q.shape[1] if q.dim() == 3 else 0
+    ld_q = _rows3(q, heads, hd, "q")
     if out is None:
-        out = torch.empty((rows, heads, hd), dtype=q.dtype, device=q.device)
-    elif out.dtype != q.dtype or out.shape != q.shape:
+        out, ld_out = torch.empty((rows, heads, hd), dtype=q.dtype, device=q.device), heads * hd
+    elif out.dtype is not q.dtype or out.shape != q.shape:
         raise ValueError("out must have q's type and shape")
-    ld_out = _rows3(out, heads, hd, "out")
+    else:
+        ld_out = _rows3(out, heads, hd, "out")
     cols = tables.shape[1] if tables.dim() == 2 else 0
     max_kv = cols * shape.page_tokens if max_kv is None else max_kv
-    need = lib.spx_kv4_attention_ws(C.byref(shape), heads, rows, n, max_kv)
-    if ws is None and need > 0:
-        ws = torch.empty(need, dtype=torch.uint8, device=q.device)
-    with _Ordered(ctx, pool, q, q_start, kv_lens, tables, out, ws):
-        check(lib.spx_kv4_attention(ctx.h, C.byref(shape), _pool(shape, pool), t, _p(q), ld_q, heads, rows, n, _p(_i32(q_start, n + 1)),
-                                    _p(_i32(kv_lens, n)), _p(_i32(tables, n, cols)), cols, scale, window, max_kv, _p(out), ld_out,
-                                    _p(ws) if ws is not None else None, ws.numel() if ws is not None else 0))
+    sh = C.byref(shape)
+    at, size, ws = _scratch(lib.spx_kv4_attention_ws(sh, heads, rows, n, max_kv), ws, q)
+    _run(ctx, (pool, q, q_start, kv_lens, tables, out, ws), lib.spx_kv4_attention, sh, _pool(shape, pool), t, q.data_ptr(), ld_q, heads, rows, n,
+         _i32(q_start, n + 1), _i32(kv_lens, n), _i32(tables, n, cols), cols, scale, window, max_kv, out.data_ptr(), ld_out, at, size)
     return out
 
 
@@ -327,22 +339,23 @@ class Logprobs:
 def logprobs(ctx, logits, targets=None, top=0, logit_scale=1.0, ws=None):
     """Log probabilities of targets [rows] (int32), the entropy and the `top` most likely tokens of
     each row of logits [rows, vocab] (spx_logprobs). ws as in kv4_attention."""
-    t = _row_type(logits)
-    if logits.dim() != 2 or logits.stride(1) != 1:
+    t = _row_type(logits.dtype)
+    if logits.dim() != 2 or (logits.stride(1) != 1 and logits.shape[1] > 1):
         raise ValueError("logits must be [rows, vocab] with dense rows")
     rows, vocab = logits.shape
-    r = Logprobs()
-    r.logp = torch.empty(rows, dtype=torch.float32, device=logits.device) if targets is not None else None
-    r.entropy = torch.empty(rows, dtype=torch.float32, device=logits.device)
-    r.top_ids = torch.empty((rows, top), dtype=torch.int32, device=logits.device)
-    r.top_logp = torch.empty((rows, top), dtype=torch.float32, device=logits.device)
-    need = lib.spx_logprobs_ws(rows, vocab, top)
-    if ws is None and need > 0:
-        ws = torch.empty(need, dtype=torch.uint8, device=logits.device)
-    with _Ordered(ctx, logits, targets, ws):
-        check(lib.spx_logprobs(ctx.h, t, _p(logits), logits.stride(0) if rows > 1 else vocab, rows, vocab, logit_scale,
-                               _p(_i32(targets, rows)) if targets is not None else None, top, _p(r.logp) if targets is not None else None,
-                               _p(r.entropy), _p(r.top_ids), _p(r.top_logp), _p(ws) if ws is not None else None, ws.numel() if ws is not None else 0))
+    r, n, dev = Logprobs(), max(top, 0), logits.device
+    both = torch.empty((2, rows), dtype=torch.float32, device=dev)
+    r.logp, r.entropy = both.unbind(0)
+    at = both.data_ptr()
+    r.top_ids = torch.empty((rows, n), dtype=torch.int32, device=dev)
+    r.top_logp = torch.empty((rows, n), dtype=torch.float32, device=dev)
+    if targets is None:
+        r.logp, ids, logp, targets = None, None, None, logits
+    else:
+        ids, logp = _i32(targets, rows), at
+    scratch, size, ws = _scratch(lib.spx_logprobs_ws(rows, vocab, top), ws, logits)
+    _run(ctx, (logits, targets, ws), lib.spx_logprobs, t, logits.data_ptr(), logits.stride(0) if rows > 1 else vocab, rows, vocab, logit_scale, ids,
+         top, logp, at + 4 * rows, r.top_ids.data_ptr(), r.top_logp.data_ptr(), scratch, size)
     return r
 
 
