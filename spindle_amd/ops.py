@@ -201,11 +201,11 @@ def _run(ctx, tensors, call, *args):
     for t in tensors:
         if t.get_device() != ctx.device:
             raise ValueError(f"expected tensors on cuda:{ctx.device}, got {t.device}")
-    theirs = torch.cuda.current_stream(ctx.device)
     ours = ctx.torch_stream()
-    if theirs == ours:
+    if torch._C._cuda_getCurrentRawStream(ctx.device) == ours.cuda_stream:  # (the stream's number, without an object around it)
         check(call(ctx.h, *args))
         return
+    theirs = torch.cuda.current_stream(ctx.device)
     ours.wait_stream(theirs)
     try:
         check(call(ctx.h, *args))
@@ -249,7 +249,7 @@ def pages_plan(ctx, lens, add, tables, free_list, n_free, page_tokens, rows):
     ins = _i32(lens, n), _i32(add, n), _i32(n_free, 1), _i32(tables, n, cols), _i32(free_list, pages)
     p, rows = PagesPlan(), max(rows, 0)
     buf = torch.empty(3 * n + 2 + 2 * rows, dtype=torch.int32, device=lens.device)
-    p.lens, p.status, p.q_start, p.n_free, p.slots, p.positions = buf.split((n, n, n + 1, 1, rows, rows))
+    p.lens, p.status, p.q_start, p.n_free, p.slots, p.positions = buf.split_with_sizes((n, n, n + 1, 1, rows, rows))
     at = buf.data_ptr()  # (the parts in this order)
     _run(ctx, (lens, add, tables, free_list, n_free), lib.spx_pages_plan, n, page_tokens, cols, pages, rows, *ins, at, at + 4 * (3 * n + 1),
          at + 8 * n, at + 4 * (3 * n + 2), at + 4 * (3 * n + 2 + rows), at + 4 * n)
