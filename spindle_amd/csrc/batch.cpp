@@ -120,8 +120,10 @@ int spx_kv4_read(spx_ctx *ctx, const spx_kv4_shape *shape, const void *pool, int
 }
 
 int64_t spx_kv4_attention_ws(const spx_kv4_shape *shape, int n_heads, int rows, int n_seq, int max_kv) {
-  (void)shape; (void)n_heads; (void)rows; (void)n_seq; (void)max_kv;
-  return 0;
+  if (shape_error(shape) || n_heads < 1 || n_heads > 1024 || n_heads % shape->n_kv || rows < 1 || rows > 1 << 18 || n_seq < 1 ||
+      n_seq > 1 << 20 || max_kv < 0)
+    return 0;
+  return kv4_attention_ws(shape->head_dim, n_heads / shape->n_kv, shape->n_kv, rows, n_seq, max_kv);
 }
 
 int spx_kv4_attention(spx_ctx *ctx, const spx_kv4_shape *shape, const void *pool, int type, const void *q, int64_t ld_q,
@@ -138,8 +140,8 @@ int spx_kv4_attention(spx_ctx *ctx, const spx_kv4_shape *shape, const void *pool
     if (max_kv < 0) return fail("spx_kv4_attention: max_kv must not be negative");
     const bool work = rows > 0 && n_seq > 0;
     if (work && (!pool || !q || !out || !q_start || !kv_lens || !tables)) return fail("spx_kv4_attention: null argument");
-    if ((work && table_cols < 1) || table_cols < 0 || (int64_t)table_cols * shape->page_tokens > INT32_MAX - 64)
-      return fail("spx_kv4_attention: table_cols must be positive, table_cols * page_tokens below 2^31");
+    if ((work && table_cols < 1) || table_cols < 0 || (int64_t)table_cols * shape->page_tokens > 1 << 30)
+      return fail("spx_kv4_attention: table_cols must be positive, table_cols * page_tokens at most 2^30");
     const int64_t width = (int64_t)n_heads * shape->head_dim;
     if (rows > 1 && (ld_q < width || ld_out < width)) return fail("spx_kv4_attention: leading dimension too small");
     if (!aligned(pool, 16) || !aligned(q, size_of(type)) || !aligned(out, size_of(type)))
@@ -170,8 +172,9 @@ int spx_kv4_attention(spx_ctx *ctx, const spx_kv4_shape *shape, const void *pool
     a.q_start = q_start;
     a.kv_lens = kv_lens;
     a.tables = tables;
+    a.part = (float *)ws;
     a.scale = (float)((scale > 0.0f ? (double)scale : 1.0 / __builtin_sqrt((double)shape->head_dim)) * 1.4426950408889634);
-    SPX_HIP(launch_kv4_attention(a, shape->head_dim, type, ctx->stream));
+    SPX_HIP(launch_kv4_attention(a, shape->head_dim, type, max_kv, ctx->stream));
     return 0;
   });
 }

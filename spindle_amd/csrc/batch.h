@@ -35,8 +35,11 @@ struct Kv4Attn {
   int n_heads, group, rows, n_seq, cols, window;
   const int32_t *q_start, *kv_lens, *tables;
   float scale;  // times log2(e)
+  int chunk;    // tokens a workgroup takes at a time
+  float *part;  // scratch: outputs, then (maximum, sum), of every job, key head, split and row
 };
-hipError_t launch_kv4_attention(const Kv4Attn &a, int hd, int type, hipStream_t s);
+int64_t kv4_attention_ws(int hd, int group, int n_kv, int rows, int n_seq, int max_kv);
+hipError_t launch_kv4_attention(Kv4Attn a, int hd, int type, int max_kv, hipStream_t s);
 
 struct LogprobArgs {
   const void *x;

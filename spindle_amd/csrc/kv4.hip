@@ -301,6 +301,9 @@ __device__ __forceinline__ float lift_of(float amax) {
   return ldexpf(1.0f, min(max(14 - e, -126), 126));
 }
 
+// Long sequences are shared by workgroups: chunk blockIdx.z of `chunk` tokens (and every
+// gridDim.z-th after it). A workgroup leaves its rows' (maximum, sum, output) for k_kv4_join where
+// there is more than one chunk to them.
 template <int HD, class R, int QP, int PP>
 __global__ __launch_bounds__(256) void k_kv4_attn(const Kv4Attn a) {
   typedef typename R::E E;
@@ -336,6 +339,8 @@ __global__ __launch_bounds__(256) void k_kv4_attn(const Kv4Attn a) {
   // all rows of the job together
   const int last = min(j.r0 + 15, rows - 1) / a.group, first = j.r0 / a.group;
   const int all_hi = min(j.n - j.nq + last + 1, j.n), all_lo = a.window > 0 ? max(j.n - j.nq + first + 1 - a.window, 0) : 0;
+  const int from = all_lo & ~31, chunks = all_hi > from ? (all_hi - from + a.chunk - 1) / a.chunk : 1;
+  if ((int)blockIdx.z >= chunks) return;
 
   f4v o[NC];
 #pragma unroll
@@ -344,7 +349,8 @@ __global__ __launch_bounds__(256) void k_kv4_attn(const Kv4Attn a) {
   const int *table = a.tables + (int64_t)j.s * a.cols;
   const int pm = (1 << a.page) - 1;
 
-  for (int t0 = (all_lo & ~31) + 32 * wave; t0 < all_hi; t0 += 32 * NW) {
+  for (int c = blockIdx.z; c < chunks; c += gridDim.z)
+  for (int t0 = from + c * a.chunk + 32 * wave; t0 < min(all_hi, from + (c + 1) * a.chunk); t0 += 32 * NW) {
     Tile4<HD> x[2];
     bool in[2];
 #pragma unroll
@@ -460,22 +466,88 @@ __global__ __launch_bounds__(256) void k_kv4_attn(const Kv4Attn a) {
     f[w] = sm[w][row] == mm ? 1.0f : __builtin_amdgcn_exp2f(sm[w][row] - mm);
     total += f[w] * sl[w][row];
   }
-  const float inv = total == 0.0f ? 0.0f : 1.0f / total;
   const int rr = j.r0 + row;
-  E *dst = (E *)a.out + (int64_t)(j.q0 + rr / a.group) * a.ld_out + (head * a.group + rr % a.group) * HD + part * NC;
+  float v[NC];
 #pragma unroll
   for (int c = 0; c < NC; c++) {
-    float v = 0.0f;
-    for (int w = 0; w < NW; w++) v = fmaf(f[w], so[w][row][part * NC + c], v);
-    dst[c] = row_put(R{}, v * inv);
+    v[c] = 0.0f;
+    for (int w = 0; w < NW; w++) v[c] = fmaf(f[w], so[w][row][part * NC + c], v[c]);
   }
+  if (min(chunks, (int)gridDim.z) == 1) {
+    const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+    E *dst = (E *)a.out + (int64_t)(j.q0 + rr / a.group) * a.ld_out + (head * a.group + rr % a.group) * HD + part * NC;
+#pragma unroll
+    for (int c = 0; c < NC; c++) dst[c] = row_put(R{}, v[c] * inv);
+    return;
+  }
+  const int64_t at = (((int64_t)blockIdx.x * a.n_kv + head) * gridDim.z + blockIdx.z) * 16 + row;
+  float *dst = a.part + at * HD + part * NC;
+#pragma unroll
+  for (int c = 0; c < NC; c += 4) *(float4 *)(dst + c) = make_float4(v[c], v[c + 1], v[c + 2], v[c + 3]);
+  if (part == 0) ((float2 *)(a.part + (int64_t)gridDim.x * a.n_kv * gridDim.z * 16 * HD))[at] = make_float2(mm, total);
 }
 
-hipError_t launch_kv4_attention(const Kv4Attn &a, int hd, int type, hipStream_t s) {
-  const int64_t jobs = (int64_t)a.rows * a.group / 16 + a.n_seq;
-#define CALL(H, R)                                                                                                      \
-  hipLaunchKernelGGL((k_kv4_attn<H, R, sizeof(R::E) == 4 ? 2 : 1, std::is_same<R, RowBF16>::value ? 1 : 2>),            \
-                     dim3((unsigned)jobs, (unsigned)a.n_kv), dim3(256), 0, s, a)
+// The chunks of a job's rows together, 16 threads a row.
+template <int HD, class R>
+__global__ __launch_bounds__(256) void k_kv4_join(const Kv4Attn a, int splits) {
+  typedef typename R::E E;
+  constexpr int NC = HD / 16;
+  Job4 j;
+  if (!job_of<16>(a, blockIdx.x, j)) return;
+  const int rows = j.nq * a.group, head = blockIdx.y, row = threadIdx.x >> 4, part = threadIdx.x & 15, rr = j.r0 + row;
+  const int last = min(j.r0 + 15, rows - 1) / a.group, first = j.r0 / a.group;
+  const int all_hi = min(j.n - j.nq + last + 1, j.n), from = (a.window > 0 ? max(j.n - j.nq + first + 1 - a.window, 0) : 0) & ~31;
+  const int n = min(all_hi > from ? (all_hi - from + a.chunk - 1) / a.chunk : 1, splits);
+  if (n == 1 || rr >= rows) return;
+  const int64_t at = ((int64_t)blockIdx.x * a.n_kv + head) * splits * 16 + row;
+  const float2 *ms = (const float2 *)(a.part + (int64_t)gridDim.x * a.n_kv * splits * 16 * HD) + at;
+  float m = -__builtin_inff();
+  for (int c = 0; c < n; c++) m = fmaxf(m, ms[c * 16].x);
+  float total = 0.0f, v[NC] = {};
+  for (int c = 0; c < n; c++) {
+    const float2 x = ms[c * 16];
+    const float f = x.x == m ? 1.0f : __builtin_amdgcn_exp2f(x.x - m);
+    total = fmaf(f, x.y, total);
+    const float *src = a.part + (at + c * 16) * HD + part * NC;
+#pragma unroll
+    for (int i = 0; i < NC; i++) v[i] = fmaf(f, src[i], v[i]);
+  }
+  const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+  E *dst = (E *)a.out + (int64_t)(j.q0 + rr / a.group) * a.ld_out + (head * a.group + rr % a.group) * HD + part * NC;
+#pragma unroll
+  for (int i = 0; i < NC; i++) dst[i] = row_put(R{}, v[i] * inv);
+}
+
+// How the work is split: jobs, chunks of a sequence (at most) and tokens a chunk. Chunks are as long
+// as leaves about KV4_WGS workgroups, 128 tokens (a tile a wave) at least.
+constexpr int KV4_WGS = 4096;
+struct Split4 { int64_t jobs; int splits, chunk; };
+static Split4 split_of(int group, int n_kv, int rows, int n_seq, int max_kv) {
+  Split4 r;
+  r.jobs = (int64_t)rows * group / 16 + n_seq;
+  const int64_t busy = (((int64_t)rows * group + n_seq - 1) / n_seq + 15) / 16 * n_seq * n_kv;  // jobs with rows, all key heads
+  const int64_t want = (KV4_WGS + busy - 1) / busy;
+  int64_t chunk = ((max_kv + want - 1) / want + 127) / 128 * 128;
+  if (chunk < 128) chunk = 128;
+  if (chunk > 1 << 20) chunk = 1 << 20;
+  r.chunk = (int)chunk;
+  r.splits = (int)((max_kv + chunk - 1) / chunk);
+  if (r.splits < 1) r.splits = 1;
+  return r;
+}
+int64_t kv4_attention_ws(int hd, int group, int n_kv, int rows, int n_seq, int max_kv) {
+  const Split4 d = split_of(group, n_kv, rows, n_seq, max_kv);
+  return d.splits > 1 ? d.jobs * n_kv * d.splits * 16 * (hd + 2) * 4 : 0;
+}
+
+hipError_t launch_kv4_attention(Kv4Attn a, int hd, int type, int max_kv, hipStream_t s) {
+  const Split4 d = split_of(a.group, a.n_kv, a.rows, a.n_seq, max_kv);
+  a.chunk = d.chunk;
+  const dim3 grid((unsigned)d.jobs, (unsigned)a.n_kv, (unsigned)d.splits);
+#define CALL(H, R)                                                                                                              \
+  hipLaunchKernelGGL((k_kv4_attn<H, R, sizeof(R::E) == 4 ? 2 : 1, std::is_same<R, RowBF16>::value ? 1 : 2>), grid, dim3(256), 0, \
+                     s, a);                                                                                                     \
+  if (d.splits > 1) hipLaunchKernelGGL((k_kv4_join<H, R>), dim3(grid.x, grid.y), dim3(256), 0, s, a, d.splits)
   KV4_BY_TYPE(hd, type, CALL)
 #undef CALL
   return hipGetLastError();
