@@ -5,6 +5,9 @@ shared library whose C ABI is include/spx.h. Compile flags:
   -ffp-contract=off   the kernels place every fused multiply-add explicitly (fmaf), so the
                       compiler must not contract a*b+c on its own (rounding is part of parity)
   -packed-fp32-ops off  no packed fp32 instructions are generated
+  -amdgpu-mfma-vgpr-form (kv4.hip)  matrix instructions accumulate in vector registers: that kernel's
+                      loops scale and start their accumulators every step, and kept in the accumulation
+                      file they cost 80 register moves of 330 instructions a step
 """
 import concurrent.futures as cf
 import glob
@@ -21,6 +24,8 @@ FLAGS = ["-O3", "--offload-arch=gfx950", "-fPIC", "-std=c++17", "-ffp-contract=o
          "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
          "-Wall", "-Wno-unused-result", "-Wno-unused-function"]
 
+EXTRA = {"kv4.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]}
+
 
 def sources():
     return sorted(glob.glob(os.path.join(CSRC, "*.hip")) + glob.glob(os.path.join(CSRC, "*.cpp")))
@@ -28,7 +33,7 @@ def sources():
 
 def _compile(src):
     obj = os.path.join(BUILD, os.path.basename(src) + ".o")
-    cmd = [HIPCC, "-x", "hip", "-c", src, "-o", obj] + FLAGS
+    cmd = [HIPCC, "-x", "hip", "-c", src, "-o", obj] + FLAGS + EXTRA.get(os.path.basename(src), [])
     r = subprocess.run(cmd, capture_output=True, text=True)
     err = "\n".join(l for l in (r.stderr or "").splitlines() if "packed-fp32-ops" not in l)
     return obj, r.returncode, err

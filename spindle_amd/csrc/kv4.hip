@@ -209,12 +209,20 @@ hipError_t launch_kv4_read(const Kv4Rows &a, int hd, int type, hipStream_t s) {
 // S^T = K Q^T on v_mfma_f32_16x16x32_f16: a lane's column is its query row (lane % 16), its four
 // rows are tokens, so a row's maximum and sum lie in four lanes and the probabilities are, as they
 // come, the right operand of O^T = V^T P^T: lane l of 16 and quarter h holds tokens 4h .. 4h + 3 of
-// each of the two tiles there. Keys and values meet the matrix cores exactly (integer * scale in
-// f16). A query row is scaled by a power of two to fill f16's range; in two parts (SPX_F32) it has
-// 22 bits. Probabilities are held relative to a running maximum, times 2^10, so that small ones
-// keep their bits in f16; a maximum that grows by less than 2^5 leaves the reference as it is. In
-// two parts (SPX_F32, SPX_F16) they have 22 bits too: one part's rounding (2^-12) would add to the
-// output's own in SPX_F16; in SPX_BF16 it is an eighth of it.
+// each of the two tiles there.
+//
+// What bounds the kernel is the vector instructions that turn codes into operands. Key codes go in as
+// they are: a nibble masked in place is a subnormal f16 (code * 2^-24, or 2^-20 from the high nibble
+// of a byte, which the query makes up for), which the matrix cores multiply exactly, so a word of
+// eight codes costs five instructions; a group's sum starts at -8 times the query's and is scaled
+// afterwards, with one multiply-add a token, row and group. Values become integer * scale in f16
+// (exact): their scale belongs to the token, which the sum runs over.
+//
+// A query row is scaled by a power of two to fill f16's range; in two parts (SPX_F32) it has 22 bits.
+// Probabilities are held relative to a running maximum, times 2^10, so that small ones keep their
+// bits in f16; a maximum that grows by less than 2^5 leaves the reference as it is. In two parts
+// (SPX_F32, SPX_F16) they have 22 bits too: one part's rounding (2^-11) would add to the output's own
+// in SPX_F16; in SPX_BF16 it is an eighth of it.
 constexpr float P_LIFT = 10.0f, P_SLACK = 5.0f;
 
 // The sequence and first row of job `job`: sequence s has jobs floor(start_s * group / BM) + s and
@@ -242,51 +250,67 @@ __device__ __forceinline__ bool job_of(const Kv4Attn &a, int job, Job4 &j) {
 
 __device__ __forceinline__ h2v bits_h2(uint32_t v) { return __builtin_bit_cast(h2v, v); }
 
-// Eight codes of a key word as eight f16 values, channels in order: pairs (nibble i, nibble i + 4)
-// become 1024 + code or 64 + code by an exponent put over them.
-__device__ __forceinline__ h8v key_frag(uint32_t w, h2v d) {
-  const h2v o0 = {(_Float16)-1032.0f, (_Float16)-1032.0f}, o1 = {(_Float16)-72.0f, (_Float16)-72.0f};
+// Constants held in registers: the instruction that masks and puts an exponent over the rest in one
+// takes one constant from the scalar file and none from the instruction stream.
+struct Const4 {
+  uint32_t lo = 0x000f000fu, hi = 0x00f000f0u;  // scalar
+  uint32_t e0 = 0x64006400u, e1 = 0x54005400u;  // vector: f16 1024 (ulp 1) and 64 (ulp 1/16)
+};
+__device__ __forceinline__ Const4 constants() {
+  Const4 c;
+  asm("" : "+s"(c.lo));
+  asm("" : "+s"(c.hi));
+  asm("" : "+v"(c.e0));
+  asm("" : "+v"(c.e1));
+  return c;
+}
+// Eight codes of a key word as eight f16 values, channels in order: subnormals code * 2^-24 in
+// elements 0, 1, 4, 5, code * 2^-20 in the others.
+__device__ __forceinline__ h8v key_codes(uint32_t w, const Const4 &k) {
   const uint32_t w8 = w >> 8;
-  h2v x[4];
-  x[0] = (bits_h2((w & 0x000f000fu) | 0x64006400u) + o0) * d;
-  x[1] = (bits_h2((w & 0x00f000f0u) | 0x54005400u) + o1) * d;
-  x[2] = (bits_h2((w8 & 0x000f000fu) | 0x64006400u) + o0) * d;
-  x[3] = (bits_h2((w8 & 0x00f000f0u) | 0x54005400u) + o1) * d;
+  const uint32_t x[4] = {w & k.lo, w & k.hi, w8 & k.lo, w8 & k.hi};
   return __builtin_bit_cast(h8v, x);
 }
-// Byte b of the value words of two tokens as two channels' pairs of tokens.
+// Byte b of the value words of two tokens as two channels' pairs of tokens: 1024 + code and 64 + code
+// by an exponent put over the nibble, less what is too much, times the tokens' scales.
 template <int HD>
-__device__ __forceinline__ void value_pairs(uint32_t w0, uint32_t w1, int b, h2v d, h2v &even, h2v &odd) {
+__device__ __forceinline__ void value_pairs(uint32_t w0, uint32_t w1, int b, h2v d, const Const4 &k, h2v &even, h2v &odd) {
   const h2v o0 = {(_Float16)-1032.0f, (_Float16)-1032.0f}, o1 = {(_Float16)-72.0f, (_Float16)-72.0f};
   // HD 128: byte b of w0 and of w1; HD 64: both tokens' bytes lie in w0
   const uint32_t p = HD == 128 ? __builtin_amdgcn_perm(w1, w0, 0x0c040c00u + (uint32_t)b * 0x00010001u)
                                : __builtin_amdgcn_perm(w0, w0, 0x0c020c00u + (uint32_t)b * 0x00010001u);
-  even = (bits_h2((p & 0x000f000fu) | 0x64006400u) + o0) * d;
-  odd = (bits_h2((p & 0x00f000f0u) | 0x54005400u) + o1) * d;
+  even = (bits_h2((p & k.lo) | k.e0) + o0) * d;
+  odd = (bits_h2((p & k.hi) | k.e1) + o1) * d;
 }
+typedef float f2r __attribute__((ext_vector_type(2)));
+// Two numbers as f16, and what that leaves of them.
+__device__ __forceinline__ h2v half_pair(float a, float b) { return __builtin_convertvector((f2r{a, b}), h2v); }
+__device__ __forceinline__ h2v half_rest(float a, float b, h2v top) { return half_pair(fmaf(-(float)top[0], 1.0f, a), fmaf(-(float)top[1], 1.0f, b)); }
 
-// What a lane holds of a tile of 16 tokens.
+// What a lane holds of a tile of 16 tokens: its token's key words, its four tokens' value words and
+// scales.
 template <int HD>
 struct Tile4 {
   uint32_t k[HD / 32], v[HD / 32];
-  h2v ks[HD / 64], vs[2];  // its token's scales; its four tokens' in its channels' group
+  h2v ks[4][HD / 64], vs[2];  // all groups' of a token; its channels' group's
 };
 template <int HD>
 __device__ __forceinline__ void tile_load(Tile4<HD> &x, const uint8_t *tile, int lane) {
   constexpr int G = HD / 32;
   const int l = lane & 15, h = lane >> 4;
-  const uint8_t *kc = tile + lane * 4 * G, *vc = kc + 8 * HD, *ks = tile + 16 * HD + l * 2 * G, *vs = tile + 17 * HD + ((l * G >> 4) * 16 + 4 * h) * 2;
+  const uint8_t *kc = tile + lane * 4 * G, *vc = kc + 8 * HD, *ks = tile + 16 * HD + h * 8 * G, *vs = tile + 17 * HD + ((l * G >> 4) * 16 + 4 * h) * 2;
   if constexpr (HD == 128) {
-    const uint4 a = *(const uint4 *)kc, b = *(const uint4 *)vc;
-    const uint2 c = *(const uint2 *)ks;
+    const uint4 a = *(const uint4 *)kc, b = *(const uint4 *)vc, c = *(const uint4 *)ks, d = *(const uint4 *)(ks + 16);
     x.k[0] = a.x; x.k[1] = a.y; x.k[2] = a.z; x.k[3] = a.w;
     x.v[0] = b.x; x.v[1] = b.y; x.v[2] = b.z; x.v[3] = b.w;
-    x.ks[0] = bits_h2(c.x); x.ks[1] = bits_h2(c.y);
+    x.ks[0][0] = bits_h2(c.x); x.ks[0][1] = bits_h2(c.y); x.ks[1][0] = bits_h2(c.z); x.ks[1][1] = bits_h2(c.w);
+    x.ks[2][0] = bits_h2(d.x); x.ks[2][1] = bits_h2(d.y); x.ks[3][0] = bits_h2(d.z); x.ks[3][1] = bits_h2(d.w);
   } else {
     const uint2 a = *(const uint2 *)kc, b = *(const uint2 *)vc;
+    const uint4 c = *(const uint4 *)ks;
     x.k[0] = a.x; x.k[1] = a.y;
     x.v[0] = b.x; x.v[1] = b.y;
-    x.ks[0] = bits_h2(*(const uint32_t *)ks);
+    x.ks[0][0] = bits_h2(c.x); x.ks[1][0] = bits_h2(c.y); x.ks[2][0] = bits_h2(c.z); x.ks[3][0] = bits_h2(c.w);
   }
   const uint2 c = *(const uint2 *)vs;
   x.vs[0] = bits_h2(c.x);
@@ -298,7 +322,7 @@ __device__ __forceinline__ float lift_of(float amax) {
   if (!(amax > 0.0f) || !(amax < __builtin_inff())) return 1.0f;
   int e;
   (void)frexpf(amax, &e);
-  return ldexpf(1.0f, min(max(14 - e, -126), 126));
+  return ldexpf(1.0f, min(max(14 - e, -100), 100));
 }
 
 // Long sequences are shared by workgroups: chunk blockIdx.z of `chunk` tokens (and every
@@ -324,16 +348,24 @@ __global__ __launch_bounds__(256) void k_kv4_attn(const Kv4Attn a) {
       amax = fmaxf(amax, fabsf(qv[g][i]));
     }
   amax = max32(max16(amax));
-  const float lift = lift_of(amax), unlift = a.scale / lift;
+  const float lift = lift_of(amax), unlift = a.scale / lift * 16777216.0f;
   h8v qh[G], ql[G];
+  f4v zero[G];  // where a group's sum starts
 #pragma unroll
-  for (int g = 0; g < G; g++)
+  for (int g = 0; g < G; g++) {
+    float all = 0.0f;
 #pragma unroll
     for (int i = 0; i < 8; i++) {
-      const float x = qv[g][i] * lift;
-      qh[g][i] = (_Float16)x;
-      if (QP == 2) ql[g][i] = (_Float16)(x - (float)qh[g][i]);
+      const float x = qv[g][i] * lift, down = i & 2 ? 0.0625f : 1.0f;
+      const _Float16 top = (_Float16)x;
+      const _Float16 low = (_Float16)(QP == 2 ? x - (float)top : 0.0f);
+      all += (float)top + (float)low;
+      qh[g][i] = (_Float16)((float)top * down);
+      ql[g][i] = (_Float16)((float)low * down);
     }
+    all = add32(add16(all)) * (-8.0f / 16777216.0f);
+    zero[g] = f4v{all, all, all, all};
+  }
   const int pos = j.n - j.nq + tok;
   const int hi = min(pos + 1, j.n), lo = a.window > 0 ? max(pos + 1 - a.window, 0) : 0;
   // all rows of the job together
@@ -349,36 +381,45 @@ __global__ __launch_bounds__(256) void k_kv4_attn(const Kv4Attn a) {
   const int *table = a.tables + (int64_t)j.s * a.cols;
   const int pm = (1 << a.page) - 1;
 
-  for (int c = blockIdx.z; c < chunks; c += gridDim.z)
-  for (int t0 = from + c * a.chunk + 32 * wave; t0 < min(all_hi, from + (c + 1) * a.chunk); t0 += 32 * NW) {
-    Tile4<HD> x[2];
-    bool in[2];
+  // tokens that every row sees: tiles of them need no masks (a NaN there reaches every row)
+  const int see_lo = a.window > 0 ? max(j.n - j.nq + last + 1 - a.window, 0) : 0, see_hi = min(j.n - j.nq + first + 1, j.n);
+
+  const Const4 kc = constants();
+  auto load = [&](Tile4<HD> *x, int t0) {  // which of the two tiles there are, as bits
+    int in = 0;
 #pragma unroll
     for (int u = 0; u < 2; u++) {
       const int t = t0 + 16 * u;
       const int pg = t < all_hi ? table[t >> a.page] : -1;
-      in[u] = pg >= 0 && pg < a.n_pages;
-      tile_load<HD>(x[u], a.pool + tile_at<HD>(in[u] ? pg : 0, a.n_kv, head, a.page, in[u] ? t & pm : 0), lane);
+      const bool ok = pg >= 0 && pg < a.n_pages;
+      in |= (int)ok << u;
+      tile_load<HD>(x[u], a.pool + tile_at<HD>(ok ? pg : 0, a.n_kv, head, a.page, ok ? t & pm : 0), lane);
     }
+    return in;
+  };
+  auto step = [&](Tile4<HD> *x, int t0, int in, auto edge_) {
+    constexpr bool edge = decltype(edge_)::value;
     float s[2][4], mt = -__builtin_inff();
 #pragma unroll
     for (int u = 0; u < 2; u++) {
-      f4v acc = {0.0f, 0.0f, 0.0f, 0.0f};
+      f4v acc[G];
 #pragma unroll
       for (int g = 0; g < G; g++) {
-        const _Float16 d = x[u].ks[g >> 1][g & 1];
-        const h8v kf = key_frag(x[u].k[g], h2v{d, d});
-        acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qh[g], acc, 0, 0, 0);
-        if (QP == 2) acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, ql[g], acc, 0, 0, 0);
+        const h8v kf = key_codes(x[u].k[g], kc);
+        acc[g] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qh[g], zero[g], 0, 0, 0);
+        if (QP == 2) acc[g] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, ql[g], acc[g], 0, 0, 0);
       }
 #pragma unroll
       for (int i = 0; i < 4; i++) {
+        float v = 0.0f;
+#pragma unroll
+        for (int g = 0; g < G; g++) v = fmaf((float)x[u].ks[i][g >> 1][g & 1], acc[g][i], v);
         const int t = t0 + 16 * u + 4 * h + i;
-        s[u][i] = in[u] && t >= lo && t < hi ? acc[i] * unlift : -__builtin_inff();
+        s[u][i] = !edge || ((in >> u & 1) && t >= lo && t < hi) ? v : -__builtin_inff();
         mt = fmaxf(mt, s[u][i]);
       }
     }
-    mt = max32(max16(mt));
+    mt = max32(max16(mt)) * unlift;  // (unlift is positive)
     if (__builtin_amdgcn_ballot_w64(mt > m + P_SLACK)) {
       const float mn = fmaxf(m, mt), f = m == mn ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
       m = mn;
@@ -386,48 +427,44 @@ __global__ __launch_bounds__(256) void k_kv4_attn(const Kv4Attn a) {
 #pragma unroll
       for (int c = 0; c < NC; c++) o[c] *= f;
     }
-    const float ref = m == -__builtin_inff() ? 0.0f : m - P_LIFT;
-    h8v ph, pl;
+    const float ref = m == -__builtin_inff() ? 0.0f : P_LIFT - m;
+    h2v p1[4], p2[4];
 #pragma unroll
     for (int u = 0; u < 2; u++)
 #pragma unroll
-      for (int i = 0; i < 4; i++) {
-        const float p = __builtin_amdgcn_exp2f(s[u][i] - ref);
-        sum += p;
-        ph[4 * u + i] = (_Float16)p;
-        if (PP == 2) pl[4 * u + i] = (_Float16)(p - (float)ph[4 * u + i]);
+      for (int i = 0; i < 4; i += 2) {
+        const float x = __builtin_amdgcn_exp2f(fmaf(s[u][i], unlift, ref)), y = __builtin_amdgcn_exp2f(fmaf(s[u][i + 1], unlift, ref));
+        sum += x + y;
+        p1[2 * u + i / 2] = half_pair(x, y);
+        if (PP == 2) p2[2 * u + i / 2] = half_rest(x, y, p1[2 * u + i / 2]);
       }
-    // values of tokens that no row may see count as zero (what lies there may be anything)
-    h2v vs[2][2];
-    bool nan = false;
-#pragma unroll
-    for (int u = 0; u < 2; u++)
-#pragma unroll
-      for (int i = 0; i < 4; i++) {
-        const int t = t0 + 16 * u + 4 * h + i;
-        const _Float16 d = x[u].vs[i >> 1][i & 1];
-        vs[u][i >> 1][i & 1] = in[u] && t >= all_lo && t < all_hi ? d : (_Float16)0.0f;
-        nan |= !(vs[u][i >> 1][i & 1] == vs[u][i >> 1][i & 1]);
-      }
-    if (__builtin_expect(__builtin_amdgcn_ballot_w64(nan) != 0, 0)) {
-      // a NaN among the values reaches the rows that see its token and no others: which they are
-      // is a product of 0s and 1s, and in the products below it counts as zero
+    const h8v ph = __builtin_bit_cast(h8v, p1), pl = __builtin_bit_cast(h8v, p2);
+    h2v vs[2][2] = {{x[0].vs[0], x[0].vs[1]}, {x[1].vs[0], x[1].vs[1]}};
+    if (edge) {
+      // values of tokens that no row may see count as zero (what lies there may be anything); a NaN
+      // among the others reaches the rows that see its token and no others: which they are is a
+      // product of 0s and 1s, and in the products below it counts as zero
+      bool nan = false;
       h8v bad, sees;
 #pragma unroll
       for (int u = 0; u < 2; u++)
 #pragma unroll
         for (int i = 0; i < 4; i++) {
+          const int t = t0 + 16 * u + 4 * h + i;
           const _Float16 d = vs[u][i >> 1][i & 1];
-          bad[4 * u + i] = (_Float16)(d == d ? 0.0f : 1.0f);
-          vs[u][i >> 1][i & 1] = d == d ? d : (_Float16)0.0f;
+          const bool is = (in >> u & 1) && t >= all_lo && t < all_hi, num = d == d;
+          nan |= is && !num;
+          bad[4 * u + i] = (_Float16)(is && !num ? 1.0f : 0.0f);
           sees[4 * u + i] = (_Float16)(s[u][i] == -__builtin_inff() ? 0.0f : 1.0f);
+          vs[u][i >> 1][i & 1] = is && num ? d : (_Float16)0.0f;
         }
-      const f4v hit = __builtin_amdgcn_mfma_f32_16x16x32_f16(bad, sees, f4v{0.0f, 0.0f, 0.0f, 0.0f}, 0, 0, 0);
+      if (__builtin_amdgcn_ballot_w64(nan)) {
+        const f4v hit = __builtin_amdgcn_mfma_f32_16x16x32_f16(bad, sees, f4v{0.0f, 0.0f, 0.0f, 0.0f}, 0, 0, 0);
 #pragma unroll
-      for (int c = 0; c < NC; c++)
+        for (int c = 0; c < NC; c++)
 #pragma unroll
-        for (int i = 0; i < 4; i++)
-          if (hit[i] > 0.0f) o[c][i] = __builtin_nanf("");
+          for (int i = 0; i < 4; i++) o[c][i] = hit[i] > 0.0f ? __builtin_nanf("") : o[c][i];
+      }
     }
 #pragma unroll
     for (int b = 0; b < NC / 2; b++) {
@@ -436,8 +473,8 @@ __global__ __launch_bounds__(256) void k_kv4_attn(const Kv4Attn a) {
       for (int u = 0; u < 2; u++)
 #pragma unroll
         for (int i = 0; i < 2; i++) {
-          if constexpr (HD == 128) value_pairs<HD>(x[u].v[2 * i], x[u].v[2 * i + 1], b, vs[u][i], e[2 * u + i], d[2 * u + i]);
-          else value_pairs<HD>(x[u].v[i], 0u, b, vs[u][i], e[2 * u + i], d[2 * u + i]);
+          if constexpr (HD == 128) value_pairs<HD>(x[u].v[2 * i], x[u].v[2 * i + 1], b, vs[u][i], kc, e[2 * u + i], d[2 * u + i]);
+          else value_pairs<HD>(x[u].v[i], 0u, b, vs[u][i], kc, e[2 * u + i], d[2 * u + i]);
         }
       const h8v ve = __builtin_bit_cast(h8v, e), vo = __builtin_bit_cast(h8v, d);
       o[2 * b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ve, ph, o[2 * b], 0, 0, 0);
@@ -446,6 +483,15 @@ __global__ __launch_bounds__(256) void k_kv4_attn(const Kv4Attn a) {
         o[2 * b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ve, pl, o[2 * b], 0, 0, 0);
         o[2 * b + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vo, pl, o[2 * b + 1], 0, 0, 0);
       }
+    }
+  };
+  for (int c = blockIdx.z; c < chunks; c += gridDim.z) {
+    const int end = min(all_hi, from + (c + 1) * a.chunk);
+    for (int t0 = from + c * a.chunk + 32 * wave; t0 < end; t0 += 32 * NW) {
+      Tile4<HD> x[2];
+      const int in = load(x, t0);
+      if (in == 3 && t0 >= see_lo && t0 + 32 <= see_hi) step(x, t0, in, std::false_type{});
+      else step(x, t0, in, std::true_type{});
     }
   }
   sum = add32(add16(sum));
@@ -487,30 +533,51 @@ __global__ __launch_bounds__(256) void k_kv4_attn(const Kv4Attn a) {
   if (part == 0) ((float2 *)(a.part + (int64_t)gridDim.x * a.n_kv * gridDim.z * 16 * HD))[at] = make_float2(mm, total);
 }
 
-// The chunks of a job's rows together, 16 threads a row.
+// The chunks of a job's rows together: a wave has four rows, 16 lanes each.
 template <int HD, class R>
-__global__ __launch_bounds__(256) void k_kv4_join(const Kv4Attn a, int splits) {
+__global__ __launch_bounds__(64) void k_kv4_join(const Kv4Attn a, int splits) {
   typedef typename R::E E;
-  constexpr int NC = HD / 16;
+  constexpr int NC = HD / 16, U = 4;
   Job4 j;
   if (!job_of<16>(a, blockIdx.x, j)) return;
-  const int rows = j.nq * a.group, head = blockIdx.y, row = threadIdx.x >> 4, part = threadIdx.x & 15, rr = j.r0 + row;
+  const int rows = j.nq * a.group, head = blockIdx.y, row = blockIdx.z * 4 + (threadIdx.x >> 4), part = threadIdx.x & 15, rr = j.r0 + row;
   const int last = min(j.r0 + 15, rows - 1) / a.group, first = j.r0 / a.group;
   const int all_hi = min(j.n - j.nq + last + 1, j.n), from = (a.window > 0 ? max(j.n - j.nq + first + 1 - a.window, 0) : 0) & ~31;
   const int n = min(all_hi > from ? (all_hi - from + a.chunk - 1) / a.chunk : 1, splits);
   if (n == 1 || rr >= rows) return;
   const int64_t at = ((int64_t)blockIdx.x * a.n_kv + head) * splits * 16 + row;
   const float2 *ms = (const float2 *)(a.part + (int64_t)gridDim.x * a.n_kv * splits * 16 * HD) + at;
+  const float *src = a.part + at * HD + part * NC;
   float m = -__builtin_inff();
-  for (int c = 0; c < n; c++) m = fmaxf(m, ms[c * 16].x);
+  for (int c = part; c < n; c += 16) m = fmaxf(m, ms[c * 16].x);
+  m = fmaxf(m, SPX_DPPF(m, 0xB1));
+  m = fmaxf(m, SPX_DPPF(m, 0x4E));
+  m = fmaxf(m, SPX_DPPF(m, 0x141));
+  m = fmaxf(m, SPX_DPPF(m, 0x140));
   float total = 0.0f, v[NC] = {};
-  for (int c = 0; c < n; c++) {
-    const float2 x = ms[c * 16];
-    const float f = x.x == m ? 1.0f : __builtin_amdgcn_exp2f(x.x - m);
-    total = fmaf(f, x.y, total);
-    const float *src = a.part + (at + c * 16) * HD + part * NC;
+  for (int c0 = 0; c0 < n; c0 += U) {  // U chunks' loads at a time
+    float2 x[U];
+    float4 y[U][NC / 4];
 #pragma unroll
-    for (int i = 0; i < NC; i++) v[i] = fmaf(f, src[i], v[i]);
+    for (int u = 0; u < U; u++) {
+      const int c = min(c0 + u, n - 1);
+      x[u] = ms[c * 16];
+#pragma unroll
+      for (int i = 0; i < NC / 4; i++) y[u][i] = *(const float4 *)(src + (int64_t)c * 16 * HD + 4 * i);
+    }
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+      const float f = x[u].x == m ? 1.0f : __builtin_amdgcn_exp2f(x[u].x - m);
+      if (c0 + u >= n) continue;  // (0 times a NaN is one)
+      total = fmaf(f, x[u].y, total);
+#pragma unroll
+      for (int i = 0; i < NC / 4; i++) {
+        v[4 * i] = fmaf(f, y[u][i].x, v[4 * i]);
+        v[4 * i + 1] = fmaf(f, y[u][i].y, v[4 * i + 1]);
+        v[4 * i + 2] = fmaf(f, y[u][i].z, v[4 * i + 2]);
+        v[4 * i + 3] = fmaf(f, y[u][i].w, v[4 * i + 3]);
+      }
+    }
   }
   const float inv = total == 0.0f ? 0.0f : 1.0f / total;
   E *dst = (E *)a.out + (int64_t)(j.q0 + rr / a.group) * a.ld_out + (head * a.group + rr % a.group) * HD + part * NC;
@@ -547,7 +614,7 @@ hipError_t launch_kv4_attention(Kv4Attn a, int hd, int type, int max_kv, hipStre
 #define CALL(H, R)                                                                                                              \
   hipLaunchKernelGGL((k_kv4_attn<H, R, sizeof(R::E) == 4 ? 2 : 1, std::is_same<R, RowBF16>::value ? 1 : 2>), grid, dim3(256), 0, \
                      s, a);                                                                                                     \
-  if (d.splits > 1) hipLaunchKernelGGL((k_kv4_join<H, R>), dim3(grid.x, grid.y), dim3(256), 0, s, a, d.splits)
+  if (d.splits > 1) hipLaunchKernelGGL((k_kv4_join<H, R>), dim3(grid.x, grid.y, 4), dim3(64), 0, s, a, d.splits)
   KV4_BY_TYPE(hd, type, CALL)
 #undef CALL
   return hipGetLastError();
