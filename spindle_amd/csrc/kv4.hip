@@ -385,12 +385,19 @@ __global__ __launch_bounds__(256) void k_kv4_attn(const Kv4Attn a) {
   const int see_lo = a.window > 0 ? max(j.n - j.nq + last + 1 - a.window, 0) : 0, see_hi = min(j.n - j.nq + first + 1, j.n);
 
   const Const4 kc = constants();
+  int base = 0, pages = -1;  // lane i holds the page id of entry base + i
+  bool have = false;
   auto load = [&](Tile4<HD> *x, int t0) {  // which of the two tiles there are, as bits
     int in = 0;
+    if (!have || ((t0 + 31) >> a.page) - base > 63) {
+      have = true;
+      base = t0 >> a.page;
+      pages = table[min(base + lane, a.cols - 1)];
+    }
 #pragma unroll
     for (int u = 0; u < 2; u++) {
       const int t = t0 + 16 * u;
-      const int pg = t < all_hi ? table[t >> a.page] : -1;
+      const int pg = t < all_hi ? lane_i(pages, (t >> a.page) - base) : -1;
       const bool ok = pg >= 0 && pg < a.n_pages;
       in |= (int)ok << u;
       tile_load<HD>(x[u], a.pool + tile_at<HD>(ok ? pg : 0, a.n_kv, head, a.page, ok ? t & pm : 0), lane);
@@ -487,6 +494,7 @@ __global__ __launch_bounds__(256) void k_kv4_attn(const Kv4Attn a) {
   };
   for (int c = blockIdx.z; c < chunks; c += gridDim.z) {
     const int end = min(all_hi, from + (c + 1) * a.chunk);
+    have = false;
     for (int t0 = from + c * a.chunk + 32 * wave; t0 < end; t0 += 32 * NW) {
       Tile4<HD> x[2];
       const int in = load(x, t0);
@@ -587,7 +595,7 @@ __global__ __launch_bounds__(64) void k_kv4_join(const Kv4Attn a, int splits) {
 
 // How the work is split: jobs, chunks of a sequence (at most) and tokens a chunk. Chunks are as long
 // as leaves about KV4_WGS workgroups, 128 tokens (a tile a wave) at least.
-constexpr int KV4_WGS = 4096;
+constexpr int KV4_WGS = 2048;
 struct Split4 { int64_t jobs; int splits, chunk; };
 static Split4 split_of(int group, int n_kv, int rows, int n_seq, int max_kv) {
   Split4 r;
@@ -604,13 +612,15 @@ static Split4 split_of(int group, int n_kv, int rows, int n_seq, int max_kv) {
 }
 int64_t kv4_attention_ws(int hd, int group, int n_kv, int rows, int n_seq, int max_kv) {
   const Split4 d = split_of(group, n_kv, rows, n_seq, max_kv);
-  return d.splits > 1 ? d.jobs * n_kv * d.splits * 16 * (hd + 2) * 4 : 0;
+  return d.splits > 1 ? (d.jobs | 1) * n_kv * d.splits * 16 * (hd + 2) * 4 : 0;
 }
 
 hipError_t launch_kv4_attention(Kv4Attn a, int hd, int type, int max_kv, hipStream_t s) {
   const Split4 d = split_of(a.group, a.n_kv, a.rows, a.n_seq, max_kv);
   a.chunk = d.chunk;
-  const dim3 grid((unsigned)d.jobs, (unsigned)a.n_kv, (unsigned)d.splits);
+  // an odd count, so that neighbouring key heads and chunks of a sequence go to other XCDs (workgroups go
+  // around the eight of them in order)
+  const dim3 grid((unsigned)d.jobs | 1, (unsigned)a.n_kv, (unsigned)d.splits);
 #define CALL(H, R)                                                                                                              \
   hipLaunchKernelGGL((k_kv4_attn<H, R, sizeof(R::E) == 4 ? 2 : 1, std::is_same<R, RowBF16>::value ? 1 : 2>), grid, dim3(256), 0, \
                      s, a);                                                                                                     \
