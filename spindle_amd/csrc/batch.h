@@ -35,8 +35,9 @@ struct Kv4Attn {
   int n_heads, group, rows, n_seq, cols, window;
   const int32_t *q_start, *kv_lens, *tables;
   float scale;  // times log2(e)
-  int chunk;    // tokens a workgroup takes at a time
-  float *part;  // scratch: outputs, then (maximum, sum), of every job, key head, split and row
+  int few;            // sequences with more rows (new tokens x query heads a key head) are k_kv4_rows'
+  int chunk, rchunk;  // tokens a workgroup takes at a time
+  float *part, *rpart;  // scratch: outputs, then (maximum, sum), of every job, key head, split and row
 };
 int64_t kv4_attention_ws(int hd, int group, int n_kv, int rows, int n_seq, int max_kv);
 hipError_t launch_kv4_attention(Kv4Attn a, int hd, int type, int max_kv, hipStream_t s);

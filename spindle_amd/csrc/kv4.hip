@@ -248,6 +248,18 @@ __device__ __forceinline__ bool job_of(const Kv4Attn &a, int job, Job4 &j) {
   return j.nq > 0 && j.r0 >= 0 && j.r0 < j.nq * a.group;
 }
 
+// k_kv4_attn's jobs: where k_kv4_rows takes the sequences of more rows, each of the others is one.
+__device__ __forceinline__ bool few_job(const Kv4Attn &a, int job, Job4 &j) {
+  if (a.few == INT32_MAX) return job_of<16>(a, job, j);
+  if (job >= a.n_seq) return false;
+  j.s = job;
+  j.q0 = min(max(a.q_start[job], 0), a.rows);
+  j.nq = min(max(a.q_start[job + 1], 0), a.rows) - j.q0;
+  j.r0 = 0;
+  j.n = (int)min((int64_t)max(a.kv_lens[job], 0), (int64_t)a.cols << a.page);
+  return j.nq > 0 && j.nq * a.group <= a.few;
+}
+
 __device__ __forceinline__ h2v bits_h2(uint32_t v) { return __builtin_bit_cast(h2v, v); }
 
 // Constants held in registers: the instruction that masks and puts an exponent over the rest in one
@@ -264,12 +276,19 @@ __device__ __forceinline__ Const4 constants() {
   asm("" : "+v"(c.e1));
   return c;
 }
-// Eight codes of a key word as eight f16 values, channels in order: subnormals code * 2^-24 in
-// elements 0, 1, 4, 5, code * 2^-20 in the others.
+// Eight codes of a key word as eight f16 values, channels in order. EXACT: the integers code - 8.
+// Otherwise the codes as subnormals, code * 2^-24 in elements 0, 1, 4, 5, code * 2^-20 in the others.
+template <bool EXACT>
 __device__ __forceinline__ h8v key_codes(uint32_t w, const Const4 &k) {
   const uint32_t w8 = w >> 8;
-  const uint32_t x[4] = {w & k.lo, w & k.hi, w8 & k.lo, w8 & k.hi};
-  return __builtin_bit_cast(h8v, x);
+  if constexpr (EXACT) {
+    const h2v o0 = {(_Float16)-1032.0f, (_Float16)-1032.0f}, o1 = {(_Float16)-72.0f, (_Float16)-72.0f};
+    const h2v x[4] = {bits_h2((w & k.lo) | k.e0) + o0, bits_h2((w & k.hi) | k.e1) + o1, bits_h2((w8 & k.lo) | k.e0) + o0, bits_h2((w8 & k.hi) | k.e1) + o1};
+    return __builtin_bit_cast(h8v, x);
+  } else {
+    const uint32_t x[4] = {w & k.lo, w & k.hi, w8 & k.lo, w8 & k.hi};
+    return __builtin_bit_cast(h8v, x);
+  }
 }
 // Byte b of the value words of two tokens as two channels' pairs of tokens: 1024 + code and 64 + code
 // by an exponent put over the nibble, less what is too much, times the tokens' scales.
@@ -332,11 +351,13 @@ template <int HD, class R, int QP, int PP>
 __global__ __launch_bounds__(256) void k_kv4_attn(const Kv4Attn a) {
   typedef typename R::E E;
   constexpr int G = HD / 32, NC = HD / 16, NW = 4;
+  constexpr bool EXACT = QP == 2;
   __shared__ float so[NW][16][HD + 4], sm[NW][16], sl[NW][16];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l = lane & 15, h = lane >> 4, head = blockIdx.y;
   Job4 j;
-  if (!job_of<16>(a, blockIdx.x, j)) return;
-  const int rows = j.nq * a.group, r = j.r0 + l, tok = min(r, rows - 1) / a.group, g0 = min(r, rows - 1) % a.group;
+  if (!few_job(a, blockIdx.x, j)) return;
+  const int rows = j.nq * a.group;
+  const int r = j.r0 + l, tok = min(r, rows - 1) / a.group, g0 = min(r, rows - 1) % a.group;
   // the row's query, its scale and what it sees
   const E *qp = (const E *)a.q + (int64_t)(j.q0 + tok) * a.ld_q + (head * a.group + g0) * HD + 8 * h;
   float qv[G][8], amax = 0.0f;
@@ -348,7 +369,7 @@ __global__ __launch_bounds__(256) void k_kv4_attn(const Kv4Attn a) {
       amax = fmaxf(amax, fabsf(qv[g][i]));
     }
   amax = max32(max16(amax));
-  const float lift = lift_of(amax), unlift = a.scale / lift * 16777216.0f;
+  const float lift = lift_of(amax), unlift = a.scale / lift * (EXACT ? 1.0f : 16777216.0f);
   h8v qh[G], ql[G];
   f4v zero[G];  // where a group's sum starts
 #pragma unroll
@@ -356,14 +377,14 @@ __global__ __launch_bounds__(256) void k_kv4_attn(const Kv4Attn a) {
     float all = 0.0f;
 #pragma unroll
     for (int i = 0; i < 8; i++) {
-      const float x = qv[g][i] * lift, down = i & 2 ? 0.0625f : 1.0f;
+      const float x = qv[g][i] * lift, down = !EXACT && i & 2 ? 0.0625f : 1.0f;
       const _Float16 top = (_Float16)x;
       const _Float16 low = (_Float16)(QP == 2 ? x - (float)top : 0.0f);
       all += (float)top + (float)low;
       qh[g][i] = (_Float16)((float)top * down);
       ql[g][i] = (_Float16)((float)low * down);
     }
-    all = add32(add16(all)) * (-8.0f / 16777216.0f);
+    all = EXACT ? 0.0f : add32(add16(all)) * (-8.0f / 16777216.0f);
     zero[g] = f4v{all, all, all, all};
   }
   const int pos = j.n - j.nq + tok;
@@ -412,7 +433,7 @@ __global__ __launch_bounds__(256) void k_kv4_attn(const Kv4Attn a) {
       f4v acc[G];
 #pragma unroll
       for (int g = 0; g < G; g++) {
-        const h8v kf = key_codes(x[u].k[g], kc);
+        const h8v kf = key_codes<EXACT>(x[u].k[g], kc);
         acc[g] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qh[g], zero[g], 0, 0, 0);
         if (QP == 2) acc[g] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, ql[g], acc[g], 0, 0, 0);
       }
@@ -541,23 +562,320 @@ __global__ __launch_bounds__(256) void k_kv4_attn(const Kv4Attn a) {
   if (part == 0) ((float2 *)(a.part + (int64_t)gridDim.x * a.n_kv * gridDim.z * 16 * HD))[at] = make_float2(mm, total);
 }
 
-// The chunks of a job's rows together: a wave has four rows, 16 lanes each.
-template <int HD, class R>
+// ------------------------------------------------------------------ attention of many rows
+// Prompt chunks: a workgroup takes 128 rows of one sequence and key head, 32 a wave, and walks the
+// tokens 64 at a time. Here the matrix cores have the work (4 * 128 operations a code and row), so
+// codes become f16 values once for all four waves, in shared memory, while the 64 before them are
+// worked on: wave w turns the w-th tile of 16 tokens. Products are v_mfma_f32_32x32x16_f16, whose
+// left operand a wave reads once for 32 rows: S^T = K Q^T and O^T = V^T P^T as above, a lane's column
+// being its row (lane % 32). Keys lie as [token][channel]; values as [channel][token] with bits 2 and 3
+// of a token's number swapped, so that the eight tokens whose probabilities a lane has in a step lie
+// together. 16-byte chunks of both are permuted by exclusive-or with row bits: a wave's reads and
+// writes spread over all banks.
+//
+// A group of 32 channels is one block of O^T, so a NaN group (written as zeros) can be given to the
+// rows that see it afterwards: what was zeroed is kept as bits, 64 tokens a group.
+typedef float f16v __attribute__((ext_vector_type(16)));
+constexpr int ROWS_BM = 128;
+
+template <int HD>
+struct Rows4 {  // a step's 64 tokens
+  h8v k[64][HD / 8];  // [token][chunk ^ key_mix(token)]
+  h8v v[HD][8];       // [channel][chunk ^ value_mix(channel)]
+  uint32_t flag[4];   // of tile w: 1, a NaN group among its values; 2, it is not there
+  unsigned long long nans[HD / 32];  // the tokens of NaN value groups
+};
+
+template <int HD>
+__device__ __forceinline__ int key_mix(int t) { return HD == 128 ? t & 15 : t >> 1 & 7; }
+// Place i of n in an order that runs backwards in every other 256.
+__device__ __forceinline__ int snake(int i, int n) {
+  const int b = i & ~255;
+  return i & 256 ? b + min(n - b, 256) - 1 - (i - b) : i;
+}
+__device__ __forceinline__ int value_mix(int ch) { return (ch >> 1 ^ ch >> 4) & 7; }
+
+template <int HD, class R, int QP, int PP>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void k_kv4_rows(const Kv4Attn a) {
+  typedef typename R::E E;
+  constexpr int G = HD / 32, KS = HD / 16, NC = HD / 16;
+  extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+  Rows4<HD> *buf = (Rows4<HD> *)lds;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 31, h = lane >> 5, head = blockIdx.x % a.n_kv;
+  // The last jobs of a sequence see the most tokens: they go first, 256 workgroups (one a CU) by falling
+  // work, the 256 after them by rising work, and so on.
+  const int rank = snake(blockIdx.x, gridDim.x) / a.n_kv, job = (int)(gridDim.x / a.n_kv) - 1 - rank;
+  Job4 j;
+  if (!job_of<ROWS_BM>(a, job, j)) return;
+  const int rows = j.nq * a.group;
+  if (rows <= a.few) return;  // k_kv4_attn's
+  const int r = j.r0 + 32 * wave + col, rc = min(r, rows - 1), tok = rc / a.group;
+  const E *qp = (const E *)a.q + (int64_t)(j.q0 + tok) * a.ld_q + (head * a.group + rc % a.group) * HD + 8 * h;
+  float amax = 0.0f;
+#pragma unroll
+  for (int k = 0; k < KS; k++)
+#pragma unroll
+    for (int i = 0; i < 8; i++) amax = fmaxf(amax, fabsf(row_get(R{}, qp[16 * k + i])));
+  amax = max32(amax);
+  const float lift = lift_of(amax), unlift = a.scale / lift;
+  h8v qh[KS], ql[KS];
+#pragma unroll
+  for (int k = 0; k < KS; k++)
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+      const float x = row_get(R{}, qp[16 * k + i]) * lift;
+      qh[k][i] = (_Float16)x;
+      if (QP == 2) ql[k][i] = (_Float16)(x - (float)qh[k][i]);
+    }
+  const int pos = j.n - j.nq + tok, hi = min(pos + 1, j.n), lo = a.window > 0 ? max(pos + 1 - a.window, 0) : 0;
+  const int last = min(j.r0 + ROWS_BM - 1, rows - 1) / a.group, first = j.r0 / a.group;
+  const int all_hi = min(j.n - j.nq + last + 1, j.n), all_lo = a.window > 0 ? max(j.n - j.nq + first + 1 - a.window, 0) : 0;
+  const int see_lo = a.window > 0 ? max(j.n - j.nq + last + 1 - a.window, 0) : 0, see_hi = min(j.n - j.nq + first + 1, j.n);
+  const int from = all_lo & ~63, chunks = all_hi > from ? (all_hi - from + a.rchunk - 1) / a.rchunk : 1;
+  if ((int)blockIdx.z >= chunks) return;
+  const int *table = a.tables + (int64_t)j.s * a.cols;
+  const int pm = (1 << a.page) - 1;
+
+  f16v o[G];
+#pragma unroll
+  for (int g = 0; g < G; g++)
+#pragma unroll
+    for (int i = 0; i < 16; i++) o[g][i] = 0.0f;
+  float m = -__builtin_inff(), sum = 0.0f;
+
+  // this wave's tile of the 64 tokens from t0
+  const int l = lane & 15, hq = lane >> 4;
+  uint32_t kw[G], vw[G];
+  h2v ks[G / 2], vs[2];
+  int in;  // whether it is there
+  auto load = [&](int t0) {
+    const int t = t0 + 16 * wave;
+    const int pg = t < all_hi ? table[t >> a.page] : -1;
+    in = pg >= 0 && pg < a.n_pages;
+    const uint8_t *tile = a.pool + tile_at<HD>(in ? pg : 0, a.n_kv, head, a.page, in ? t & pm : 0);
+    const uint8_t *kp = tile + lane * 4 * G, *vp = kp + 8 * HD;
+    if constexpr (HD == 128) {
+      const uint4 x = *(const uint4 *)kp, y = *(const uint4 *)vp;
+      kw[0] = x.x; kw[1] = x.y; kw[2] = x.z; kw[3] = x.w;
+      vw[0] = y.x; vw[1] = y.y; vw[2] = y.z; vw[3] = y.w;
+      const uint2 z = *(const uint2 *)(tile + 16 * HD + l * 2 * G);
+      ks[0] = bits_h2(z.x); ks[1] = bits_h2(z.y);
+    } else {
+      const uint2 x = *(const uint2 *)kp, y = *(const uint2 *)vp;
+      kw[0] = x.x; kw[1] = x.y;
+      vw[0] = y.x; vw[1] = y.y;
+      ks[0] = bits_h2(*(const uint32_t *)(tile + 16 * HD + l * 2 * G));
+    }
+    const uint2 z = *(const uint2 *)(tile + 17 * HD + ((l * G >> 4) * 16 + 4 * hq) * 2);
+    vs[0] = bits_h2(z.x); vs[1] = bits_h2(z.y);
+  };
+  const Const4 kc = constants();
+  auto store = [&](Rows4<HD> &b, int t0) {
+    const h2v o0 = {(_Float16)-1032.0f, (_Float16)-1032.0f}, o1 = {(_Float16)-72.0f, (_Float16)-72.0f};
+    const int t = 16 * wave + l;
+#pragma unroll
+    for (int g = 0; g < G; g++) {
+      const _Float16 d1 = ks[g >> 1][g & 1];
+      const h2v d = {d1, d1};
+      const uint32_t w = kw[g], w8 = w >> 8;
+      const h2v x[4] = {(bits_h2((w & kc.lo) | kc.e0) + o0) * d, (bits_h2((w & kc.hi) | kc.e1) + o1) * d,
+                        (bits_h2((w8 & kc.lo) | kc.e0) + o0) * d, (bits_h2((w8 & kc.hi) | kc.e1) + o1) * d};
+      b.k[t][(4 * g + hq) ^ key_mix<HD>(t)] = __builtin_bit_cast(h8v, x);
+    }
+    // tokens that are not there or that no row sees count as zero; so do NaN groups, marked
+    uint32_t bad = 0;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const int tt = t0 + 16 * wave + 4 * hq + i;
+      const _Float16 d = vs[i >> 1][i & 1];
+      const bool is = in && tt >= all_lo && tt < all_hi, num = d == d;
+      if (is && !num) bad |= 1u << i;
+      vs[i >> 1][i & 1] = is && num ? d : (_Float16)0.0f;
+    }
+    // four tokens of this lane's channels: 8 bytes of each channel's row
+    const int chunk = 2 * wave + (hq & 1), half = hq >> 1;
+#pragma unroll
+    for (int c = 0; c < NC / 2; c++) {
+      h2v e[2], d[2];
+#pragma unroll
+      for (int i = 0; i < 2; i++) {
+        if constexpr (HD == 128) value_pairs<HD>(vw[2 * i], vw[2 * i + 1], c, vs[i], kc, e[i], d[i]);
+        else value_pairs<HD>(vw[i], 0u, c, vs[i], kc, e[i], d[i]);
+      }
+#pragma unroll
+      for (int p = 0; p < 2; p++) {
+        const int ch = l * NC + 2 * c + p;
+        const uint2 x = p ? make_uint2(__builtin_bit_cast(uint32_t, d[0]), __builtin_bit_cast(uint32_t, d[1]))
+                          : make_uint2(__builtin_bit_cast(uint32_t, e[0]), __builtin_bit_cast(uint32_t, e[1]));
+        ((uint2 *)&b.v[ch][chunk ^ value_mix(ch)])[half] = x;
+      }
+    }
+    const bool any = __builtin_amdgcn_ballot_w64(bad != 0) != 0;
+    if (lane == 0) b.flag[wave] = (any ? 1 : 0) | (in ? 0 : 2);
+    if (any) {  // (rare) the 16 tokens' bits of each group
+      const int span = 16 / G;  // lanes of l that share a group
+#pragma unroll
+      for (int g = 0; g < G; g++) {
+        uint32_t w = l == g * span ? bad << (4 * hq) : 0;
+        w |= (uint32_t)__shfl_xor((int)w, 16);
+        w |= (uint32_t)__shfl_xor((int)w, 32);
+        if (lane == g * span) ((uint16_t *)&b.nans[g])[wave] = (uint16_t)w;
+      }
+    } else if (lane < G) {
+      ((uint16_t *)&b.nans[lane])[wave] = 0;
+    }
+  };
+
+  // NB blocks of 32 tokens at once: two let the matrix cores work on one block while the other's
+  // probabilities are made, but do not fit the registers where queries have two parts
+  constexpr int NB = QP == 2 ? 1 : 2;
+  int kat[KS], vat[2 * G];  // a lane's chunks of a block's keys and values
+#pragma unroll
+  for (int k = 0; k < KS; k++) kat[k] = col * (HD / 8) + ((2 * k + h) ^ key_mix<HD>(col));
+#pragma unroll
+  for (int g = 0; g < G; g++) {
+    const int ch = 32 * g + col;
+    vat[2 * g] = ch * 8 + (h ^ value_mix(ch));
+    vat[2 * g + 1] = ch * 8 + ((2 + h) ^ value_mix(ch));
+  }
+  for (int c = blockIdx.z; c < chunks; c += gridDim.z) {
+    const int begin = from + c * a.rchunk, end = min(all_hi, begin + a.rchunk);
+    if (begin >= end) break;
+    load(begin);
+    store(buf[0], begin);  // (a chunk before this one ended with a barrier)
+    if (begin + 64 < end) load(begin + 64);
+    __syncthreads();
+    int at = 0;
+    for (int t0 = begin; t0 < end; t0 += 64, at ^= 1) {
+      const Rows4<HD> &b = buf[at];
+      const h8v *bk = &b.k[0][0], *bv = &b.v[0][0];
+      const uint4 flag = *(const uint4 *)b.flag;
+      const uint32_t gone = (flag.x >> 1) | (flag.y & 2) | (flag.z & 2) << 1 | (flag.w & 2) << 2;
+      const bool masks = t0 < see_lo || t0 + 64 > see_hi || gone, nans = ((flag.x | flag.y | flag.z | flag.w) & 1) != 0;
+#pragma unroll 1
+      for (int u0 = 0; u0 < 2; u0 += NB) {
+        f16v s[NB];
+#pragma unroll
+        for (int u = 0; u < NB; u++) {
+#pragma unroll
+          for (int i = 0; i < 16; i++) s[u][i] = 0.0f;
+#pragma unroll
+          for (int k = 0; k < KS; k++) {
+            // (32 tokens on, key_mix is what it was)
+            const h8v kf = bk[kat[k] + (u0 + u) * 32 * (HD / 8)];
+            s[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, qh[k], s[u], 0, 0, 0);
+            if (QP == 2) s[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, ql[k], s[u], 0, 0, 0);
+          }
+        }
+        // the next tile's codes become values while the products run
+        if (u0 == 0 && t0 + 64 < end) store(buf[at ^ 1], t0 + 64);
+        if (masks) {
+#pragma unroll
+          for (int u = 0; u < NB; u++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) {
+              const int q = 32 * (u0 + u) + 8 * (i >> 2) + 4 * h + (i & 3), t = t0 + q;
+              const bool hide = (bool)((int)(t < lo) | (int)(t >= hi) | (int)(gone >> (q >> 4) & 1));
+              s[u][i] = hide ? -__builtin_inff() : s[u][i];
+            }
+        }
+        float mt = s[0][0];
+#pragma unroll
+        for (int u = 0; u < NB; u++)
+#pragma unroll
+          for (int i = 0; i < 16; i++) mt = fmaxf(mt, s[u][i]);
+        mt = max32(mt) * unlift;
+        if (__builtin_amdgcn_ballot_w64(mt > m + P_SLACK)) {
+          const float mn = fmaxf(m, mt), f = m == mn ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
+          m = mn;
+          sum *= f;
+#pragma unroll
+          for (int g = 0; g < G; g++) o[g] *= f;
+        }
+        if (__builtin_expect(nans, 0)) {
+#pragma unroll
+          for (int u = 0; u < NB; u++)
+#pragma unroll
+            for (int g = 0; g < G; g++) {
+              const uint32_t bits = (uint32_t)(b.nans[g] >> (32 * (u0 + u) + 4 * h));
+              bool hit = false;
+#pragma unroll
+              for (int i = 0; i < 16; i++) hit |= (bits >> (8 * (i >> 2) + (i & 3)) & 1) && !(s[u][i] == -__builtin_inff());
+              if (max32(hit ? 1.0f : 0.0f) > 0.0f)
+#pragma unroll
+                for (int i = 0; i < 16; i++) o[g][i] = __builtin_nanf("");
+            }
+        }
+        const float ref = m == -__builtin_inff() ? 0.0f : P_LIFT - m;
+#pragma unroll
+        for (int u = 0; u < NB; u++) {
+          h2v p1[8], p2[8];
+#pragma unroll
+          for (int i = 0; i < 16; i += 2) {
+            const float x = __builtin_amdgcn_exp2f(fmaf(s[u][i], unlift, ref)), y = __builtin_amdgcn_exp2f(fmaf(s[u][i + 1], unlift, ref));
+            sum += x + y;
+            p1[i / 2] = half_pair(x, y);
+            if (PP == 2) p2[i / 2] = half_rest(x, y, p1[i / 2]);
+          }
+#pragma unroll
+          for (int k = 0; k < 2; k++) {
+            const h2v q1[4] = {p1[4 * k], p1[4 * k + 1], p1[4 * k + 2], p1[4 * k + 3]}, q2[4] = {p2[4 * k], p2[4 * k + 1], p2[4 * k + 2], p2[4 * k + 3]};
+            const h8v ph = __builtin_bit_cast(h8v, q1), pl = __builtin_bit_cast(h8v, q2);
+#pragma unroll
+            for (int g = 0; g < G; g++) {
+              const h8v vf = bv[vat[2 * g + k] ^ (u0 + u) << 2];
+              o[g] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, ph, o[g], 0, 0, 0);
+              if (PP == 2) o[g] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, pl, o[g], 0, 0, 0);
+            }
+          }
+        }
+      }
+      if (t0 + 128 < end) load(t0 + 128);
+      __syncthreads();
+    }
+  }
+  sum = add32(sum);
+  if (r >= rows) return;
+  // element i of a block is channel 8 (i / 4) + 4 h + i % 4
+  if (min(chunks, (int)gridDim.z) == 1) {
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    E *dst = (E *)a.out + (int64_t)(j.q0 + tok) * a.ld_out + (head * a.group + r % a.group) * HD + 4 * h;
+#pragma unroll
+    for (int g = 0; g < G; g++)
+#pragma unroll
+      for (int i = 0; i < 16; i++) dst[32 * g + 8 * (i >> 2) + (i & 3)] = row_put(R{}, o[g][i] * inv);
+    return;
+  }
+  const int64_t row = (((int64_t)job * a.n_kv + head) * gridDim.z + blockIdx.z) * ROWS_BM + 32 * wave + col;
+  float *dst = a.rpart + row * HD + 4 * h;
+#pragma unroll
+  for (int g = 0; g < G; g++)
+#pragma unroll
+    for (int i = 0; i < 16; i += 4) *(float4 *)(dst + 32 * g + 2 * i) = make_float4(o[g][i], o[g][i + 1], o[g][i + 2], o[g][i + 3]);
+  if (h == 0) ((float2 *)(a.rpart + (int64_t)gridDim.x * gridDim.z * ROWS_BM * HD))[row] = make_float2(m, sum);
+}
+
+// The chunks of a job's rows together: a wave has four rows, 16 lanes each. BM: rows a job, of
+// k_kv4_attn (16) or k_kv4_rows.
+template <int HD, class R, int BM>
 __global__ __launch_bounds__(64) void k_kv4_join(const Kv4Attn a, int splits) {
   typedef typename R::E E;
   constexpr int NC = HD / 16, U = 4;
   Job4 j;
-  if (!job_of<16>(a, blockIdx.x, j)) return;
+  if (BM > 16 ? !job_of<BM>(a, blockIdx.x, j) : !few_job(a, blockIdx.x, j)) return;
   const int rows = j.nq * a.group, head = blockIdx.y, row = blockIdx.z * 4 + (threadIdx.x >> 4), part = threadIdx.x & 15, rr = j.r0 + row;
-  const int last = min(j.r0 + 15, rows - 1) / a.group, first = j.r0 / a.group;
-  const int all_hi = min(j.n - j.nq + last + 1, j.n), from = (a.window > 0 ? max(j.n - j.nq + first + 1 - a.window, 0) : 0) & ~31;
-  const int n = min(all_hi > from ? (all_hi - from + a.chunk - 1) / a.chunk : 1, splits);
+  if (BM > 16 && rows <= a.few) return;
+  const int chunk = BM > 16 ? a.rchunk : a.chunk;
+  const int last = min(j.r0 + BM - 1, rows - 1) / a.group, first = j.r0 / a.group;
+  const int all_hi = min(j.n - j.nq + last + 1, j.n), from = (a.window > 0 ? max(j.n - j.nq + first + 1 - a.window, 0) : 0) & (BM > 16 ? ~63 : ~31);
+  const int n = min(all_hi > from ? (all_hi - from + chunk - 1) / chunk : 1, splits);
   if (n == 1 || rr >= rows) return;
-  const int64_t at = ((int64_t)blockIdx.x * a.n_kv + head) * splits * 16 + row;
-  const float2 *ms = (const float2 *)(a.part + (int64_t)gridDim.x * a.n_kv * splits * 16 * HD) + at;
-  const float *src = a.part + at * HD + part * NC;
+  const float *whole = BM > 16 ? a.rpart : a.part;
+  const int64_t at = ((int64_t)blockIdx.x * a.n_kv + head) * splits * BM + row;
+  const float2 *ms = (const float2 *)(whole + (int64_t)gridDim.x * a.n_kv * splits * BM * HD) + at;
+  const float *src = whole + at * HD + part * NC;
   float m = -__builtin_inff();
-  for (int c = part; c < n; c += 16) m = fmaxf(m, ms[c * 16].x);
+  for (int c = part; c < n; c += 16) m = fmaxf(m, ms[c * BM].x);
   m = fmaxf(m, SPX_DPPF(m, 0xB1));
   m = fmaxf(m, SPX_DPPF(m, 0x4E));
   m = fmaxf(m, SPX_DPPF(m, 0x141));
@@ -569,9 +887,9 @@ __global__ __launch_bounds__(64) void k_kv4_join(const Kv4Attn a, int splits) {
 #pragma unroll
     for (int u = 0; u < U; u++) {
       const int c = min(c0 + u, n - 1);
-      x[u] = ms[c * 16];
+      x[u] = ms[c * BM];
 #pragma unroll
-      for (int i = 0; i < NC / 4; i++) y[u][i] = *(const float4 *)(src + (int64_t)c * 16 * HD + 4 * i);
+      for (int i = 0; i < NC / 4; i++) y[u][i] = *(const float4 *)(src + (int64_t)c * BM * HD + 4 * i);
     }
 #pragma unroll
     for (int u = 0; u < U; u++) {
@@ -593,41 +911,75 @@ __global__ __launch_bounds__(64) void k_kv4_join(const Kv4Attn a, int splits) {
   for (int i = 0; i < NC; i++) dst[i] = row_put(R{}, v[i] * inv);
 }
 
-// How the work is split: jobs, chunks of a sequence (at most) and tokens a chunk. Chunks are as long
-// as leaves about KV4_WGS workgroups, 128 tokens (a tile a wave) at least.
-constexpr int KV4_WGS = 2048;
+// How the work is split: jobs (an odd number, so that neighbouring key heads and chunks of a sequence
+// go to other XCDs: workgroups go around the eight of them in order), chunks of a sequence (at most)
+// and tokens a chunk. Chunks are as long as leaves about `wgs` workgroups, a multiple of `step`.
+//   KV4_WGS, workgroups of four waves, three or four a CU: 64 sequences of up to 16K (32 heads over 4)
+//   took 107 / 99 / 109 us with 4096 / 2048 / 1024.
+constexpr int KV4_WGS = 2048, KV4_RWGS = 512;
 struct Split4 { int64_t jobs; int splits, chunk; };
-static Split4 split_of(int group, int n_kv, int rows, int n_seq, int max_kv) {
+static Split4 split_of(int bm, int64_t rows, int64_t seq_rows, int n_kv, int n_seq, int max_kv, int wgs, int step) {
   Split4 r;
-  r.jobs = (int64_t)rows * group / 16 + n_seq;
-  const int64_t busy = (((int64_t)rows * group + n_seq - 1) / n_seq + 15) / 16 * n_seq * n_kv;  // jobs with rows, all key heads
-  const int64_t want = (KV4_WGS + busy - 1) / busy;
-  int64_t chunk = ((max_kv + want - 1) / want + 127) / 128 * 128;
-  if (chunk < 128) chunk = 128;
+  r.jobs = (rows / bm + n_seq) | 1;
+  const int64_t busy = (seq_rows + bm - 1) / bm * n_seq * n_kv;  // jobs with rows, all key heads
+  const int64_t want = (wgs + busy - 1) / busy;
+  int64_t chunk = ((max_kv + want - 1) / want + step - 1) / step * step;
+  if (chunk < step) chunk = step;
   if (chunk > 1 << 20) chunk = 1 << 20;
   r.chunk = (int)chunk;
   r.splits = (int)((max_kv + chunk - 1) / chunk);
   if (r.splits < 1) r.splits = 1;
   return r;
 }
+// Both kernels' shares. Sequences with more rows than KV4_FEW (times query heads a key head) are
+// k_kv4_rows'; where there are no more rows than sequences the launch is spared and k_kv4_attn takes all.
+constexpr int KV4_FEW = 16;
+struct Plan4 { Split4 few, many; bool both; int64_t few_floats, many_floats; };
+static Plan4 plan_of(int hd, int group, int n_kv, int rows, int n_seq, int max_kv) {
+  Plan4 p{};
+  const int64_t all = (int64_t)rows * group, each = (all + n_seq - 1) / n_seq;
+  p.both = rows > n_seq && all > KV4_FEW;
+  p.few = split_of(16, all, p.both && each > KV4_FEW ? KV4_FEW : each, n_kv, n_seq, max_kv, KV4_WGS, 128);
+  if (p.both) p.few.jobs = n_seq | 1;
+  if (p.few.splits > 1) p.few_floats = p.few.jobs * n_kv * p.few.splits * 16 * (hd + 2);
+  if (p.both) {
+    p.many = split_of(ROWS_BM, all, each, n_kv, n_seq, max_kv, KV4_RWGS, 256);
+    if (p.many.splits > 1) p.many_floats = p.many.jobs * n_kv * p.many.splits * ROWS_BM * (hd + 2);
+  }
+  return p;
+}
 int64_t kv4_attention_ws(int hd, int group, int n_kv, int rows, int n_seq, int max_kv) {
-  const Split4 d = split_of(group, n_kv, rows, n_seq, max_kv);
-  return d.splits > 1 ? (d.jobs | 1) * n_kv * d.splits * 16 * (hd + 2) * 4 : 0;
+  const Plan4 p = plan_of(hd, group, n_kv, rows, n_seq, max_kv);
+  return 4 * (p.few_floats + p.many_floats);
+}
+
+template <int HD, class R>
+static hipError_t launch_attention(Kv4Attn &a, const Plan4 &p, hipStream_t s) {
+  constexpr int QP = sizeof(typename R::E) == 4 ? 2 : 1, PP = std::is_same<R, RowBF16>::value ? 1 : 2;
+  const unsigned nk = (unsigned)a.n_kv;
+  a.few = p.both ? KV4_FEW : INT32_MAX;
+  a.chunk = p.few.chunk;
+  a.rchunk = p.many.chunk;
+  a.rpart = a.part + p.few_floats;
+  hipLaunchKernelGGL((k_kv4_attn<HD, R, QP, PP>), dim3((unsigned)p.few.jobs, nk, p.few.splits), dim3(256), 0, s, a);
+  if (p.few.splits > 1) hipLaunchKernelGGL((k_kv4_join<HD, R, 16>), dim3((unsigned)p.few.jobs, nk, 4), dim3(64), 0, s, a, p.few.splits);
+  if (p.both) {
+    constexpr unsigned bytes = 2 * sizeof(Rows4<HD>);
+    static_assert(bytes <= 65536 + 1024, "two buffers");
+    const hipError_t e = hipFuncSetAttribute((const void *)k_kv4_rows<HD, R, QP, PP>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+    if (e != hipSuccess) return e;
+    hipLaunchKernelGGL((k_kv4_rows<HD, R, QP, PP>), dim3((unsigned)p.many.jobs * nk, 1, p.many.splits), dim3(256), bytes, s, a);
+    if (p.many.splits > 1)
+      hipLaunchKernelGGL((k_kv4_join<HD, R, ROWS_BM>), dim3((unsigned)p.many.jobs, nk, ROWS_BM / 4), dim3(64), 0, s, a, p.many.splits);
+  }
+  return hipGetLastError();
 }
 
 hipError_t launch_kv4_attention(Kv4Attn a, int hd, int type, int max_kv, hipStream_t s) {
-  const Split4 d = split_of(a.group, a.n_kv, a.rows, a.n_seq, max_kv);
-  a.chunk = d.chunk;
-  // an odd count, so that neighbouring key heads and chunks of a sequence go to other XCDs (workgroups go
-  // around the eight of them in order)
-  const dim3 grid((unsigned)d.jobs | 1, (unsigned)a.n_kv, (unsigned)d.splits);
-#define CALL(H, R)                                                                                                              \
-  hipLaunchKernelGGL((k_kv4_attn<H, R, sizeof(R::E) == 4 ? 2 : 1, std::is_same<R, RowBF16>::value ? 1 : 2>), grid, dim3(256), 0, \
-                     s, a);                                                                                                     \
-  if (d.splits > 1) hipLaunchKernelGGL((k_kv4_join<H, R>), dim3(grid.x, grid.y, 4), dim3(64), 0, s, a, d.splits)
+  const Plan4 p = plan_of(hd, a.group, a.n_kv, a.rows, a.n_seq, max_kv);
+#define CALL(H, R) return launch_attention<H, R>(a, p, s)
   KV4_BY_TYPE(hd, type, CALL)
 #undef CALL
-  return hipGetLastError();
 }
 
 }  // namespace spx
