@@ -579,7 +579,7 @@ typedef float f16v __attribute__((ext_vector_type(16)));
 constexpr int ROWS_BM = 128;
 
 template <int HD>
-struct Rows4 {  // a step's 64 tokens
+struct alignas(256) Rows4 {  // a step's 64 tokens
   h8v k[64][HD / 8];  // [token][chunk ^ key_mix(token)]
   h8v v[HD][8];       // [channel][chunk ^ value_mix(channel)]
   uint32_t flag[4];   // of tile w: 1, a NaN group among its values; 2, it is not there
@@ -729,15 +729,10 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void k
   // NB blocks of 32 tokens at once: two let the matrix cores work on one block while the other's
   // probabilities are made, but do not fit the registers where queries have two parts
   constexpr int NB = QP == 2 ? 1 : 2;
-  int kat[KS], vat[2 * G];  // a lane's chunks of a block's keys and values
-#pragma unroll
-  for (int k = 0; k < KS; k++) kat[k] = col * (HD / 8) + ((2 * k + h) ^ key_mix<HD>(col));
-#pragma unroll
-  for (int g = 0; g < G; g++) {
-    const int ch = 32 * g + col;
-    vat[2 * g] = ch * 8 + (h ^ value_mix(ch));
-    vat[2 * g + 1] = ch * 8 + ((2 + h) ^ value_mix(ch));
-  }
+  // A lane's chunks: the permutations leave what the step k, the block u and the group g add to a chunk's
+  // number an exclusive-or as well, so one base serves them all.
+  //   keys: (32 u + col) HD / 8 + (2 k + h ^ key_mix);   values: (32 g + col) 8 + (4 u + 2 k + h ^ value_mix ^ 2 g)
+  const int kat = col * (HD / 8) + (h ^ key_mix<HD>(col)), vat = col * 8 + (h ^ value_mix(col));
   for (int c = blockIdx.z; c < chunks; c += gridDim.z) {
     const int begin = from + c * a.rchunk, end = min(all_hi, begin + a.rchunk);
     if (begin >= end) break;
@@ -761,8 +756,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void k
           for (int i = 0; i < 16; i++) s[u][i] = 0.0f;
 #pragma unroll
           for (int k = 0; k < KS; k++) {
-            // (32 tokens on, key_mix is what it was)
-            const h8v kf = bk[kat[k] + (u0 + u) * 32 * (HD / 8)];
+            const h8v kf = bk[(kat ^ 2 * k) + (u0 + u) * 32 * (HD / 8)];
             s[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, qh[k], s[u], 0, 0, 0);
             if (QP == 2) s[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, ql[k], s[u], 0, 0, 0);
           }
@@ -823,7 +817,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void k
             const h8v ph = __builtin_bit_cast(h8v, q1), pl = __builtin_bit_cast(h8v, q2);
 #pragma unroll
             for (int g = 0; g < G; g++) {
-              const h8v vf = bv[vat[2 * g + k] ^ (u0 + u) << 2];
+              const h8v vf = bv[(vat ^ (2 * k ^ (2 * g & 7)) ^ 4 * (u0 + u)) + 256 * g];
               o[g] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, ph, o[g], 0, 0, 0);
               if (PP == 2) o[g] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, pl, o[g], 0, 0, 0);
             }
@@ -918,10 +912,9 @@ __global__ __launch_bounds__(64) void k_kv4_join(const Kv4Attn a, int splits) {
 //   took 107 / 99 / 109 us with 4096 / 2048 / 1024.
 constexpr int KV4_WGS = 2048, KV4_RWGS = 512;
 struct Split4 { int64_t jobs; int splits, chunk; };
-static Split4 split_of(int bm, int64_t rows, int64_t seq_rows, int n_kv, int n_seq, int max_kv, int wgs, int step) {
+static Split4 split_of(int64_t jobs, int64_t busy, int max_kv, int wgs, int step) {  // busy: jobs with rows, all key heads
   Split4 r;
-  r.jobs = (rows / bm + n_seq) | 1;
-  const int64_t busy = (seq_rows + bm - 1) / bm * n_seq * n_kv;  // jobs with rows, all key heads
+  r.jobs = jobs | 1;
   const int64_t want = (wgs + busy - 1) / busy;
   int64_t chunk = ((max_kv + want - 1) / want + step - 1) / step * step;
   if (chunk < step) chunk = step;
@@ -939,11 +932,11 @@ static Plan4 plan_of(int hd, int group, int n_kv, int rows, int n_seq, int max_k
   Plan4 p{};
   const int64_t all = (int64_t)rows * group, each = (all + n_seq - 1) / n_seq;
   p.both = rows > n_seq && all > KV4_FEW;
-  p.few = split_of(16, all, p.both && each > KV4_FEW ? KV4_FEW : each, n_kv, n_seq, max_kv, KV4_WGS, 128);
-  if (p.both) p.few.jobs = n_seq | 1;
+  if (p.both) p.few = split_of(n_seq, (int64_t)n_seq * n_kv, max_kv, KV4_WGS, 128);
+  else p.few = split_of(all / 16 + n_seq, (each + 15) / 16 * n_seq * n_kv, max_kv, KV4_WGS, 128);
   if (p.few.splits > 1) p.few_floats = p.few.jobs * n_kv * p.few.splits * 16 * (hd + 2);
   if (p.both) {
-    p.many = split_of(ROWS_BM, all, each, n_kv, n_seq, max_kv, KV4_RWGS, 256);
+    p.many = split_of(all / ROWS_BM + n_seq, (all / ROWS_BM + 1) * n_kv, max_kv, KV4_RWGS, 256);
     if (p.many.splits > 1) p.many_floats = p.many.jobs * n_kv * p.many.splits * ROWS_BM * (hd + 2);
   }
   return p;
