@@ -5,6 +5,7 @@
 // 18 * head_dim bytes, in which each lane of a wave finds the codes that it feeds to the matrix
 // instructions in one load. Scales have 8 significant bits, so integer * scale (at most 3 + 8
 // bits, or 8 times the scale) is exact in f16 and the matrix cores read the values themselves.
+#include <atomic>
 #include <type_traits>
 
 #include "batch.h"
@@ -248,16 +249,20 @@ __device__ __forceinline__ bool job_of(const Kv4Attn &a, int job, Job4 &j) {
   return j.nq > 0 && j.r0 >= 0 && j.r0 < j.nq * a.group;
 }
 
-// k_kv4_attn's jobs: where k_kv4_rows takes the sequences of more rows, each of the others is one.
+// k_kv4_attn's jobs: where k_kv4_rows takes the sequences of more than KV4_FEW rows, each of the others
+// has KV4_FEW / 16, whether it needs them or not.
+constexpr int KV4_FEW = 64;
 __device__ __forceinline__ bool few_job(const Kv4Attn &a, int job, Job4 &j) {
   if (a.few == INT32_MAX) return job_of<16>(a, job, j);
-  if (job >= a.n_seq) return false;
-  j.s = job;
-  j.q0 = min(max(a.q_start[job], 0), a.rows);
-  j.nq = min(max(a.q_start[job + 1], 0), a.rows) - j.q0;
-  j.r0 = 0;
-  j.n = (int)min((int64_t)max(a.kv_lens[job], 0), (int64_t)a.cols << a.page);
-  return j.nq > 0 && j.nq * a.group <= a.few;
+  const int s = job / (KV4_FEW / 16);
+  if (s >= a.n_seq) return false;
+  j.s = s;
+  j.q0 = min(max(a.q_start[s], 0), a.rows);
+  j.nq = min(max(a.q_start[s + 1], 0), a.rows) - j.q0;
+  j.r0 = job % (KV4_FEW / 16) * 16;
+  j.n = (int)min((int64_t)max(a.kv_lens[s], 0), (int64_t)a.cols << a.page);
+  const int rows = j.nq * a.group;
+  return j.nq > 0 && rows <= a.few && j.r0 < rows;
 }
 
 __device__ __forceinline__ h2v bits_h2(uint32_t v) { return __builtin_bit_cast(h2v, v); }
@@ -576,7 +581,7 @@ __global__ __launch_bounds__(256) void k_kv4_attn(const Kv4Attn a) {
 // A group of 32 channels is one block of O^T, so a NaN group (written as zeros) can be given to the
 // rows that see it afterwards: what was zeroed is kept as bits, 64 tokens a group.
 typedef float f16v __attribute__((ext_vector_type(16)));
-constexpr int ROWS_BM = 128;
+constexpr int ROWS_BM = 128, SCHED_R = 4, SCHED_V = 10;
 
 template <int HD>
 struct alignas(256) Rows4 {  // a step's 64 tokens
@@ -647,10 +652,19 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void k
   const int l = lane & 15, hq = lane >> 4;
   uint32_t kw[G], vw[G];
   h2v ks[G / 2], vs[2];
-  int in;  // whether it is there
+  int in;                          // whether it is there
+  int base = INT32_MIN, pages = -1;  // lane i holds the page id of entry base + i
   auto load = [&](int t0) {
     const int t = t0 + 16 * wave;
-    const int pg = t < all_hi ? table[t >> a.page] : -1;
+    int pg = -1;
+    if (t < all_hi) {
+      const int e = t >> a.page;
+      if (base < 0 || e - base > 63) {
+        base = e;
+        pages = table[min(base + lane, a.cols - 1)];
+      }
+      pg = lane_i(pages, e - base);
+    }
     in = pg >= 0 && pg < a.n_pages;
     const uint8_t *tile = a.pool + tile_at<HD>(in ? pg : 0, a.n_kv, head, a.page, in ? t & pm : 0);
     const uint8_t *kp = tile + lane * 4 * G, *vp = kp + 8 * HD;
@@ -670,7 +684,24 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void k
     vs[0] = bits_h2(z.x); vs[1] = bits_h2(z.y);
   };
   const Const4 kc = constants();
-  auto store = [&](Rows4<HD> &b, int t0) {
+  // Where not every row sees all of the 64 tokens, what no row sees or is not there counts as zero, and so
+  // do NaN groups, which are marked. (Elsewhere a NaN reaches every row by itself.)
+  uint32_t bad = 0, mark = 0;
+  auto edge = [&](int t0) {
+    bad = 0;
+    mark = in ? 0 : 2;
+    if (in && t0 >= see_lo && t0 + 64 <= see_hi) return;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const int tt = t0 + 16 * wave + 4 * hq + i;
+      const _Float16 d = vs[i >> 1][i & 1];
+      const bool is = in && tt >= all_lo && tt < all_hi, num = d == d;
+      if (is && !num) bad |= 1u << i;
+      vs[i >> 1][i & 1] = is && num ? d : (_Float16)0.0f;
+    }
+    if (__builtin_amdgcn_ballot_w64(bad != 0)) mark |= 1;
+  };
+  auto store = [&](Rows4<HD> &b) {
     const h2v o0 = {(_Float16)-1032.0f, (_Float16)-1032.0f}, o1 = {(_Float16)-72.0f, (_Float16)-72.0f};
     const int t = 16 * wave + l;
 #pragma unroll
@@ -681,16 +712,6 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void k
       const h2v x[4] = {(bits_h2((w & kc.lo) | kc.e0) + o0) * d, (bits_h2((w & kc.hi) | kc.e1) + o1) * d,
                         (bits_h2((w8 & kc.lo) | kc.e0) + o0) * d, (bits_h2((w8 & kc.hi) | kc.e1) + o1) * d};
       b.k[t][(4 * g + hq) ^ key_mix<HD>(t)] = __builtin_bit_cast(h8v, x);
-    }
-    // tokens that are not there or that no row sees count as zero; so do NaN groups, marked
-    uint32_t bad = 0;
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-      const int tt = t0 + 16 * wave + 4 * hq + i;
-      const _Float16 d = vs[i >> 1][i & 1];
-      const bool is = in && tt >= all_lo && tt < all_hi, num = d == d;
-      if (is && !num) bad |= 1u << i;
-      vs[i >> 1][i & 1] = is && num ? d : (_Float16)0.0f;
     }
     // four tokens of this lane's channels: 8 bytes of each channel's row
     const int chunk = 2 * wave + (hq & 1), half = hq >> 1;
@@ -710,9 +731,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void k
         ((uint2 *)&b.v[ch][chunk ^ value_mix(ch)])[half] = x;
       }
     }
-    const bool any = __builtin_amdgcn_ballot_w64(bad != 0) != 0;
-    if (lane == 0) b.flag[wave] = (any ? 1 : 0) | (in ? 0 : 2);
-    if (any) {  // (rare) the 16 tokens' bits of each group
+    if (lane == 0) b.flag[wave] = mark;
+    if (mark & 1) {  // (rare) the 16 tokens' bits of each group
       const int span = 16 / G;  // lanes of l that share a group
 #pragma unroll
       for (int g = 0; g < G; g++) {
@@ -736,18 +756,21 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void k
   for (int c = blockIdx.z; c < chunks; c += gridDim.z) {
     const int begin = from + c * a.rchunk, end = min(all_hi, begin + a.rchunk);
     if (begin >= end) break;
+    base = -1;
     load(begin);
-    store(buf[0], begin);  // (a chunk before this one ended with a barrier)
-    if (begin + 64 < end) load(begin + 64);
+    edge(begin);
+    store(buf[0]);  // (a chunk before this one ended with a barrier)
+    load(begin + 64);      // (tiles behind the last are not there)
     __syncthreads();
     int at = 0;
     for (int t0 = begin; t0 < end; t0 += 64, at ^= 1) {
+      edge(t0 + 64);
       const Rows4<HD> &b = buf[at];
       const h8v *bk = &b.k[0][0], *bv = &b.v[0][0];
       const uint4 flag = *(const uint4 *)b.flag;
       const uint32_t gone = (flag.x >> 1) | (flag.y & 2) | (flag.z & 2) << 1 | (flag.w & 2) << 2;
       const bool masks = t0 < see_lo || t0 + 64 > see_hi || gone, nans = ((flag.x | flag.y | flag.z | flag.w) & 1) != 0;
-#pragma unroll 1
+#pragma unroll
       for (int u0 = 0; u0 < 2; u0 += NB) {
         f16v s[NB];
 #pragma unroll
@@ -761,8 +784,20 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void k
             if (QP == 2) s[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, ql[k], s[u], 0, 0, 0);
           }
         }
-        // the next tile's codes become values while the products run
-        if (u0 == 0 && t0 + 64 < end) store(buf[at ^ 1], t0 + 64);
+        if (u0 == 0) {
+          // the next tile's codes become values while the products run: a product, the read of another's
+          // keys and ten vector instructions at a time
+          store(buf[at ^ 1]);
+          __builtin_amdgcn_sched_group_barrier(0x100, SCHED_R, 0);
+#pragma unroll
+          for (int i = 0; i < 16; i++) {
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x002, SCHED_V, 0);
+            if (i > 3) __builtin_amdgcn_sched_group_barrier(0x200, 1, 0);
+          }
+        }
+        if (u0 == 0) load(t0 + 128);
         if (masks) {
 #pragma unroll
           for (int u = 0; u < NB; u++)
@@ -807,9 +842,13 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void k
 #pragma unroll
           for (int i = 0; i < 16; i += 2) {
             const float x = __builtin_amdgcn_exp2f(fmaf(s[u][i], unlift, ref)), y = __builtin_amdgcn_exp2f(fmaf(s[u][i + 1], unlift, ref));
-            sum += x + y;
             p1[i / 2] = half_pair(x, y);
-            if (PP == 2) p2[i / 2] = half_rest(x, y, p1[i / 2]);
+            if (PP == 2) {
+              p2[i / 2] = half_rest(x, y, p1[i / 2]);
+              sum += x + y;
+            } else {  // the sum of what the products take, two at a time
+              sum = __builtin_amdgcn_fdot2(p1[i / 2], h2v{(_Float16)1.0f, (_Float16)1.0f}, sum, false);
+            }
           }
 #pragma unroll
           for (int k = 0; k < 2; k++) {
@@ -824,7 +863,6 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void k
           }
         }
       }
-      if (t0 + 128 < end) load(t0 + 128);
       __syncthreads();
     }
   }
@@ -849,46 +887,55 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void k
   if (h == 0) ((float2 *)(a.rpart + (int64_t)gridDim.x * gridDim.z * ROWS_BM * HD))[row] = make_float2(m, sum);
 }
 
-// The chunks of a job's rows together: a wave has four rows, 16 lanes each. BM: rows a job, of
-// k_kv4_attn (16) or k_kv4_rows.
-template <int HD, class R, int BM>
-__global__ __launch_bounds__(64) void k_kv4_join(const Kv4Attn a, int splits) {
+// The chunks of a row together, a wave a row, four rows a workgroup: sixteen lanes have a row's
+// channels, each of the four quarters of the wave takes every fourth chunk. Workgroups below
+// few_jobs * 4 are k_kv4_attn's rows, the others k_kv4_rows'.
+template <int HD, class R>
+__global__ __launch_bounds__(256) void k_kv4_join(const Kv4Attn a, int few_jobs, int few_splits, int many_splits) {
   typedef typename R::E E;
   constexpr int NC = HD / 16, U = 4;
+  const int head = blockIdx.y, part = threadIdx.x & 15, quarter = threadIdx.x >> 4 & 3;
+  const bool many = (int)blockIdx.x >= few_jobs * 4;
+  const int bm = many ? ROWS_BM : 16, at0 = (many ? blockIdx.x - few_jobs * 4 : blockIdx.x) * 4, job = at0 / bm;
+  const int row = __builtin_amdgcn_readfirstlane(at0 % bm + (threadIdx.x >> 6));
+  const int splits = many ? many_splits : few_splits, chunk = many ? a.rchunk : a.chunk, step = many ? 64 : 32;
+  if (splits == 1) return;
   Job4 j;
-  if (BM > 16 ? !job_of<BM>(a, blockIdx.x, j) : !few_job(a, blockIdx.x, j)) return;
-  const int rows = j.nq * a.group, head = blockIdx.y, row = blockIdx.z * 4 + (threadIdx.x >> 4), part = threadIdx.x & 15, rr = j.r0 + row;
-  if (BM > 16 && rows <= a.few) return;
-  const int chunk = BM > 16 ? a.rchunk : a.chunk;
-  const int last = min(j.r0 + BM - 1, rows - 1) / a.group, first = j.r0 / a.group;
-  const int all_hi = min(j.n - j.nq + last + 1, j.n), from = (a.window > 0 ? max(j.n - j.nq + first + 1 - a.window, 0) : 0) & (BM > 16 ? ~63 : ~31);
+  if (!(many ? job_of<ROWS_BM>(a, job, j) : few_job(a, job, j))) return;
+  const int rows = j.nq * a.group, rr = j.r0 + row;
+  if (rr >= rows || (many && rows <= a.few)) return;
+  const int last = min(j.r0 + bm - 1, rows - 1) / a.group, first = j.r0 / a.group;
+  const int all_hi = min(j.n - j.nq + last + 1, j.n), from = (a.window > 0 ? max(j.n - j.nq + first + 1 - a.window, 0) : 0) & -step;
   const int n = min(all_hi > from ? (all_hi - from + chunk - 1) / chunk : 1, splits);
-  if (n == 1 || rr >= rows) return;
-  const float *whole = BM > 16 ? a.rpart : a.part;
-  const int64_t at = ((int64_t)blockIdx.x * a.n_kv + head) * splits * BM + row;
-  const float2 *ms = (const float2 *)(whole + (int64_t)gridDim.x * a.n_kv * splits * BM * HD) + at;
+  if (n == 1) return;
+  const int jobs = many ? (int)(gridDim.x - few_jobs * 4) / (ROWS_BM / 4) : few_jobs;
+  const float *whole = many ? a.rpart : a.part;
+  const int64_t at = ((int64_t)job * a.n_kv + head) * splits * bm + row;
+  const float2 *ms = (const float2 *)(whole + (int64_t)jobs * a.n_kv * splits * bm * HD) + at;
   const float *src = whole + at * HD + part * NC;
-  float m = -__builtin_inff();
-  for (int c = part; c < n; c += 16) m = fmaxf(m, ms[c * BM].x);
-  m = fmaxf(m, SPX_DPPF(m, 0xB1));
-  m = fmaxf(m, SPX_DPPF(m, 0x4E));
-  m = fmaxf(m, SPX_DPPF(m, 0x141));
-  m = fmaxf(m, SPX_DPPF(m, 0x140));
-  float total = 0.0f, v[NC] = {};
-  for (int c0 = 0; c0 < n; c0 += U) {  // U chunks' loads at a time
+  float m = -__builtin_inff(), total = 0.0f, v[NC] = {};
+  for (int c0 = quarter; c0 < n; c0 += 4 * U) {  // U chunks' loads at a time
     float2 x[U];
     float4 y[U][NC / 4];
 #pragma unroll
     for (int u = 0; u < U; u++) {
-      const int c = min(c0 + u, n - 1);
-      x[u] = ms[c * BM];
+      const int c = min(c0 + 4 * u, n - 1);
+      x[u] = ms[(int64_t)c * bm];
 #pragma unroll
-      for (int i = 0; i < NC / 4; i++) y[u][i] = *(const float4 *)(src + (int64_t)c * BM * HD + 4 * i);
+      for (int i = 0; i < NC / 4; i++) y[u][i] = *(const float4 *)(src + (int64_t)c * bm * HD + 4 * i);
     }
+    float mn = m;
+#pragma unroll
+    for (int u = 0; u < U; u++) mn = fmaxf(mn, x[u].x);  // (a chunk twice does no harm here)
+    const float f0 = m == mn ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
+    total *= f0;
+#pragma unroll
+    for (int i = 0; i < NC; i++) v[i] *= f0;
+    m = mn;
 #pragma unroll
     for (int u = 0; u < U; u++) {
+      if (c0 + 4 * u >= n) continue;
       const float f = x[u].x == m ? 1.0f : __builtin_amdgcn_exp2f(x[u].x - m);
-      if (c0 + u >= n) continue;  // (0 times a NaN is one)
       total = fmaf(f, x[u].y, total);
 #pragma unroll
       for (int i = 0; i < NC / 4; i++) {
@@ -899,10 +946,15 @@ __global__ __launch_bounds__(64) void k_kv4_join(const Kv4Attn a, int splits) {
       }
     }
   }
+  const float mm = max32(max16(m)), f = m == mm ? 1.0f : __builtin_amdgcn_exp2f(m - mm);
+  total = add32(add16(total * f));
   const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+#pragma unroll
+  for (int i = 0; i < NC; i++) v[i] = add32(add16(v[i] * f)) * inv;
+  if (quarter) return;
   E *dst = (E *)a.out + (int64_t)(j.q0 + rr / a.group) * a.ld_out + (head * a.group + rr % a.group) * HD + part * NC;
 #pragma unroll
-  for (int i = 0; i < NC; i++) dst[i] = row_put(R{}, v[i] * inv);
+  for (int i = 0; i < NC; i++) dst[i] = row_put(R{}, v[i]);
 }
 
 // How the work is split: jobs (an odd number, so that neighbouring key heads and chunks of a sequence
@@ -915,7 +967,7 @@ struct Split4 { int64_t jobs; int splits, chunk; };
 static Split4 split_of(int64_t jobs, int64_t busy, int max_kv, int wgs, int step) {  // busy: jobs with rows, all key heads
   Split4 r;
   r.jobs = jobs | 1;
-  const int64_t want = (wgs + busy - 1) / busy;
+  const int64_t want = wgs > busy ? wgs / busy : 1;
   int64_t chunk = ((max_kv + want - 1) / want + step - 1) / step * step;
   if (chunk < step) chunk = step;
   if (chunk > 1 << 20) chunk = 1 << 20;
@@ -924,15 +976,15 @@ static Split4 split_of(int64_t jobs, int64_t busy, int max_kv, int wgs, int step
   if (r.splits < 1) r.splits = 1;
   return r;
 }
-// Both kernels' shares. Sequences with more rows than KV4_FEW (times query heads a key head) are
-// k_kv4_rows'; where there are no more rows than sequences the launch is spared and k_kv4_attn takes all.
-constexpr int KV4_FEW = 16;
+// Both kernels' shares. Sequences with more rows than KV4_FEW rows (new tokens times query heads a
+// key head) are k_kv4_rows'; where there are no more new tokens than sequences that launch is spared and
+// k_kv4_attn takes all.
 struct Plan4 { Split4 few, many; bool both; int64_t few_floats, many_floats; };
 static Plan4 plan_of(int hd, int group, int n_kv, int rows, int n_seq, int max_kv) {
   Plan4 p{};
   const int64_t all = (int64_t)rows * group, each = (all + n_seq - 1) / n_seq;
   p.both = rows > n_seq && all > KV4_FEW;
-  if (p.both) p.few = split_of(n_seq, (int64_t)n_seq * n_kv, max_kv, KV4_WGS, 128);
+  if (p.both) p.few = split_of((int64_t)n_seq * (KV4_FEW / 16), (each > 16 ? 2 : 1) * (int64_t)n_seq * n_kv, max_kv, KV4_WGS, 128);
   else p.few = split_of(all / 16 + n_seq, (each + 15) / 16 * n_seq * n_kv, max_kv, KV4_WGS, 128);
   if (p.few.splits > 1) p.few_floats = p.few.jobs * n_kv * p.few.splits * 16 * (hd + 2);
   if (p.both) {
@@ -955,16 +1007,21 @@ static hipError_t launch_attention(Kv4Attn &a, const Plan4 &p, hipStream_t s) {
   a.rchunk = p.many.chunk;
   a.rpart = a.part + p.few_floats;
   hipLaunchKernelGGL((k_kv4_attn<HD, R, QP, PP>), dim3((unsigned)p.few.jobs, nk, p.few.splits), dim3(256), 0, s, a);
-  if (p.few.splits > 1) hipLaunchKernelGGL((k_kv4_join<HD, R, 16>), dim3((unsigned)p.few.jobs, nk, 4), dim3(64), 0, s, a, p.few.splits);
   if (p.both) {
     constexpr unsigned bytes = 2 * sizeof(Rows4<HD>);
-    static_assert(bytes <= 65536 + 1024, "two buffers");
-    const hipError_t e = hipFuncSetAttribute((const void *)k_kv4_rows<HD, R, QP, PP>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+    static std::atomic<uint64_t> set{0};  // devices on which the kernel has been allowed that much shared memory
+    int dev = 0;
+    hipError_t e = hipGetDevice(&dev);
     if (e != hipSuccess) return e;
+    if (dev > 63 || !(set.load() >> dev & 1)) {
+      e = hipFuncSetAttribute((const void *)k_kv4_rows<HD, R, QP, PP>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+      if (e != hipSuccess) return e;
+      if (dev < 64) set |= 1ull << dev;
+    }
     hipLaunchKernelGGL((k_kv4_rows<HD, R, QP, PP>), dim3((unsigned)p.many.jobs * nk, 1, p.many.splits), dim3(256), bytes, s, a);
-    if (p.many.splits > 1)
-      hipLaunchKernelGGL((k_kv4_join<HD, R, ROWS_BM>), dim3((unsigned)p.many.jobs, nk, ROWS_BM / 4), dim3(64), 0, s, a, p.many.splits);
   }
+  const unsigned f = p.few.splits > 1 ? (unsigned)p.few.jobs : 0, m = p.both && p.many.splits > 1 ? (unsigned)p.many.jobs : 0;
+  if (f || m) hipLaunchKernelGGL((k_kv4_join<HD, R>), dim3(f * 4 + m * (ROWS_BM / 4), nk), dim3(256), 0, s, a, (int)f, p.few.splits, p.many.splits);
   return hipGetLastError();
 }
 
