@@ -49,108 +49,152 @@ __device__ __forceinline__ bool slot_of(int slot, int page, int n_pages, int &pg
   return slot >= 0 && pg < n_pages;
 }
 
-// A thread's piece of a row: eight channels of the key (kv = 0) or the value (1) of one head.
+// A thread's piece of a row: eight channels of the key (kv = 0) or the value (1) of one head. Rows run
+// fastest above the pieces of a row, so that a wave fills whole cache lines of a tile. (Four rows a
+// thread, all loads under way at once, gain nothing: 8191 rows of 8 heads of 128 take 20 instead of 18
+// us to write, 11.4 instead of 12.0 to read.)
 template <int HD>
 struct Piece {
   int row, head, kv, c8;  // c8: channels 8 c8 ..
 };
-// Rows run fastest above the pieces of a row, so that a wave fills whole cache lines of a tile.
 template <int HD>
-__device__ __forceinline__ bool piece_of(const Kv4Rows &a, int64_t i, Piece<HD> &p) {
+__device__ __forceinline__ Piece<HD> piece_of() {
   constexpr int PC = HD / 8;
-  p.c8 = (int)(i % PC);
-  i /= PC;
-  p.row = (int)(i % a.rows);
-  i /= a.rows;
-  p.kv = (int)(i & 1);
-  p.head = (int)(i >> 1);
-  return p.head < a.n_kv;
+  return {(int)(blockIdx.x * (256 / PC) + threadIdx.x / PC), (int)(blockIdx.y >> 1), (int)(blockIdx.y & 1), (int)(threadIdx.x % PC)};
+}
+// Eight values of a row. VEC: rows lie at multiples of 16 bytes.
+template <class R, bool VEC>
+__device__ __forceinline__ void get8(const typename R::E *src, float *x) {
+  alignas(16) typename R::E e[8];
+  if constexpr (VEC) {
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(e) / 16; i++) ((uint4 *)e)[i] = ((const uint4 *)src)[i];
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; j++) e[j] = src[j];
+  }
+#pragma unroll
+  for (int j = 0; j < 8; j++) x[j] = row_get(R{}, e[j]);
+}
+template <class R, bool VEC>
+__device__ __forceinline__ void put8(typename R::E *dst, const float *x) {
+  alignas(16) typename R::E e[8];
+#pragma unroll
+  for (int j = 0; j < 8; j++) e[j] = row_put(R{}, x[j]);
+  if constexpr (VEC) {
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(e) / 16; i++) ((uint4 *)dst)[i] = ((const uint4 *)e)[i];
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; j++) dst[j] = e[j];
+  }
 }
 
 // ------------------------------------------------------------------ append
 // The integer nearest to x / d, half to even, exactly: the quotient's estimate is off by at most
 // one, and x - c d is exact (c d has at most 12 bits and is within a factor of two of x, or zero).
-__device__ __forceinline__ int kv4_code(float x, float d, float inv) {
+__device__ __forceinline__ float kv4_code_exact(float x, float d, float inv) {
   float c = rintf(x * inv);
   c = fminf(fmaxf(c, -9.0f), 9.0f);
   const float e = fmaf(-c, d, x) * (d < 0.0f ? -1.0f : 1.0f), h = 0.5f * fabsf(d);  // e: the rest, in d's direction
   const bool odd = ((int)c & 1) != 0;
   if (e > h || (e == h && odd)) c += 1.0f;
   else if (e < -h || (e == -h && odd)) c -= 1.0f;
-  return (int)fminf(fmaxf(c, -8.0f), 7.0f);
+  return c;
+}
+// Eight of them. x * inv is within 1.5e-6 of the quotient (at most 12, two roundings), so that only
+// where one lies that near to a half is more than its rounding needed.
+__device__ __forceinline__ void kv4_codes(const float *x, float d, float inv, uint32_t *c) {
+  float f[8], off = 0.0f;
+#pragma unroll
+  for (int j = 0; j < 8; j++) {
+    const float y = x[j] * inv;
+    f[j] = rintf(y);
+    off = fmaxf(off, fabsf(y - f[j]));
+  }
+  if (off > 0.49999f)
+#pragma unroll
+    for (int j = 0; j < 8; j++) f[j] = kv4_code_exact(x[j], d, inv);
+#pragma unroll
+  for (int j = 0; j < 8; j++) c[j] = (uint32_t)(fminf(fmaxf(f[j], -8.0f), 7.0f) + 8.0f);
 }
 
 // A thread quantizes eight channels; the four threads of a quad share a group's scale.
 // Bound by bytes: each value is read once (4 or 2 bytes) and 4.5 bits are written.
-template <int HD, class R>
-__global__ __launch_bounds__(256) void k_kv4_append(const Kv4Rows a) {
-  typedef typename R::E E;
-  Piece<HD> p;
-  if (!piece_of<HD>(a, (int64_t)blockIdx.x * 256 + threadIdx.x, p)) return;
+template <int HD>
+__device__ __forceinline__ void append_piece(const Kv4Rows &a, float *x, int kv, int head, int c8, int slot) {
   int pg, t;
-  if (!slot_of(a.slots[p.row], a.page, a.n_pages, pg, t)) return;  // (a quad has one row)
-  const E *src = (p.kv ? (const E *)a.v + (int64_t)p.row * a.ld_v : (const E *)a.k + (int64_t)p.row * a.ld_k) + p.head * HD + p.c8 * 8;
-  float x[8];
+  const bool is = slot_of(slot, a.page, a.n_pages, pg, t);
   uint32_t m = 0;
 #pragma unroll
-  for (int j = 0; j < 8; j++) {
-    x[j] = row_get(R{}, src[j]);
-    m = max(m, __float_as_uint(x[j]) & 0x7fffffffu);  // magnitudes order as integers, NaN above all
-  }
+  for (int j = 0; j < 8; j++) m = max(m, __float_as_uint(x[j]) & 0x7fffffffu);  // magnitudes order as integers, NaN above all
   m = max(m, (uint32_t)__builtin_amdgcn_mov_dpp((int)m, 0xB1, 0xF, 0xF, true));
   m = max(m, (uint32_t)__builtin_amdgcn_mov_dpp((int)m, 0x4E, 0xF, 0xF, true));
   // the first value of that magnitude gives the sign: place << 1 | negative, the smallest of all
   uint32_t key = ~0u;
 #pragma unroll
   for (int j = 7; j >= 0; j--)
-    if ((__float_as_uint(x[j]) & 0x7fffffffu) == m) key = (uint32_t)(((p.c8 & 3) * 8 + j) << 1) | (__float_as_uint(x[j]) >> 31);
+    if ((__float_as_uint(x[j]) & 0x7fffffffu) == m) key = (uint32_t)(((c8 & 3) * 8 + j) << 1) | (__float_as_uint(x[j]) >> 31);
   key = min(key, (uint32_t)__builtin_amdgcn_mov_dpp((int)key, 0xB1, 0xF, 0xF, true));
   key = min(key, (uint32_t)__builtin_amdgcn_mov_dpp((int)key, 0x4E, 0xF, 0xF, true));
+  if (!is) return;
   const bool bad = m >= 0x7f800000u;
   const float most = __uint_as_float(m | (key << 31));
   float d = row_get(RowBF16{}, bf16_rne(most * -0.125f));
   d = (float)(_Float16)fminf(fmaxf(d, -KV4_DMAX), KV4_DMAX) + 0.0f;  // (a scale of zero is +0)
   const float inv = d == 0.0f ? 0.0f : 1.0f / d;
-  int c[8];
+  uint32_t c[8];
+  if (bad) {  // (codes of a NaN group are 0)
 #pragma unroll
-  for (int j = 0; j < 8; j++) c[j] = bad || d == 0.0f ? 8 : kv4_code(x[j], d, inv) + 8;
+    for (int j = 0; j < 8; j++) x[j] = 0.0f;
+  }
+  kv4_codes(x, d, inv, c);  // (a scale of zero has inv = 0: codes 0)
   const _Float16 dh = bad ? (_Float16)__builtin_nanf("") : (_Float16)d;
   constexpr int G = HD / 32;
-  uint8_t *tile = a.pool + tile_at<HD>(pg, a.n_kv, p.head, a.page, t);
-  const int ti = t & 15, g = p.c8 >> 2, h = p.c8 & 3;
-  if (!p.kv) {
+  uint8_t *tile = a.pool + tile_at<HD>(pg, a.n_kv, head, a.page, t);
+  const int ti = t & 15, g = c8 >> 2, h = c8 & 3;
+  if (!kv) {
     uint32_t w = 0;
 #pragma unroll
-    for (int j = 0; j < 8; j++) w |= (uint32_t)c[j] << (4 * ((j >> 1) + 4 * (j & 1)));
+    for (int j = 0; j < 8; j++) w |= c[j] << (4 * ((j >> 1) + 4 * (j & 1)));
     *(uint32_t *)(tile + ((h * 16 + ti) * G + g) * 4) = w;
     if (h == 0) *(_Float16 *)(tile + 16 * HD + (ti * G + g) * 2) = dh;
   } else {
     uint32_t w = 0;
 #pragma unroll
-    for (int j = 0; j < 8; j++) w |= (uint32_t)c[j] << (4 * j);
+    for (int j = 0; j < 8; j++) w |= c[j] << (4 * j);
     uint8_t *vc = tile + 8 * HD + (ti >> 2) * 64 * G + (ti & 3) * G;
     if (HD == 128) {
-      *(uint32_t *)(vc + p.c8 * 16) = w;
+      *(uint32_t *)(vc + c8 * 16) = w;
     } else {  // a lane of the attention kernels has four channels: two lanes' halves
-      *(uint16_t *)(vc + (2 * p.c8) * 8) = (uint16_t)w;
-      *(uint16_t *)(vc + (2 * p.c8 + 1) * 8) = (uint16_t)(w >> 16);
+      *(uint16_t *)(vc + (2 * c8) * 8) = (uint16_t)w;
+      *(uint16_t *)(vc + (2 * c8 + 1) * 8) = (uint16_t)(w >> 16);
     }
     if (h == 0) *(_Float16 *)(tile + 17 * HD + (g * 16 + ti) * 2) = dh;
   }
 }
+template <int HD, class R, bool VEC>
+__global__ __launch_bounds__(256) void k_kv4_append(const Kv4Rows a) {
+  typedef typename R::E E;
+  const Piece<HD> p = piece_of<HD>();
+  if (p.row >= a.rows) return;  // (a quad has one row)
+  const E *base = (p.kv ? (const E *)a.v : (const E *)a.k) + p.head * HD + p.c8 * 8;
+  float x[8];
+  get8<R, VEC>(base + p.row * (p.kv ? a.ld_v : a.ld_k), x);
+  append_piece<HD>(a, x, p.kv, p.head, p.c8, a.slots[p.row]);
+}
 
 // ------------------------------------------------------------------ read
-template <int HD, class R>
+template <int HD, class R, bool VEC>
 __global__ __launch_bounds__(256) void k_kv4_read(const Kv4Rows a) {
   typedef typename R::E E;
-  Piece<HD> p;
-  if (!piece_of<HD>(a, (int64_t)blockIdx.x * 256 + threadIdx.x, p)) return;
-  int pg, t;
-  const bool in = slot_of(a.slots[p.row], a.page, a.n_pages, pg, t);
-  E *dst = (p.kv ? (E *)a.v + (int64_t)p.row * a.ld_v : (E *)a.k + (int64_t)p.row * a.ld_k) + p.head * HD + p.c8 * 8;
+  constexpr int G = HD / 32;
+  const Piece<HD> p = piece_of<HD>();
+  if (p.row >= a.rows) return;
+  E *base = (p.kv ? (E *)a.v : (E *)a.k) + p.head * HD + p.c8 * 8;
   float x[8] = {};
-  if (in) {
-    constexpr int G = HD / 32;
+  int pg, t;
+  if (slot_of(a.slots[p.row], a.page, a.n_pages, pg, t)) {
     const uint8_t *tile = a.pool + tile_at<HD>(pg, a.n_kv, p.head, a.page, t);
     const int ti = t & 15, g = p.c8 >> 2, h = p.c8 & 3;
     uint32_t w;
@@ -170,10 +214,8 @@ __global__ __launch_bounds__(256) void k_kv4_read(const Kv4Rows a) {
       x[j] = (float)((int)((w >> (4 * nib)) & 15) - 8) * d;
     }
   }
-#pragma unroll
-  for (int j = 0; j < 8; j++) dst[j] = row_put(R{}, x[j]);
+  put8<R, VEC>(base + p.row * (p.kv ? a.ld_v : a.ld_k), x);
 }
-
 
 #define KV4_BY_TYPE(hd, type, CALL)                                                 \
   switch ((hd) * 64 + (type)) {                                                     \
@@ -186,17 +228,24 @@ __global__ __launch_bounds__(256) void k_kv4_read(const Kv4Rows a) {
   default: return hipErrorInvalidValue;                                             \
   }
 
+static bool rows_aligned(const Kv4Rows &a, int size) {
+  return (uintptr_t)a.k % 16 == 0 && (uintptr_t)a.v % 16 == 0 && a.ld_k * size % 16 == 0 && a.ld_v * size % 16 == 0;
+}
+static dim3 rows_grid(const Kv4Rows &a, int hd) { return dim3((unsigned)(((int64_t)a.rows * (hd / 8) + 255) / 256), 2u * a.n_kv); }
+
 hipError_t launch_kv4_append(const Kv4Rows &a, int hd, int type, hipStream_t s) {
-  const int64_t n = (int64_t)a.rows * a.n_kv * 2 * (hd / 8);
-#define CALL(H, R) hipLaunchKernelGGL((k_kv4_append<H, R>), dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s, a)
+#define CALL(H, R)                                                  \
+  if (rows_aligned(a, sizeof(R::E))) hipLaunchKernelGGL((k_kv4_append<H, R, true>), rows_grid(a, H), dim3(256), 0, s, a); \
+  else hipLaunchKernelGGL((k_kv4_append<H, R, false>), rows_grid(a, H), dim3(256), 0, s, a)
   KV4_BY_TYPE(hd, type, CALL)
 #undef CALL
   return hipGetLastError();
 }
 
 hipError_t launch_kv4_read(const Kv4Rows &a, int hd, int type, hipStream_t s) {
-  const int64_t n = (int64_t)a.rows * a.n_kv * 2 * (hd / 8);
-#define CALL(H, R) hipLaunchKernelGGL((k_kv4_read<H, R>), dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s, a)
+#define CALL(H, R)                                                \
+  if (rows_aligned(a, sizeof(R::E))) hipLaunchKernelGGL((k_kv4_read<H, R, true>), rows_grid(a, H), dim3(256), 0, s, a); \
+  else hipLaunchKernelGGL((k_kv4_read<H, R, false>), rows_grid(a, H), dim3(256), 0, s, a)
   KV4_BY_TYPE(hd, type, CALL)
 #undef CALL
   return hipGetLastError();

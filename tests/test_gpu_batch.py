@@ -95,6 +95,31 @@ def test_append_one_row_rewrites_it(ctx):
     assert k.shape == (0, 2, 64)
 
 
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("kv,hd", [(8, 128), (13, 64)])
+def test_append_and_read_many_rows(ctx, dtype, kv, hd):
+    """A prompt's thousands of rows, more than a thread each, at odd counts and addresses, against the
+    same in small calls."""
+    from spindle_amd import ops
+    n, page = 9001, 64
+    shape = ops.Kv4Shape(kv, hd, page, n // page + 2)
+    g = torch.Generator(device="cuda")
+    g.manual_seed(n)
+    slots = torch.randperm(shape.n_pages * page, generator=g, device="cuda")[:n].to(torch.int32)
+    slots[[5, 8000]] = -1
+    for off in (0, 1):
+        k, v = (torch.randn(n * kv * hd + 1, generator=g, device="cuda").to(dtype)[off:off + n * kv * hd].view(n, kv, hd) for _ in range(2))
+        many, few = shape.pool(), shape.pool()
+        ops.kv4_append(ctx, shape, many, k, v, slots)
+        for a in range(0, n, 500):
+            ops.kv4_append(ctx, shape, few, k[a:a + 500], v[a:a + 500], slots[a:a + 500])
+        assert torch.equal(many, few)
+        got = ops.kv4_read(ctx, shape, many, slots, dtype)
+        for a in range(0, n, 500):
+            one = ops.kv4_read(ctx, shape, few, slots[a:a + 500], dtype)
+            assert all(torch.equal(x[a:a + 500], y) for x, y in zip(got, one))
+
+
 # --------------------------------------------------------------------------------------- the plan
 def run_plan(ctx, lens, add, tables, free, n_free, page, rows):
     from spindle_amd import ops
