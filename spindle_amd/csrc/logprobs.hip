@@ -52,18 +52,26 @@ __device__ __forceinline__ void best_offer(Best &b, unsigned long long key) {
     if (k > b.last) best_insert(b, k);
   }
 }
-// The list from one key a lane (0: none): each goes to the lane of its rank.
+// The list from one key a lane (0: none): for few the largest one after the other, else each goes to the
+// lane of its rank.
 __device__ __forceinline__ void best_start(Best &b, unsigned long long key, int top) {
   const int lane = threadIdx.x & 63;
-  int rank = 0;
-#pragma unroll
-  for (int j = 0; j < 64; j++) {
-    const unsigned long long k = lane_u64(key, j);
-    rank += k > key || (k == key && j < lane);  // (equal: both 0)
-  }
-  const uint32_t hi = (uint32_t)__builtin_amdgcn_ds_permute(rank * 4, (int)(key >> 32)), lo = (uint32_t)__builtin_amdgcn_ds_permute(rank * 4, (int)(uint32_t)key);
-  b.mine = (unsigned long long)hi << 32 | lo;
   b.top = top;
+  if (top <= 4) {
+    b.mine = 0;
+    for (int n = 0; n < top; n++) {
+      const unsigned long long k = wave_max_u64(key);
+      if (lane == n) b.mine = k;
+      if (key == k) key = 0;
+    }
+  } else {
+    if (key == 0) key = lane + 1;  // (numbers of their own, below every key)
+    int rank = 0;
+#pragma unroll
+    for (int j = 0; j < 64; j++) rank += lane_u64(key, j) > key;
+    const uint32_t hi = (uint32_t)__builtin_amdgcn_ds_permute(rank * 4, (int)(key >> 32)), lo = (uint32_t)__builtin_amdgcn_ds_permute(rank * 4, (int)(uint32_t)key);
+    b.mine = hi ? (unsigned long long)hi << 32 | lo : 0ull;
+  }
   b.last = lane_u64(b.mine, top - 1);
 }
 
@@ -132,8 +140,15 @@ __device__ __forceinline__ void take(const float *v, F id, int top, bool &begun,
 #pragma unroll
     for (int i = 0; i < N; i++) { const unsigned long long c = key_of(i); k = c > k ? c : k; }
     best_start(b, k, top);
+    if (N > 1) {  // the others that may be among them (equal ones too: ids are in no order here)
+      const float bar = b.last ? alt_logit(b.last) : -__builtin_inff();
 #pragma unroll
-    for (int i = 0; i < N; i++) { const unsigned long long c = key_of(i); best_offer(b, c == k ? 0ull : c); }
+      for (int i = 0; i < N; i++)
+        if (__builtin_amdgcn_ballot_w64(v[i] >= bar)) {
+          const unsigned long long c = key_of(i);
+          best_offer(b, c == k ? 0ull : c);
+        }
+    }
   } else {
     const float bar = b.last ? alt_logit(b.last) : -__builtin_inff();
     if (__builtin_amdgcn_ballot_w64(best > bar)) {
@@ -169,22 +184,24 @@ __device__ __forceinline__ void finish(const LogprobArgs &a, int row, const Sums
   }
 }
 
-// The waves' sums and lists together, in wave 0.
+// The waves' sums and lists together, in wave 0: the first sixteen of each list are sorted at once, the
+// others offered.
 __device__ __forceinline__ void join_waves(Sums &s, Best &b, int top) {
   __shared__ Sums ss[LP_W];
   __shared__ unsigned long long sk[LP_W][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  if (wave) {
-    if (lane == 0) ss[wave] = s;
-    if (top) sk[wave][lane] = b.mine;
-  }
+  if (lane == 0) ss[wave] = s;
+  if (top) sk[wave][lane] = b.mine;
   __syncthreads();
   if (wave) return;
-  for (int w = 1; w < LP_W; w++) {
-    sums_join(s, ss[w]);
-    if (top) best_offer(b, lane < top ? sk[w][lane] : 0ull);
+  for (int w = 1; w < LP_W; w++) sums_join(s, ss[w]);
+  if (top) {
+    const int w = lane >> 4, i = lane & 15;
+    best_start(b, i < top ? sk[w][i] : 0ull, top);
+    if (top > 16) best_offer(b, 16 + i < top ? sk[w][16 + i] : 0ull);
   }
 }
+static_assert(LP_W == 4, "a quarter of the wave a list");
 
 // A workgroup takes a part of a row, its waves shares of that one after the other
 // (ids ascend within a wave), 64 vectors of 16 bytes a load, four loads at a time. Elements before
