@@ -5,6 +5,7 @@
 // 18 * head_dim bytes, in which each lane of a wave finds the codes that it feeds to the matrix
 // instructions in one load. Scales have 8 significant bits, so integer * scale (at most 3 + 8
 // bits, or 8 times the scale) is exact in f16 and the matrix cores read the values themselves.
+#include <algorithm>
 #include <atomic>
 #include <type_traits>
 
@@ -936,28 +937,42 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void k
   if (h == 0) ((float2 *)(a.rpart + (int64_t)gridDim.x * gridDim.z * ROWS_BM * HD))[row] = make_float2(m, sum);
 }
 
-// The chunks of a row together, a wave a row, four rows a workgroup: sixteen lanes have a row's
-// channels, each of the four quarters of the wave takes every fourth chunk. Workgroups below
-// few_jobs * 4 are k_kv4_attn's rows, the others k_kv4_rows'.
+// The chunks of a row together, a wave a row: sixteen lanes have a row's channels, each of the four
+// quarters of the wave takes every fourth chunk. Workgroups below few_jobs * 4 have four of k_kv4_attn's
+// rows, the others 16 of k_kv4_rows' (fewer workgroups where a job has no rows at all).
+constexpr int JOIN_ROWS = 4;  // k_kv4_rows' rows a wave
+template <int HD, class R>
+__device__ __forceinline__ void join_row(const Kv4Attn &a, const Job4 &j, bool many, int job, int row, int splits, int jobs);
+
 template <int HD, class R>
 __global__ __launch_bounds__(256) void k_kv4_join(const Kv4Attn a, int few_jobs, int few_splits, int many_splits) {
+  const bool many = (int)blockIdx.x >= few_jobs * 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  Job4 j;
+  if (many) {
+    constexpr int PER = ROWS_BM / (4 * JOIN_ROWS);
+    const int at = blockIdx.x - few_jobs * 4, job = at / PER, row = at % PER * (4 * JOIN_ROWS) + wave * JOIN_ROWS;
+    if (many_splits == 1 || !job_of<ROWS_BM>(a, job, j) || j.nq * a.group <= a.few) return;
+    for (int i = 0; i < JOIN_ROWS; i++) join_row<HD, R>(a, j, true, job, row + i, many_splits, (int)(gridDim.x - few_jobs * 4) / PER);
+  } else {
+    const int job = blockIdx.x / 4;
+    if (few_splits == 1 || !few_job(a, job, j)) return;
+    join_row<HD, R>(a, j, false, job, blockIdx.x % 4 * 4 + wave, few_splits, few_jobs);
+  }
+}
+
+template <int HD, class R>
+__device__ __forceinline__ void join_row(const Kv4Attn &a, const Job4 &j, bool many, int job, int row, int splits, int jobs) {
   typedef typename R::E E;
   constexpr int NC = HD / 16, U = 4;
-  const int head = blockIdx.y, part = threadIdx.x & 15, quarter = threadIdx.x >> 4 & 3;
-  const bool many = (int)blockIdx.x >= few_jobs * 4;
-  const int bm = many ? ROWS_BM : 16, at0 = (many ? blockIdx.x - few_jobs * 4 : blockIdx.x) * 4, job = at0 / bm;
-  const int row = __builtin_amdgcn_readfirstlane(at0 % bm + (threadIdx.x >> 6));
-  const int splits = many ? many_splits : few_splits, chunk = many ? a.rchunk : a.chunk, step = many ? 64 : 32;
-  if (splits == 1) return;
-  Job4 j;
-  if (!(many ? job_of<ROWS_BM>(a, job, j) : few_job(a, job, j))) return;
+  const int head = blockIdx.y, part = threadIdx.x & 15, quarter = threadIdx.x >> 4 & 3, bm = many ? ROWS_BM : 16;
+  const int chunk = many ? a.rchunk : a.chunk, step = many ? 64 : 32;
   const int rows = j.nq * a.group, rr = j.r0 + row;
-  if (rr >= rows || (many && rows <= a.few)) return;
+  if (rr >= rows) return;
   const int last = min(j.r0 + bm - 1, rows - 1) / a.group, first = j.r0 / a.group;
   const int all_hi = min(j.n - j.nq + last + 1, j.n), from = (a.window > 0 ? max(j.n - j.nq + first + 1 - a.window, 0) : 0) & -step;
   const int n = min(all_hi > from ? (all_hi - from + chunk - 1) / chunk : 1, splits);
   if (n == 1) return;
-  const int jobs = many ? (int)(gridDim.x - few_jobs * 4) / (ROWS_BM / 4) : few_jobs;
   const float *whole = many ? a.rpart : a.part;
   const int64_t at = ((int64_t)job * a.n_kv + head) * splits * bm + row;
   const float2 *ms = (const float2 *)(whole + (int64_t)jobs * a.n_kv * splits * bm * HD) + at;
@@ -1009,41 +1024,57 @@ __global__ __launch_bounds__(256) void k_kv4_join(const Kv4Attn a, int few_jobs,
 // How the work is split: jobs (an odd number, so that neighbouring key heads and chunks of a sequence
 // go to other XCDs: workgroups go around the eight of them in order), chunks of a sequence (at most)
 // and tokens a chunk. Chunks are as long as leaves about `wgs` workgroups, a multiple of `step`.
-//   KV4_WGS, workgroups of four waves, three or four a CU: 64 sequences of up to 16K (32 heads over 4)
-//   took 107 / 99 / 109 us with 4096 / 2048 / 1024.
+//   KV4_WGS: 64 sequences of up to 16K (32 heads over 4) took 107 / 99 / 109 us with 4096 / 2048 / 1024
+//   workgroups; where that makes chunks of less than 512 tokens (four tiles a wave), half of it, which is
+//   what is resident at a time: a verify of 9 rows over twelve sequences of up to 2050 tokens (16 heads
+//   over 8 of 64) 18 / 16 us with 2048 / 1024.
+//   KV4_RWGS, k_kv4_rows': two a CU.
 constexpr int KV4_WGS = 2048, KV4_RWGS = 512;
 struct Split4 { int64_t jobs; int splits, chunk; };
-static Split4 split_of(int64_t jobs, int64_t busy, int max_kv, int wgs, int step) {  // busy: jobs with rows, all key heads
+static Split4 split_of(int64_t jobs, int64_t busy, int64_t span, int wgs, int step) {  // busy: jobs with rows, all key heads
   Split4 r;
   r.jobs = jobs | 1;
-  const int64_t want = wgs > busy ? wgs / busy : 1;
-  int64_t chunk = ((max_kv + want - 1) / want + step - 1) / step * step;
-  if (chunk < step) chunk = step;
-  if (chunk > 1 << 20) chunk = 1 << 20;
+  auto chunk_for = [&](int64_t n) {
+    const int64_t want = n > busy ? n / busy : 1;
+    return std::max<int64_t>(((span + want - 1) / want + step - 1) / step * step, step);
+  };
+  int64_t chunk = chunk_for(wgs);
+  if (wgs == KV4_WGS && chunk < 512) chunk = std::min<int64_t>(512, chunk_for(wgs / 2));
+  chunk = std::min<int64_t>(chunk, 1 << 20);
   r.chunk = (int)chunk;
-  r.splits = (int)((max_kv + chunk - 1) / chunk);
-  if (r.splits < 1) r.splits = 1;
+  r.splits = (int)std::max<int64_t>((span + chunk - 1) / chunk, 1);
   return r;
+}
+// The same under a window, of which a job of `tokens` new tokens walks no more than the window, those
+// and a tile: shorter chunks, but no more of them than without (the scratch is for so many; a workgroup
+// takes a second chunk where there are more).
+static Split4 split_window(int64_t jobs, int64_t busy, int max_kv, int window, int tokens, int wgs, int step) {
+  Split4 all = split_of(jobs, busy, max_kv, wgs, step);
+  if (window <= 0) return all;
+  const Split4 r = split_of(jobs, busy, std::min<int64_t>(max_kv, (int64_t)window + tokens + 64), wgs, step);
+  all.chunk = r.chunk;
+  all.splits = std::min(all.splits, r.splits);
+  return all;
 }
 // Both kernels' shares. Sequences with more rows than KV4_FEW rows (new tokens times query heads a
 // key head) are k_kv4_rows'; where there are no more new tokens than sequences that launch is spared and
 // k_kv4_attn takes all.
 struct Plan4 { Split4 few, many; bool both; int64_t few_floats, many_floats; };
-static Plan4 plan_of(int hd, int group, int n_kv, int rows, int n_seq, int max_kv) {
+static Plan4 plan_of(int hd, int group, int n_kv, int rows, int n_seq, int max_kv, int window) {
   Plan4 p{};
   const int64_t all = (int64_t)rows * group, each = (all + n_seq - 1) / n_seq;
   p.both = rows > n_seq && all > KV4_FEW;
-  if (p.both) p.few = split_of((int64_t)n_seq * (KV4_FEW / 16), (each > 16 ? 2 : 1) * (int64_t)n_seq * n_kv, max_kv, KV4_WGS, 128);
-  else p.few = split_of(all / 16 + n_seq, (each + 15) / 16 * n_seq * n_kv, max_kv, KV4_WGS, 128);
+  if (p.both) p.few = split_window((int64_t)n_seq * (KV4_FEW / 16), (each > 16 ? 2 : 1) * (int64_t)n_seq * n_kv, max_kv, window, 16 / group + 2, KV4_WGS, 128);
+  else p.few = split_window(all / 16 + n_seq, (each + 15) / 16 * n_seq * n_kv, max_kv, window, 16 / group + 2, KV4_WGS, 128);
   if (p.few.splits > 1) p.few_floats = p.few.jobs * n_kv * p.few.splits * 16 * (hd + 2);
   if (p.both) {
-    p.many = split_of(all / ROWS_BM + n_seq, (all / ROWS_BM + 1) * n_kv, max_kv, KV4_RWGS, 256);
+    p.many = split_window(all / ROWS_BM + n_seq, (all / ROWS_BM + 1) * n_kv, max_kv, window, ROWS_BM / group + 2, KV4_RWGS, 64);
     if (p.many.splits > 1) p.many_floats = p.many.jobs * n_kv * p.many.splits * ROWS_BM * (hd + 2);
   }
   return p;
 }
 int64_t kv4_attention_ws(int hd, int group, int n_kv, int rows, int n_seq, int max_kv) {
-  const Plan4 p = plan_of(hd, group, n_kv, rows, n_seq, max_kv);
+  const Plan4 p = plan_of(hd, group, n_kv, rows, n_seq, max_kv, 0);
   return 4 * (p.few_floats + p.many_floats);
 }
 
@@ -1070,12 +1101,12 @@ static hipError_t launch_attention(Kv4Attn &a, const Plan4 &p, hipStream_t s) {
     hipLaunchKernelGGL((k_kv4_rows<HD, R, QP, PP>), dim3((unsigned)p.many.jobs * nk, 1, p.many.splits), dim3(256), bytes, s, a);
   }
   const unsigned f = p.few.splits > 1 ? (unsigned)p.few.jobs : 0, m = p.both && p.many.splits > 1 ? (unsigned)p.many.jobs : 0;
-  if (f || m) hipLaunchKernelGGL((k_kv4_join<HD, R>), dim3(f * 4 + m * (ROWS_BM / 4), nk), dim3(256), 0, s, a, (int)f, p.few.splits, p.many.splits);
+  if (f || m) hipLaunchKernelGGL((k_kv4_join<HD, R>), dim3(f * 4 + m * (ROWS_BM / (4 * JOIN_ROWS)), nk), dim3(256), 0, s, a, (int)f, p.few.splits, p.many.splits);
   return hipGetLastError();
 }
 
 hipError_t launch_kv4_attention(Kv4Attn a, int hd, int type, int max_kv, hipStream_t s) {
-  const Plan4 p = plan_of(hd, a.group, a.n_kv, a.rows, a.n_seq, max_kv);
+  const Plan4 p = plan_of(hd, a.group, a.n_kv, a.rows, a.n_seq, max_kv, a.window);
 #define CALL(H, R) return launch_attention<H, R>(a, p, s)
   KV4_BY_TYPE(hd, type, CALL)
 #undef CALL
