@@ -173,7 +173,7 @@ int spx_kv4_read(spx_ctx *ctx, const spx_kv4_shape *shape, const void *pool, int
  * not depend on its being right. Sums, maxima and probabilities are held in 32 bits; SPX_F32 rows
  * meet the cache as two f16 parts (22 bits), SPX_F16 and SPX_BF16 rows as they are.
  * ws: spx_kv4_attention_ws bytes, a multiple of 16 in address. n_heads <= 1024, rows <= 262144,
- * table_cols * page_tokens <= 2^30. */
+ * n_seq <= 4096, table_cols * page_tokens <= 2^30. */
 int64_t spx_kv4_attention_ws(const spx_kv4_shape *shape, int n_heads, int rows, int n_seq, int max_kv);
 int spx_kv4_attention(spx_ctx *ctx, const spx_kv4_shape *shape, const void *pool, int type, const void *q, int64_t ld_q,
                       int n_heads, int rows, int n_seq, const int32_t *q_start, const int32_t *kv_lens, const int32_t *tables,

@@ -121,7 +121,7 @@ int spx_kv4_read(spx_ctx *ctx, const spx_kv4_shape *shape, const void *pool, int
 
 int64_t spx_kv4_attention_ws(const spx_kv4_shape *shape, int n_heads, int rows, int n_seq, int max_kv) {
   if (shape_error(shape) || n_heads < 1 || n_heads > 1024 || n_heads % shape->n_kv || rows < 1 || rows > 1 << 18 || n_seq < 1 ||
-      n_seq > 1 << 20 || max_kv < 0)
+      n_seq > PLAN_MAX_SEQ || max_kv < 0)
     return 0;
   return kv4_attention_ws(shape->head_dim, n_heads / shape->n_kv, shape->n_kv, rows, n_seq, max_kv);
 }
@@ -135,7 +135,7 @@ int spx_kv4_attention(spx_ctx *ctx, const spx_kv4_shape *shape, const void *pool
     if (!row_type(type)) return fail("spx_kv4_attention: type must be SPX_F32, SPX_F16 or SPX_BF16");
     if (n_heads < 1 || n_heads > 1024 || n_heads % shape->n_kv) return fail("spx_kv4_attention: n_heads must be a multiple of n_kv, at most 1024");
     if (rows < 0 || rows > 1 << 18) return fail("spx_kv4_attention: rows must be in 0..262144");
-    if (n_seq < 0 || n_seq > 1 << 20) return fail("spx_kv4_attention: n_seq must be in 0..2^20");
+    if (n_seq < 0 || n_seq > PLAN_MAX_SEQ) return fail("spx_kv4_attention: n_seq must be in 0..4096");
     if (window < 0) return fail("spx_kv4_attention: window must not be negative");
     if (max_kv < 0) return fail("spx_kv4_attention: max_kv must not be negative");
     const bool work = rows > 0 && n_seq > 0;
@@ -168,7 +168,7 @@ int spx_kv4_attention(spx_ctx *ctx, const spx_kv4_shape *shape, const void *pool
     a.rows = rows;
     a.n_seq = n_seq;
     a.cols = table_cols;
-    a.window = window;
+    a.window = window > 1 << 30 ? 0 : window;  // (no sequence is longer)
     a.q_start = q_start;
     a.kv_lens = kv_lens;
     a.tables = tables;

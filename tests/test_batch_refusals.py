@@ -85,7 +85,7 @@ def attention(lib, s, **kw):
 @pytest.mark.parametrize("kw,word", [
     (dict(pool=None), "null"), (dict(q=None), "null"), (dict(out=None), "null"), (dict(q_start=None), "null"), (dict(lens=None), "null"),
     (dict(tables=None), "null"), (dict(type=12), "type"), (dict(heads=3), "n_heads"), (dict(heads=0), "n_heads"), (dict(heads=1026), "n_heads"),
-    (dict(rows=-1), "rows"), (dict(rows=1 << 19), "rows"), (dict(n_seq=-1), "n_seq"), (dict(window=-1), "window"), (dict(cols=0), "table_cols"),
+    (dict(rows=-1), "rows"), (dict(rows=1 << 19), "rows"), (dict(n_seq=-1), "n_seq"), (dict(n_seq=4097), "n_seq"), (dict(window=-1), "window"), (dict(cols=0), "table_cols"),
     (dict(cols=1 << 26), "table_cols"), (dict(ld_q=511), "leading"), (dict(ld_out=511), "leading"), (dict(pool=A + 4), "multiple of 16"),
     (dict(q=A + 2), "multiple"), (dict(scale=float("inf")), "scale"), (dict(scale=float("nan")), "scale"), (dict(max_kv=-1), "max_kv"), ({}, "context")])
 def test_attention(lib, kw, word):

@@ -330,11 +330,66 @@ def test_attention_scales(ctx, dtype, q_spread, kv_spread):
     b.check(queries(8, 5, 4, 128, dtype, q_spread), [4, 1], dtype, scale=0.02)
 
 
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("rows", [1, 70])
+def test_attention_one_token_outweighs_the_rest(ctx, dtype, rows):
+    """A token that takes nearly all of the weight, thousands of others with some 2^-24 of its: what they
+    have together is kept (their probabilities lie among f16's subnormals)."""
+    n, hd = 6000, 128
+    b = Batch(ctx, [n], 1, hd, 64, seed=30, spread=0.05)
+    u = np.zeros(hd)
+    u[::2], u[1::2] = 1.0, -1.0
+    for at, far in ((0, 17.0), (n - rows - 1, 16.0)):  # exp(-17) = 2^-24.5
+        b = Batch(ctx, [n], 1, hd, 64, seed=31, spread=0.05)
+        b.put(0, at, k=(u * far / np.sqrt(hd))[None], v=np.full((1, hd), 0.5))
+        q = torch.from_numpy(np.tile(u, (rows, 2, 1))).to(dtype).cuda()
+        b.check(q, [rows], dtype)
+
+
+def test_attention_window_past_everything(ctx):
+    """The largest window there is sees what no window sees, rows before position 0 among them."""
+    b = Batch(ctx, [300, 40], 2, 64, 16, seed=32)
+    for counts in ([3, 1], [100, 45]):
+        q = queries(32, sum(counts), 4, 64, F32)
+        want, _ = b.check(q, counts, F32)
+        for window in (2 ** 31 - 1, 2 ** 30 + 1, 2 ** 30, 301):
+            got, _ = b.check(q, counts, F32, window=window)
+            assert np.allclose(f64(got), f64(want), rtol=0, atol=1e-5)
+
+
+def test_attention_captured_prompt(ctx):
+    """A prompt's call captured, in its first use of the type, and replayed over other lengths, tables
+    and queries, with eager calls and waits between."""
+    from spindle_amd import ops
+    with torch.cuda.stream(ctx.torch_stream()):
+        for dtype in (F32, F16, BF16):
+            b = Batch(ctx, [400, 90], 2, 128, 16, seed=33)
+            q, start, lens, tables = queries(33, 130, 8, 128, dtype), ints([0, 120, 123]), ints([400, 90]), ints(b.tables)
+            out = torch.full_like(q, 7.0)
+            torch.cuda.synchronize()
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g, stream=ctx.torch_stream()):
+                ops.kv4_attention(ctx, b.shape, b.pool, q, start, lens, tables, out=out)
+            for i, (s, n) in enumerate([([0, 120, 123], [400, 90]), ([0, 1, 130], [300, 80]), ([0, 0, 50], [5, 90]), ([0, 130, 130], [255, 1])]):
+                start.copy_(ints(s)), lens.copy_(ints(n)), q.copy_(queries(40 + i, 130, 8, 128, dtype)), out.fill_(7.0)
+                want = torch.full_like(q, 7.0)
+                ops.kv4_attention(ctx, b.shape, b.pool, q, start, lens, tables, out=want)
+                g.replay()
+                if i % 2:
+                    torch.cuda.synchronize()
+                assert torch.equal(out, want) and (out[s[2]:] == 7.0).all()
+
+
 def test_attention_many_sequences(ctx):
     rng = np.random.default_rng(6)
     lens = [int(v) for v in rng.integers(1, 60, 300)]
     b = Batch(ctx, lens, 1, 64, 16, seed=6)
     b.check(queries(6, 300, 2, 64, F16), [1] * 300, F16)
+    counts = [int(v) for v in rng.integers(0, 3, 300)]  # more rows than sequences, some of them idle
+    b.check(queries(7, sum(counts), 2, 64, F16), counts, F16)
+    lens = [int(v) for v in rng.integers(1, 20, 4096)]
+    b = Batch(ctx, lens, 1, 64, 16, seed=7)
+    b.check(queries(8, 4096, 1, 64, BF16), [1] * 4096, BF16)
 
 
 def test_attention_rows_it_leaves(ctx):
