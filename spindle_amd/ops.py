@@ -29,7 +29,7 @@ class Context:
         h = P()
         check(lib.spx_create(device, C.byref(h)))  # fails (SpxError) without a visible GPU
         self.h = h
-        self._stream = None
+        self._stream, self.raw_stream = None, lib.spx_get_stream(h)
         self._children = weakref.WeakSet()   # engines / tensors to release before the context
 
     def adopt(self, obj):
@@ -42,7 +42,7 @@ class Context:
         """The context's stream as a torch stream: a program that makes it torch's current one
         (torch.cuda.set_stream) orders its own work and the operators' on one stream."""
         if self._stream is None:
-            self._stream = torch.cuda.ExternalStream(lib.spx_get_stream(self.h), device=self.device)
+            self._stream = torch.cuda.ExternalStream(self.raw_stream, device=self.device)
         return self._stream
 
     def close(self):
@@ -201,11 +201,10 @@ def _run(ctx, tensors, call, *args):
     for t in tensors:
         if t.get_device() != ctx.device:
             raise ValueError(f"expected tensors on cuda:{ctx.device}, got {t.device}")
-    ours = ctx.torch_stream()
-    if torch._C._cuda_getCurrentRawStream(ctx.device) == ours.cuda_stream:  # (the stream's number, without an object around it)
+    if torch._C._cuda_getCurrentRawStream(ctx.device) == ctx.raw_stream:  # (the stream's number, without an object around it)
         check(call(ctx.h, *args))
         return
-    theirs = torch.cuda.current_stream(ctx.device)
+    ours, theirs = ctx.torch_stream(), torch.cuda.current_stream(ctx.device)
     ours.wait_stream(theirs)
     try:
         check(call(ctx.h, *args))
@@ -291,10 +290,9 @@ def kv4_read(ctx, shape, pool, slots, dtype=None):
     """(k, v) [rows, n_kv, head_dim]: the values that the pool's slots [rows] stand for (spx_kv4_read)."""
     dtype = dtype or torch.float32
     t, n, w = _row_type(dtype), slots.numel(), shape.n_kv * shape.head_dim
-    both = torch.empty((2, n, shape.n_kv, shape.head_dim), dtype=dtype, device=pool.device)
-    k, v = both.unbind(0)
-    at = both.data_ptr()
-    _run(ctx, (pool, slots), lib.spx_kv4_read, C.byref(shape), _pool(shape, pool), t, n, _i32(slots, n), at, w, at + n * w * dtype.itemsize, w)
+    size = (n, shape.n_kv, shape.head_dim)
+    k, v = pool.new_empty(size, dtype=dtype), pool.new_empty(size, dtype=dtype)
+    _run(ctx, (pool, slots), lib.spx_kv4_read, C.byref(shape), _pool(shape, pool), t, n, _i32(slots, n), k.data_ptr(), w, v.data_ptr(), w)
     return k, v
 
 
@@ -303,7 +301,7 @@ def _scratch(need, ws, like):
     if ws is None:
         if need <= 0:
             return None, 0, like
-        ws = torch.empty(need, dtype=torch.uint8, device=like.device)
+        ws = like.new_empty(need, dtype=torch.uint8)
     return ws.data_ptr(), ws.numel() * ws.element_size(), ws
 
 
@@ -316,7 +314,7 @@ def kv4_attention(ctx, shape, pool, q, q_start, kv_lens, tables, scale=0.0, wind
     rows, heads = q.shape[0], q.shape[1] if q.dim() == 3 else 0
     ld_q = _rows3(q, heads, hd, "q")
     if out is None:
-        out, ld_out = torch.empty((rows, heads, hd), dtype=q.dtype, device=q.device), heads * hd
+        out, ld_out = q.new_empty((rows, heads, hd)), heads * hd
     elif out.dtype is not q.dtype or out.shape != q.shape:
         raise ValueError("out must have q's type and shape")
     else:
@@ -324,7 +322,7 @@ def kv4_attention(ctx, shape, pool, q, q_start, kv_lens, tables, scale=0.0, wind
     cols = tables.shape[1] if tables.dim() == 2 else 0
     max_kv = cols * shape.page_tokens if max_kv is None else max_kv
     sh = C.byref(shape)
-    at, size, ws = _scratch(lib.spx_kv4_attention_ws(sh, heads, rows, n, max_kv), ws, q)
+    at, size, ws = _scratch(lib.spx_kv4_attention_ws(sh, heads, rows, n, max_kv), ws, pool)
     _run(ctx, (pool, q, q_start, kv_lens, tables, out, ws), lib.spx_kv4_attention, sh, _pool(shape, pool), t, q.data_ptr(), ld_q, heads, rows, n,
          _i32(q_start, n + 1), _i32(kv_lens, n), _i32(tables, n, cols), cols, scale, window, max_kv, out.data_ptr(), ld_out, at, size)
     return out
@@ -343,19 +341,17 @@ def logprobs(ctx, logits, targets=None, top=0, logit_scale=1.0, ws=None):
     if logits.dim() != 2 or (logits.stride(1) != 1 and logits.shape[1] > 1):
         raise ValueError("logits must be [rows, vocab] with dense rows")
     rows, vocab = logits.shape
-    r, n, dev = Logprobs(), max(top, 0), logits.device
-    both = torch.empty((2, rows), dtype=torch.float32, device=dev)
-    r.logp, r.entropy = both.unbind(0)
-    at = both.data_ptr()
-    r.top_ids = torch.empty((rows, n), dtype=torch.int32, device=dev)
-    r.top_logp = torch.empty((rows, n), dtype=torch.float32, device=dev)
+    r, n = Logprobs(), max(top, 0)
+    r.entropy = logits.new_empty(rows, dtype=torch.float32)
+    r.top_ids, r.top_logp = logits.new_empty((rows, n), dtype=torch.int32), logits.new_empty((rows, n), dtype=torch.float32)
     if targets is None:
         r.logp, ids, logp, targets = None, None, None, logits
     else:
-        ids, logp = _i32(targets, rows), at
+        r.logp, ids = logits.new_empty(rows, dtype=torch.float32), _i32(targets, rows)
+        logp = r.logp.data_ptr()
     scratch, size, ws = _scratch(lib.spx_logprobs_ws(rows, vocab, top), ws, logits)
     _run(ctx, (logits, targets, ws), lib.spx_logprobs, t, logits.data_ptr(), logits.stride(0) if rows > 1 else vocab, rows, vocab, logit_scale, ids,
-         top, logp, at + 4 * rows, r.top_ids.data_ptr(), r.top_logp.data_ptr(), scratch, size)
+         top, logp, r.entropy.data_ptr(), r.top_ids.data_ptr(), r.top_logp.data_ptr(), scratch, size)
     return r
 
 
