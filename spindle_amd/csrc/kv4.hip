@@ -1034,15 +1034,17 @@ __device__ __forceinline__ void join_row(const Kv4Attn &a, const Job4 &j, bool m
 //   workgroups; where that makes chunks of less than 512 tokens (four tiles a wave), half of it, which is
 //   what is resident at a time: a verify of 9 rows over twelve sequences of up to 2050 tokens (16 heads
 //   over 8 of 64) 18 / 16 us with 2048 / 1024.
-//   KV4_RWGS, k_kv4_rows': two a CU.
-constexpr int KV4_WGS = 2048, KV4_RWGS = 512;
+//   KV4_RWGS, k_kv4_rows': two a CU. Its chunks have KV4_RLEAST tokens at least, four steps: a launch
+//   whose sequences all turn out to be k_kv4_attn's costs as many rounds of empty workgroups as it has
+//   chunks (shared memory lets two of them onto a CU).
+constexpr int KV4_WGS = 2048, KV4_RWGS = 512, KV4_RLEAST = 256;
 struct Split4 { int64_t jobs; int splits, chunk; };
-static Split4 split_of(int64_t jobs, int64_t busy, int64_t span, int wgs, int step) {  // busy: jobs with rows, all key heads
+static Split4 split_of(int64_t jobs, int64_t busy, int64_t span, int wgs, int step, int least) {  // busy: jobs with rows, all key heads
   Split4 r;
   r.jobs = jobs | 1;
   auto chunk_for = [&](int64_t n) {
     const int64_t want = n > busy ? n / busy : 1;
-    return std::max<int64_t>(((span + want - 1) / want + step - 1) / step * step, step);
+    return std::max<int64_t>(((span + want - 1) / want + step - 1) / step * step, least);
   };
   int64_t chunk = chunk_for(wgs);
   if (wgs == KV4_WGS && chunk < 512) chunk = std::min<int64_t>(512, chunk_for(wgs / 2));
@@ -1054,10 +1056,10 @@ static Split4 split_of(int64_t jobs, int64_t busy, int64_t span, int wgs, int st
 // The same under a window, of which a job of `tokens` new tokens walks no more than the window, those
 // and a tile: shorter chunks, but no more of them than without (the scratch is for so many; a workgroup
 // takes a second chunk where there are more).
-static Split4 split_window(int64_t jobs, int64_t busy, int max_kv, int window, int tokens, int wgs, int step) {
-  Split4 all = split_of(jobs, busy, max_kv, wgs, step);
+static Split4 split_window(int64_t jobs, int64_t busy, int max_kv, int window, int tokens, int wgs, int step, int least) {
+  Split4 all = split_of(jobs, busy, max_kv, wgs, step, least);
   if (window <= 0) return all;
-  const Split4 r = split_of(jobs, busy, std::min<int64_t>(max_kv, (int64_t)window + tokens + 64), wgs, step);
+  const Split4 r = split_of(jobs, busy, std::min<int64_t>(max_kv, (int64_t)window + tokens + 64), wgs, step, least);
   all.chunk = r.chunk;
   all.splits = std::min(all.splits, r.splits);
   return all;
@@ -1070,11 +1072,11 @@ static Plan4 plan_of(int hd, int group, int n_kv, int rows, int n_seq, int max_k
   Plan4 p{};
   const int64_t all = (int64_t)rows * group, each = (all + n_seq - 1) / n_seq;
   p.both = rows > n_seq && all > KV4_FEW;
-  if (p.both) p.few = split_window((int64_t)n_seq * (KV4_FEW / 16), (each > 16 ? 2 : 1) * (int64_t)n_seq * n_kv, max_kv, window, 16 / group + 2, KV4_WGS, 128);
-  else p.few = split_window(all / 16 + n_seq, (each + 15) / 16 * n_seq * n_kv, max_kv, window, 16 / group + 2, KV4_WGS, 128);
+  if (p.both) p.few = split_window((int64_t)n_seq * (KV4_FEW / 16), (each > 16 ? 2 : 1) * (int64_t)n_seq * n_kv, max_kv, window, 16 / group + 2, KV4_WGS, 128, 128);
+  else p.few = split_window(all / 16 + n_seq, (each + 15) / 16 * n_seq * n_kv, max_kv, window, 16 / group + 2, KV4_WGS, 128, 128);
   if (p.few.splits > 1) p.few_floats = p.few.jobs * n_kv * p.few.splits * 16 * (hd + 2);
   if (p.both) {
-    p.many = split_window(all / ROWS_BM + n_seq, (all / ROWS_BM + 1) * n_kv, max_kv, window, ROWS_BM / group + 2, KV4_RWGS, 64);
+    p.many = split_window(all / ROWS_BM + n_seq, (all / ROWS_BM + 1) * n_kv, max_kv, window, ROWS_BM / group + 2, KV4_RWGS, 64, KV4_RLEAST);
     if (p.many.splits > 1) p.many_floats = p.many.jobs * n_kv * p.many.splits * ROWS_BM * (hd + 2);
   }
   return p;
