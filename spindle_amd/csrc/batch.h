@@ -35,6 +35,7 @@ struct Kv4Attn {
   int n_heads, group, rows, n_seq, cols, window;
   const int32_t *q_start, *kv_lens, *tables;
   float scale;  // times log2(e)
+  int qvec, ovec;     // queries / outputs lie at multiples of 16 bytes
   int few;            // sequences with more rows (new tokens x query heads a key head) are k_kv4_rows'
   int chunk, rchunk;  // tokens a workgroup takes at a time
   float *part, *rpart;  // scratch: outputs, then (maximum, sum), of every job, key head, split and row

@@ -91,6 +91,29 @@ __device__ __forceinline__ void put8(typename R::E *dst, const float *x) {
   }
 }
 
+// The same by a flag that is one for the launch; N values out.
+template <class R>
+__device__ __forceinline__ void get8_if(bool vec, const typename R::E *src, float *x) {
+  if (vec) get8<R, true>(src, x);
+  else get8<R, false>(src, x);
+}
+template <class R, int N>
+__device__ __forceinline__ void put_if(bool vec, typename R::E *dst, const float *x) {
+  typedef typename R::E E;
+  alignas(16) E e[N];
+#pragma unroll
+  for (int i = 0; i < N; i++) e[i] = row_put(R{}, x[i]);
+  if (vec) {
+    if constexpr (sizeof(e) == 8) *(uint2 *)dst = *(const uint2 *)e;
+    else
+#pragma unroll
+      for (int i = 0; i < (int)sizeof(e) / 16; i++) ((uint4 *)dst)[i] = ((const uint4 *)e)[i];
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; i++) dst[i] = e[i];
+  }
+}
+
 // ------------------------------------------------------------------ append
 // The integer nearest to x / d, half to even, exactly: the quotient's estimate is off by at most
 // one, and x - c d is exact (c d has at most 12 bits and is within a factor of two of x, or zero).
@@ -423,12 +446,11 @@ __global__ __launch_bounds__(256) void k_kv4_attn(const Kv4Attn a) {
   const E *qp = (const E *)a.q + (int64_t)(j.q0 + tok) * a.ld_q + (head * a.group + g0) * HD + 8 * h;
   float qv[G][8], amax = 0.0f;
 #pragma unroll
-  for (int g = 0; g < G; g++)
+  for (int g = 0; g < G; g++) {
+    get8_if<R>(a.qvec, qp + 32 * g, qv[g]);
 #pragma unroll
-    for (int i = 0; i < 8; i++) {
-      qv[g][i] = row_get(R{}, qp[32 * g + i]);
-      amax = fmaxf(amax, fabsf(qv[g][i]));
-    }
+    for (int i = 0; i < 8; i++) amax = fmaxf(amax, fabsf(qv[g][i]));
+  }
   amax = max32(max16(amax));
   const float lift = lift_of(amax), unlift = a.scale / lift * (EXACT ? 1.0f : 16777216.0f);
   h8v qh[G], ql[G];
@@ -613,7 +635,8 @@ __global__ __launch_bounds__(256) void k_kv4_attn(const Kv4Attn a) {
     const float inv = total == 0.0f ? 0.0f : 1.0f / total;
     E *dst = (E *)a.out + (int64_t)(j.q0 + rr / a.group) * a.ld_out + (head * a.group + rr % a.group) * HD + part * NC;
 #pragma unroll
-    for (int c = 0; c < NC; c++) dst[c] = row_put(R{}, v[c] * inv);
+    for (int c = 0; c < NC; c++) v[c] *= inv;
+    put_if<R, NC>(a.ovec, dst, v);
     return;
   }
   const int64_t at = (((int64_t)blockIdx.x * a.n_kv + head) * gridDim.z + blockIdx.z) * 16 + row;
@@ -674,20 +697,25 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void k
   const E *qp = (const E *)a.q + (int64_t)(j.q0 + tok) * a.ld_q + (head * a.group + rc % a.group) * HD + 8 * h;
   float amax = 0.0f;
 #pragma unroll
-  for (int k = 0; k < KS; k++)
+  for (int k = 0; k < KS; k++) {
+    float x[8];
+    get8_if<R>(a.qvec, qp + 16 * k, x);
 #pragma unroll
-    for (int i = 0; i < 8; i++) amax = fmaxf(amax, fabsf(row_get(R{}, qp[16 * k + i])));
+    for (int i = 0; i < 8; i++) amax = fmaxf(amax, fabsf(x[i]));
+  }
   amax = max32(amax);
   const float lift = lift_of(amax), unlift = a.scale / lift;
   h8v qh[KS], ql[KS];
 #pragma unroll
-  for (int k = 0; k < KS; k++)
+  for (int k = 0; k < KS; k++) {
+    float x[8];
+    get8_if<R>(a.qvec, qp + 16 * k, x);
 #pragma unroll
     for (int i = 0; i < 8; i++) {
-      const float x = row_get(R{}, qp[16 * k + i]) * lift;
-      qh[k][i] = (_Float16)x;
-      if (QP == 2) ql[k][i] = (_Float16)(x - (float)qh[k][i]);
+      qh[k][i] = (_Float16)(x[i] * lift);
+      if (QP == 2) ql[k][i] = (_Float16)(x[i] * lift - (float)qh[k][i]);
     }
+  }
   const int pos = j.n - j.nq + tok, hi = min(pos + 1, j.n), lo = a.window > 0 ? max(pos + 1 - a.window, 0) : 0;
   const int last = min(j.r0 + ROWS_BM - 1, rows - 1) / a.group, first = j.r0 / a.group;
   const int all_hi = min(j.n - j.nq + last + 1, j.n), all_lo = a.window > 0 ? max(j.n - j.nq + first + 1 - a.window, 0) : 0;
@@ -931,7 +959,10 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void k
 #pragma unroll
     for (int g = 0; g < G; g++)
 #pragma unroll
-      for (int i = 0; i < 16; i++) dst[32 * g + 8 * (i >> 2) + (i & 3)] = row_put(R{}, o[g][i] * inv);
+      for (int i = 0; i < 16; i += 4) {
+        const float x[4] = {o[g][i] * inv, o[g][i + 1] * inv, o[g][i + 2] * inv, o[g][i + 3] * inv};
+        put_if<R, 4>(a.ovec, dst + 32 * g + 2 * i, x);
+      }
     return;
   }
   const int64_t row = (((int64_t)job * a.n_kv + head) * gridDim.z + blockIdx.z) * ROWS_BM + 32 * wave + col;
@@ -1023,8 +1054,7 @@ __device__ __forceinline__ void join_row(const Kv4Attn &a, const Job4 &j, bool m
   for (int i = 0; i < NC; i++) v[i] = add32(add16(v[i] * f)) * inv;
   if (quarter) return;
   E *dst = (E *)a.out + (int64_t)(j.q0 + rr / a.group) * a.ld_out + (head * a.group + rr % a.group) * HD + part * NC;
-#pragma unroll
-  for (int i = 0; i < NC; i++) dst[i] = row_put(R{}, v[i]);
+  put_if<R, NC>(a.ovec, dst, v);
 }
 
 // How the work is split: jobs (an odd number, so that neighbouring key heads and chunks of a sequence
@@ -1094,6 +1124,9 @@ static hipError_t launch_attention(Kv4Attn &a, const Plan4 &p, hipStream_t s) {
   a.chunk = p.few.chunk;
   a.rchunk = p.many.chunk;
   a.rpart = a.part + p.few_floats;
+  constexpr int ES = sizeof(typename R::E);
+  a.qvec = (uintptr_t)a.q % 16 == 0 && a.ld_q * ES % 16 == 0;
+  a.ovec = (uintptr_t)a.out % 16 == 0 && a.ld_out * ES % 16 == 0;
   hipLaunchKernelGGL((k_kv4_attn<HD, R, QP, PP>), dim3((unsigned)p.few.jobs, nk, p.few.splits), dim3(256), 0, s, a);
   if (p.both) {
     constexpr unsigned bytes = 2 * sizeof(Rows4<HD>);
