@@ -143,8 +143,9 @@ __device__ __forceinline__ void kv4_codes(const float *x, float d, float inv, ui
   for (int j = 0; j < 8; j++) c[j] = (uint32_t)(fminf(fmaxf(f[j], -8.0f), 7.0f) + 8.0f);
 }
 
-// A thread quantizes eight channels; the four threads of a quad share a group's scale.
-// Bound by bytes: each value is read once (4 or 2 bytes) and 4.5 bits are written.
+// A thread quantizes eight channels; the four threads of a quad share a group's scale. 8191 rows of 8
+// heads of 128 (bf16, 43 MB in and out) take 18 us, where bytes alone would take 8: what bounds it are
+// its narrow stores, a word of codes a thread and two bytes of scale a quad; 24 rows of four heads 3.5 us.
 template <int HD>
 __device__ __forceinline__ void append_piece(const Kv4Rows &a, float *x, int kv, int head, int c8, int slot) {
   int pg, t;
@@ -209,6 +210,7 @@ __global__ __launch_bounds__(256) void k_kv4_append(const Kv4Rows a) {
 }
 
 // ------------------------------------------------------------------ read
+// The other way round: a word of codes and a scale in, 16 or 32 bytes out; 12 and 2.5 us for the same.
 template <int HD, class R, bool VEC>
 __global__ __launch_bounds__(256) void k_kv4_read(const Kv4Rows a) {
   typedef typename R::E E;
@@ -656,6 +658,13 @@ __global__ __launch_bounds__(256) void k_kv4_attn(const Kv4Attn a) {
 // of a token's number swapped, so that the eight tokens whose probabilities a lane has in a step lie
 // together. 16-byte chunks of both are permuted by exclusive-or with row bits: a wave's reads and
 // writes spread over all banks.
+//
+// Bound by the vector instructions beside the products: about 150 a block of 32 x 32 scores (a third
+// of them conversions of codes, the rest maxima, exponentials and their rounding), where its products
+// take 512 cycles. 2048 rows at 4096 tokens (32 heads over 4 of 128, bf16, 103 GFLOP) take 139 us, 742
+// TFLOP/s, where an 8192^3 product of the library reaches 1100. 32 rows a wave and two workgroups a CU,
+// because 64 rows would leave one wave a SIMD, and 256 rows a workgroup no second one to even out what
+// the rows of a prompt see.
 //
 // A group of 32 channels is one block of O^T, so a NaN group (written as zeros) can be given to the
 // rows that see it afterwards: what was zeroed is kept as bits, 64 tokens a group.

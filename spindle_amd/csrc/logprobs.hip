@@ -5,7 +5,10 @@
 // log p_i = x_i - m - log S and the entropy is log S - T / S. One pass over the logits keeps m, S
 // and T a lane (a larger maximum m' turns them into f S and f (T + (m - m') S), f = exp(m - m')) and
 // the alternatives a wave: lane i holds the i-th best key. Bound by the bytes of the logits where
-// there are many rows, by the latency of two launches where there are few.
+// there are many rows (500 rows of 151936 in fp32, one alternative: 66 us, 4.6 TB/s; twenty: 87), by the
+// latency of two launches where there are few (one row: 6 us, with five alternatives 10). 72 rows of
+// 49155 in 16 bits take 9 us, with twenty alternatives 20: the wave's first list is a sort by rank of its
+// lanes' largest, later keys only those above the list's last.
 #include "batch.h"
 #include "dev.h"
 
