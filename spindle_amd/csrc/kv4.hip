@@ -661,7 +661,7 @@ __global__ __launch_bounds__(256) void k_kv4_attn(const Kv4Attn a) {
 //
 // Bound by the vector instructions beside the products: about 150 a block of 32 x 32 scores (a third
 // of them conversions of codes, the rest maxima, exponentials and their rounding), where its products
-// take 512 cycles. 2048 rows at 4096 tokens (32 heads over 4 of 128, bf16, 103 GFLOP) take 139 us, 742
+// take 512 cycles. 2048 rows at 4096 tokens (32 heads over 4 of 128, bf16, 103 GFLOP) take 137 us, 750
 // TFLOP/s, where an 8192^3 product of the library reaches 1100. 32 rows a wave and two workgroups a CU,
 // because 64 rows would leave one wave a SIMD, and 256 rows a workgroup no second one to even out what
 // the rows of a prompt see.
@@ -999,6 +999,7 @@ __global__ __launch_bounds__(256) void k_kv4_join(const Kv4Attn a, int few_jobs,
     constexpr int PER = ROWS_BM / (4 * JOIN_ROWS);
     const int at = blockIdx.x - few_jobs * 4, job = at / PER, row = at % PER * (4 * JOIN_ROWS) + wave * JOIN_ROWS;
     if (many_splits == 1 || !job_of<ROWS_BM>(a, job, j) || j.nq * a.group <= a.few) return;
+#pragma unroll
     for (int i = 0; i < JOIN_ROWS; i++) join_row<HD, R>(a, j, true, job, row + i, many_splits, (int)(gridDim.x - few_jobs * 4) / PER);
   } else {
     const int job = blockIdx.x / 4;
@@ -1106,12 +1107,16 @@ static Split4 split_window(int64_t jobs, int64_t busy, int max_kv, int window, i
 // Both kernels' shares. Sequences with more rows than KV4_FEW rows (new tokens times query heads a
 // key head) are k_kv4_rows'; where there are no more new tokens than sequences that launch is spared and
 // k_kv4_attn takes all.
-struct Plan4 { Split4 few, many; bool both; int64_t few_floats, many_floats; };
+// A single sequence of that many rows is k_kv4_rows' alone, however many of them q_start leaves it:
+// without the launches that would have nothing to do a 2048-row prompt takes 137 us instead of 139.
+struct Plan4 { Split4 few, many; bool both, alone; int64_t few_floats, many_floats; };
 static Plan4 plan_of(int hd, int group, int n_kv, int rows, int n_seq, int max_kv, int window) {
   Plan4 p{};
   const int64_t all = (int64_t)rows * group, each = (all + n_seq - 1) / n_seq;
   p.both = rows > n_seq && all > KV4_FEW;
-  if (p.both) p.few = split_window((int64_t)n_seq * (KV4_FEW / 16), (each > 16 ? 2 : 1) * (int64_t)n_seq * n_kv, max_kv, window, 16 / group + 2, KV4_WGS, 128, 128);
+  p.alone = p.both && n_seq == 1;
+  if (p.alone) p.few = {0, 1, 128};
+  else if (p.both) p.few = split_window((int64_t)n_seq * (KV4_FEW / 16), (each > 16 ? 2 : 1) * (int64_t)n_seq * n_kv, max_kv, window, 16 / group + 2, KV4_WGS, 128, 128);
   else p.few = split_window(all / 16 + n_seq, (each + 15) / 16 * n_seq * n_kv, max_kv, window, 16 / group + 2, KV4_WGS, 128, 128);
   if (p.few.splits > 1) p.few_floats = p.few.jobs * n_kv * p.few.splits * 16 * (hd + 2);
   if (p.both) {
@@ -1129,14 +1134,14 @@ template <int HD, class R>
 static hipError_t launch_attention(Kv4Attn &a, const Plan4 &p, hipStream_t s) {
   constexpr int QP = sizeof(typename R::E) == 4 ? 2 : 1, PP = std::is_same<R, RowBF16>::value ? 1 : 2;
   const unsigned nk = (unsigned)a.n_kv;
-  a.few = p.both ? KV4_FEW : INT32_MAX;
+  a.few = p.alone ? 0 : p.both ? KV4_FEW : INT32_MAX;
   a.chunk = p.few.chunk;
   a.rchunk = p.many.chunk;
   a.rpart = a.part + p.few_floats;
   constexpr int ES = sizeof(typename R::E);
   a.qvec = (uintptr_t)a.q % 16 == 0 && a.ld_q * ES % 16 == 0;
   a.ovec = (uintptr_t)a.out % 16 == 0 && a.ld_out * ES % 16 == 0;
-  hipLaunchKernelGGL((k_kv4_attn<HD, R, QP, PP>), dim3((unsigned)p.few.jobs, nk, p.few.splits), dim3(256), 0, s, a);
+  if (!p.alone) hipLaunchKernelGGL((k_kv4_attn<HD, R, QP, PP>), dim3((unsigned)p.few.jobs, nk, p.few.splits), dim3(256), 0, s, a);
   if (p.both) {
     constexpr unsigned bytes = 2 * sizeof(Rows4<HD>);
     static std::atomic<uint64_t> set{0};  // devices on which the kernel has been allowed that much shared memory

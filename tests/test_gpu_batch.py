@@ -380,6 +380,24 @@ def test_attention_captured_prompt(ctx):
                 assert torch.equal(out, want) and (out[s[2]:] == 7.0).all()
 
 
+@pytest.mark.parametrize("start,n", [([0, 130], 700), ([0, 1], 333), ([4, 9], 9), ([0, 0], 50), ([100, 130], 64), ([0, 130], 100)])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_attention_one_sequence_room_to_spare(ctx, dtype, start, n):
+    """One sequence in a call with room for a prompt: a whole one, a row, some in the middle, none."""
+    from spindle_amd import ops
+    b = Batch(ctx, [n], 2, 64, 16, seed=34)
+    q = queries(34, 130, 8, 64, dtype)
+    out = torch.full_like(q, 7.0)
+    ops.kv4_attention(ctx, b.shape, b.pool, q, ints(start), ints([n]), ints(b.tables), out=out)
+    lo, hi = start
+    assert (out[:lo] == 7.0).all() and (out[hi:] == 7.0).all()
+    at, half, parts = b.slots(0), torch.finfo(dtype).eps / 2, (2, 2) if dtype == F32 else (1, 1)
+    got, qd = f64(out), f64(q)
+    for i in range(lo, hi):
+        want, tol = R.attention(qd[i], b.k[at], b.v[at], n - (hi - i), 0, 64 ** -0.5, *parts)
+        assert (np.abs(got[i] - want) <= tol + half * (np.abs(want) + tol)).all(), i
+
+
 def test_attention_many_sequences(ctx):
     rng = np.random.default_rng(6)
     lens = [int(v) for v in rng.integers(1, 60, 300)]
