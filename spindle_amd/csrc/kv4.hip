@@ -16,7 +16,6 @@ namespace spx {
 
 typedef _Float16 h2v __attribute__((ext_vector_type(2)));
 typedef _Float16 h8v __attribute__((ext_vector_type(8)));
-typedef uint32_t u4v __attribute__((ext_vector_type(4)));
 
 constexpr float KV4_DMAX = 8160.0f;  // 8 * d stays finite in f16
 
@@ -669,7 +668,7 @@ __global__ __launch_bounds__(256) void k_kv4_attn(const Kv4Attn a) {
 // A group of 32 channels is one block of O^T, so a NaN group (written as zeros) can be given to the
 // rows that see it afterwards: what was zeroed is kept as bits, 64 tokens a group.
 typedef float f16v __attribute__((ext_vector_type(16)));
-constexpr int ROWS_BM = 128, SCHED_R = 4, SCHED_V = 10;
+constexpr int ROWS_BM = 128;
 
 template <int HD>
 struct alignas(256) Rows4 {  // a step's 64 tokens
@@ -877,19 +876,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void k
             if (QP == 2) s[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, ql[k], s[u], 0, 0, 0);
           }
         }
-        if (u0 == 0) {
-          // the next tile's codes become values while the products run: a product, the read of another's
-          // keys and ten vector instructions at a time
-          store(buf[at ^ 1]);
-          __builtin_amdgcn_sched_group_barrier(0x100, SCHED_R, 0);
-#pragma unroll
-          for (int i = 0; i < 16; i++) {
-            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-            __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-            __builtin_amdgcn_sched_group_barrier(0x002, SCHED_V, 0);
-            if (i > 3) __builtin_amdgcn_sched_group_barrier(0x200, 1, 0);
-          }
-        }
+        if (u0 == 0) store(buf[at ^ 1]);  // the next tile's codes become values while the products run
         if (u0 == 0) load(t0 + 128);
         if (masks) {
 #pragma unroll
@@ -999,7 +986,6 @@ __global__ __launch_bounds__(256) void k_kv4_join(const Kv4Attn a, int few_jobs,
     constexpr int PER = ROWS_BM / (4 * JOIN_ROWS);
     const int at = blockIdx.x - few_jobs * 4, job = at / PER, row = at % PER * (4 * JOIN_ROWS) + wave * JOIN_ROWS;
     if (many_splits == 1 || !job_of<ROWS_BM>(a, job, j) || j.nq * a.group <= a.few) return;
-#pragma unroll
     for (int i = 0; i < JOIN_ROWS; i++) join_row<HD, R>(a, j, true, job, row + i, many_splits, (int)(gridDim.x - few_jobs * 4) / PER);
   } else {
     const int job = blockIdx.x / 4;
