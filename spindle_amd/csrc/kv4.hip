@@ -11,6 +11,7 @@
 
 #include "batch.h"
 #include "dev.h"
+#include "kv4_order.h"
 
 namespace spx {
 
@@ -680,11 +681,6 @@ struct alignas(256) Rows4 {  // a step's 64 tokens
 
 template <int HD>
 __device__ __forceinline__ int key_mix(int t) { return HD == 128 ? t & 15 : t >> 1 & 7; }
-// Place i of n in an order that runs backwards in every other 256.
-__device__ __forceinline__ int snake(int i, int n) {
-  const int b = i & ~255;
-  return i & 256 ? b + min(n - b, 256) - 1 - (i - b) : i;
-}
 __device__ __forceinline__ int value_mix(int ch) { return (ch >> 1 ^ ch >> 4) & 7; }
 
 template <int HD, class R, int QP, int PP>
@@ -693,10 +689,9 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void k
   constexpr int G = HD / 32, KS = HD / 16, NC = HD / 16;
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
   Rows4<HD> *buf = (Rows4<HD> *)lds;
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 31, h = lane >> 5, head = blockIdx.x % a.n_kv;
-  // The last jobs of a sequence see the most tokens: they go first, 256 workgroups (one a CU) by falling
-  // work, the 256 after them by rising work, and so on.
-  const int rank = snake(blockIdx.x, gridDim.x) / a.n_kv, job = (int)(gridDim.x / a.n_kv) - 1 - rank;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 31, h = lane >> 5;
+  const RowsPlace place = rows_place(blockIdx.x, gridDim.x, a.n_kv);
+  const int job = place.job, head = place.head;
   Job4 j;
   if (!job_of<ROWS_BM>(a, job, j)) return;
   const int rows = j.nq * a.group;

@@ -1,0 +1,82 @@
+"""The operators for batches of sequences at the ends of their ranges: launches of many workgroups, numbers
+at their types' limits, lengths near 2^31. References in 64 bits."""
+import numpy as np
+import pytest
+
+from test_gpu_batch import BF16, F16, F32, Batch, ctx, f64, ints, queries  # noqa: F401 (ctx: a fixture)
+
+pytestmark = pytest.mark.gpu
+torch = pytest.importorskip("torch")
+
+PARTS = {F32: (2, 2), F16: (1, 2), BF16: (1, 1)}
+
+
+def reference(b, q, counts, dtype, window=0, scale=None, lens=None):
+    """batch_ref.attention and its bound for every row at once, in 64 bits on the device, the output's own
+    rounding included. (Products of two-dimensional matrices, the right one made dense.)"""
+    parts_q, parts_p = PARTS[dtype]
+    rows, heads, hd = q.shape
+    scale = scale or hd ** -0.5
+    out, tol = (torch.zeros(rows, heads, hd, dtype=torch.float64, device="cuda") for _ in range(2))
+    at = 0
+    for s, c in enumerate(counts):
+        n = b.lens[s] if lens is None else lens[s]
+        k, v = (torch.from_numpy(x[b.slots(s, n)]).cuda() for x in (b.k, b.v))
+        tok = torch.arange(n, device="cuda")
+        for a in range(0, c, 1024):
+            z = min(c, a + 1024)
+            pos = (n - c + torch.arange(a, z, device="cuda"))[:, None]
+            seen = (tok <= pos) & (tok > pos - window) if window else tok <= pos
+            some = seen.any(1, keepdim=True)
+            for h in range(heads):
+                kh, vh, qh = k[:, h // (heads // b.kv)].contiguous(), v[:, h // (heads // b.kv)].contiguous(), q[at + a:at + z, h].double()
+                x = (qh @ kh.t().contiguous()) * scale
+                mag = (qh.abs() @ kh.abs().t().contiguous()) * scale
+                split = 2.0 ** -22 * qh.abs().amax(1, keepdim=True) * kh.abs().sum(1) * scale if parts_q == 2 else 0.0
+                ds = torch.where(seen, mag * (hd + 8) * 2.0 ** -24 + split + x.abs() * 3 * 2.0 ** -24, 0.0).amax(1, keepdim=True)
+                p = torch.where(some, torch.softmax(torch.where(seen, x, -torch.inf), 1), 0.0)
+                rel = 2 * ds + (2.0 ** -22 if parts_p == 2 else 2.0 ** -11) * 2 + (seen.sum(1, keepdim=True) / 8 + 64) * 2.0 ** -24
+                out[at + a:at + z, h] = p @ vh
+                tol[at + a:at + z, h] = torch.where(some, rel * (p @ vh.abs()) + 2.0 ** -35 * (seen.double() @ vh.abs()) + 1e-37, 0.0)
+        at += c
+    half = torch.finfo(dtype).eps / 2
+    return out, tol + half * (out.abs() + tol) + (2.0 ** -25 if dtype == F16 else 0.0)
+
+
+def held(ctx, b, q, counts, dtype, window=0, scale=None, **kw):
+    """Runs the operator into an output of NaN and holds every row to its bound."""
+    from spindle_amd import ops
+    start = np.concatenate([[0], np.cumsum(counts)])
+    out = torch.full_like(q, float("nan"))
+    ops.kv4_attention(ctx, b.shape, b.pool, q, ints(start), ints(b.lens), ints(b.tables), scale=scale or 0.0, window=window, out=out, **kw)
+    want, tol = reference(b, q, counts, dtype, window, scale)
+    n = int(start[-1])
+    bad = ~((out[:n].double() - want[:n]).abs() <= tol[:n])
+    assert not bad.any(), (int(bad.any(-1).sum()), bad.nonzero()[0].tolist())
+    assert out[n:].isnan().all()
+    return out
+
+
+# -------------------------------------------------------------------- launches of many workgroups
+@pytest.mark.parametrize("heads,kv,hd,lens,counts,dtype", [
+    (9, 3, 64, [8192], [8192], BF16),                                        # 579 workgroups of the prompt kernel, one chunk
+    (9, 3, 64, [100] * 64, [78] * 63 + [86], F32),                           # 5000 rows over 64 sequences
+    (12, 6, 64, [4096], [4096], F16),
+    (40, 10, 128, [2100, 2048], [2000, 2048], BF16),
+    (40, 10, 128, [4096], [4096], F32),
+    (5, 5, 64, [3000, 40, 2900], [2700, 0, 2500], BF16),
+])
+def test_prompts_of_many_workgroups(ctx, heads, kv, hd, lens, counts, dtype):  # noqa: F811
+    """Row tiles times key heads past 512, numbers of key heads that are no power of two."""
+    b = Batch(ctx, lens, kv, hd, 64, seed=kv)
+    held(ctx, b, queries(kv, sum(counts), heads, hd, dtype), counts, dtype)
+
+
+@pytest.mark.parametrize("heads,kv,hd", [(9, 3, 64), (12, 6, 64), (20, 5, 128)])
+@pytest.mark.parametrize("window", [0, 700])
+def test_many_workgroups_split(ctx, heads, kv, hd, window):  # noqa: F811
+    """The same where sequences are split into chunks, whose outputs are joined: many short row tiles."""
+    n = 220
+    lens, counts = [[1500, 260, 90][i % 3] for i in range(n)], [[30, 1, 3][i % 3] for i in range(n)]
+    b = Batch(ctx, lens, kv, hd, 16, seed=heads)
+    held(ctx, b, queries(heads, sum(counts), heads, hd, F32), counts, F32, window=window)
