@@ -304,7 +304,13 @@ hipError_t launch_kv4_read(const Kv4Rows &a, int hd, int type, hipStream_t s) {
 // bits in f16; a maximum that grows by less than 2^5 leaves the reference as it is. In two parts
 // (SPX_F32, SPX_F16) they have 22 bits too: one part's rounding (2^-11) would add to the output's own
 // in SPX_F16; in SPX_BF16 it is an eighth of it.
-constexpr float P_LIFT = 10.0f, P_SLACK = 5.0f;
+// The reference is kept in the units of the sums, unscaled: a probability's exponent is one multiply-add
+// s * unlift + (10 - m * unlift), whose last term is rounded. Where that is past 2^12 (P_FAR) the sums have
+// the reference taken off first: at 2^30 the rounding would be more than f16's whole range.
+constexpr float P_LIFT = 10.0f, P_SLACK = 5.0f, P_FAR = 4096.0f;
+// What the exponents add to s * unlift, for a reference of top = m * unlift (0 where no token has been seen).
+__device__ __forceinline__ float p_ref(float top) { return top == -__builtin_inff() ? 0.0f : P_LIFT - top; }
+__device__ __forceinline__ bool p_far(float top) { return fabsf(top) > P_FAR && top != -__builtin_inff(); }
 
 // The sequence and first row of job `job`: sequence s has jobs floor(start_s * group / BM) + s and
 // on, enough for its rows whatever their number, and f ascends, so that one pass over q_start in
@@ -532,15 +538,24 @@ __global__ __launch_bounds__(256) void k_kv4_attn(const Kv4Attn a) {
         mt = fmaxf(mt, s[u][i]);
       }
     }
-    mt = max32(max16(mt)) * unlift;  // (unlift is positive)
-    if (__builtin_amdgcn_ballot_w64(mt > m + P_SLACK)) {
-      const float mn = fmaxf(m, mt), f = m == mn ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
+    mt = max32(max16(mt));
+    if (__builtin_amdgcn_ballot_w64((mt - m) * unlift > P_SLACK)) {  // (unlift is positive)
+      const float mn = fmaxf(m, mt), f = m == mn ? 1.0f : __builtin_amdgcn_exp2f((m - mn) * unlift);
       m = mn;
       sum *= f;
 #pragma unroll
       for (int c = 0; c < NC; c++) o[c] *= f;
     }
-    const float ref = m == -__builtin_inff() ? 0.0f : P_LIFT - m;
+    const float top = m * unlift;
+    float ref = p_ref(top);
+    if (__builtin_expect(__builtin_amdgcn_ballot_w64(p_far(top)) != 0, 0)) {
+      const float off = p_far(top) ? m : 0.0f;
+      ref = p_far(top) ? P_LIFT : ref;
+#pragma unroll
+      for (int u = 0; u < 2; u++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) s[u][i] -= off;
+    }
     h2v p1[4], p2[4];
 #pragma unroll
     for (int u = 0; u < 2; u++)
@@ -609,7 +624,7 @@ __global__ __launch_bounds__(256) void k_kv4_attn(const Kv4Attn a) {
     }
   }
   sum = add32(add16(sum));
-  if (h == 0) { sm[wave][l] = m; sl[wave][l] = sum; }
+  if (h == 0) { sm[wave][l] = m * unlift; sl[wave][l] = sum; }
   // row i of a lane's four is channels (4h + i) NC .. + NC - 1
 #pragma unroll
   for (int i = 0; i < 4; i++)
@@ -888,9 +903,9 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void k
         for (int u = 0; u < NB; u++)
 #pragma unroll
           for (int i = 0; i < 16; i++) mt = fmaxf(mt, s[u][i]);
-        mt = max32(mt) * unlift;
-        if (__builtin_amdgcn_ballot_w64(mt > m + P_SLACK)) {
-          const float mn = fmaxf(m, mt), f = m == mn ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
+        mt = max32(mt);
+        if (__builtin_amdgcn_ballot_w64((mt - m) * unlift > P_SLACK)) {
+          const float mn = fmaxf(m, mt), f = m == mn ? 1.0f : __builtin_amdgcn_exp2f((m - mn) * unlift);
           m = mn;
           sum *= f;
 #pragma unroll
@@ -910,7 +925,16 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void k
                 for (int i = 0; i < 16; i++) o[g][i] = __builtin_nanf("");
             }
         }
-        const float ref = m == -__builtin_inff() ? 0.0f : P_LIFT - m;
+        const float top = m * unlift;
+        float ref = p_ref(top);
+        if (__builtin_expect(__builtin_amdgcn_ballot_w64(p_far(top)) != 0, 0)) {
+          const float off = p_far(top) ? m : 0.0f;
+          ref = p_far(top) ? P_LIFT : ref;
+#pragma unroll
+          for (int u = 0; u < NB; u++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) s[u][i] -= off;
+        }
 #pragma unroll
         for (int u = 0; u < NB; u++) {
           h2v p1[8], p2[8];
@@ -962,7 +986,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void k
   for (int g = 0; g < G; g++)
 #pragma unroll
     for (int i = 0; i < 16; i += 4) *(float4 *)(dst + 32 * g + 2 * i) = make_float4(o[g][i], o[g][i + 1], o[g][i + 2], o[g][i + 3]);
-  if (h == 0) ((float2 *)(a.rpart + (int64_t)gridDim.x * gridDim.z * ROWS_BM * HD))[row] = make_float2(m, sum);
+  if (h == 0) ((float2 *)(a.rpart + (int64_t)gridDim.x * gridDim.z * ROWS_BM * HD))[row] = make_float2(m * unlift, sum);
 }
 
 // The chunks of a row together, a wave a row: sixteen lanes have a row's channels, each of the four

@@ -80,3 +80,99 @@ def test_many_workgroups_split(ctx, heads, kv, hd, window):  # noqa: F811
     lens, counts = [[1500, 260, 90][i % 3] for i in range(n)], [[30, 1, 3][i % 3] for i in range(n)]
     b = Batch(ctx, lens, kv, hd, 16, seed=heads)
     held(ctx, b, queries(heads, sum(counts), heads, hd, F32), counts, F32, window=window)
+
+
+# ----------------------------------------------------------------------- scores far from zero
+def whole_keys(b, step, seed):
+    """Keys of whole multiples of `step` (a power of two) in every slot: -7 .. 7 times it, the first channel of
+    each group -8 times, so that the cache holds them exactly."""
+    from spindle_amd import ops
+    rng = np.random.default_rng(seed)
+    k = rng.integers(-7, 8, (b.pages * b.page, b.kv, b.hd)).astype(np.float32)
+    k[:, :, ::32] = -8.0
+    v = torch.from_numpy(b.v).float().cuda()
+    ops.kv4_append(b.ctx, b.shape, b.pool, torch.from_numpy(k * np.float32(step)).cuda(), v, ints(np.arange(b.pages * b.page)))
+    b.refresh()
+    assert np.array_equal(b.k, k.astype(np.float64) * step)
+
+
+def run_into_nan(ctx, b, q, counts, **kw):  # noqa: F811
+    from spindle_amd import ops
+    out = torch.full_like(q, float("nan"))
+    ops.kv4_attention(ctx, b.shape, b.pool, q, ints(np.concatenate([[0], np.cumsum(counts)])), ints(b.lens), ints(b.tables), out=out, **kw)
+    return out
+
+
+def check_largest_scores(ctx, dtype, hd, size, step, scale, lens, counts):  # noqa: F811
+    """Queries with one channel of +-size: a row's scores are exact and further apart than any
+    exponential's range, so that it is the mean of the values of its largest keys. Bound: n / 8 + 64
+    roundings of a 32-bit sum; every probability is the same power of two."""
+    b = Batch(ctx, lens, 2, hd, 16, seed=50)
+    whole_keys(b, step, 51)
+    rows, heads = sum(counts), 8
+    rng = np.random.default_rng(52)
+    ch = rng.integers(1, 32, (rows, heads)) + 32 * rng.integers(0, hd // 32, (rows, heads))
+    sign = rng.choice([-1.0, 1.0], (rows, heads))
+    q = torch.zeros(rows, heads, hd, dtype=dtype, device="cuda")
+    q[torch.arange(rows)[:, None], torch.arange(heads)[None], torch.from_numpy(ch)] = torch.from_numpy(sign * size).to(dtype).cuda()
+    got = f64(run_into_nan(ctx, b, q, counts, scale=scale))
+    half, at = torch.finfo(dtype).eps / 2, 0
+    for s, c in enumerate(counts):
+        slots = b.slots(s)
+        for i in range(c):
+            n = lens[s] - c + i + 1
+            for h in range(heads):
+                k, v = b.k[slots[:n], h // 4, ch[at, h]] * sign[at, h], b.v[slots[:n], h // 4]
+                best = v[k == k.max()]
+                want = best.mean(0)
+                tol = (n / 8 + 64) * 2.0 ** -24 * np.abs(best).mean(0)
+                tol += half * (np.abs(want) + tol) + 2.0 ** -25
+                assert (np.abs(got[at, h] - want) <= tol).all(), (s, i, h)
+            at += 1
+
+
+FAR = [(F32, 2.0 ** 30, 1.0, 0.0), (F32, 2.0 ** 100, 1.0, 0.0), (BF16, 2.0 ** 30, 1.0, 0.0), (BF16, 2.0 ** 100, 1.0, 0.0), (F16, 2.0 ** 15, 2.0 ** 12, 1.0)]
+
+
+@pytest.mark.parametrize("dtype,size,step,scale", FAR)
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("counts", [[2, 1], [60, 1]])
+def test_scores_far_apart(ctx, dtype, size, step, scale, hd, counts):  # noqa: F811
+    """Scores past 2^28, where the rounding of the largest one alone is more than f16's range."""
+    check_largest_scores(ctx, dtype, hd, size, step, scale, [150, 70], counts)
+
+
+@pytest.mark.parametrize("dtype,size,step,scale", FAR)
+def test_scores_far_apart_split(ctx, dtype, size, step, scale):  # noqa: F811
+    check_largest_scores(ctx, dtype, 128, size, step, scale, [3000, 700], [2, 1])
+    check_largest_scores(ctx, dtype, 64, size, step, scale, [1500, 70], [70, 3])
+
+
+@pytest.mark.parametrize("dtype,size,scale", [(F32, 1e10, 0.0), (F32, 1e30, 0.0), (BF16, 1e10, 0.0), (BF16, 1e30, 0.0), (F16, 3e3, 1e6)])
+@pytest.mark.parametrize("counts", [[2, 1], [60, 1]])
+def test_large_queries(ctx, dtype, size, scale, counts):  # noqa: F811
+    """Ordinary rows times a large number: where the largest score is further from the next than what
+    rounding can move them (and 50 more), the row is that token's value; elsewhere it lies among the values."""
+    b = Batch(ctx, [300, 90], 2, 128, 16, seed=53)
+    q = queries(53, sum(counts), 8, 128, dtype, size)
+    got, sc = run_into_nan(ctx, b, q, counts, scale=scale).double(), scale or 128 ** -0.5
+    parts_q, parts_p = PARTS[dtype]
+    at, sure = 0, 0
+    for s, c in enumerate(counts):
+        k, v = (torch.from_numpy(x[b.slots(s)]).cuda() for x in (b.k, b.v))
+        for i in range(c):
+            n = b.lens[s] - c + i + 1
+            for h in range(8):
+                kh, vh, qh = k[:n, h // 4], v[:n, h // 4], q[at, h].double()
+                x = kh @ qh * sc
+                ds = ((kh.abs() @ qh.abs()) * 136 * 2.0 ** -24 + qh.abs().max() * kh.abs().sum(1) * (2.0 ** -22 if parts_q == 2 else 0.0) + x.abs() / sc * 3 * 2.0 ** -24).max() * sc
+                top = x.topk(2)
+                assert (got[at, h].abs() <= vh.abs().max() * (1 + 2.0 ** -7)).all()
+                if float(top.values[0] - top.values[1]) > 2 * float(ds) + 50:
+                    want = vh[top.indices[0]]
+                    tol = (2.0 ** -21 if parts_p == 2 else 2.0 ** -11) * want.abs() + 2.0 ** -20
+                    tol = tol + torch.finfo(dtype).eps / 2 * (want.abs() + tol)
+                    assert ((got[at, h] - want).abs() <= tol).all(), (s, i, h)
+                    sure += 1
+            at += 1
+    assert sure > 0.9 * at * 8
