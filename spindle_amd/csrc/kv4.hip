@@ -428,13 +428,19 @@ __device__ __forceinline__ void tile_load(Tile4<HD> &x, const uint8_t *tile, int
 }
 
 // The largest power of two that leaves |amax| at most 2^14 (1 for zero or what is not finite; at most
-// 2^100, so that its inverse times the softmax scale stays a normal number).
+// 2^100).
 __device__ __forceinline__ float lift_of(float amax) {
   if (!(amax > 0.0f) || !(amax < __builtin_inff())) return 1.0f;
   int e;
   (void)frexpf(amax, &e);
   return ldexpf(1.0f, min(max(14 - e, -126), 100));
 }
+
+// What turns a sum of lifted queries and keys into an exponent, kept where it is a normal number and the
+// sums (at most 2^14 * 2^16 * 128) times it stay finite. The limits change no result: sums are whole
+// multiples of 2^-48, so that at 2^90 two that differ are further apart than any exponential's range, and
+// at 2^-126 all are alike.
+__device__ __forceinline__ float unlift_of(float scale, float lift) { return fminf(fmaxf(scale / lift, 0x1p-126f), 0x1p90f); }
 
 // Long sequences are shared by workgroups: chunk blockIdx.z of `chunk` tokens (and every
 // gridDim.z-th after it). A workgroup leaves its rows' (maximum, sum, output) for k_kv4_join where
@@ -460,7 +466,7 @@ __global__ __launch_bounds__(256) void k_kv4_attn(const Kv4Attn a) {
     for (int i = 0; i < 8; i++) amax = fmaxf(amax, fabsf(qv[g][i]));
   }
   amax = max32(max16(amax));
-  const float lift = lift_of(amax), unlift = a.scale / lift * (EXACT ? 1.0f : 16777216.0f);
+  const float lift = lift_of(amax), unlift = unlift_of(a.scale, lift) * (EXACT ? 1.0f : 16777216.0f);
   h8v qh[G], ql[G];
   f4v zero[G];  // where a group's sum starts
 #pragma unroll
@@ -722,7 +728,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void k
     for (int i = 0; i < 8; i++) amax = fmaxf(amax, fabsf(x[i]));
   }
   amax = max32(amax);
-  const float lift = lift_of(amax), unlift = a.scale / lift;
+  const float lift = lift_of(amax), unlift = unlift_of(a.scale, lift);
   h8v qh[KS], ql[KS];
 #pragma unroll
   for (int k = 0; k < KS; k++) {

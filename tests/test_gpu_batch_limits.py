@@ -154,7 +154,7 @@ def test_large_queries(ctx, dtype, size, scale, counts):  # noqa: F811
     """Ordinary rows times a large number: where the largest score is further from the next than what
     rounding can move them (and 50 more), the row is that token's value; elsewhere it lies among the values."""
     b = Batch(ctx, [300, 90], 2, 128, 16, seed=53)
-    q = queries(53, sum(counts), 8, 128, dtype, size)
+    q = queries(53, sum(counts), 8, 128, dtype, size).clamp(-torch.finfo(dtype).max, torch.finfo(dtype).max)
     got, sc = run_into_nan(ctx, b, q, counts, scale=scale).double(), scale or 128 ** -0.5
     parts_q, parts_p = PARTS[dtype]
     at, sure = 0, 0
@@ -176,3 +176,30 @@ def test_large_queries(ctx, dtype, size, scale, counts):  # noqa: F811
                     sure += 1
             at += 1
     assert sure > 0.9 * at * 8
+
+
+@pytest.mark.parametrize("dtype,size,scale", [(t, 2.0 ** e, s) for t in (F32, BF16) for e, s in ((121, 0.0), (127, 0.0), (110, 1e9), (20, 3e38), (127, 3e38))] +
+                         [(F16, 2.0 ** 15, 3e38)])
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("counts", [[2, 1], [60, 1]])
+def test_queries_at_their_types_end(ctx, dtype, size, scale, hd, counts):  # noqa: F811
+    """Queries and scales up to the largest numbers there are."""
+    check_largest_scores(ctx, dtype, hd, size, 1.0, scale, [150, 70], counts)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("size", [1e36, 1e38])
+@pytest.mark.parametrize("counts", [[2, 1], [60, 1]])
+def test_largest_queries(ctx, dtype, size, counts):  # noqa: F811
+    test_large_queries(ctx, dtype, size, 0.0, counts)
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("counts", [[2, 1], [60, 1]])
+def test_vanishing_scores(ctx, dtype, counts):  # noqa: F811
+    """Scores that are zero in 32 bits: a row is the mean of the values it sees, what it does not see counts
+    for nothing."""
+    b = Batch(ctx, [150, 70], 2, 64, 16, seed=54)
+    for size, scale in ((1e-38 if dtype != F16 else 6e-8, 1e-38), (1.0, 1e-45)):
+        for window in (0, 20):
+            held(ctx, b, queries(54, sum(counts), 8, 64, dtype, size), counts, dtype, window=window, scale=scale)
