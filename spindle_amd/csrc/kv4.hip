@@ -427,10 +427,12 @@ __device__ __forceinline__ void tile_load(Tile4<HD> &x, const uint8_t *tile, int
   x.vs[1] = bits_h2(c.y);
 }
 
-// The largest power of two that leaves |amax| at most 2^14 (1 for zero or what is not finite; at most
-// 2^100).
+// The largest power of two that leaves |amax| at most 2^14 (1 for zero; at most 2^100). NaN for an
+// infinity: its scores would be infinities, of which a row that saw only -inf would look like one that sees
+// nothing.
 __device__ __forceinline__ float lift_of(float amax) {
-  if (!(amax > 0.0f) || !(amax < __builtin_inff())) return 1.0f;
+  if (!(amax > 0.0f)) return 1.0f;
+  if (amax == __builtin_inff()) return __builtin_nanf("");
   int e;
   (void)frexpf(amax, &e);
   return ldexpf(1.0f, min(max(14 - e, -126), 100));
@@ -439,7 +441,7 @@ __device__ __forceinline__ float lift_of(float amax) {
 // What turns a sum of lifted queries and keys into an exponent, kept where it is a normal number and the
 // sums (at most 2^14 * 2^16 * 128) times it stay finite. The limits change no result: sums are whole
 // multiples of 2^-48, so that at 2^90 two that differ are further apart than any exponential's range, and
-// at 2^-126 all are alike.
+// at 2^-126 all are alike. (A lift of NaN gives the lower limit: what is masked stays -inf.)
 __device__ __forceinline__ float unlift_of(float scale, float lift) { return fminf(fmaxf(scale / lift, 0x1p-126f), 0x1p90f); }
 
 // Long sequences are shared by workgroups: chunk blockIdx.z of `chunk` tokens (and every

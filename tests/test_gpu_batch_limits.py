@@ -203,3 +203,26 @@ def test_vanishing_scores(ctx, dtype, counts):  # noqa: F811
     for size, scale in ((1e-38 if dtype != F16 else 6e-8, 1e-38), (1.0, 1e-45)):
         for window in (0, 20):
             held(ctx, b, queries(54, sum(counts), 8, 64, dtype, size), counts, dtype, window=window, scale=scale)
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("counts", [[3, 2], [60, 2]])
+def test_infinite_queries(ctx, dtype, hd, counts):  # noqa: F811
+    """A row with an infinity or a NaN among its queries is NaN, also where all its scores are -inf (every key's
+    first channel is negative), unless it sees nothing; its neighbours keep their bits."""
+    b = Batch(ctx, [100, 1], 2, hd, 16, seed=55)
+    whole_keys(b, 1.0, 56)
+    b.lens[0] = counts[0] - 1  # the first row of either sequence sits before position 0
+    q = queries(55, sum(counts), 8, hd, dtype)
+    want = run_into_nan(ctx, b, q, counts)
+    bad = torch.zeros(sum(counts), 8, dtype=torch.bool, device="cuda")
+    for row, head, ch, x in ((0, 0, 0, np.inf), (1, 0, 0, np.inf), (1, 5, 32, np.inf), (1, 6, 7, -np.inf), (2, 3, 0, -np.inf), (2, 4, 9, np.nan),
+                             (counts[0], 1, 0, np.inf), (counts[0] + 1, 2, 0, np.inf), (counts[0] + 1, 7, 0, np.nan)):
+        q[row, head, ch], bad[row, head] = x, True
+    got = run_into_nan(ctx, b, q, counts)
+    nothing = torch.zeros_like(bad)
+    nothing[0], nothing[counts[0]] = True, True
+    assert (want[nothing] == 0).all() and (got[nothing] == 0).all()
+    assert torch.equal(got[~bad & ~nothing], want[~bad & ~nothing])
+    assert got[bad & ~nothing].isnan().all()
