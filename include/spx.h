@@ -123,8 +123,9 @@ int spx_moe_dev(spx_ctx *ctx, const spx_tensor *gate, const spx_tensor *up, cons
  *     there, by sequence and place), its new length is 0;
  *   add[s] >= 0: add[s] tokens follow. Sequences take the pages they lack in order, the k-th page
  *     taken being the (k + 1)-th last of the free list, as long as what they and all before them
- *     need is there; a sequence that needs pages after that, whose table is too short, or whose
- *     rows end behind `rows`, is refused: status[s] = 1, its length stays and its rows get no slot.
+ *     need is there; a sequence that needs pages after that, whose table is too short (or whose
+ *     length would pass 2^31 - 1), or whose rows end behind `rows`, is refused: status[s] = 1, its
+ *     length stays and its rows get no slot.
  * Outputs: lens_out[n_seq], n_free_out[1] (either may be its input), tables and free_list[n_pages]
  * updated in place, q_start[n_seq + 1] (the first row of each sequence: add's running sum, refused
  * ones counted; at most `rows`), and for each of `rows` <= 262144 rows its slot

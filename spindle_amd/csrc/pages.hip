@@ -76,17 +76,18 @@ __device__ __forceinline__ void plan_row(const PlanArgs &a, const int *start, in
   a.positions[r] = pos;
 }
 
-// One workgroup does it all: what it reads and writes is a few words a sequence, a page and a row,
-// so a launch's latency and the dependent steps (read lengths, three scans, look up pages) bound it:
-// 6.5 us for 24 sequences of a token each, 8.3 us for 500 with 21000 rows, 3.7 us more for the rows.
+// One workgroup does it all but the rows of large steps, which k_pages_rows places: what it reads and writes
+// is a few words a sequence, a page and a row, so a launch's latency and the dependent steps (read lengths,
+// three scans, look up pages) bound it: 6.5 us for 24 sequences of a token each, 8.3 us for 500 with 21000 rows, 3.7 us more for the rows.
 __global__ __launch_bounds__(PLAN_T) void k_pages_plan(const PlanArgs a) {
   __shared__ int back[PLAN_MAX_SEQ + 1], need[PLAN_MAX_SEQ + 1], start[PLAN_MAX_SEQ + 1], tmp[PLAN_T / 64];
   const int t = threadIdx.x, n = a.n_seq, P = 1 << a.page;
-  const int64_t cap = (int64_t)a.cols << a.page;
+  // (a table may have room for more than 2^31 tokens, a length never: what is past it does not fit)
+  const int64_t cap = min((int64_t)a.cols << a.page, (int64_t)INT32_MAX);
   const int had = min(max(a.n_free[0], 0), a.n_pages);
   auto held_of = [&](int s) { return (int)min((int64_t)max(a.lens[s], 0), cap); };
   for (int s = t; s < n; s += PLAN_T) {
-    const int l = held_of(s), add = a.add[s], held = (l + P - 1) >> a.page;
+    const int l = held_of(s), add = a.add[s], held = (int)(((int64_t)l + P - 1) >> a.page);
     const bool fits = add >= 0 && (int64_t)l + add <= cap;
     back[s] = add < 0 ? held : 0;
     need[s] = fits ? (int)(((int64_t)l + add + P - 1) >> a.page) - held : 0;
@@ -100,11 +101,12 @@ __global__ __launch_bounds__(PLAN_T) void k_pages_plan(const PlanArgs a) {
     if (start[s + 1] > a.rows) need[s] = 0;
   __syncthreads();
   block_prefix(need, n, tmp);
-  for (int k = t; k < back[n]; k += PLAN_T) {
+  const int freed = min(back[n], a.n_pages - had);  // (more than the list holds only from lengths that are not the pool's)
+  for (int k = t; k < freed; k += PLAN_T) {
     const int s = find_share(back, n, k);
-    if (had + k < a.n_pages) a.free_list[had + k] = a.tables[(int64_t)s * a.cols + (k - back[s])];
+    a.free_list[had + k] = a.tables[(int64_t)s * a.cols + (k - back[s])];
   }
-  const int avail = min(had + back[n], a.n_pages);
+  const int avail = had + freed;
   __syncthreads();  // (the released pages are on the list, the lengths still as they came)
   int taken = 0;
   for (int s = t; s < n; s += PLAN_T) {
@@ -122,7 +124,7 @@ __global__ __launch_bounds__(PLAN_T) void k_pages_plan(const PlanArgs a) {
   for (int k = t; k < taken; k += PLAN_T) {
     const int s = find_share(need, n, k);
     const int total = a.lens_out[s], mine = need[s + 1] - need[s];  // granted: its length with the new rows
-    const int first = ((total + P - 1) >> a.page) - mine;
+    const int first = (int)(((int64_t)total + P - 1) >> a.page) - mine;
     a.tables[(int64_t)s * a.cols + first + (k - need[s])] = a.free_list[avail - 1 - k];
   }
   for (int s = t; s <= n; s += PLAN_T) a.q_start[s] = min(start[s], a.rows);

@@ -226,3 +226,32 @@ def test_infinite_queries(ctx, dtype, hd, counts):  # noqa: F811
     assert (want[nothing] == 0).all() and (got[nothing] == 0).all()
     assert torch.equal(got[~bad & ~nothing], want[~bad & ~nothing])
     assert got[bad & ~nothing].isnan().all()
+
+
+# ------------------------------------------------------------------------ lengths near 2^31
+def test_plan_lengths_at_their_end(ctx):  # noqa: F811
+    """Tables with room for more than 2^31 tokens: a sequence of the longest length there is gives back the
+    pages that the list has room for, one that would pass it is refused and takes no pages from those after
+    it."""
+    from spindle_amd import ops
+    top, cols, pages = 2 ** 31 - 1, 2 ** 23 + 1, 20
+    tables = torch.arange(3 * cols, dtype=torch.int32, device="cuda").view(3, cols)
+    tables[1, 0] = 5
+    free = ints([90, 91, 92] + [-1] * (pages - 3))
+
+    def plan(lens, add, rows):
+        t, f = tables.clone(), free.clone()
+        p = ops.pages_plan(ctx, ints(lens), ints(add), t, f, ints([3]), 256, rows)
+        return p, t, f
+
+    p, t, f = plan([top, 10, 300], [-1, 5, -1], 6)
+    assert p.lens.tolist() == [0, 15, 0] and p.status.tolist() == [0, 0, 0] and p.n_free.tolist() == [pages]
+    assert f.tolist() == [90, 91, 92] + list(range(17)) and torch.equal(t, tables)
+    assert p.slots.tolist() == [5 * 256 + i for i in range(10, 15)] + [-1] and p.positions.tolist() == [10, 11, 12, 13, 14, -1]
+    p, t, f = plan([top - 3, 250, top], [4, 10, 0], 14)
+    assert p.lens.tolist() == [top - 3, 260, top] and p.status.tolist() == [1, 0, 0] and p.n_free.tolist() == [2]
+    assert p.q_start.tolist() == [0, 4, 14, 14] and t[1, 1] == 92 and torch.equal(f, free)
+    assert p.slots.tolist() == [-1] * 4 + [5 * 256 + i for i in range(250, 256)] + [92 * 256 + i for i in range(4)]
+    p, t, f = plan([top - 3, 0, 0], [3, 0, 0], 3)
+    assert p.lens.tolist() == [top, 0, 0] and p.status.tolist() == [0, 0, 0] and p.n_free.tolist() == [3]
+    assert p.positions.tolist() == [top - 3, top - 2, top - 1] and torch.equal(t, tables)
