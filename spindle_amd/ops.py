@@ -226,6 +226,12 @@ def _i32(t, *shape):
     return t.data_ptr()
 
 
+def _not_c_ints(names):
+    """Raised where one of a call's numbers (their bits together, past bit 31) does not fit the C entry's
+    ints: ctypes would cut it off without a word."""
+    return ValueError(f"{names} must be in 0..2^31 - 1")
+
+
 def _rows3(t, heads, hd, name):
     """The distance between the rows of a [rows, heads, hd] tensor whose rows are dense."""
     n, w = t.shape[0], heads * hd
@@ -245,8 +251,10 @@ def pages_plan(ctx, lens, add, tables, free_list, n_free, page_tokens, rows):
     updated in place, the rest comes back new (pass the plan's lens and n_free to the next step).
     rows: how many rows the step has room for, at least the sum of the positive adds."""
     n, cols, pages = lens.numel(), tables.shape[1] if tables.dim() == 2 else 0, free_list.numel()
+    if (n | cols | pages | page_tokens | rows) >> 31:
+        raise _not_c_ints("page_tokens, rows and the tensors' sizes")
     ins = _i32(lens, n), _i32(add, n), _i32(n_free, 1), _i32(tables, n, cols), _i32(free_list, pages)
-    p, rows = PagesPlan(), max(rows, 0)
+    p = PagesPlan()
     buf = torch.empty(3 * n + 2 + 2 * rows, dtype=torch.int32, device=lens.device)
     p.lens, p.status, p.q_start, p.n_free, p.slots, p.positions = buf.split_with_sizes((n, n, n + 1, 1, rows, rows))
     at = buf.data_ptr()  # (the parts in this order)
@@ -280,6 +288,8 @@ def _pool(shape, pool):
 def kv4_append(ctx, shape, pool, k, v, slots):
     """Puts rows k, v [rows, n_kv, head_dim] into the pool's slots [rows] (spx_kv4_append)."""
     t, n, kv, hd = _row_type(k.dtype), slots.numel(), shape.n_kv, shape.head_dim
+    if n >> 31:
+        raise _not_c_ints("the rows")
     if v.dtype is not k.dtype or k.shape[0] != n or v.shape[0] != n:
         raise ValueError("k and v must have one type and a row for each slot")
     _run(ctx, (pool, k, v, slots), lib.spx_kv4_append, C.byref(shape), _pool(shape, pool), t, k.data_ptr(), _rows3(k, kv, hd, "k"), v.data_ptr(),
@@ -290,6 +300,8 @@ def kv4_read(ctx, shape, pool, slots, dtype=None):
     """(k, v) [rows, n_kv, head_dim]: the values that the pool's slots [rows] stand for (spx_kv4_read)."""
     dtype = dtype or torch.float32
     t, n, w = _row_type(dtype), slots.numel(), shape.n_kv * shape.head_dim
+    if n >> 31:
+        raise _not_c_ints("the rows")
     size = (n, shape.n_kv, shape.head_dim)
     k, v = pool.new_empty(size, dtype=dtype), pool.new_empty(size, dtype=dtype)
     _run(ctx, (pool, slots), lib.spx_kv4_read, C.byref(shape), _pool(shape, pool), t, n, _i32(slots, n), k.data_ptr(), w, v.data_ptr(), w)
@@ -321,6 +333,8 @@ def kv4_attention(ctx, shape, pool, q, q_start, kv_lens, tables, scale=0.0, wind
         ld_out = _rows3(out, heads, hd, "out")
     cols = tables.shape[1] if tables.dim() == 2 else 0
     max_kv = cols * shape.page_tokens if max_kv is None else max_kv
+    if (rows | heads | n | cols | window | max_kv) >> 31:
+        raise _not_c_ints("window, max_kv and the tensors' sizes")
     sh = C.byref(shape)
     at, size, ws = _scratch(lib.spx_kv4_attention_ws(sh, heads, rows, n, max_kv), ws, pool)
     _run(ctx, (pool, q, q_start, kv_lens, tables, out, ws), lib.spx_kv4_attention, sh, _pool(shape, pool), t, q.data_ptr(), ld_q, heads, rows, n,
@@ -341,7 +355,9 @@ def logprobs(ctx, logits, targets=None, top=0, logit_scale=1.0, ws=None):
     if logits.dim() != 2 or (logits.stride(1) != 1 and logits.shape[1] > 1):
         raise ValueError("logits must be [rows, vocab] with dense rows")
     rows, vocab = logits.shape
-    r, n = Logprobs(), max(top, 0)
+    if (rows | vocab | top) >> 31:
+        raise _not_c_ints("top and the logits' sizes")
+    r, n = Logprobs(), min(top, 32)  # (more are refused)
     r.entropy = logits.new_empty(rows, dtype=torch.float32)
     r.top_ids, r.top_logp = logits.new_empty((rows, n), dtype=torch.int32), logits.new_empty((rows, n), dtype=torch.float32)
     if targets is None:

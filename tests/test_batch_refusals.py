@@ -162,3 +162,35 @@ def test_reference_rounds_as_stated():
     assert list(R.codes_of(x, R.scale_of(x))[:3]) == [-8, 0, 2]
     assert np.isnan(R.values(np.where(np.arange(32) == 3, np.inf, 1.0))).all()
     assert R.scale_of(np.full(32, 1e9)) == -8160.0 and R.scale_of(np.zeros(32)) == 0.0
+
+
+def test_python_numbers_past_the_c_ints():
+    """Numbers that a C int would cut off are refused before anything else happens, negative ones too."""
+    from spindle_amd import ops
+    i32 = lambda *s: torch.zeros(s, dtype=torch.int32)  # noqa: E731
+    sh, q = shape(), torch.zeros(2, 4, 128)
+    pool = torch.zeros(4 * 2 * 2 * 18 * 128, dtype=torch.uint8)
+    for bad in (2 ** 31, 2 ** 32, 2 ** 32 + 16, -1, -2 ** 31, -2 ** 32 + 16):
+        calls = [lambda: ops.pages_plan(None, i32(2), i32(2), i32(2, 3), i32(5), i32(1), 16, bad),
+                 lambda: ops.pages_plan(None, i32(2), i32(2), i32(2, 3), i32(5), i32(1), bad, 4),
+                 lambda: ops.kv4_attention(None, sh, pool, q, i32(2), i32(1), i32(1, 4), window=bad),
+                 lambda: ops.kv4_attention(None, sh, pool, q, i32(2), i32(1), i32(1, 4), max_kv=bad),
+                 lambda: ops.logprobs(None, torch.zeros(2, 50), top=bad)]
+        for f in calls:
+            with pytest.raises(ValueError, match="2.31"):
+                f()
+
+
+def test_python_largest_numbers_reach_the_checks(lib):
+    """2^31 - 1 goes through to the C entry's own checks (here as far as the tensors' device)."""
+    from spindle_amd import ops
+
+    class Ctx:
+        device, h, raw_stream = 0, None, 0
+    i32 = lambda *s: torch.zeros(s, dtype=torch.int32)  # noqa: E731
+    pool = torch.zeros(4 * 2 * 2 * 18 * 128, dtype=torch.uint8)
+    for kw in (dict(window=2 ** 31 - 1), dict(max_kv=2 ** 31 - 1)):
+        with pytest.raises(ValueError, match="cuda:0"):
+            ops.kv4_attention(Ctx, shape(), pool, torch.zeros(2, 4, 128), i32(2), i32(1), i32(1, 4), ws=pool, **kw)
+    with pytest.raises(ValueError, match="cuda:0"):
+        ops.logprobs(Ctx, torch.zeros(2, 50), top=2 ** 31 - 1)
