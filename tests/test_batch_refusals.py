@@ -194,3 +194,25 @@ def test_python_largest_numbers_reach_the_checks(lib):
             ops.kv4_attention(Ctx, shape(), pool, torch.zeros(2, 4, 128), i32(2), i32(1), i32(1, 4), ws=pool, **kw)
     with pytest.raises(ValueError, match="cuda:0"):
         ops.logprobs(Ctx, torch.zeros(2, 50), top=2 ** 31 - 1)
+
+
+# ------------------------------------------------------------------ scratch that calls do need
+def test_split_calls_need_scratch(lib):
+    """What is split among workgroups needs scratch, and is refused without it; what is not needs none."""
+    s = shape(n_pages=4096)
+    need = lib.spx_kv4_attention_ws(C.byref(s), 4, 1, 1, 65536)
+    assert need >= 4 * 2 * 16 * (128 + 2) * 2  # two parts of 16 rows of two key heads at the least
+    big = dict(rows=1, cols=2048, max_kv=65536)
+    for kw in (dict(ws_bytes=need - 1), dict(ws_bytes=0), dict(ws=A + 8)):
+        assert "ws must hold" in error(lib, attention(lib, s, **kw, **big))
+    none = lambda **kw: lib.spx_kv4_attention(None, C.byref(s), A, 0, A, 512, 4, kw["rows"], 1, A, A, A, kw["cols"], 0.0, 0, kw["max_kv"], A, 512, None, 0)  # noqa: E731
+    assert "ws must hold" in error(lib, none(**big))
+    assert lib.spx_kv4_attention_ws(C.byref(s), 4, 1, 1, 64) == 0
+    assert "context" in error(lib, none(rows=1, cols=2, max_kv=64))
+    need = lib.spx_logprobs_ws(1, 151936, 5)
+    assert need >= 2 * (16 + 8 * 5)
+    big = dict(rows=1, vocab=151936, ld=151936, top=5)
+    for kw in (dict(ws_bytes=need - 1), dict(ws=None), dict(ws=A + 8)):
+        assert "ws must hold" in error(lib, lib.spx_logprobs(None, *(LP | big | kw).values()))
+    assert lib.spx_logprobs_ws(2, 1000, 3) == 0
+    assert "context" in error(lib, lib.spx_logprobs(None, *(LP | dict(ws=None, ws_bytes=0)).values()))
