@@ -114,7 +114,8 @@ int spx_moe_dev(spx_ctx *ctx, const spx_tensor *gate, const spx_tensor *up, cons
  * allocates, waits on the host or copies to it, so a step of them can be captured into a graph;
  * scratch memory is the caller's (the *_ws functions say how much), and calls that may run at the
  * same time need scratch of their own. Activations are SPX_F32, SPX_F16 or SPX_BF16 (`type`), with
- * rows `ld` elements apart; every rounding to 16 bits is to nearest even. */
+ * rows `ld` elements apart; every rounding to 16 bits is to nearest even. Addresses are multiples
+ * of their elements' size, where no more is asked for. */
 
 /* One step's bookkeeping for n_seq <= 4096 sequences with block tables [n_seq][table_cols] of page
  * ids, pages of page_tokens (a power of two, 16..256) tokens. Sequence s holds lens[s] tokens in

@@ -37,6 +37,9 @@ int log2_of(int v) { return 31 - __builtin_clz((unsigned)v); }
 bool row_type(int t) { return t == SPX_F32 || t == SPX_F16 || t == SPX_BF16; }
 int64_t size_of(int t) { return t == SPX_F32 ? 4 : 2; }
 bool aligned(const void *p, int64_t a) { return (uintptr_t)p % (uintptr_t)a == 0; }
+// Arrays of 32-bit numbers. (Kernels read some of them by scalar loads, which drop an address's last two bits.)
+template <class... T>
+bool words(T... p) { return (aligned(p, 4) && ...); }
 
 // nullptr, or what is wrong with the shape.
 const char *shape_error(const spx_kv4_shape *s) {
@@ -95,6 +98,8 @@ int spx_pages_plan(spx_ctx *ctx, int n_seq, int page_tokens, int table_cols, int
     if (n_pages < 1 || (int64_t)n_pages * page_tokens > INT32_MAX) return fail("spx_pages_plan: n_pages must be positive, n_pages * page_tokens below 2^31");
     if (rows < 0 || rows > 1 << 18) return fail("spx_pages_plan: rows must be in 0..262144");
     if (rows > 0 && (!slots || !positions)) return fail("spx_pages_plan: null argument");
+    if (!words(lens, add, n_free, tables, free_list, lens_out, n_free_out, q_start, slots, positions, status))
+      return fail("spx_pages_plan: addresses must be multiples of 4");
     if (!ctx) return fail("spx_pages_plan: null context");
     OnDevice dev(ctx->device);
     if (dev.err != hipSuccess) return hip_fail(dev.err, "spx_pages_plan");
@@ -144,7 +149,7 @@ int spx_kv4_attention(spx_ctx *ctx, const spx_kv4_shape *shape, const void *pool
       return fail("spx_kv4_attention: table_cols must be positive, table_cols * page_tokens at most 2^30");
     const int64_t width = (int64_t)n_heads * shape->head_dim;
     if (rows > 1 && (ld_q < width || ld_out < width)) return fail("spx_kv4_attention: leading dimension too small");
-    if (!aligned(pool, 16) || !aligned(q, size_of(type)) || !aligned(out, size_of(type)))
+    if (!aligned(pool, 16) || !aligned(q, size_of(type)) || !aligned(out, size_of(type)) || !words(q_start, kv_lens, tables))
       return fail("spx_kv4_attention: the pool's address must be a multiple of 16, the others of their elements' size");
     if (!(scale < __builtin_inff())) return fail("spx_kv4_attention: scale must be finite");
     const int64_t want = spx_kv4_attention_ws(shape, n_heads, rows, n_seq, max_kv);
@@ -197,7 +202,8 @@ int spx_logprobs(spx_ctx *ctx, int type, const void *logits, int64_t ld, int row
     if (rows > 0 && (!logits || (top_n > 0 && (!top_ids || !top_logp)))) return fail("spx_logprobs: null argument");
     if ((targets != nullptr) != (logp != nullptr)) return fail("spx_logprobs: targets and logp go together");
     if (rows > 1 && ld < vocab) return fail("spx_logprobs: leading dimension too small");
-    if (!aligned(logits, size_of(type))) return fail("spx_logprobs: the logits' address must be a multiple of their size");
+    if (!aligned(logits, size_of(type)) || !words(targets, logp, entropy, top_ids, top_logp))
+      return fail("spx_logprobs: addresses must be multiples of the elements' size");
     const int64_t want = spx_logprobs_ws(rows, vocab, top_n);
     if (rows > 0 && want > 0 && (!ws || ws_bytes < want || !aligned(ws, 16)))
       return fail("spx_logprobs: ws must hold " + std::to_string(want) + " bytes at an address that is a multiple of 16");

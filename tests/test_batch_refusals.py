@@ -216,3 +216,19 @@ def test_split_calls_need_scratch(lib):
         assert "ws must hold" in error(lib, lib.spx_logprobs(None, *(LP | big | kw).values()))
     assert lib.spx_logprobs_ws(2, 1000, 3) == 0
     assert "context" in error(lib, lib.spx_logprobs(None, *(LP | dict(ws=None, ws_bytes=0)).values()))
+
+
+# ------------------------------------------------------------------ addresses of 32-bit numbers
+@pytest.mark.parametrize("name", list(PLAN)[5:])
+def test_plan_addresses(lib, name):
+    assert "multiples of 4" in error(lib, lib.spx_pages_plan(None, *(PLAN | {name: A + 2}).values()))
+
+
+@pytest.mark.parametrize("name", ["q_start", "lens", "tables"])
+def test_attention_addresses(lib, name):
+    assert "multiple" in error(lib, attention(lib, shape(), **{name: A + 2}))
+
+
+@pytest.mark.parametrize("name", ["targets", "logp", "entropy", "ids", "best"])
+def test_logprobs_addresses(lib, name):
+    assert "multiples" in error(lib, lib.spx_logprobs(None, *(LP | {name: A + 2}).values()))
