@@ -171,9 +171,11 @@ int spx_kv4_read(spx_ctx *ctx, const spx_kv4_shape *shape, const void *pool, int
  * (query head h reads key head h / (n_heads / n_kv)), scale <= 0 meaning 1 / sqrt(head_dim). A row
  * that sees nothing gets zeros; rows behind q_start[n_seq] are left as they were. A page id outside
  * the pool makes its tokens unseen; lengths beyond the table and row numbers beyond `rows` are cut
- * there. max_kv says how long sequences are at most: it steers how the work is split, results do
- * not depend on its being right. Sums, maxima and probabilities are held in 32 bits; SPX_F32 rows
- * meet the cache as two f16 parts (22 bits), SPX_F16 and SPX_BF16 rows as they are.
+ * there. max_kv says how long sequences are at most: it steers how the work is split; a wrong one
+ * costs time, and the order of sums, no more. Maxima and sums are held in 32 bits. SPX_F32 rows meet
+ * the keys as two f16 parts (22 bits), SPX_F16 and SPX_BF16 rows as they are; probabilities are made in
+ * 32 bits and meet the values as two f16 parts (22 bits), for SPX_BF16 as one (11 bits). Scores may be of any
+ * size; a query head that holds a NaN or an infinity gives NaN where its row sees anything.
  * ws: spx_kv4_attention_ws bytes, a multiple of 16 in address. n_heads <= 1024, rows <= 262144,
  * n_seq <= 4096, table_cols * page_tokens <= 2^30. */
 int64_t spx_kv4_attention_ws(const spx_kv4_shape *shape, int n_heads, int rows, int n_seq, int max_kv);

@@ -168,7 +168,6 @@ int spx_kv4_attention(spx_ctx *ctx, const spx_kv4_shape *shape, const void *pool
     a.out = out;
     a.ld_q = ld_q;
     a.ld_out = ld_out;
-    a.n_heads = n_heads;
     a.group = n_heads / shape->n_kv;
     a.rows = rows;
     a.n_seq = n_seq;

@@ -32,7 +32,7 @@ struct Kv4Attn {
   const void *q;
   void *out;
   int64_t ld_q, ld_out;
-  int n_heads, group, rows, n_seq, cols, window;
+  int group, rows, n_seq, cols, window;
   const int32_t *q_start, *kv_lens, *tables;
   float scale;  // times log2(e)
   int qvec, ovec;     // queries / outputs lie at multiples of 16 bytes

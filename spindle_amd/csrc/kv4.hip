@@ -295,15 +295,20 @@ hipError_t launch_kv4_read(const Kv4Rows &a, int hd, int type, hipStream_t s) {
 // the sum: harmless beside 16-bit rows, but SPX_F32 rows came out 6.5e-6 off instead of 3e-7, so theirs
 // meet the integers -8 .. 7, at four more instructions a word. Values become integer * scale in f16
 // (exact): their scale belongs to the token, which the sum runs over. 64 sequences of up to 16K tokens
-// (32 heads over 4 of 128) read 382 MB in 93 us, 4.1 TB/s, where a copy reaches 5.1; three waves a SIMD,
-// the vector units about half busy. Loads of the next tiles issued before this one's work (209
-// registers, two waves a SIMD) gained nothing, nor did fewer registers with spills.
+// (32 heads over 4 of 128) read 382 MB in 93 us, 4.1 TB/s, where a copy reaches 5.1. By the counters the
+// vector units are busy 71% of the time in which a CU has waves (2.6 a SIMD on average, which spend 43% of
+// theirs at waits), and a CU has none for a quarter of the kernel's time. Loads of the next tiles issued before this one's work (209 registers, two waves a SIMD)
+// gained nothing, nor did fewer registers with spills.
 //
 // A query row is scaled by a power of two to fill f16's range; in two parts (SPX_F32) it has 22 bits.
 // Probabilities are held relative to a running maximum, times 2^10, so that small ones keep their
-// bits in f16; a maximum that grows by less than 2^5 leaves the reference as it is. In two parts
-// (SPX_F32, SPX_F16) they have 22 bits too: one part's rounding (2^-11) would add to the output's own
-// in SPX_F16; in SPX_BF16 it is an eighth of it.
+// bits in f16; a maximum that grows by less than 5 (a factor of 2^5) leaves the reference as it is.
+// They are made in 32 bits and enter the second product in f16: in two parts (SPX_F32, SPX_F16), 22 bits,
+// because one part's rounding (2^-11) would add to the output's own in SPX_F16; in one part, 11 bits, for
+// SPX_BF16, where it is an eighth of the output's (2048 rows at 4096 tokens: 1.67e-3 off in norm with it,
+// 1.66e-3 by the output's rounding alone). Their sum is of the unrounded ones here, of the rounded ones
+// where k_kv4_rows has one part.
+//
 // The reference is kept in the units of the sums, unscaled: a probability's exponent is one multiply-add
 // s * unlift + (10 - m * unlift), whose last term is rounded. Where that is past 2^12 (P_FAR) the sums have
 // the reference taken off first: at 2^30 the rounding would be more than f16's whole range.
@@ -336,7 +341,14 @@ __device__ __forceinline__ bool job_of(const Kv4Attn &a, int job, Job4 &j) {
 }
 
 // k_kv4_attn's jobs: where k_kv4_rows takes the sequences of more than KV4_FEW rows, each of the others
-// has KV4_FEW / 16, whether it needs them or not.
+// has KV4_FEW / 16, whether it needs them or not. KV4_FEW by both kernels' times (k_kv4_attn / k_kv4_rows, us;
+// 32 heads over 4 of 128, the same number of rows in every sequence):
+//   rows              48         64         72         96         128
+//   64 x 4096, bf16   99 / 121   122 / 122  148 / 128  174 / 150  224 / 113
+//   64 x 4096, fp32   117 / 181  145 / 188  177 / 196  212 / 237  274 / 190
+//   12 x 2048, bf16   26 / 32    30 / 34    34 / 35    39 / 37    46 / 37
+//   1 x 4096, bf16    15 / 22    16 / 23    17 / 23    18 / 23    21 / 24
+// 64 is where 16-bit batches change over; few or short sequences and fp32 would change over later, at about 96.
 constexpr int KV4_FEW = 64;
 __device__ __forceinline__ bool few_job(const Kv4Attn &a, int job, Job4 &j) {
   if (a.few == INT32_MAX) return job_of<16>(a, job, j);
