@@ -314,8 +314,8 @@ hipError_t launch_kv4_read(const Kv4Rows &a, int hd, int type, hipStream_t s) {
 // the reference taken off first: at 2^30 the rounding would be more than f16's whole range.
 constexpr float P_LIFT = 10.0f, P_SLACK = 5.0f, P_FAR = 4096.0f;
 // What the exponents add to s * unlift, for a reference of top = m * unlift (0 where no token has been seen).
-__device__ __forceinline__ float p_ref(float top) { return top == -__builtin_inff() ? 0.0f : P_LIFT - top; }
 __device__ __forceinline__ bool p_far(float top) { return fabsf(top) > P_FAR && top != -__builtin_inff(); }
+__device__ __forceinline__ float p_ref(float top) { return top == -__builtin_inff() ? 0.0f : p_far(top) ? P_LIFT : P_LIFT - top; }
 
 // The sequence and first row of job `job`: sequence s has jobs floor(start_s * group / BM) + s and
 // on, enough for its rows whatever their number, and f ascends, so that one pass over q_start in
@@ -439,21 +439,20 @@ __device__ __forceinline__ void tile_load(Tile4<HD> &x, const uint8_t *tile, int
   x.vs[1] = bits_h2(c.y);
 }
 
-// The largest power of two that leaves |amax| at most 2^14 (1 for zero; at most 2^100). NaN for an
-// infinity: its scores would be infinities, of which a row that saw only -inf would look like one that sees
-// nothing.
+// The largest power of two that leaves |amax| at most 2^14 (1 for zero; at most 2^100). Zero for an
+// infinity, which it makes a NaN: its scores would be infinities, of which a row that saw only -inf would
+// look like one that sees nothing.
 __device__ __forceinline__ float lift_of(float amax) {
-  if (!(amax > 0.0f)) return 1.0f;
-  if (amax == __builtin_inff()) return __builtin_nanf("");
   int e;
   (void)frexpf(amax, &e);
-  return ldexpf(1.0f, min(max(14 - e, -126), 100));
+  const float lift = ldexpf(1.0f, min(max(14 - e, -126), 100));
+  return amax == __builtin_inff() ? 0.0f : amax > 0.0f ? lift : 1.0f;
 }
 
 // What turns a sum of lifted queries and keys into an exponent, kept where it is a normal number and the
 // sums (at most 2^14 * 2^16 * 128) times it stay finite. The limits change no result: sums are whole
 // multiples of 2^-48, so that at 2^90 two that differ are further apart than any exponential's range, and
-// at 2^-126 all are alike. (A lift of NaN gives the lower limit: what is masked stays -inf.)
+// at 2^-126 all are alike. (A lift of zero gives the upper limit: what is masked stays -inf.)
 __device__ __forceinline__ float unlift_of(float scale, float lift) { return fminf(fmaxf(scale / lift, 0x1p-126f), 0x1p90f); }
 
 // Long sequences are shared by workgroups: chunk blockIdx.z of `chunk` tokens (and every
@@ -509,7 +508,8 @@ __global__ __launch_bounds__(256) void k_kv4_attn(const Kv4Attn a) {
   f4v o[NC];
 #pragma unroll
   for (int c = 0; c < NC; c++) o[c] = f4v{0.0f, 0.0f, 0.0f, 0.0f};
-  float m = -__builtin_inff(), sum = 0.0f;
+  float m = -__builtin_inff(), sum = 0.0f, ref = 0.0f;
+  bool far = false;  // whether some lane's reference is past P_FAR
   const int *table = a.tables + (int64_t)j.s * a.cols;
   const int pm = (1 << a.page) - 1;
 
@@ -562,15 +562,14 @@ __global__ __launch_bounds__(256) void k_kv4_attn(const Kv4Attn a) {
     if (__builtin_amdgcn_ballot_w64((mt - m) * unlift > P_SLACK)) {  // (unlift is positive)
       const float mn = fmaxf(m, mt), f = m == mn ? 1.0f : __builtin_amdgcn_exp2f((m - mn) * unlift);
       m = mn;
+      ref = p_ref(m * unlift);
+      far = __builtin_amdgcn_ballot_w64(p_far(m * unlift)) != 0;
       sum *= f;
 #pragma unroll
       for (int c = 0; c < NC; c++) o[c] *= f;
     }
-    const float top = m * unlift;
-    float ref = p_ref(top);
-    if (__builtin_expect(__builtin_amdgcn_ballot_w64(p_far(top)) != 0, 0)) {
-      const float off = p_far(top) ? m : 0.0f;
-      ref = p_far(top) ? P_LIFT : ref;
+    if (__builtin_expect(far, 0)) {
+      const float off = p_far(m * unlift) ? m : 0.0f;
 #pragma unroll
       for (int u = 0; u < 2; u++)
 #pragma unroll
@@ -769,6 +768,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void k
 #pragma unroll
     for (int i = 0; i < 16; i++) o[g][i] = 0.0f;
   float m = -__builtin_inff(), sum = 0.0f;
+  bool far = false;  // whether some lane's reference is past P_FAR
 
   // this wave's tile of the 64 tokens from t0
   const int l = lane & 15, hq = lane >> 4;
@@ -927,6 +927,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void k
         if (__builtin_amdgcn_ballot_w64((mt - m) * unlift > P_SLACK)) {
           const float mn = fmaxf(m, mt), f = m == mn ? 1.0f : __builtin_amdgcn_exp2f((m - mn) * unlift);
           m = mn;
+          far = __builtin_amdgcn_ballot_w64(p_far(m * unlift)) != 0;
           sum *= f;
 #pragma unroll
           for (int g = 0; g < G; g++) o[g] *= f;
@@ -945,11 +946,10 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void k
                 for (int i = 0; i < 16; i++) o[g][i] = __builtin_nanf("");
             }
         }
-        const float top = m * unlift;
-        float ref = p_ref(top);
-        if (__builtin_expect(__builtin_amdgcn_ballot_w64(p_far(top)) != 0, 0)) {
-          const float off = p_far(top) ? m : 0.0f;
-          ref = p_far(top) ? P_LIFT : ref;
+        float ref = m == -__builtin_inff() ? 0.0f : P_LIFT - m * unlift;  // (kept, it would cost a register too many)
+        if (__builtin_expect(far, 0)) {
+          const float off = p_far(m * unlift) ? m : 0.0f;
+          ref = p_ref(m * unlift);
 #pragma unroll
           for (int u = 0; u < NB; u++)
 #pragma unroll
