@@ -696,9 +696,9 @@ __global__ __launch_bounds__(256) void k_kv4_attn(const Kv4Attn a) {
 // Bound by the vector instructions beside the products: about 150 a block of 32 x 32 scores (a third
 // of them conversions of codes, the rest maxima, exponentials and their rounding), where its products
 // take 512 cycles. 2048 rows at 4096 tokens (32 heads over 4 of 128, bf16, 103 GFLOP) take 133 to
-// 142 us by card, 725 to 775 TFLOP/s, where an 8192^3 product of the library reaches 1100. 32 rows a wave and two workgroups a CU,
-// because 64 rows would leave one wave a SIMD, and 256 rows a workgroup no second one to even out what
-// the rows of a prompt see.
+// 142 us by card, 725 to 775 TFLOP/s, where an 8192^3 product of the library reaches 1100. 32 rows a wave
+// and two workgroups a CU, because 64 rows would leave one wave a SIMD, and 256 rows a workgroup no second
+// one to even out what the rows of a prompt see.
 //
 // A group of 32 channels is one block of O^T, so a NaN group (written as zeros) can be given to the
 // rows that see it afterwards: what was zeroed is kept as bits, 64 tokens a group.

@@ -255,3 +255,10 @@ def test_plan_lengths_at_their_end(ctx):  # noqa: F811
     p, t, f = plan([top - 3, 0, 0], [3, 0, 0], 3)
     assert p.lens.tolist() == [top, 0, 0] and p.status.tolist() == [0, 0, 0] and p.n_free.tolist() == [3]
     assert p.positions.tolist() == [top - 3, top - 2, top - 1] and torch.equal(t, tables)
+
+
+@pytest.mark.parametrize("kv,counts", [(300, [150, 2]), (300, [3, 1]), (1024, [70, 1]), (1024, [1, 1])])
+def test_many_key_heads(ctx, kv, counts):  # noqa: F811
+    """As many key heads as there may be, more than a turn of the prompt kernel's order."""
+    b = Batch(ctx, [160, 40], kv, 64, 16, seed=57)
+    held(ctx, b, queries(57, sum(counts), kv, 64, BF16), counts, BF16)
