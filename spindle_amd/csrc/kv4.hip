@@ -297,8 +297,9 @@ hipError_t launch_kv4_read(const Kv4Rows &a, int hd, int type, hipStream_t s) {
 // (exact): their scale belongs to the token, which the sum runs over. 64 sequences of up to 16K tokens
 // (32 heads over 4 of 128) read 382 MB in 93 us, 4.1 TB/s, where a copy reaches 5.1. By the counters the
 // vector units are busy 71% of the time in which a CU has waves (2.6 a SIMD on average, which spend 43% of
-// theirs at waits), and a CU has none for a quarter of the kernel's time. Loads of the next tiles issued before this one's work (209 registers, two waves a SIMD)
-// gained nothing, nor did fewer registers with spills.
+// theirs at waits), and a CU has none for a quarter of the kernel's time. Loads of the next
+// tiles issued before this one's work (209 registers, two waves a SIMD) gained nothing, nor did fewer
+// registers with spills.
 //
 // A query row is scaled by a power of two to fill f16's range; in two parts (SPX_F32) it has 22 bits.
 // Probabilities are held relative to a running maximum, times 2^10, so that small ones keep their

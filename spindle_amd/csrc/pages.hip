@@ -78,7 +78,8 @@ __device__ __forceinline__ void plan_row(const PlanArgs &a, const int *start, in
 
 // One workgroup does it all but the rows of large steps, which k_pages_rows places: what it reads and writes
 // is a few words a sequence, a page and a row, so a launch's latency and the dependent steps (read lengths,
-// three scans, look up pages) bound it: 6.5 us for 24 sequences of a token each, 8.3 us for 500 with 21000 rows, 3.7 us more for the rows.
+// three scans, look up pages) bound it: 6.5 us for 24 sequences of a token each, 8.3 us
+// for 500 with 21000 rows, 3.7 us more for the rows.
 __global__ __launch_bounds__(PLAN_T) void k_pages_plan(const PlanArgs a) {
   __shared__ int back[PLAN_MAX_SEQ + 1], need[PLAN_MAX_SEQ + 1], start[PLAN_MAX_SEQ + 1], tmp[PLAN_T / 64];
   const int t = threadIdx.x, n = a.n_seq, P = 1 << a.page;
