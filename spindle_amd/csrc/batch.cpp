@@ -1,45 +1,15 @@
 // C entries of the operators for batches of sequences: checks of arguments, then the launches.
-#include <exception>
 #include <string>
 
 #include "batch.h"
-#include "internal.h"
+#include "entry.h"
 
 using namespace spx;
 
 namespace {
 
-// The context's device for the length of a call, the caller's afterwards.
-struct OnDevice {
-  int was = -1;
-  hipError_t err;
-  explicit OnDevice(int device) {
-    err = hipGetDevice(&was);
-    if (err == hipSuccess && was != device) err = hipSetDevice(device);
-    else was = -1;
-  }
-  ~OnDevice() { if (was >= 0) (void)hipSetDevice(was); }
-};
-
-// No exception leaves a C entry (error texts allocate).
-template <class F>
-int entry(F f) {
-  try {
-    return f();
-  } catch (const std::exception &) {
-    return -1;
-  }
-}
-
 bool pow2(int v) { return v > 0 && (v & (v - 1)) == 0; }
 bool page_ok(int p) { return pow2(p) && p >= 16 && p <= 256; }
-int log2_of(int v) { return 31 - __builtin_clz((unsigned)v); }
-bool row_type(int t) { return t == SPX_F32 || t == SPX_F16 || t == SPX_BF16; }
-int64_t size_of(int t) { return t == SPX_F32 ? 4 : 2; }
-bool aligned(const void *p, int64_t a) { return (uintptr_t)p % (uintptr_t)a == 0; }
-// Arrays of 32-bit numbers. (Kernels read some of them by scalar loads, which drop an address's last two bits.)
-template <class... T>
-bool words(T... p) { return (aligned(p, 4) && ...); }
 
 // nullptr, or what is wrong with the shape.
 const char *shape_error(const spx_kv4_shape *s) {

@@ -76,6 +76,16 @@ __device__ __forceinline__ unsigned long long wave_max_u64(unsigned long long v)
   v = max_u64_x(v, false);
   return max_u64_x(v, true);
 }
+// Inclusive running sum over the wave's lanes.
+__device__ __forceinline__ int wave_scan(int v) {
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int u = __shfl_up(v, o);
+    if (lane >= o) v += u;
+  }
+  return v;
+}
 // Lane i's value of lane src (src wave-uniform).
 __device__ __forceinline__ float lane_f(float v, int src) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), src)); }
 __device__ __forceinline__ int lane_i(int v, int src) { return __builtin_amdgcn_readlane(v, src); }

@@ -16,17 +16,6 @@ constexpr int PLAN_T = 1024;
 // is quicker than its turns: 21000 rows of 500 sequences 28 us in one launch, 14 us in two.
 constexpr int PLAN_ROWS = 2048;
 
-// Inclusive running sum over the wave's lanes.
-__device__ __forceinline__ int wave_scan(int v) {
-  const int lane = threadIdx.x & 63;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const int u = __shfl_up(v, o);
-    if (lane >= o) v += u;
-  }
-  return v;
-}
-
 // Turns arr[0 .. n) into its running sum, arr[n] being the total, in place: arr[i] = sum of the
 // values before i. Every thread of the workgroup calls it.
 __device__ __forceinline__ void block_prefix(int *arr, int n, int *tmp) {
