@@ -197,6 +197,86 @@ int spx_logprobs(spx_ctx *ctx, int type, const void *logits, int64_t ld, int row
                  const int32_t *targets, int top_n, float *logp, float *entropy, int32_t *top_ids, float *top_logp, void *ws,
                  int64_t ws_bytes);
 
+/* ------------------------------------------------------------------ experts over a batch */
+/* Operators of a mixture of experts over a batch's rows, for the same host: the router's choice, rows
+ * sorted by expert and joined again, with the gradients that tuning a router takes, and products with
+ * matrices in microscaled 4-bit floats, dense or by expert. spx_moe and spx_moe_dev above run whole
+ * experts in GGUF formats for up to 16 and 128 rows. No counterpart in the reference, which routes on
+ * the host and has neither sort, format nor gradient. What the batch operators above promise holds
+ * here too: nothing is allocated, waited for or copied to the host, scratch is the caller's, types are
+ * SPX_F32, SPX_F16 and SPX_BF16, roundings to 16 bits are to nearest even, addresses are multiples of their
+ * elements' size. Outputs are memory of their own. A call's outputs have the same bits every time. */
+
+/* The k experts of each row of router logits [rows][n_expert]: chosen [rows][k] gets the ids of the
+ * largest logits, larger first, equal ones by ascending id, weights [rows][k] their softmax
+ * probabilities over all experts (norm 0) or over the chosen ones (norm 1, the probabilities over
+ * their sum). Logits of -inf have weight zero; a row of nothing but -inf has weights 0, a row that holds
+ * a NaN or +inf NaN weights (its ids are distinct and in range all the same). n_expert <= 1024,
+ * k <= 32, k <= n_expert, rows <= 262144. */
+int spx_moe_route(spx_ctx *ctx, int type, const void *logits, int64_t ld, int rows, int n_expert, int k, int norm, int32_t *chosen,
+                  float *weights);
+/* Its gradient: from d_weights [rows][k] and the ids that spx_moe_route left, d_logits [rows][n_expert]
+ * (rows ld_d apart, of the logits' type) with ids held fixed. norm 1: w_j (g_j - sum_i w_i g_i) at the
+ * chosen ids, zero elsewhere; norm 0: p_e (g of e, if chosen, - sum_i p_i g_i) everywhere. A row of nothing but
+ * -inf gets zeros, a row with a NaN or +inf, or with an id out of range, NaN. */
+int spx_moe_route_grad(spx_ctx *ctx, int type, const void *logits, int64_t ld, int rows, int n_expert, int k, int norm,
+                       const int32_t *chosen, const float *d_weights, void *d_logits, int64_t ld_d);
+
+/* The entries of chosen [rows][k] in order of their expert, equal ones in order of entry (row * k + j):
+ * starts[n_expert + 1] (expert e's entries stand at places starts[e] .. starts[e + 1] - 1),
+ * order[rows * k] (the entry at each place) and place[rows][k] (each entry's place). An id outside
+ * 0..n_expert - 1 belongs to no expert here: its place is -1, and as many places at order's end hold -1.
+ * ws: spx_moe_sort_ws bytes, a multiple of 16 in address. n_expert <= 1024, k <= 32, rows <= 262144. */
+int64_t spx_moe_sort_ws(int rows, int k, int n_expert);
+int spx_moe_sort(spx_ctx *ctx, int rows, int k, int n_expert, const int32_t *chosen, int32_t *starts, int32_t *order, int32_t *place,
+                 void *ws, int64_t ws_bytes);
+/* Rows in sorted order: out[i] = x[order[i] / k], times weights[order[i]] where weights [rows][k] are given;
+ * i < rows * k, x [rows][width]. Zeros where order holds no entry. Its gradient is spx_moe_combine
+ * (without weights: the sum over the places that a row went to). width <= 2^20. */
+int spx_moe_gather(spx_ctx *ctx, int type, const void *x, int64_t ld_x, int rows, int k, int width, const int32_t *order,
+                   const float *weights, void *out, int64_t ld_out);
+/* Rows joined again: out[r] = sum over j of weights[r][j] * y[place[r][j]] (weights NULL: of the rows
+ * themselves), y [rows * k][width], summed in 32 bits in order of j. A place outside y adds nothing. */
+int spx_moe_combine(spx_ctx *ctx, int type, const void *y, int64_t ld_y, int rows, int k, int width, const int32_t *place,
+                    const float *weights, void *out, int64_t ld_out);
+/* The weighted joining's gradient: from d_out [rows][width], d_y[place[r][j]] = weights[r][j] * d_out[r] and
+ * d_weights[r][j] = d_out[r] . y[place[r][j]] (0 where the place is none), in 32 bits; d_y is zero where order holds
+ * no entry. order and place are those of one spx_moe_sort. */
+int spx_moe_combine_grad(spx_ctx *ctx, int type, const void *d_out, int64_t ld_d, const void *y, int64_t ld_y, int rows, int k, int width,
+                         const int32_t *order, const int32_t *place, const float *weights, void *d_y, int64_t ld_dy, float *d_weights);
+
+/* A matrix in microscaled 4-bit floats (the Open Compute Project's microscaling formats 1.0, MXFP4):
+ * each row's blocks of 32 columns share a scale 2^E, E = floor(log2 of the block's largest magnitude) - 2,
+ * at least -127 (a block of zeros: -127); a value is held as a sign and the nearest of 0, 0.5, 1, 1.5, 2, 3,
+ * 4, 6 (codes 0..7) to its magnitude over the scale, a tie going to the even code, 6 standing for all
+ * above. A block that holds a NaN or an infinity stands for NaN throughout.
+ * Layout, with cols padded by zeros to a multiple of 128 (P): codes [rows][P / 2], two a byte, the lower
+ * column in the low half, the sign above the code; then scale bytes [rows][P / 32]: E + 127, 255 for NaN. The
+ * products take any bytes: 255 is NaN, 253 and 254 may overflow; padding columns hold codes 0 and scales other than 255. */
+enum { SPX_MX4 = 39 };
+typedef struct {
+  void *data;  /* spx_mx4_bytes bytes, a multiple of 16 in address */
+  int rows, cols;
+} spx_mx4;
+int64_t spx_mx4_bytes(int rows, int cols); /* 0 when rows is not positive or cols not in 1..2^20 */
+
+/* Rows x [m->rows][m->cols] into m, and the values that m stands for out of it. */
+int spx_mx4_quantize(spx_ctx *ctx, int type, const void *x, int64_t ld_x, const spx_mx4 *m);
+int spx_mx4_read(spx_ctx *ctx, const spx_mx4 *m, int type, void *out, int64_t ld_out);
+
+/* Products with such matrices: out[i] = W x_i, or with `up` out[i] = silu(W x_i) * (up x_i), i < rows,
+ * silu(v) = v / (1 + exp(-v)); w (and up, of one shape) holds n_expert matrices of n = w->rows / n_expert
+ * rows one after the other, n <= 2^20, n_expert <= 1024. Without starts n_expert is 1 and order NULL. With starts
+ * [n_expert + 1] (as spx_moe_sort leaves it) row i takes the matrices of the expert whose places it is among; rows behind
+ * starts[n_expert] are left as they were. x_i is row order[i] / k of x, or without order row i; a row whose
+ * order holds no entry (or one of a row behind x_rows) is left as it was. x [x_rows][w->cols]: rows
+ * ld_x apart of type SPX_F32, SPX_F16 or SPX_BF16, or SPX_MX4: x is an spx_mx4's data of x_rows rows (ld_x is not used).
+ * out: rows ld_out apart, of out_type (SPX_F32, SPX_F16, SPX_BF16), rounded once. Sums are held in 32
+ * bits; every value of x meets the matrices with all its bits (an fp32 value as three bf16 parts, an f16 value as two;
+ * what is below 2^-133 in magnitude is lost). rows <= 2^23, x_rows <= 2^23. */
+int spx_mx4_matmul(spx_ctx *ctx, int type, const void *x, int64_t ld_x, int x_rows, const spx_mx4 *w, const spx_mx4 *up, int n_expert,
+                   const int32_t *starts, const int32_t *order, int k, int rows, int out_type, void *out, int64_t ld_out);
+
 /* ------------------------------------------------------------------ synthetic weights */
 /* Seeded synthetic tensor in GGUF block layout (n_expert slabs of rows x cols). kind 0:
  * quantized weights (Q4_K/Q6_K/Q8_0/Q5_0) whose dequantised values have std sigma; kind 1:

@@ -40,6 +40,17 @@ SIGNATURES = {
                                     P, I64, P, I64]),
     "spx_logprobs_ws": (I64, [C.c_int, C.c_int, C.c_int]),
     "spx_logprobs": (C.c_int, [P, C.c_int, P, I64, C.c_int, C.c_int, C.c_float, P, C.c_int, P, P, P, P, P, I64]),
+    "spx_moe_route": (C.c_int, [P, C.c_int, P, I64] + [C.c_int] * 4 + [P, P]),
+    "spx_moe_route_grad": (C.c_int, [P, C.c_int, P, I64] + [C.c_int] * 4 + [P, P, P, I64]),
+    "spx_moe_sort_ws": (I64, [C.c_int, C.c_int, C.c_int]),
+    "spx_moe_sort": (C.c_int, [P, C.c_int, C.c_int, C.c_int, P, P, P, P, P, I64]),
+    "spx_moe_gather": (C.c_int, [P, C.c_int, P, I64, C.c_int, C.c_int, C.c_int, P, P, P, I64]),
+    "spx_moe_combine": (C.c_int, [P, C.c_int, P, I64, C.c_int, C.c_int, C.c_int, P, P, P, I64]),
+    "spx_moe_combine_grad": (C.c_int, [P, C.c_int, P, I64, P, I64, C.c_int, C.c_int, C.c_int, P, P, P, P, I64, P]),
+    "spx_mx4_bytes": (I64, [C.c_int, C.c_int]),
+    "spx_mx4_quantize": (C.c_int, [P, C.c_int, P, I64, P]),
+    "spx_mx4_read": (C.c_int, [P, P, C.c_int, P, I64]),
+    "spx_mx4_matmul": (C.c_int, [P, C.c_int, P, I64, C.c_int, P, P, C.c_int, P, P, C.c_int, C.c_int, C.c_int, P, I64]),
     "spx_synth_tensor": (C.c_int, [C.c_int, I64, I64, C.c_int, C.c_uint64, C.c_float, C.c_int, P]),
     "spx_engine_create": (C.c_int, [P, P, C.POINTER(P)]),
     "spx_engine_set_tensor": (C.c_int, [P, C.c_char_p, C.c_int, I64, I64, C.c_int, P]),

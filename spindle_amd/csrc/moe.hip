@@ -1,0 +1,412 @@
+// A mixture of experts over a batch: the router's choice and its gradient, rows sorted by expert, gathered,
+// joined again and that gradient (spx_moe_route .. spx_moe_combine_grad).
+#include "dev.h"
+#include "experts.h"
+#include "rows.h"
+
+namespace spx {
+
+// ------------------------------------------------------------------ the router
+// A wave has a row, its lane l the logits l, l + 64, ...; NV of them.
+
+// Logits' order as numbers: larger logit, larger number; -0 as 0; NaN above all. 0: none.
+__device__ __forceinline__ uint32_t logit_key(float v) {
+  const uint32_t u = __float_as_uint(v + 0.0f);
+  if ((u & 0x7fffffffu) > 0x7f800000u) return 0xffffffffu;
+  return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+
+template <class R, int NV>
+__device__ __forceinline__ void route_logits(const RouteArgs &a, int row, float (&x)[NV]) {
+  const int lane = threadIdx.x & 63;
+  const typename R::E *src = (const typename R::E *)a.logits + (int64_t)row * a.ld;
+#pragma unroll
+  for (int v = 0; v < NV; v++) {
+    const int e = lane + 64 * v;
+    x[v] = e < a.n_expert ? row_get(R{}, src[e]) : -INFINITY;
+  }
+}
+
+// k rounds of: the wave's largest key, the lowest id that holds it. Lane i keeps the i-th.
+template <class R, int NV>
+__global__ __launch_bounds__(256) void k_moe_route(const RouteArgs a) {
+  const int row = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+  if (row >= a.rows) return;
+  float x[NV];
+  route_logits<R, NV>(a, row, x);
+  uint32_t key[NV];
+#pragma unroll
+  for (int v = 0; v < NV; v++) key[v] = lane + 64 * v < a.n_expert ? logit_key(x[v]) : 0u;
+  int my_e = 0;
+  float my_x = 0.0f, m = 0.0f;
+  for (int i = 0; i < a.k; i++) {
+    uint32_t best = key[0];
+#pragma unroll
+    for (int v = 1; v < NV; v++) best = max(best, key[v]);
+    best = wave_max_u32(best);
+    int e = 0;
+    float at = 0.0f;
+#pragma unroll
+    for (int v = NV - 1; v >= 0; v--) {
+      const unsigned long long holds = __builtin_amdgcn_ballot_w64(key[v] == best);
+      if (holds) {
+        const int l = (int)__builtin_ctzll(holds);
+        e = 64 * v + l;
+        at = lane_f(x[v], l);
+      }
+    }
+    if (i == 0) m = at;
+    if (lane == i) { my_e = e; my_x = at; }
+#pragma unroll
+    for (int v = 0; v < NV; v++)
+      if (lane + 64 * v == e) key[v] = 0u;
+  }
+  // m is the row's maximum, or a NaN if it holds one. -inf: nothing is likely, weights are 0.
+  const float p = lane < a.k && m != -INFINITY ? expf(my_x - m) : 0.0f;
+  float total = 0.0f;
+  if (a.norm) total = p;
+  else
+#pragma unroll
+    for (int v = 0; v < NV; v++) total += expf(x[v] - m);
+  total = wave_sum(total);
+  if (lane < a.k) {
+    a.chosen[(int64_t)row * a.k + lane] = my_e;
+    a.weights[(int64_t)row * a.k + lane] = m == -INFINITY ? 0.0f : p / total;
+  }
+}
+
+// With w the weights and g their gradient, s = sum w g: d x_c = w_c (g_c - s), where the weights are over all
+// experts also d x_e = -p_e s of the others. Lane i holds the i-th chosen id, its weight and gradient.
+template <class R, int NV>
+__global__ __launch_bounds__(256) void k_moe_route_grad(const RouteArgs a) {
+  const int row = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+  if (row >= a.rows) return;
+  typedef typename R::E E;
+  float x[NV];
+  route_logits<R, NV>(a, row, x);
+  bool bad = false;
+  float m = -INFINITY;
+#pragma unroll
+  for (int v = 0; v < NV; v++) {
+    bad |= isnan(x[v]) || x[v] == INFINITY;
+    m = fmaxf(m, x[v]);
+  }
+  m = wave_max(m);
+  int id = -1;
+  float g = 0.0f, xc = -INFINITY;
+  if (lane < a.k) {
+    id = a.chosen[(int64_t)row * a.k + lane];
+    g = a.d_weights[(int64_t)row * a.k + lane];
+    bad |= id < 0 || id >= a.n_expert;
+    if (id >= 0 && id < a.n_expert) xc = row_get(R{}, ((const E *)a.logits)[(int64_t)row * a.ld + id]);
+  }
+  bad = __builtin_amdgcn_ballot_w64(bad) != 0;
+  const float mc = a.norm ? wave_max(xc) : m;  // (the weights' own maximum, whatever ids are given)
+  const float pc = xc == -INFINITY ? 0.0f : expf(xc - mc);
+  float p[NV], total = pc;
+  if (!a.norm) {
+    total = 0.0f;
+#pragma unroll
+    for (int v = 0; v < NV; v++) { p[v] = x[v] == -INFINITY ? 0.0f : expf(x[v] - m); total += p[v]; }
+  }
+  total = wave_sum(total);
+  const float inv = total > 0.0f ? 1.0f / total : 0.0f, w = pc * inv, s = wave_sum(lane < a.k ? w * g : 0.0f);
+  const float mine = a.norm ? w * (g - s) : w * g;
+  E *out = (E *)a.d_logits + (int64_t)row * a.ld_d;
+  float d[NV];
+#pragma unroll
+  for (int v = 0; v < NV; v++) d[v] = a.norm ? 0.0f : -(p[v] * inv) * s;
+  for (int j = 0; j < a.k; j++) {
+    const int e = lane_i(id, j);
+    const float add = lane_f(mine, j);
+#pragma unroll
+    for (int v = 0; v < NV; v++)
+      if (lane + 64 * v == e) d[v] += add;
+  }
+#pragma unroll
+  for (int v = 0; v < NV; v++)
+    if (lane + 64 * v < a.n_expert) out[lane + 64 * v] = row_put(R{}, bad ? __builtin_nanf("") : d[v]);
+}
+
+#define MOE_BY_TYPE(type, CALL)               \
+  switch (type) {                             \
+  case T_F32: { CALL(RowF32); break; }        \
+  case T_F16: { CALL(RowF16); break; }        \
+  case T_BF16: { CALL(RowBF16); break; }      \
+  default: return hipErrorInvalidValue;       \
+  }
+
+template <class R>
+static void route(const RouteArgs &a, bool grad, hipStream_t s) {
+  const dim3 grid((unsigned)(a.rows + 3) / 4), block(256);
+#define ROUTE(NV)                                                                              \
+  if (grad) hipLaunchKernelGGL((k_moe_route_grad<R, NV>), grid, block, 0, s, a);               \
+  else hipLaunchKernelGGL((k_moe_route<R, NV>), grid, block, 0, s, a)
+  if (a.n_expert <= 64) { ROUTE(1); }
+  else if (a.n_expert <= 128) { ROUTE(2); }
+  else if (a.n_expert <= 256) { ROUTE(4); }
+  else if (a.n_expert <= 512) { ROUTE(8); }
+  else { ROUTE(16); }
+#undef ROUTE
+}
+hipError_t launch_moe_route(const RouteArgs &a, int type, hipStream_t s) {
+#define CALL(R) route<R>(a, false, s)
+  MOE_BY_TYPE(type, CALL)
+#undef CALL
+  return hipGetLastError();
+}
+hipError_t launch_moe_route_grad(const RouteArgs &a, int type, hipStream_t s) {
+#define CALL(R) route<R>(a, true, s)
+  MOE_BY_TYPE(type, CALL)
+#undef CALL
+  return hipGetLastError();
+}
+
+// ------------------------------------------------------------------ sorting by expert
+// A counting sort that keeps the order of equal ones. A workgroup has a run of entries, each of its waves
+// a run of those; entries of no expert are those of a last, (n_expert + 1)-th bucket. An entry's place is its
+// bucket's start, plus the bucket's entries in earlier workgroups, in the workgroup's earlier waves, earlier in the
+// wave's run and at lower lanes. Counts are sums of integers: no order of additions changes them.
+constexpr int SORT_T = 512, SORT_W = SORT_T / 64;
+constexpr int SORT_ALONE = 4096;  // so many entries are one workgroup's
+
+static int sort_run(int64_t n) {  // a workgroup's entries
+  if (n <= SORT_ALONE) return SORT_ALONE;
+  const int64_t per = ((n + 255) / 256 + SORT_T - 1) / SORT_T * SORT_T;
+  return (int)(per < 2 * SORT_T ? 2 * SORT_T : per);
+}
+int moe_sort_blocks(int64_t n) { return (int)((n + sort_run(n) - 1) / sort_run(n)); }
+
+__device__ __forceinline__ int bucket_of(const SortArgs &a, int i) {
+  const int e = a.chosen[i];
+  return e >= 0 && e < a.n_expert ? e : a.n_expert;
+}
+
+__global__ __launch_bounds__(SORT_T) void k_moe_count(const SortArgs a, int run) {
+  __shared__ int count[MOE_MAX_E + 1];
+  const int nb = a.n_expert + 1;
+  for (int e = threadIdx.x; e < nb; e += SORT_T) count[e] = 0;
+  __syncthreads();
+  const int begin = blockIdx.x * run, end = min(begin + run, a.n);
+  for (int i = begin + threadIdx.x; i < end; i += SORT_T) atomicAdd(&count[bucket_of(a, i)], 1);
+  __syncthreads();
+  for (int e = threadIdx.x; e < nb; e += SORT_T) a.counts[(int64_t)blockIdx.x * nb + e] = count[e];
+}
+
+__global__ __launch_bounds__(SORT_T) void k_moe_place(const SortArgs a, int run) {
+  extern __shared__ int at[];  // [SORT_W][n_expert + 1]: counts, then the next place of each bucket
+  __shared__ int up[SORT_W];
+  const int t = threadIdx.x, wave = t >> 6, lane = t & 63, nb = a.n_expert + 1;
+  for (int i = t; i < SORT_W * nb; i += SORT_T) at[i] = 0;
+  __syncthreads();
+  const int begin = blockIdx.x * run + wave * (run / SORT_W), end = min(begin + run / SORT_W, a.n);
+  int *mine = at + wave * nb;
+  for (int i = begin + lane; i < end; i += 64) atomicAdd(&mine[bucket_of(a, i)], 1);
+  __syncthreads();
+  int carry = 0;
+  for (int b = 0; b < nb; b += SORT_T) {  // a thread a bucket
+    const int e = b + t;
+    int before = 0, all = 0;
+    if (e < nb) {
+      if (gridDim.x == 1) {
+        for (int w = 0; w < SORT_W; w++) all += at[w * nb + e];
+      } else {
+        for (int g = 0; g < (int)gridDim.x; g++) {
+          const int c = a.counts[(int64_t)g * nb + e];
+          all += c;
+          before += g < (int)blockIdx.x ? c : 0;
+        }
+      }
+    }
+    const int sum = wave_scan(all);
+    if (lane == 63) up[wave] = sum;
+    __syncthreads();
+    int start = carry + sum - all;
+    for (int w = 0; w < SORT_W; w++) {
+      if (w < wave) start += up[w];
+      carry += up[w];
+    }
+    if (e < nb) {
+      if (blockIdx.x == 0) a.starts[e] = start;  // (the last bucket's: where the entries of experts end)
+      int next = start + before;
+      for (int w = 0; w < SORT_W; w++) {
+        const int c = at[w * nb + e];
+        at[w * nb + e] = next;
+        next += c;
+      }
+    }
+    __syncthreads();
+  }
+  const int bits = 32 - __builtin_clz(nb - 1);
+  for (int i = begin + lane; i - lane < end; i += 64) {
+    const bool in = i < end;
+    const int e = in ? bucket_of(a, i) : 0;
+    unsigned long long same = __builtin_amdgcn_ballot_w64(in);
+    for (int b = 0; b < bits; b++) {
+      const unsigned long long set = __builtin_amdgcn_ballot_w64((e >> b & 1) != 0);
+      same &= e >> b & 1 ? set : ~set;
+    }
+    const unsigned long long lower = same & ((1ull << lane) - 1ull);
+    const int p = in ? mine[e] + __builtin_popcountll(lower) : 0;
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    if (in && (same >> lane) == 1ull) mine[e] = p + 1;  // the last of them
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    if (in) {
+      const bool none = e == a.n_expert;
+      a.order[p] = none ? -1 : i;
+      a.place[i] = none ? -1 : p;
+    }
+  }
+}
+
+hipError_t launch_moe_sort(const SortArgs &a, hipStream_t s) {
+  const int run = sort_run(a.n), blocks = a.n > 0 ? moe_sort_blocks(a.n) : 1;
+  if (blocks > 1) hipLaunchKernelGGL(k_moe_count, dim3(blocks), dim3(SORT_T), 0, s, a, run);
+  hipLaunchKernelGGL(k_moe_place, dim3(blocks), dim3(SORT_T), SORT_W * (a.n_expert + 1) * sizeof(int), s, a, run);
+  return hipGetLastError();
+}
+
+// ------------------------------------------------------------------ rows there and back
+// A power of two of threads has a row, each piece of it 16 bytes (VEC: all rows lie at multiples of 16 bytes
+// and are as long) or one element.
+template <class R, bool VEC>
+struct RowPiece {
+  typedef typename R::E E;
+  static constexpr int N = VEC ? 16 / (int)sizeof(E) : 1;
+  static __device__ __forceinline__ void get(const E *p, float (&x)[N]) {
+    alignas(16) E e[N];
+    if constexpr (VEC) *(uint4 *)e = *(const uint4 *)p;
+    else e[0] = *p;
+#pragma unroll
+    for (int i = 0; i < N; i++) x[i] = row_get(R{}, e[i]);
+  }
+  static __device__ __forceinline__ void put(E *p, const float (&x)[N]) {
+    alignas(16) E e[N];
+#pragma unroll
+    for (int i = 0; i < N; i++) e[i] = row_put(R{}, x[i]);
+    if constexpr (VEC) *(uint4 *)p = *(const uint4 *)e;
+    else *p = e[0];
+  }
+};
+
+template <class R, bool VEC>
+__global__ __launch_bounds__(256) void k_moe_gather(const JoinArgs a, int log_t) {
+  typedef RowPiece<R, VEC> P;
+  typedef typename R::E E;
+  const int i = blockIdx.x * (256 >> log_t) + (threadIdx.x >> log_t), t = threadIdx.x & ((1 << log_t) - 1);
+  const int n = a.rows * a.k;
+  if (i >= n) return;
+  const int entry = a.order[i];
+  const bool is = entry >= 0 && entry < n;
+  const E *src = (const E *)a.x + (int64_t)(is ? entry / a.k : 0) * a.ld_x;
+  E *dst = (E *)a.out + (int64_t)i * a.ld_out;
+  const float w = a.weights && is ? a.weights[entry] : 1.0f;
+  for (int c = t; c < a.width / P::N; c += 1 << log_t) {
+    float x[P::N] = {};
+    if (is) P::get(src + c * P::N, x);
+    if (a.weights)
+#pragma unroll
+      for (int j = 0; j < P::N; j++) x[j] *= w;
+    if (!is)
+#pragma unroll
+      for (int j = 0; j < P::N; j++) x[j] = 0.0f;
+    P::put(dst + c * P::N, x);
+  }
+}
+
+template <class R, bool VEC>
+__global__ __launch_bounds__(256) void k_moe_combine(const JoinArgs a, int log_t) {
+  typedef RowPiece<R, VEC> P;
+  typedef typename R::E E;
+  const int r = blockIdx.x * (256 >> log_t) + (threadIdx.x >> log_t), t = threadIdx.x & ((1 << log_t) - 1);
+  if (r >= a.rows) return;
+  const int n = a.rows * a.k;
+  for (int c = t; c < a.width / P::N; c += 1 << log_t) {
+    float sum[P::N] = {};
+#pragma unroll 4
+    for (int j = 0; j < a.k; j++) {
+      const int p = a.place[(int64_t)r * a.k + j];
+      const bool is = p >= 0 && p < n;
+      const float w = a.weights ? a.weights[(int64_t)r * a.k + j] : 1.0f;
+      float x[P::N];
+      P::get((const E *)a.x + (is ? p : 0) * a.ld_x + c * P::N, x);
+#pragma unroll
+      for (int i = 0; i < P::N; i++) sum[i] = is ? fmaf(w, x[i], sum[i]) : sum[i];
+    }
+    P::put((E *)a.out + (int64_t)r * a.ld_out + c * P::N, sum);
+  }
+}
+
+// A wave has an entry: its row's d_out against its sorted row of y.
+template <class R, bool VEC>
+__global__ __launch_bounds__(256) void k_moe_combine_grad(const JoinArgs a) {
+  typedef RowPiece<R, VEC> P;
+  typedef typename R::E E;
+  const int entry = blockIdx.x * 4 + (threadIdx.x >> 6), t = threadIdx.x & 63, n = a.rows * a.k;
+  if (entry >= n) return;
+  const int p = a.place[entry];
+  const bool is = p >= 0 && p < n;
+  float dot = 0.0f;
+  if (is) {
+    const float w = a.weights[entry];
+    const E *d = (const E *)a.d + (int64_t)(entry / a.k) * a.ld_d, *y = (const E *)a.x + (int64_t)p * a.ld_x;
+    E *out = (E *)a.out + (int64_t)p * a.ld_out;
+    for (int c = t; c < a.width / P::N; c += 64) {
+      float u[P::N], v[P::N];
+      P::get(d + c * P::N, u);
+      P::get(y + c * P::N, v);
+#pragma unroll
+      for (int i = 0; i < P::N; i++) {
+        dot = fmaf(u[i], v[i], dot);
+        u[i] *= w;
+      }
+      P::put(out + c * P::N, u);
+    }
+  }
+  dot = wave_sum(dot);
+  if (t == 0) a.d_weights[entry] = dot;
+  const int none = a.order[entry];  // (as a place)
+  if (none < 0 || none >= n) {
+    E *out = (E *)a.out + (int64_t)entry * a.ld_out;
+    const float zero[P::N] = {};
+    for (int c = t; c < a.width / P::N; c += 64) P::put(out + c * P::N, zero);
+  }
+}
+
+// Whether rows at p, ld apart, lie at multiples of 16 bytes.
+static bool on16(const void *p, int64_t ld, int size) { return (uintptr_t)p % 16 == 0 && ld * size % 16 == 0; }
+
+template <class R>
+static void join(const JoinArgs &a, int what, hipStream_t s) {
+  constexpr int size = sizeof(typename R::E);
+  const bool vec = a.width * size % 16 == 0 && on16(a.x, a.ld_x, size) && on16(a.out, a.ld_out, size) && (what != 2 || on16(a.d, a.ld_d, size));
+  const int pieces = vec ? a.width * size / 16 : a.width;
+  int log_t = 0;
+  while (log_t < 8 && (1 << log_t) < pieces) log_t++;
+  const int rows = what == 0 ? a.rows * a.k : a.rows, each = 256 >> log_t;
+  const dim3 grid((unsigned)((rows + each - 1) / each)), block(256);
+  if (what == 0) {
+    if (vec) hipLaunchKernelGGL((k_moe_gather<R, true>), grid, block, 0, s, a, log_t);
+    else hipLaunchKernelGGL((k_moe_gather<R, false>), grid, block, 0, s, a, log_t);
+  } else if (what == 1) {
+    if (vec) hipLaunchKernelGGL((k_moe_combine<R, true>), grid, block, 0, s, a, log_t);
+    else hipLaunchKernelGGL((k_moe_combine<R, false>), grid, block, 0, s, a, log_t);
+  } else {
+    const dim3 waves((unsigned)((a.rows * a.k + 3) / 4));
+    if (vec) hipLaunchKernelGGL((k_moe_combine_grad<R, true>), waves, block, 0, s, a);
+    else hipLaunchKernelGGL((k_moe_combine_grad<R, false>), waves, block, 0, s, a);
+  }
+}
+static hipError_t launch_join(const JoinArgs &a, int type, int what, hipStream_t s) {
+#define CALL(R) join<R>(a, what, s)
+  MOE_BY_TYPE(type, CALL)
+#undef CALL
+  return hipGetLastError();
+}
+hipError_t launch_moe_gather(const JoinArgs &a, int type, hipStream_t s) { return launch_join(a, type, 0, s); }
+hipError_t launch_moe_combine(const JoinArgs &a, int type, hipStream_t s) { return launch_join(a, type, 1, s); }
+hipError_t launch_moe_combine_grad(const JoinArgs &a, int type, hipStream_t s) { return launch_join(a, type, 2, s); }
+
+}  // namespace spx

@@ -1,0 +1,358 @@
+// Matrices in microscaled 4-bit floats: rows in (spx_mx4_quantize), values out (spx_mx4_read) and products
+// (spx_mx4_matmul). include/spx.h states the format and its layout.
+//
+// The layout is the matrix cores': an instruction's 128 columns of a row are 64 bytes of codes and four scale
+// bytes, of which lane group g of a wave takes the g-th 16 bytes and the g-th scale, one block of 32.
+#include "dev.h"
+#include "experts.h"
+#include "rows.h"
+
+namespace spx {
+
+typedef int i8v __attribute__((ext_vector_type(8)));
+typedef __bf16 b2v __attribute__((ext_vector_type(2)));
+typedef __bf16 b8v __attribute__((ext_vector_type(8)));
+
+// ------------------------------------------------------------------ rows in and out
+// A thread has eight columns, the four threads of a quad a block, sixteen threads a step of 128 columns.
+struct Eight {
+  int row, c8;  // columns 8 c8 ..
+};
+__device__ __forceinline__ Eight eight_of(const Mx4Rows &a, int log_t, int &step) {
+  step = 1 << log_t;
+  return {(int)((blockIdx.x + blockIdx.y * gridDim.x) * (256 >> log_t) + (threadIdx.x >> log_t)), (int)(threadIdx.x & ((1 << log_t) - 1))};
+}
+
+// Magnitudes order as integers, NaN above all. With u the largest one's bits, floor(log2) - 2 + 127 is u >> 23 less
+// 2, at least 0 (what is below the normal numbers included).
+template <class R, bool VEC>
+__global__ __launch_bounds__(256) void k_mx4_quantize(const Mx4Rows a, int log_t) {
+  typedef typename R::E E;
+  int step;
+  const Eight p = eight_of(a, log_t, step);
+  if ((uint32_t)p.row >= (uint32_t)a.rows) return;
+  const E *src = (const E *)a.x + (int64_t)p.row * a.ld_x;
+  for (int c = p.c8; c < a.steps * 16; c += step) {  // (threads of a step of columns stay together)
+    float x[8];
+    if (c * 8 + 8 <= a.cols) get8<R, VEC>(src + c * 8, x);
+    else
+#pragma unroll
+      for (int j = 0; j < 8; j++) x[j] = c * 8 + j < a.cols ? row_get(R{}, src[c * 8 + j]) : 0.0f;
+    uint32_t m = 0;
+#pragma unroll
+    for (int j = 0; j < 8; j++) m = max(m, __float_as_uint(x[j]) & 0x7fffffffu);
+    m = max(m, (uint32_t)__builtin_amdgcn_mov_dpp((int)m, 0xB1, 0xF, 0xF, true));
+    m = max(m, (uint32_t)__builtin_amdgcn_mov_dpp((int)m, 0x4E, 0xF, 0xF, true));
+    const bool bad = m >= 0x7f800000u;
+    const uint32_t e = m >> 23, byte = bad ? 255u : e > 2u ? e - 2u : 0u;
+    uint32_t w = 0;
+    if (!bad) {
+      // the conversion rounds value / scale to nearest, ties to the even code, and takes the scale's exponent alone
+      const float scale = __uint_as_float(byte << 23);
+      w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[0], x[1], scale, 0);
+      w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[2], x[3], scale, 1);
+      w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[4], x[5], scale, 2);
+      w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[6], x[7], scale, 3);
+    }
+    *(uint32_t *)(a.m.codes + (int64_t)p.row * (a.steps * 64) + c * 4) = w;
+    // a step's four scales as one word: each quad's byte at its place, joined across the sixteen lanes
+    uint32_t s = byte << (8 * (c >> 2 & 3));
+    s |= (uint32_t)__builtin_amdgcn_mov_dpp((int)s, 0x124, 0xF, 0xF, true);
+    s |= (uint32_t)__builtin_amdgcn_mov_dpp((int)s, 0x128, 0xF, 0xF, true);
+    if ((c & 15) == 0) *(uint32_t *)(a.m.scales + (int64_t)p.row * (a.steps * 4) + (c >> 2)) = s;
+  }
+}
+
+template <class R, bool VEC>
+__global__ __launch_bounds__(256) void k_mx4_read(const Mx4Rows a, int log_t) {
+  typedef typename R::E E;
+  int step;
+  const Eight p = eight_of(a, log_t, step);
+  if ((uint32_t)p.row >= (uint32_t)a.rows) return;
+  E *dst = (E *)a.x + (int64_t)p.row * a.ld_x;
+  for (int c = p.c8; c * 8 < a.cols; c += step) {
+    const uint32_t w = *(const uint32_t *)(a.m.codes + (int64_t)p.row * (a.steps * 64) + c * 4);
+    const float scale = __uint_as_float((uint32_t)a.m.scales[(int64_t)p.row * (a.steps * 4) + (c >> 2)] << 23);
+    f2v v[4];
+    v[0] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, scale, 0);
+    v[1] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, scale, 1);
+    v[2] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, scale, 2);
+    v[3] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, scale, 3);
+    const float x[8] = {v[0].x, v[0].y, v[1].x, v[1].y, v[2].x, v[2].y, v[3].x, v[3].y};
+    if (c * 8 + 8 <= a.cols) put8<R, VEC>(dst + c * 8, x);
+    else
+      for (int j = 0; c * 8 + j < a.cols; j++) dst[c * 8 + j] = row_put(R{}, x[j]);
+  }
+}
+
+// Whether rows at p, ld apart, lie at multiples of 16 bytes.
+static bool on16(const void *p, int64_t ld, int64_t size) { return (uintptr_t)p % 16 == 0 && ld * size % 16 == 0; }
+
+template <class R>
+static void rows_in_out(const Mx4Rows &a, bool in, hipStream_t s) {
+  const bool vec = on16(a.x, a.ld_x, sizeof(typename R::E));
+  int log_t = 4;
+  while (log_t < 8 && (1 << log_t) < a.steps * 16) log_t++;
+  const int each = 256 >> log_t;
+  const int64_t blocks = ((int64_t)a.rows + each - 1) / each, wide = blocks < 1 << 20 ? blocks : 1 << 20;
+  const dim3 grid((unsigned)wide, (unsigned)((blocks + wide - 1) / wide)), block(256);
+  if (in) {
+    if (vec) hipLaunchKernelGGL((k_mx4_quantize<R, true>), grid, block, 0, s, a, log_t);
+    else hipLaunchKernelGGL((k_mx4_quantize<R, false>), grid, block, 0, s, a, log_t);
+  } else {
+    if (vec) hipLaunchKernelGGL((k_mx4_read<R, true>), grid, block, 0, s, a, log_t);
+    else hipLaunchKernelGGL((k_mx4_read<R, false>), grid, block, 0, s, a, log_t);
+  }
+}
+#define MX4_BY_TYPE(type, CALL)               \
+  switch (type) {                             \
+  case T_F32: { CALL(RowF32); break; }        \
+  case T_F16: { CALL(RowF16); break; }        \
+  case T_BF16: { CALL(RowBF16); break; }      \
+  default: return hipErrorInvalidValue;       \
+  }
+hipError_t launch_mx4_quantize(const Mx4Rows &a, int type, hipStream_t s) {
+#define CALL(R) rows_in_out<R>(a, true, s)
+  MX4_BY_TYPE(type, CALL)
+#undef CALL
+  return hipGetLastError();
+}
+hipError_t launch_mx4_read(const Mx4Rows &a, int type, hipStream_t s) {
+#define CALL(R) rows_in_out<R>(a, false, s)
+  MX4_BY_TYPE(type, CALL)
+#undef CALL
+  return hipGetLastError();
+}
+
+// ------------------------------------------------------------------ products
+// Kinds of x: 4-bit, or 16- and 32-bit rows as bf16 parts whose sum is the value (bf16 one, f16 two, fp32 three).
+struct XMx4 { typedef RowF32 R; static constexpr int PARTS = 0; };
+struct XBF16 { typedef RowBF16 R; static constexpr int PARTS = 1; };
+struct XF16 { typedef RowF16 R; static constexpr int PARTS = 2; };
+struct XF32 { typedef RowF32 R; static constexpr int PARTS = 3; };
+
+// The rows of a tile: which expert's, where they start, how many (0: there is no such tile).
+struct Tile { int expert, row, count; };
+// The t-th tile of `most` rows: without starts of all rows, with them expert by expert (each one's last may be part
+// filled). Every lane of a wave gets it.
+__device__ __forceinline__ Tile tile_of(const Mx4Product &a, int t, int most) {
+  if (!a.starts) {
+    const int r = t * most;
+    return {0, r, r < a.rows ? min(most, a.rows - r) : 0};
+  }
+  const int lane = threadIdx.x & 63;
+  int before = 0;
+  for (int b = 0; b < a.n_expert; b += 64) {
+    const int e = b + lane;
+    int lo = 0, hi = 0;
+    if (e < a.n_expert) {
+      lo = min(max(a.starts[e], 0), a.rows);
+      hi = min(max(a.starts[e + 1], lo), a.rows);
+    }
+    const int tiles = (hi - lo + most - 1) / most, upto = before + wave_scan(tiles);
+    const unsigned long long past = __builtin_amdgcn_ballot_w64(upto > t);
+    if (past) {
+      const int l = (int)__builtin_ctzll(past), r = lane_i(lo, l) + (t - (lane_i(upto, l) - lane_i(tiles, l))) * most;
+      return {b + l, r, min(most, lane_i(hi, l) - r)};
+    }
+    before = lane_i(upto, 63);
+  }
+  return {0, 0, 0};
+}
+// Tiles of `most` rows that there may be.
+static int64_t tiles_most(const Mx4Product &a, int most) {
+  if (!a.starts) return ((int64_t)a.rows + most - 1) / most;
+  const int64_t t = (int64_t)a.rows / most + a.n_expert;
+  return t < a.rows ? t : a.rows;
+}
+
+// Row i's row of x, -1: none.
+__device__ __forceinline__ int source_of(const Mx4Product &a, int i) {
+  int r = i;
+  if (a.order) {
+    const int entry = a.order[i];
+    r = entry >= 0 ? entry / a.k : -1;
+  }
+  return r < a.x_rows ? r : -1;
+}
+
+// Eight columns of a row of x from column c on, zeros behind the last.
+template <class R>
+__device__ __forceinline__ void x8(const Mx4Product &a, const typename R::E *row, int c, bool vec, float *x) {
+  if (c + 8 <= a.cols) get8_if<R>(vec, row + c, x);
+  else
+#pragma unroll
+    for (int j = 0; j < 8; j++) x[j] = c + j < a.cols ? row_get(R{}, row[c + j]) : 0.0f;
+}
+// A value as bf16 parts, each the upper half of what is left: 8 bits a part, and what is taken off is exact. An infinity
+// or a NaN is its first part.
+template <int P>
+__device__ __forceinline__ void parts_of(const float *x, b8v (&part)[P]) {
+  uint32_t u[P][8];
+#pragma unroll
+  for (int j = 0; j < 8; j++) {
+    float r = x[j];
+    if (P == 3 && isnan(r)) r = __builtin_nanf("");  // (its upper half might be infinity's)
+#pragma unroll
+    for (int p = 0; p < P; p++) {
+      u[p][j] = __float_as_uint(r);
+      if (p + 1 < P) {
+        const float rest = r - __uint_as_float(u[p][j] & 0xffff0000u);
+        r = (u[p][j] & 0x7f800000u) == 0x7f800000u ? 0.0f : rest;
+      }
+    }
+  }
+#pragma unroll
+  for (int p = 0; p < P; p++) {
+    i4v w;
+#pragma unroll
+    for (int j = 0; j < 4; j++) w[j] = (int)__builtin_amdgcn_perm(u[p][2 * j + 1], u[p][2 * j], 0x07060302u);
+    part[p] = __builtin_bit_cast(b8v, w);
+  }
+}
+// Eight codes as values in bf16, which holds them exactly.
+__device__ __forceinline__ b8v values_of(uint32_t w, float scale) {
+  b2v v[4];
+  v[0] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 0);
+  v[1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 1);
+  v[2] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 2);
+  v[3] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 3);
+  b8v r;
+#pragma unroll
+  for (int j = 0; j < 4; j++) { r[2 * j] = v[j][0]; r[2 * j + 1] = v[j][1]; }
+  return r;
+}
+__device__ __forceinline__ f4v mfma_mx4(i4v w, int ws, i4v x, int xs, f4v acc) {
+  const i8v A = {w[0], w[1], w[2], w[3], 0, 0, 0, 0}, B = {x[0], x[1], x[2], x[3], 0, 0, 0, 0};
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(A, B, acc, 4, 4, 0, ws, 0, xs);
+}
+
+__device__ __forceinline__ float silu(float v) { return v / (1.0f + expf(-v)); }
+
+struct Vecs { int x, out; };  // rows of x lie at multiples of 16 bytes, of out at multiples of four elements
+
+// Four neighbours of a row of out.
+template <int T>
+__device__ __forceinline__ void put4(const Mx4Product &a, int i, int c, f4v v, bool vec) {
+  typedef typename std::conditional<T == T_F32, RowF32, typename std::conditional<T == T_F16, RowF16, RowBF16>::type>::type R;
+  typedef typename R::E E;
+  E *dst = (E *)a.out + (int64_t)i * a.ld_out + c;
+  if (c + 4 <= a.n) {
+    const float x[4] = {v[0], v[1], v[2], v[3]};
+    put_if<R, 4>(vec, dst, x);
+  } else {
+    for (int j = 0; c + j < a.n; j++) dst[j] = row_put(R{}, v[j]);
+  }
+}
+__device__ __forceinline__ void put4_by(const Mx4Product &a, int out_type, int i, int c, f4v v, bool vec) {
+  if (out_type == T_F32) put4<T_F32>(a, i, c, v, vec);
+  else if (out_type == T_F16) put4<T_F16>(a, i, c, v, vec);
+  else put4<T_BF16>(a, i, c, v, vec);
+}
+
+// Sixteen rows of x against 16 RT rows of the matrix (and of up): W X^T, a lane's four sums being four neighbours of
+// one row of out. The workgroup's four waves take the steps of 128 columns in turn and are joined at the end.
+template <class X, int RT, bool GATED>
+__global__ __launch_bounds__(256) void k_mx4_rows(const Mx4Product a, const Vecs vec, int out_type) {
+  constexpr int P = X::PARTS, H = GATED ? 2 : 1;
+  typedef typename X::R R;
+  typedef typename R::E E;
+  __shared__ f4v sums[4][RT * H][64];
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
+  const Tile tile = tile_of(a, blockIdx.y + blockIdx.z * gridDim.y, 16);
+  if (tile.count <= 0) return;
+  const int i = tile.row + m, src = m < tile.count ? source_of(a, i) : -1, n0 = blockIdx.x * (16 * RT);
+  const uint8_t *wc[H][RT], *wsc[H][RT];
+#pragma unroll
+  for (int h = 0; h < H; h++)
+#pragma unroll
+    for (int t = 0; t < RT; t++) {
+      const int64_t row = (int64_t)tile.expert * a.n + min(n0 + 16 * t + m, a.n - 1);
+      const Mx4 w = h ? a.up : a.w;
+      wc[h][t] = w.codes + row * (a.steps * 64) + g * 16;
+      wsc[h][t] = w.scales + row * (a.steps * 4) + g;
+    }
+  f4v acc[H][RT] = {};
+  for (int s = wave; s < a.steps; s += 4) {
+    i4v w[H][RT];
+    int ws[H][RT];
+#pragma unroll
+    for (int h = 0; h < H; h++)
+#pragma unroll
+      for (int t = 0; t < RT; t++) {
+        w[h][t] = *(const i4v *)(wc[h][t] + s * 64);
+        ws[h][t] = wsc[h][t][s * 4];
+      }
+    if constexpr (P == 0) {
+      i4v x = {};
+      int xs = 0;
+      if (src >= 0) {
+        x = *(const i4v *)((const uint8_t *)a.x + (int64_t)src * (a.steps * 64) + s * 64 + g * 16);
+        xs = a.x_scales[(int64_t)src * (a.steps * 4) + s * 4 + g];
+      }
+#pragma unroll
+      for (int h = 0; h < H; h++)
+#pragma unroll
+        for (int t = 0; t < RT; t++) acc[h][t] = mfma_mx4(w[h][t], ws[h][t], x, xs, acc[h][t]);
+    } else {
+#pragma unroll
+      for (int c = 0; c < 4; c++) {
+        float x[8] = {};
+        if (src >= 0) x8<R>(a, (const E *)a.x + (int64_t)src * a.ld_x, s * 128 + g * 32 + c * 8, vec.x, x);
+        b8v part[P < 1 ? 1 : P];
+        parts_of(x, part);
+#pragma unroll
+        for (int h = 0; h < H; h++)
+#pragma unroll
+          for (int t = 0; t < RT; t++) {
+            const b8v v = values_of((uint32_t)w[h][t][c], __uint_as_float((uint32_t)ws[h][t] << 23));
+#pragma unroll
+            for (int p = P - 1; p >= 0; p--) acc[h][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, part[p], acc[h][t], 0, 0, 0);
+          }
+      }
+    }
+  }
+#pragma unroll
+  for (int h = 0; h < H; h++)
+#pragma unroll
+    for (int t = 0; t < RT; t++) sums[wave][h * RT + t][lane] = acc[h][t];
+  __syncthreads();
+  if (src < 0) return;
+  for (int t = wave; t < RT; t += 4) {
+    f4v v[H];
+#pragma unroll
+    for (int h = 0; h < H; h++) v[h] = (sums[0][h * RT + t][lane] + sums[1][h * RT + t][lane]) + (sums[2][h * RT + t][lane] + sums[3][h * RT + t][lane]);
+    if (GATED)
+#pragma unroll
+      for (int j = 0; j < 4; j++) v[0][j] = silu(v[0][j]) * v[H - 1][j];
+    if (n0 + 16 * t + 4 * g < a.n) put4_by(a, out_type, i, n0 + 16 * t + 4 * g, v[0], vec.out);
+  }
+}
+
+// Tiles over the launch's second and third dimension.
+static dim3 tile_grid(int64_t columns, int64_t tiles) {
+  const int64_t y = tiles < 32768 ? tiles : 32768;
+  return dim3((unsigned)columns, (unsigned)y, (unsigned)((tiles + y - 1) / y));
+}
+
+template <class X>
+static hipError_t product(const Mx4Product &a, int out_type, hipStream_t s) {
+  constexpr int RT = 2;
+  const Vecs vec = {X::PARTS == 0 || on16(a.x, a.ld_x, sizeof(typename X::R::E)),
+                    (uintptr_t)a.out % (out_type == T_F32 ? 16 : 8) == 0 && a.ld_out % 4 == 0};
+  const dim3 grid = tile_grid((a.n + 16 * RT - 1) / (16 * RT), tiles_most(a, 16));
+  if (a.up.codes) hipLaunchKernelGGL((k_mx4_rows<X, RT, true>), grid, dim3(256), 0, s, a, vec, out_type);
+  else hipLaunchKernelGGL((k_mx4_rows<X, RT, false>), grid, dim3(256), 0, s, a, vec, out_type);
+  return hipGetLastError();
+}
+hipError_t launch_mx4_matmul(const Mx4Product &a, int type, int out_type, hipStream_t s) {
+  switch (type) {
+  case SPX_MX4: return product<XMx4>(a, out_type, s);
+  case T_F32: return product<XF32>(a, out_type, s);
+  case T_F16: return product<XF16>(a, out_type, s);
+  case T_BF16: return product<XBF16>(a, out_type, s);
+  }
+  return hipErrorInvalidValue;
+}
+
+}  // namespace spx

@@ -371,6 +371,202 @@ def logprobs(ctx, logits, targets=None, top=0, logit_scale=1.0, ws=None):
     return r
 
 
+# ------------------------------------------------------------------ experts over a batch
+# A step of a mixture of experts over a batch's rows: moe_route, moe_sort, mx4_matmul over the sorted rows
+# (gated, then down), moe_combine. As above: on the context's stream in order with torch's, nothing waits on
+# the host, everything can be captured.
+def _rows2(t, name, width=None):
+    """The distance between the rows of a [rows, width] tensor whose rows are dense."""
+    if t.dim() != 2 or (width is not None and t.shape[1] != width) or (t.stride(1) != 1 and t.shape[1] > 1):
+        raise ValueError(f"{name}: expected [rows, {'width' if width is None else width}] with dense rows, got {tuple(t.shape)}, strides {t.stride()}")
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def _f32(t, shape, name):
+    """The address of a dense float32 tensor of this shape."""
+    if t.dtype is not torch.float32 or tuple(t.shape) != tuple(shape) or not t.is_contiguous():
+        raise ValueError(f"{name}: expected a contiguous float32 tensor {tuple(shape)}, got {t.dtype} {tuple(t.shape)}")
+    return t.data_ptr()
+
+
+def _out2(out, like, rows, width, dtype, name="out"):
+    """(a call's output [rows, width], the distance between its rows): the caller's, or a new one."""
+    if out is None:
+        return like.new_empty((rows, width), dtype=dtype), width
+    if out.dtype is not dtype or out.shape[0] != rows:
+        raise ValueError(f"{name} must be [{rows}, {width}] of {dtype}, got {tuple(out.shape)} of {out.dtype}")
+    return out, _rows2(out, name, width)
+
+
+def moe_route(ctx, logits, k, norm=True):
+    """(chosen [rows, k] int32, weights [rows, k] float32): the k experts of each row of router logits [rows,
+    n_expert] and their softmax weights, over the chosen ones (norm) or over all (spx_moe_route)."""
+    t, ld = _row_type(logits.dtype), _rows2(logits, "logits")
+    rows, n = logits.shape
+    if (rows | n | k) >> 31:
+        raise _not_c_ints("k and the logits' sizes")
+    chosen, weights = logits.new_empty((rows, k), dtype=torch.int32), logits.new_empty((rows, k), dtype=torch.float32)
+    _run(ctx, (logits,), lib.spx_moe_route, t, logits.data_ptr(), ld, rows, n, k, 1 if norm else 0, chosen.data_ptr(), weights.data_ptr())
+    return chosen, weights
+
+
+def moe_route_grad(ctx, logits, chosen, d_weights, norm=True):
+    """The logits' gradient from that of moe_route's weights, its ids held fixed (spx_moe_route_grad)."""
+    t, ld = _row_type(logits.dtype), _rows2(logits, "logits")
+    rows, n = logits.shape
+    k = chosen.shape[1] if chosen.dim() == 2 else 0
+    if (rows | n | k) >> 31:
+        raise _not_c_ints("the tensors' sizes")
+    ids, g = _i32(chosen, rows, k), _f32(d_weights, (rows, k), "d_weights")
+    d = logits.new_empty((rows, n))
+    _run(ctx, (logits, chosen, d_weights), lib.spx_moe_route_grad, t, logits.data_ptr(), ld, rows, n, k, 1 if norm else 0, ids, g, d.data_ptr(), n)
+    return d
+
+
+class MoeOrder:
+    """What moe_sort leaves: starts [n_expert + 1], order [rows * k], place [rows, k] (int32)."""
+    __slots__ = ("starts", "order", "place")
+
+
+def moe_sort(ctx, chosen, n_expert, ws=None):
+    """The entries of chosen [rows, k] (int32) in order of their expert (spx_moe_sort); ids outside
+    0..n_expert - 1 belong to no expert here. ws as in kv4_attention."""
+    rows, k = chosen.shape if chosen.dim() == 2 else (0, 0)
+    if (rows | k | n_expert) >> 31:
+        raise _not_c_ints("n_expert and chosen's sizes")
+    ids = _i32(chosen, rows, k)
+    o = MoeOrder()
+    buf = chosen.new_empty(2 * rows * k + n_expert + 1)
+    order, place, o.starts = buf.split_with_sizes((rows * k, rows * k, n_expert + 1))
+    o.order, o.place = order, place.view(rows, k)
+    scratch, size, ws = _scratch(lib.spx_moe_sort_ws(rows, k, n_expert), ws, chosen)
+    at = buf.data_ptr()  # (the parts in this order)
+    _run(ctx, (chosen, ws), lib.spx_moe_sort, rows, k, n_expert, ids, at + 8 * rows * k, at, at + 4 * rows * k, scratch, size)
+    return o
+
+
+def moe_gather(ctx, x, order, k, weights=None, out=None):
+    """Rows x [rows, width] in sorted order [rows * k, width], times weights [rows, k] where given
+    (spx_moe_gather). Its gradient is moe_combine with the order's place and the same weights."""
+    t, ld = _row_type(x.dtype), _rows2(x, "x")
+    rows, width = x.shape
+    if (rows | width | k | rows * k) >> 31:
+        raise _not_c_ints("k and the tensors' sizes")
+    o, w = _i32(order, rows * k), None if weights is None else _f32(weights, (rows, k), "weights")
+    out, ld_out = _out2(out, x, rows * k, width, x.dtype)
+    _run(ctx, (x, order, x if weights is None else weights, out), lib.spx_moe_gather, t, x.data_ptr(), ld, rows, k, width, o, w, out.data_ptr(), ld_out)
+    return out
+
+
+def moe_combine(ctx, y, place, weights=None, out=None):
+    """Sorted rows y [rows * k, width] joined into [rows, width]: the sum over place [rows, k], times weights
+    [rows, k] where given (spx_moe_combine)."""
+    t, ld = _row_type(y.dtype), _rows2(y, "y")
+    rows, k = place.shape if place.dim() == 2 else (0, 0)
+    width = y.shape[1]
+    if (rows | width | k | rows * k) >> 31:
+        raise _not_c_ints("the tensors' sizes")
+    if y.shape[0] != rows * k:
+        raise ValueError(f"y must have a row for each entry of place ({rows * k}), got {y.shape[0]}")
+    p, w = _i32(place, rows, k), None if weights is None else _f32(weights, (rows, k), "weights")
+    out, ld_out = _out2(out, y, rows, width, y.dtype)
+    _run(ctx, (y, place, y if weights is None else weights, out), lib.spx_moe_combine, t, y.data_ptr(), ld, rows, k, width, p, w, out.data_ptr(), ld_out)
+    return out
+
+
+def moe_combine_grad(ctx, d_out, y, order, place, weights):
+    """(d_y [rows * k, width], d_weights [rows, k]): the gradient of moe_combine(y, place, weights) from
+    d_out [rows, width]; order and place are one moe_sort's (spx_moe_combine_grad)."""
+    t, ld_d, ld_y = _row_type(y.dtype), _rows2(d_out, "d_out"), _rows2(y, "y")
+    rows, width = d_out.shape
+    k = place.shape[1] if place.dim() == 2 else 0
+    if (rows | width | k | rows * k) >> 31:
+        raise _not_c_ints("the tensors' sizes")
+    if d_out.dtype is not y.dtype or tuple(y.shape) != (rows * k, width):
+        raise ValueError(f"y must be [{rows * k}, {width}] of d_out's type, got {tuple(y.shape)} of {y.dtype}")
+    o, p, w = _i32(order, rows * k), _i32(place, rows, k), _f32(weights, (rows, k), "weights")
+    d_y, d_w = y.new_empty((rows * k, width)), y.new_empty((rows, k), dtype=torch.float32)
+    _run(ctx, (d_out, y, order, place, weights), lib.spx_moe_combine_grad, t, d_out.data_ptr(), ld_d, y.data_ptr(), ld_y, rows, k, width, o, p, w,
+         d_y.data_ptr(), width, d_w.data_ptr())
+    return d_y, d_w
+
+
+class _Mx4C(C.Structure):
+    _fields_ = [("data", P), ("rows", C.c_int), ("cols", C.c_int)]
+
+
+class Mx4:
+    """A matrix in microscaled 4-bit floats (spx_mx4): its bytes, a uint8 tensor, and what they hold."""
+    __slots__ = ("data", "rows", "cols", "_c")
+
+    def __init__(self, data, rows, cols):
+        if (rows | cols) >> 31:
+            raise _not_c_ints("rows and cols")
+        need = lib.spx_mx4_bytes(rows, cols)
+        if need <= 0:
+            raise ValueError("a 4-bit matrix has 1 or more rows, and columns in 1..2^20")
+        if data.dtype is not torch.uint8 or not data.is_contiguous() or data.numel() < need:
+            raise ValueError(f"the bytes must be a contiguous uint8 tensor of {need}")
+        self.data, self.rows, self.cols, self._c = data, rows, cols, _Mx4C(data.data_ptr(), rows, cols)
+
+    @staticmethod
+    def nbytes(rows, cols):
+        return lib.spx_mx4_bytes(rows, cols) if not (rows | cols) >> 31 else 0
+
+    @staticmethod
+    def empty(rows, cols, device="cuda"):
+        return Mx4(torch.empty(Mx4.nbytes(rows, cols), dtype=torch.uint8, device=device), rows, cols)
+
+
+def mx4_quantize(ctx, x, out=None):
+    """Rows x [rows, cols] as an Mx4 (spx_mx4_quantize)."""
+    t, ld = _row_type(x.dtype), _rows2(x, "x")
+    if out is None:
+        out = Mx4.empty(*x.shape, device=x.device)
+    elif (out.rows, out.cols) != tuple(x.shape):
+        raise ValueError(f"out must be of {tuple(x.shape)}, got {(out.rows, out.cols)}")
+    _run(ctx, (x, out.data), lib.spx_mx4_quantize, t, x.data_ptr(), ld, C.byref(out._c))
+    return out
+
+
+def mx4_read(ctx, m, dtype=None, out=None):
+    """The values [rows, cols] that an Mx4 stands for (spx_mx4_read)."""
+    dtype = dtype or torch.float32
+    t = _row_type(dtype)
+    out, ld = _out2(out, m.data, m.rows, m.cols, dtype)
+    _run(ctx, (m.data, out), lib.spx_mx4_read, C.byref(m._c), t, out.data_ptr(), ld)
+    return out
+
+
+def mx4_matmul(ctx, x, w, up=None, starts=None, order=None, k=1, dtype=None, out=None):
+    """Products with 4-bit matrices (spx_mx4_matmul): x [rows, cols] (a tensor or an Mx4) against w's rows, or
+    silu(x w) * (x up). With starts [n_expert + 1] w holds n_expert matrices one after the other and out's rows are in
+    moe_sort's order: row i is x's row order[i] / k, without order x's row i. dtype: out's type (x's, for an Mx4
+    bfloat16). Rows of out behind starts' last are left as they were."""
+    four = isinstance(x, Mx4)
+    if four:
+        t, rows_x, cols, ld, data = 39, x.rows, x.cols, 0, x.data
+    else:
+        t, ld, data = _row_type(x.dtype), _rows2(x, "x"), x
+        rows_x, cols = x.shape
+    dtype = dtype or (torch.bfloat16 if four else x.dtype)
+    if cols != w.cols:
+        raise ValueError(f"x has {cols} columns, w {w.cols}")
+    experts = 1 if starts is None else starts.numel() - 1
+    if experts < 1 or w.rows % experts:
+        raise ValueError(f"w's {w.rows} rows are no {experts} matrices")
+    rows = rows_x if order is None else order.numel()
+    if (rows | rows_x | cols | k) >> 31:
+        raise _not_c_ints("k and the tensors' sizes")
+    n = w.rows // experts
+    at_s, at_o = None if starts is None else _i32(starts, experts + 1), None if order is None else _i32(order, rows)
+    out, ld_out = _out2(out, data, rows, n, dtype)
+    tensors = [data, w.data, out] + [v for v in (None if up is None else up.data, starts, order) if v is not None]
+    _run(ctx, tensors, lib.spx_mx4_matmul, t, data.data_ptr(), ld, rows_x, C.byref(w._c), None if up is None else C.byref(up._c), experts, at_s, at_o, k, rows,
+         _row_type(dtype), out.data_ptr(), ld_out)
+    return out
+
+
 class SamplerParams(C.Structure):
     """spx_sampler_params (SamplerConfig, smollm_chat.rs:1523-1555)."""
     _fields_ = [("temperature", C.c_float), ("top_k", C.c_int), ("top_p", C.c_float), ("min_p", C.c_float),

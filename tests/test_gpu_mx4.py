@@ -1,0 +1,420 @@
+"""Matrices in microscaled 4-bit floats (include/spx.h: spx_mx4_quantize, spx_mx4_read, spx_mx4_matmul) against
+64-bit evaluations of their definitions (moe_ref.py), and a layer of experts put together."""
+import numpy as np
+import pytest
+
+import moe_ref as R
+
+pytestmark = pytest.mark.gpu
+torch = pytest.importorskip("torch")
+
+F32, F16, BF16 = torch.float32, torch.float16, torch.bfloat16
+PARTS = {F32: 3, F16: 2, BF16: 1, "mx4": 0}
+
+
+@pytest.fixture(scope="module")
+def ctx():
+    from spindle_amd import ops
+    if not torch.cuda.is_available():
+        pytest.skip("no GPU")
+    c = ops.Context(0)
+    yield c
+    c.close()
+
+
+def ints(v):
+    return torch.tensor(np.asarray(v), dtype=torch.int32, device="cuda")
+
+
+def f64(t):
+    return t.detach().cpu().double().numpy()
+
+
+def close(got, want, tol, what=""):
+    got = f64(got) if isinstance(got, torch.Tensor) else got
+    assert np.array_equal(np.isnan(got), np.isnan(want)), what
+    with np.errstate(invalid="ignore"):
+        off = np.where(np.isnan(want) | (got == want), 0.0, np.abs(got - want) - tol)
+    assert (off <= 0).all(), (what, float(np.nanmax(off)))
+
+
+# ----------------------------------------------------------------------------------- the format
+def rows_for(rng, rows, cols, dtype):
+    x = rng.standard_normal((rows, cols)) * np.exp2(rng.integers(-12, 12, (rows, 1)))
+    big = {F32: 3.4e38, F16: 65504.0, BF16: 3.38e38}[dtype]
+    for r in range(rows):
+        kind = r % 11
+        if kind == 1:
+            x[r] = 0.0
+        elif kind == 2:
+            x[r, rng.integers(cols)] = [np.nan, np.inf, -np.inf][r // 11 % 3]
+        elif kind == 3:  # every quotient on the grid's halves, the largest 6 or 7.99
+            x[r] = rng.choice([0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0, 6.0, 7.0], cols) * rng.choice([-1, 1], cols)
+        elif kind == 4:
+            x[r] *= 1e-7 if dtype == F16 else 1e-38  # around and below the smallest normal numbers
+        elif kind == 5:
+            x[r] = rng.choice([-big, big, 1.0], cols)
+        elif kind == 6:
+            x[r] = rng.choice([-0.0, 0.0], cols)
+        elif kind == 7:
+            x[r] = np.exp2(rng.integers(-10, 10, cols))
+    return torch.from_numpy(np.clip(x, -big, big)).to(dtype)
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("rows,cols", [(1, 1), (3, 31), (22, 32), (23, 33), (5, 127), (12, 128), (34, 129), (11, 576), (3, 2050)])
+@pytest.mark.parametrize("pad,off", [(0, 0), (16, 0), (3, 1)])
+def test_quantize_and_read(ctx, dtype, rows, cols, pad, off):
+    from spindle_amd import ops
+    rng = np.random.default_rng(rows + cols)
+    wide = torch.full((rows, cols + pad + off), float("nan"), dtype=dtype)
+    wide[:, off:off + cols] = rows_for(rng, rows, cols, dtype)
+    x = wide.cuda()[:, off:off + cols]
+    m = ops.Mx4(torch.full((ops.Mx4.nbytes(rows, cols) + 8,), 0xA5, dtype=torch.uint8, device="cuda"), rows, cols)
+    assert ops.mx4_quantize(ctx, x, out=m) is m
+    want = R.pack(*R.quantize(f64(x)))
+    got = m.data.cpu().numpy()
+    assert np.array_equal(got[:-8], want) and (got[-8:] == 0xA5).all()
+    values = torch.from_numpy(R.unpack(want, rows, cols))
+    for t in (F32, F16, BF16):
+        v = ops.mx4_read(ctx, m, t)
+        ref = values.float().to(t)
+        assert torch.equal(v.cpu().nan_to_num(nan=77.0), ref.nan_to_num(nan=77.0))
+        into = torch.zeros(rows, cols + pad + off, dtype=t, device="cuda")
+        ops.mx4_read(ctx, m, t, out=into[:, off:off + cols])
+        assert torch.equal(into[:, off:off + cols].nan_to_num(nan=77.0), v.nan_to_num(nan=77.0)) and not into[:, :off].any() and not into[:, off + cols:].any()
+
+
+def test_read_every_code_and_scale(ctx):
+    from spindle_amd import ops
+    data = np.concatenate([np.tile(np.arange(16, dtype=np.uint8) * 17, 256 * 4), np.repeat(np.arange(256, dtype=np.uint8), 4)])
+    m = ops.Mx4(torch.from_numpy(data).cuda(), 256, 128)
+    with np.errstate(over="ignore"):
+        want = R.unpack(data, 256, 128).astype(np.float32)
+    assert np.array_equal(ops.mx4_read(ctx, m).cpu().numpy(), want, equal_nan=True)
+
+
+def test_quantize_many_rows(ctx):
+    """As many rows as a prompt has, against the same in small calls."""
+    from spindle_amd import ops
+    g = torch.Generator(device="cuda")
+    g.manual_seed(2)
+    x = torch.randn(9001, 700, generator=g, device="cuda", dtype=BF16)
+    got = ops.mx4_read(ctx, ops.mx4_quantize(ctx, x), BF16)
+    for a in range(0, 9001, 1000):
+        assert torch.equal(ops.mx4_read(ctx, ops.mx4_quantize(ctx, x[a:a + 1000]), BF16), got[a:a + 1000])
+
+
+# --------------------------------------------------------------------------------------- products
+def matrix(rng, rows, cols, spread=6):
+    """A random matrix's bytes (padding columns zeros)."""
+    from spindle_amd import ops
+    p = R.padded(cols)
+    codes = rng.integers(0, 16, (rows, p))
+    codes[:, cols:] = 0
+    data = R.pack(codes, rng.integers(127 - spread, 128 + spread, (rows, p // 32)))
+    return ops.Mx4(torch.from_numpy(data).cuda(), rows, cols), R.unpack(data, rows, cols)
+
+
+def rows_of_x(rng, kind, rows, cols, pad=0, off=0):
+    """x as the call takes it, its values in 64 bits."""
+    if kind == "mx4":
+        m, v = matrix(rng, max(rows, 1), cols)
+        return m, v
+    x = torch.from_numpy(rng.standard_normal((rows, cols + pad + off)) * np.exp2(rng.integers(-4, 4, (rows, 1)))).to(kind).cuda()[:, off:off + cols]
+    return x, f64(x)
+
+
+def check(got, x, w, up, kind, dtype):
+    want, tol = R.product(x, w, up, PARTS[kind])
+    got = f64(got)
+    # What lies half a step or more above a type's largest number rounds to infinity: in f16 from 65504 + 32 / 2 on.
+    # Where the exact value is that near to it, its infinity is as right as a finite result.
+    limit = {F32: 2.0 ** 128, BF16: 2.0 ** 128, F16: 65520.0}[dtype]
+    over = np.isinf(got) & (np.abs(want) + tol >= limit) & (np.sign(got) == np.sign(want))
+    assert not (np.isfinite(got) & (np.abs(want) - tol >= limit)).any()
+    close(np.where(over, want, got), want, tol + R.rounding(np.abs(want) + tol, dtype), (x.shape, w.shape))
+
+
+SIZES = [(1, 1, 1), (1, 2048, 33), (2, 128, 16), (3, 100, 31), (16, 129, 64), (17, 576, 65), (33, 256, 129), (64, 1000, 40), (130, 384, 200), (257, 64, 300)]
+
+
+@pytest.mark.parametrize("kind", [F32, F16, BF16, "mx4"])
+@pytest.mark.parametrize("rows,cols,n", SIZES)
+@pytest.mark.parametrize("gated", [False, True])
+def test_dense(ctx, kind, rows, cols, n, gated):
+    from spindle_amd import ops
+    rng = np.random.default_rng(rows * 7 + cols + n)
+    x, xv = rows_of_x(rng, kind, rows, cols)
+    w, wv = matrix(rng, n, cols)
+    up, uv = matrix(rng, n, cols) if gated else (None, None)
+    for dtype in (F32, F16, BF16) if kind == "mx4" else (kind,):
+        scale = 2.0 ** -9 if dtype == F16 else 1.0  # (sums stay in f16's range)
+        if scale != 1.0:
+            w2, wv2 = lowered(w, wv, scale)
+            check(ops.mx4_matmul(ctx, x, w2, up=up, dtype=dtype) if not gated else ops.mx4_matmul(ctx, x, w2, up=lowered(up, uv, scale)[0], dtype=dtype),
+                  xv, wv2, uv * scale if gated else None, kind, dtype)
+        else:
+            check(ops.mx4_matmul(ctx, x, w, up=up, dtype=dtype), xv, wv, uv, kind, dtype)
+
+
+def lowered(m, v, scale):
+    """The matrix with its scales lowered by a power of two."""
+    from spindle_amd import ops
+    data = m.data.clone()
+    codes = m.rows * R.padded(m.cols) // 2
+    data[codes:] -= int(-np.log2(scale))
+    return ops.Mx4(data, m.rows, m.cols), v * scale
+
+
+@pytest.mark.parametrize("kind", [F32, F16, BF16])
+@pytest.mark.parametrize("pad,off", [(8, 0), (3, 1)])
+def test_strides(ctx, kind, pad, off):
+    """Rows of x and out apart by more than their width, at odd addresses; what lies between rows of out stays."""
+    from spindle_amd import ops
+    rng = np.random.default_rng(pad)
+    rows, cols, n = 37, 200, 53
+    x, xv = rows_of_x(rng, kind, rows, cols, pad, off)
+    w, wv = lowered(*matrix(rng, n, cols), 2.0 ** -9)
+    into = torch.full((rows, n + pad + off), 5.0, dtype=kind, device="cuda")
+    ops.mx4_matmul(ctx, x, w, out=into[:, off:off + n])
+    check(into[:, off:off + n], xv, wv, None, kind, kind)
+    assert (into[:, :off] == 5.0).all() and (into[:, off + n:] == 5.0).all()
+
+
+GROUPS = [(1, 8, 128, 128, 40), (5, 2, 4, 100, 33), (24, 8, 32, 256, 64), (100, 4, 6, 300, 100), (90, 8, 3, 64, 130), (300, 2, 5, 160, 72)]
+
+
+@pytest.mark.parametrize("kind", [F32, F16, BF16, "mx4"])
+@pytest.mark.parametrize("rows,k,experts,cols,n", GROUPS)
+@pytest.mark.parametrize("gated,sort_first,drop", [(True, False, False), (False, True, True), (False, False, True)])
+def test_by_expert(ctx, kind, rows, k, experts, cols, n, gated, sort_first, drop):
+    from spindle_amd import ops
+    rng = np.random.default_rng(rows + cols)
+    ids = rng.integers(0, experts, (rows, k))
+    ids[: rows // 3] = ids[0, 0]  # a crowded expert, others with few rows or none
+    if drop:
+        ids[rng.random(ids.shape) < 0.4] = -1
+    o = ops.moe_sort(ctx, ints(ids), experts)
+    starts, order, _ = R.sort(ids, experts)
+    x, xv = rows_of_x(rng, kind, rows * k if sort_first else rows, cols)
+    w, wv = lowered(*matrix(rng, experts * n, cols), 2.0 ** -9)
+    up, uv = lowered(*matrix(rng, experts * n, cols), 2.0 ** -9) if gated else (None, None)
+    dtype = BF16 if kind == "mx4" else kind
+    out = torch.full((rows * k, n), 123.0, dtype=dtype, device="cuda")
+    ops.mx4_matmul(ctx, x, w, up=up, starts=o.starts, order=None if sort_first else o.order, k=k, dtype=dtype, out=out)
+    assert (out[starts[-1]:] == 123.0).all()  # rows behind the last one stay
+    for e in range(experts):
+        a, b = starts[e], starts[e + 1]
+        if a < b:
+            rows_e = xv[a:b] if sort_first else xv[order[a:b] // k]
+            at = slice(e * n, (e + 1) * n)
+            check(out[a:b], rows_e, wv[at], uv[at] if gated else None, kind, dtype)
+
+
+@pytest.mark.parametrize("kind", [F32, BF16, "mx4"])
+@pytest.mark.parametrize("rows", [6, 150])
+def test_rows_without_an_entry(ctx, kind, rows):
+    """A row whose order names no row of x stays as it was, among rows that have one; so do rows that starts leave out."""
+    from spindle_amd import ops
+    rng = np.random.default_rng(rows)
+    cols, n = 128, 48
+    x, xv = rows_of_x(rng, kind, rows, cols)
+    w, wv = matrix(rng, 2 * n, cols)
+    dtype = F32
+    order = rng.integers(0, rows * 2, rows)
+    order[[1, 4]] = -1, rows * 2  # k = 2: that is a row behind x
+    out = torch.full((rows, n), 7.0, dtype=dtype, device="cuda")
+    cut = rows // 2
+    ops.mx4_matmul(ctx, x, w, starts=ints([1, cut, rows - 1]), order=ints(order), k=2, dtype=dtype, out=out)
+    for i in range(rows):
+        if i in (0, 1, 4, rows - 1):
+            assert (out[i] == 7.0).all()
+        else:
+            at = slice(0, n) if i < cut else slice(n, 2 * n)
+            check(out[i:i + 1], xv[order[i] // 2][None], wv[at], None, kind, dtype)
+    # starts past the rows are cut there
+    out.fill_(7.0)
+    ops.mx4_matmul(ctx, x, w, starts=ints([-5, cut, 10 ** 6]), order=ints(order), k=2, dtype=dtype, out=out)
+    check(out[rows - 1:], xv[order[rows - 1] // 2][None], wv[n:], None, kind, dtype)
+
+
+@pytest.mark.parametrize("kind", [F32, F16, BF16, "mx4"])
+@pytest.mark.parametrize("rows", [3, 70, 200])
+def test_special_values(ctx, kind, rows):
+    """NaN and infinities stay in their rows, NaN scales in their matrix's; scales to the ends of their range."""
+    from spindle_amd import ops
+    rng = np.random.default_rng(5)
+    cols, n = 260, 36
+    w, wv = matrix(rng, n, cols)
+    w.data[n * R.padded(cols) // 2 + 4 * R.padded(cols) // 32] = 255  # the first block of row 4
+    if kind == "mx4":
+        x, xv = matrix(rng, rows, cols)
+        x.data[rows * R.padded(cols) // 2 + 2 * R.padded(cols) // 32 + 3] = 255
+        xv = R.unpack(x.data.cpu().numpy(), rows, cols)
+    else:
+        x = torch.from_numpy(rng.standard_normal((rows, cols))).to(kind).cuda()
+        x[2, 100] = float("nan")
+        x[1, 7] = float("inf")
+        xv = f64(x)
+        if kind == F32:  # a NaN whose upper half is infinity's
+            x.view(torch.int32)[2, 100] = 0x7F800001
+    wv = R.unpack(w.data.cpu().numpy(), n, cols)
+    got = f64(ops.mx4_matmul(ctx, x, w, dtype=F32))
+    assert np.isnan(got[:, 4]).all() and np.isnan(got[2]).all()
+    with np.errstate(invalid="ignore"):
+        want = xv @ wv.T
+    if kind != "mx4":
+        rest = [j for j in range(n) if j != 4]
+        inf = wv[rest, 7]
+        assert np.array_equal(np.isnan(got[1, rest]), inf == 0) and np.array_equal(got[1, rest][inf != 0], np.sign(inf[inf != 0]) * np.inf)
+    keep = [i for i in range(rows) if i not in (1, 2)]
+    others = [j for j in range(n) if j != 4]
+    if kind == "mx4":
+        keep = [i for i in range(rows) if i != 2]
+    ref, tol = R.product(xv[keep], wv[others], None, PARTS[kind])
+    close(got[np.ix_(keep, others)], ref, tol + R.rounding(np.abs(ref) + tol, F32))
+    assert not np.isnan(want[np.ix_(keep, others)]).any()
+
+
+@pytest.mark.parametrize("rows", [2, 40])
+def test_wide_scales(ctx, rows):
+    """Products whose scales lie far apart, each way, keep their values: x times 2^40, the matrix times 2^-60."""
+    from spindle_amd import ops
+    rng = np.random.default_rng(rows)
+    cols, n = 256, 24
+    w, wv = lowered(*matrix(rng, n, cols, 30), 2.0 ** -60)
+    m, mv = matrix(rng, rows, cols, 30)
+    m.data[rows * cols // 2:] += 40
+    got = ops.mx4_matmul(ctx, m, w, dtype=F32)
+    check(got, mv * 2.0 ** 40, wv, None, "mx4", F32)
+    x = torch.from_numpy(mv * 2.0 ** 40).float().cuda()
+    check(ops.mx4_matmul(ctx, x, w), f64(x), wv, None, F32, F32)
+
+
+def test_no_rows(ctx):
+    from spindle_amd import ops
+    w, _ = matrix(np.random.default_rng(1), 8, 64)
+    assert ops.mx4_matmul(ctx, torch.zeros(0, 64, device="cuda"), w).shape == (0, 8)
+
+
+def test_same_bits_every_time(ctx):
+    from spindle_amd import ops
+    rng = np.random.default_rng(11)
+    w, _ = matrix(rng, 3 * 200, 700)
+    for kind in (F32, BF16, "mx4"):
+        for rows in (5, 90, 400):
+            x, _ = rows_of_x(rng, kind, rows, 700)
+            starts = ints([0, rows // 5, rows // 2, rows])
+            a = ops.mx4_matmul(ctx, x, w, starts=starts, dtype=F32)
+            for _ in range(3):
+                assert torch.equal(ops.mx4_matmul(ctx, x, w, starts=starts, dtype=F32), a)
+
+
+# ------------------------------------------------------------------------- a layer put together
+def layer(ops, ctx, x, logits, k, gate, up, down, experts, four):
+    """A mixture of experts over rows x: router, sort, gated products, down, joined."""
+    chosen, weights = ops.moe_route(ctx, logits, k)
+    o = ops.moe_sort(ctx, chosen, experts)
+    h = ops.mx4_matmul(ctx, ops.mx4_quantize(ctx, x) if four else x, gate, up=up, starts=o.starts, order=o.order, k=k, dtype=x.dtype)
+    y = ops.mx4_matmul(ctx, ops.mx4_quantize(ctx, h) if four else h, down, starts=o.starts, dtype=x.dtype)
+    return ops.moe_combine(ctx, y, o.place, weights), (chosen, weights, o, h, y)
+
+
+def layer_case(rng, rows, dtype):
+    experts, k, dim, inner = 16, 4, 256, 96
+    mats = []
+    for r, c in ((inner, dim), (inner, dim), (dim, inner)):
+        mats.append(lowered(*matrix(rng, experts * r, c, 2), 2.0 ** -5))
+    x = torch.from_numpy(rng.standard_normal((rows, dim))).to(dtype).cuda()
+    logits = torch.from_numpy(rng.standard_normal((rows, experts)) * 2).float().cuda()
+    return experts, k, mats, x, logits
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("rows", [1, 7, 150])
+@pytest.mark.parametrize("four", [False, True])
+def test_layer(ctx, dtype, rows, four):
+    """Each step of the layer against its definition on the step's own inputs."""
+    from spindle_amd import ops
+    rng = np.random.default_rng(rows)
+    experts, k, ((gate, gv), (up, uv), (down, dv)), x, logits = layer_case(rng, rows, dtype)
+    got, (chosen, weights, o, h, y) = layer(ops, ctx, x, logits, k, gate, up, down, experts, four)
+    ids, w, tol = R.route(f64(logits), k, True)
+    assert np.array_equal(chosen.cpu().numpy(), ids)
+    close(weights, w, tol)
+    starts, order, place = R.sort(ids, experts)
+    stand = lambda v: R.unpack(R.pack(*R.quantize(f64(v))), *v.shape) if four else f64(v)  # noqa: E731
+    xv, hv, kind = stand(x), stand(h), "mx4" if four else dtype
+    for e in range(experts):
+        a, b = starts[e], starts[e + 1]
+        if a < b:
+            n, d = slice(e * 96, e * 96 + 96), slice(e * 256, e * 256 + 256)
+            check(h[a:b], xv[order[a:b] // k], gv[n], uv[n], kind, dtype)
+            check(y[a:b], hv[a:b], dv[d], None, kind, dtype)
+    terms = f64(y)[place] * f64(weights)[..., None]
+    want, tol = terms.sum(1), np.abs(terms).sum(1) * k * R.U
+    close(got, want, tol + R.rounding(np.abs(want) + tol, dtype))
+
+
+def test_layer_in_a_graph(ctx):
+    """A captured layer, replayed over changing inputs with eager work between, gives the eager bits each time; on the
+    context's stream and with another stream's work in order."""
+    from spindle_amd import ops
+    rng = np.random.default_rng(21)
+    experts, k, ((gate, _), (up, _), (down, _)), x, logits = layer_case(rng, 200, BF16)
+    inputs = [(torch.randn_like(x), torch.randn_like(logits)) for _ in range(4)]
+    run = lambda: layer(ops, ctx, x, logits, k, gate, up, down, experts, True)[0]  # noqa: E731
+    want = []
+    side = torch.cuda.Stream()
+    for i, (a, b) in enumerate(inputs):
+        with torch.cuda.stream(side if i % 2 else torch.cuda.current_stream()):
+            side.wait_stream(torch.cuda.default_stream())
+            x.copy_(a)
+            logits.copy_(b)
+            want.append(run().clone())
+            torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=ctx.torch_stream()):
+        out = run()
+    for turn in range(3):
+        for (a, b), w in zip(inputs, want):
+            x.copy_(a)
+            logits.copy_(b)
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(out, w)
+            assert torch.equal(run(), w)  # eager work between replays
+
+
+def test_tuning_step_in_a_graph(ctx):
+    """A router's way back, captured and replayed: the eager bits each time."""
+    from spindle_amd import ops
+    rng = np.random.default_rng(22)
+    rows, k, experts, width = 300, 4, 12, 64
+    logits = torch.from_numpy(rng.standard_normal((rows, experts))).float().cuda()
+    y = torch.from_numpy(rng.standard_normal((rows * k, width))).to(BF16).cuda()
+    d = torch.from_numpy(rng.standard_normal((rows, width))).to(BF16).cuda()
+
+    def step():
+        chosen, weights = ops.moe_route(ctx, logits, k)
+        o = ops.moe_sort(ctx, chosen, experts)
+        out = ops.moe_combine(ctx, y, o.place, weights)
+        d_y, d_w = ops.moe_combine_grad(ctx, d, y, o.order, o.place, weights)
+        return out, d_y, ops.moe_route_grad(ctx, logits, chosen, d_w)
+
+    first = [torch.randn_like(logits) for _ in range(3)]
+    want = []
+    for v in first:
+        logits.copy_(v)
+        want.append([t.clone() for t in step()])
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for _ in range(3):
+        for v, w in zip(first, want):
+            logits.copy_(v)
+            graph.replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, b) for a, b in zip(got, w))
+            step()
