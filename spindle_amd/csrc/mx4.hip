@@ -329,17 +329,255 @@ __global__ __launch_bounds__(256) void k_mx4_rows(const Mx4Product a, const Vecs
   }
 }
 
+// ------------------------------------------------------------------ products of many rows
+// MT rows of x against 64 rows of the matrix a wave (gated: 32 of each), 256 a workgroup. A wave's rows of the matrix are
+// its own, so their codes come straight from memory into its registers, an iteration ahead; the rows of x are all four
+// waves' and go through LDS as the matrix instructions take them: 16 rows x 64 bytes a fragment, the 16 bytes of row
+// r and lane group g at 64 r + 16 (g ^ (r / 2 & 3)), which spreads what eight lanes read or write over the banks.
+__device__ __forceinline__ int frag_at(int r, int g) { return r * 64 + ((g ^ (r >> 1 & 3)) * 16); }
+
+// Tiles' order: those of one expert and row tile lie beside each other on one XCD (workgroups go to the eight in turn),
+// so that its L2 gives the rows of x and the matrices again. False: there is no such tile.
+__device__ __forceinline__ bool tile_place(const Mx4Product &a, int most, int columns, Tile &tile, int &column) {
+  int tiles = 0;
+  if (!a.starts) tiles = (a.rows + most - 1) / most;
+  else {
+    const int lane = threadIdx.x & 63;
+    for (int b = 0; b < a.n_expert; b += 64) {
+      const int e = b + lane;
+      int c = 0;
+      if (e < a.n_expert) {
+        const int lo = min(max(a.starts[e], 0), a.rows);
+        c = (min(max(a.starts[e + 1], lo), a.rows) - lo + most - 1) / most;
+      }
+      tiles += lane_i(wave_scan(c), 63);
+    }
+  }
+  const int64_t all = (int64_t)tiles * columns, each = (all + 7) / 8, id = blockIdx.x + (int64_t)blockIdx.y * gridDim.x;
+  const int64_t at = (id & 7) * each + (id >> 3);
+  if ((id >> 3) >= each || at >= all) return false;
+  tile = tile_of(a, (int)(at / columns), most);
+  column = (int)(at % columns);
+  return tile.count > 0;
+}
+
+// Eight columns of a row of x as they lie in memory, zeros behind the last and where there is no row.
+template <class E>
+struct Raw8 { uint4 v[sizeof(E) / 2]; };
+template <class E>
+__device__ __forceinline__ Raw8<E> raw8(const Mx4Product &a, const E *row, int c, bool vec) {
+  Raw8<E> r;
+  if (row && vec && c + 8 <= a.cols) {
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(E) / 2; i++) r.v[i] = ((const uint4 *)(row + c))[i];
+  } else {
+    alignas(16) E e[8];
+#pragma unroll
+    for (int j = 0; j < 8; j++) e[j] = row && c + j < a.cols ? row[c + j] : (E)0;
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(E) / 2; i++) r.v[i] = ((const uint4 *)e)[i];
+  }
+  return r;
+}
+
+template <class X, int MT>
+struct TileX {
+  static constexpr int P = X::PARTS, KS = P == 0 ? 2 : 1;              // steps of 128 columns an iteration
+  static constexpr int PLANES = P == 0 ? 2 : 4 * P;                    // fragments of 64 bytes a row
+  static constexpr int PLANE = MT * 64 + 64;                           // (planes start 16 banks apart)
+  static constexpr int UNITS = P == 0 ? MT * 8 : MT * 16;              // pieces of 16 bytes, or of eight columns, an iteration
+  static constexpr int PER = (UNITS + 255) / 256;
+  static constexpr int SCALES = P == 0 ? 2 * MT * 4 : 0;
+  static constexpr int BYTES = PLANES * PLANE + SCALES;
+  static constexpr int BUFS = 2 * BYTES <= 65536 ? 2 : 1;
+};
+
+template <class X, int MT, bool GATED>
+__global__ __launch_bounds__(256, 2) void k_mx4_tile(const Mx4Product a, const Vecs vec, int out_type, int columns) {
+  typedef TileX<X, MT> T;
+  typedef typename X::R::E E;
+  constexpr int P = T::P, KS = T::KS, MF = MT / 16, WF = GATED ? 2 : 4;  // WF: fragments of out's columns a wave
+  extern __shared__ __align__(16) uint8_t lds[];
+  __shared__ int s_src[MT];
+  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, m = lane & 15, g = lane >> 4;
+  Tile tile;
+  int column;
+  if (!tile_place(a, MT, columns, tile, column)) return;
+  if (tid < MT) s_src[tid] = tid < tile.count ? source_of(a, tile.row + tid) : -1;
+  __syncthreads();
+  const int n0 = (column * 4 + wave) * (16 * WF);
+  const int64_t wrow = (int64_t)tile.expert * a.n;
+  // a lane's row of each fragment of the matrix
+  const uint8_t *wc[4], *wsc[4];
+#pragma unroll
+  for (int t = 0; t < 4; t++) {
+    const Mx4 w = GATED && t >= 2 ? a.up : a.w;
+    const int64_t row = wrow + min(n0 + 16 * (GATED ? t & 1 : t) + m, a.n - 1);
+    wc[t] = w.codes + row * (a.steps * 64) + g * 16;
+    wsc[t] = w.scales + row * (a.steps * 4) + g;
+  }
+  // a thread's pieces of x: unit u is row u / U, piece u % U of the iteration's columns
+  constexpr int U = P == 0 ? 8 : 16;
+  const void *xr[T::PER];
+#pragma unroll
+  for (int j = 0; j < T::PER; j++) {
+    const int u = tid + 256 * j, r = u / U;
+    const int src = u < T::UNITS ? s_src[r] : -1;
+    if (P == 0) xr[j] = src >= 0 ? (const uint8_t *)a.x + (int64_t)src * (a.steps * 64) : nullptr;
+    else xr[j] = src >= 0 ? (const E *)a.x + (int64_t)src * a.ld_x : nullptr;
+  }
+  const uint8_t *xs = P == 0 && tid < MT && s_src[tid] >= 0 ? a.x_scales + (int64_t)s_src[tid] * (a.steps * 4) : nullptr;
+
+  i4v w[4 * KS], wn[4 * KS];
+  int ws[4 * KS], wsn[4 * KS];
+  uint4 xc[P == 0 ? T::PER : 1];
+  uint32_t xsc[2];
+  Raw8<E> xw[P == 0 ? 1 : T::PER];
+  const auto load_w = [&](int s) {
+#pragma unroll
+    for (int h = 0; h < KS; h++) {
+      const int sh = min(s + h, a.steps - 1);  // (behind the last: x is zero there)
+#pragma unroll
+      for (int t = 0; t < 4; t++) {
+        wn[h * 4 + t] = *(const i4v *)(wc[t] + sh * 64);
+        wsn[h * 4 + t] = wsc[t][sh * 4];
+      }
+    }
+  };
+  const auto load_x = [&](int s) {
+    if constexpr (P == 0) {
+#pragma unroll
+      for (int j = 0; j < T::PER; j++) {
+        const int q = (tid + 256 * j) % U;
+        xc[j] = make_uint4(0, 0, 0, 0);
+        if (xr[j] && s + (q >> 2) < a.steps) xc[j] = *(const uint4 *)((const uint8_t *)xr[j] + s * 64 + q * 16);
+      }
+      xsc[0] = xsc[1] = 0;
+      if (xs) {
+        xsc[0] = *(const uint32_t *)(xs + s * 4);
+        if (s + 1 < a.steps) xsc[1] = *(const uint32_t *)(xs + s * 4 + 4);
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < T::PER; j++) xw[j] = raw8<E>(a, (const E *)xr[j], s * 128 + (tid + 256 * j) % U * 8, vec.x);
+    }
+  };
+  const auto put_x = [&](uint8_t *buf) {
+#pragma unroll
+    for (int j = 0; j < T::PER; j++) {
+      const int u = tid + 256 * j, r = u / U, q = u % U;
+      if (T::UNITS % 256 && u >= T::UNITS) break;
+      if constexpr (P == 0) {
+        *(uint4 *)(buf + (q >> 2) * T::PLANE + (r >> 4) * 1024 + frag_at(r & 15, q & 3)) = xc[j];
+      } else {
+        uint8_t *dst = buf + (q & 3) * T::PLANE + (r >> 4) * 1024 + frag_at(r & 15, q >> 2);
+        if constexpr (P == 1) *(uint4 *)dst = xw[j].v[0];
+        else {
+          alignas(16) E e[8];
+#pragma unroll
+          for (int i = 0; i < (int)sizeof(E) / 2; i++) ((uint4 *)e)[i] = xw[j].v[i];
+          float x[8];
+#pragma unroll
+          for (int i = 0; i < 8; i++) x[i] = row_get(typename X::R{}, e[i]);
+          b8v part[P];
+          parts_of(x, part);
+#pragma unroll
+          for (int p = 0; p < P; p++) *(b8v *)(dst + p * 4 * T::PLANE) = part[p];
+        }
+      }
+    }
+    if (P == 0 && tid < MT) {
+      uint32_t *sc = (uint32_t *)(buf + T::PLANES * T::PLANE);
+      sc[tid] = xsc[0];
+      sc[MT + tid] = xsc[1];
+    }
+  };
+
+  f4v acc[MF][4] = {};
+  load_x(0);
+  load_w(0);
+  int buf = 0;
+  for (int s = 0; s < a.steps; s += KS) {
+    uint8_t *b = lds + buf * T::BYTES;
+    if (T::BUFS == 1) __syncthreads();  // the last iteration's reads are done
+    put_x(b);
+#pragma unroll
+    for (int t = 0; t < 4 * KS; t++) { w[t] = wn[t]; ws[t] = wsn[t]; }
+    __syncthreads();
+    if (s + KS < a.steps) {
+      load_x(s + KS);
+      load_w(s + KS);
+    }
+    if constexpr (P == 0) {
+#pragma unroll
+      for (int h = 0; h < 2; h++)
+#pragma unroll
+        for (int f = 0; f < MF; f++) {
+          const i4v x = *(const i4v *)(b + h * T::PLANE + f * 1024 + frag_at(m, g));
+          const int sx = b[T::PLANES * T::PLANE + (h * MT + f * 16 + m) * 4 + g];
+#pragma unroll
+          for (int t = 0; t < 4; t++) acc[f][t] = mfma_mx4(w[h * 4 + t], ws[h * 4 + t], x, sx, acc[f][t]);
+        }
+    } else {
+#pragma unroll
+      for (int c = 0; c < 4; c++) {
+        b8v v[4];
+#pragma unroll
+        for (int t = 0; t < 4; t++) v[t] = values_of((uint32_t)w[t][c], __uint_as_float((uint32_t)ws[t] << 23));
+#pragma unroll
+        for (int f = 0; f < MF; f++)
+#pragma unroll
+          for (int p = P - 1; p >= 0; p--) {
+            const b8v x = *(const b8v *)(b + (p * 4 + c) * T::PLANE + f * 1024 + frag_at(m, g));
+#pragma unroll
+            for (int t = 0; t < 4; t++) acc[f][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v[t], x, acc[f][t], 0, 0, 0);
+          }
+      }
+    }
+    if (T::BUFS == 2) buf ^= 1;
+  }
+#pragma unroll
+  for (int f = 0; f < MF; f++) {
+    if (s_src[f * 16 + m] < 0) continue;
+#pragma unroll
+    for (int t = 0; t < WF; t++) {
+      f4v v = acc[f][t];
+      if (GATED)
+#pragma unroll
+        for (int j = 0; j < 4; j++) v[j] = silu(v[j]) * acc[f][(t + 2) & 3][j];
+      const int c = n0 + 16 * t + 4 * g;
+      if (c < a.n) put4_by(a, out_type, tile.row + f * 16 + m, c, v, vec.out);
+    }
+  }
+}
+
 // Tiles over the launch's second and third dimension.
 static dim3 tile_grid(int64_t columns, int64_t tiles) {
   const int64_t y = tiles < 32768 ? tiles : 32768;
   return dim3((unsigned)columns, (unsigned)y, (unsigned)((tiles + y - 1) / y));
 }
 
+template <class X, int MT>
+static hipError_t tiled(const Mx4Product &a, const Vecs &vec, int out_type, hipStream_t s) {
+  typedef TileX<X, MT> T;
+  const int wide = a.up.codes ? 128 : 256, columns = (a.n + wide - 1) / wide;
+  const int64_t blocks = (tiles_most(a, MT) * columns + 7) / 8 * 8, x = blocks < 1 << 20 ? blocks : 1 << 20;
+  const dim3 grid((unsigned)x, (unsigned)((blocks + x - 1) / x));
+  constexpr unsigned bytes = T::BUFS * T::BYTES;
+  if (a.up.codes) hipLaunchKernelGGL((k_mx4_tile<X, MT, true>), grid, dim3(256), bytes, s, a, vec, out_type, columns);
+  else hipLaunchKernelGGL((k_mx4_tile<X, MT, false>), grid, dim3(256), bytes, s, a, vec, out_type, columns);
+  return hipGetLastError();
+}
+
 template <class X>
 static hipError_t product(const Mx4Product &a, int out_type, hipStream_t s) {
-  constexpr int RT = 2;
+  constexpr int RT = 2, MOST = X::PARTS <= 1 ? 128 : 64;
   const Vecs vec = {X::PARTS == 0 || on16(a.x, a.ld_x, sizeof(typename X::R::E)),
                     (uintptr_t)a.out % (out_type == T_F32 ? 16 : 8) == 0 && a.ld_out % 4 == 0};
+  const int64_t each = a.starts ? a.rows / a.n_expert : a.rows;  // rows of a matrix, where they are even
+  if (each > 64 && MOST == 128) return tiled<X, MOST>(a, vec, out_type, s);
+  if (each > 24) return tiled<X, 64>(a, vec, out_type, s);
+  if (each > 8) return tiled<X, 32>(a, vec, out_type, s);
   const dim3 grid = tile_grid((a.n + 16 * RT - 1) / (16 * RT), tiles_most(a, 16));
   if (a.up.codes) hipLaunchKernelGGL((k_mx4_rows<X, RT, true>), grid, dim3(256), 0, s, a, vec, out_type);
   else hipLaunchKernelGGL((k_mx4_rows<X, RT, false>), grid, dim3(256), 0, s, a, vec, out_type);
