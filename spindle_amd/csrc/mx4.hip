@@ -222,9 +222,11 @@ __device__ __forceinline__ b8v values_of(uint32_t w, float scale) {
   for (int j = 0; j < 4; j++) { r[2 * j] = v[j][0]; r[2 * j + 1] = v[j][1]; }
   return r;
 }
+// BYTE: which byte of ws and xs is the scale.
+template <int BYTE>
 __device__ __forceinline__ f4v mfma_mx4(i4v w, int ws, i4v x, int xs, f4v acc) {
   const i8v A = {w[0], w[1], w[2], w[3], 0, 0, 0, 0}, B = {x[0], x[1], x[2], x[3], 0, 0, 0, 0};
-  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(A, B, acc, 4, 4, 0, ws, 0, xs);
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(A, B, acc, 4, 4, BYTE, ws, BYTE, xs);
 }
 
 __device__ __forceinline__ float silu(float v) { return v / (1.0f + expf(-v)); }
@@ -293,7 +295,7 @@ __global__ __launch_bounds__(256) void k_mx4_rows(const Mx4Product a, const Vecs
 #pragma unroll
       for (int h = 0; h < H; h++)
 #pragma unroll
-        for (int t = 0; t < RT; t++) acc[h][t] = mfma_mx4(w[h][t], ws[h][t], x, xs, acc[h][t]);
+        for (int t = 0; t < RT; t++) acc[h][t] = mfma_mx4<0>(w[h][t], ws[h][t], x, xs, acc[h][t]);
     } else {
 #pragma unroll
       for (int c = 0; c < 4; c++) {
@@ -385,62 +387,69 @@ struct TileX {
   static constexpr int P = X::PARTS, KS = P == 0 ? 2 : 1;              // steps of 128 columns an iteration
   static constexpr int PLANES = P == 0 ? 2 : 4 * P;                    // fragments of 64 bytes a row
   static constexpr int PLANE = MT * 64 + 64;                           // (planes start 16 banks apart)
-  static constexpr int UNITS = P == 0 ? MT * 8 : MT * 16;              // pieces of 16 bytes, or of eight columns, an iteration
-  static constexpr int PER = (UNITS + 255) / 256;
-  static constexpr int SCALES = P == 0 ? 2 * MT * 4 : 0;
+  static constexpr int U = P == 0 ? 8 : 16;                            // a row's pieces of 16 bytes, or of eight columns, an iteration
+  static constexpr int PER = (MT * U + 255) / 256;
+  static constexpr int SCALES = P == 0 ? MT * 8 : 0;
   static constexpr int BYTES = PLANES * PLANE + SCALES;
   static constexpr int BUFS = 2 * BYTES <= 65536 ? 2 : 1;
 };
 
+// Of an iteration's 256 columns of 4-bit rows lane group g takes blocks 2g and 2g + 1, one an instruction: 32
+// bytes of codes that lie together and two scale bytes that one load brings. Of 128 columns of others it takes block g,
+// eight columns an instruction.
 template <class X, int MT, bool GATED>
 __global__ __launch_bounds__(256, 2) void k_mx4_tile(const Mx4Product a, const Vecs vec, int out_type, int columns) {
   typedef TileX<X, MT> T;
   typedef typename X::R::E E;
-  constexpr int P = T::P, KS = T::KS, MF = MT / 16, WF = GATED ? 2 : 4;  // WF: fragments of out's columns a wave
+  constexpr int P = T::P, KS = T::KS, U = T::U, MF = MT / 16, WF = GATED ? 2 : 4;  // WF: fragments of out's columns a wave
   extern __shared__ __align__(16) uint8_t lds[];
   __shared__ int s_src[MT];
-  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, m = lane & 15, g = lane >> 4;
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, m = lane & 15, g = lane >> 4;
   Tile tile;
   int column;
   if (!tile_place(a, MT, columns, tile, column)) return;
   if (tid < MT) s_src[tid] = tid < tile.count ? source_of(a, tile.row + tid) : -1;
   __syncthreads();
   const int n0 = (column * 4 + wave) * (16 * WF);
-  const int64_t wrow = (int64_t)tile.expert * a.n;
-  // a lane's row of each fragment of the matrix
-  const uint8_t *wc[4], *wsc[4];
+  // the matrix from the wave's first row on, a lane's row of each fragment
+  const int first = min(n0, a.n - 1);
+  const int64_t row0 = (int64_t)tile.expert * a.n + first;
+  const uint8_t *wbase[2] = {a.w.codes + row0 * (a.steps * 64), GATED ? a.up.codes + row0 * (a.steps * 64) : nullptr};
+  const uint8_t *sbase[2] = {a.w.scales + row0 * (a.steps * 4), GATED ? a.up.scales + row0 * (a.steps * 4) : nullptr};
+  uint32_t wrow[WF];
 #pragma unroll
-  for (int t = 0; t < 4; t++) {
-    const Mx4 w = GATED && t >= 2 ? a.up : a.w;
-    const int64_t row = wrow + min(n0 + 16 * (GATED ? t & 1 : t) + m, a.n - 1);
-    wc[t] = w.codes + row * (a.steps * 64) + g * 16;
-    wsc[t] = w.scales + row * (a.steps * 4) + g;
-  }
-  // a thread's pieces of x: unit u is row u / U, piece u % U of the iteration's columns
-  constexpr int U = P == 0 ? 8 : 16;
-  const void *xr[T::PER];
+  for (int t = 0; t < WF; t++) wrow[t] = (uint32_t)(min(n0 + 16 * t + m, a.n - 1) - first) * (uint32_t)(a.steps * 4);
+  const int q = tid % U, r0 = tid / U;  // a thread's pieces of x: piece q of rows r0, r0 + 256 / U, ...
+  const uint8_t *xr[P == 0 ? T::PER : 1];
+  if constexpr (P == 0)
 #pragma unroll
-  for (int j = 0; j < T::PER; j++) {
-    const int u = tid + 256 * j, r = u / U;
-    const int src = u < T::UNITS ? s_src[r] : -1;
-    if (P == 0) xr[j] = src >= 0 ? (const uint8_t *)a.x + (int64_t)src * (a.steps * 64) : nullptr;
-    else xr[j] = src >= 0 ? (const E *)a.x + (int64_t)src * a.ld_x : nullptr;
-  }
+    for (int j = 0; j < T::PER; j++) {
+      const int r = r0 + 256 / U * j, src = r < MT ? s_src[r] : -1;
+      xr[j] = src >= 0 ? (const uint8_t *)a.x + (int64_t)src * (a.steps * 64) + q * 16 : nullptr;
+    }
   const uint8_t *xs = P == 0 && tid < MT && s_src[tid] >= 0 ? a.x_scales + (int64_t)s_src[tid] * (a.steps * 4) : nullptr;
 
   i4v w[4 * KS], wn[4 * KS];
-  int ws[4 * KS], wsn[4 * KS];
+  uint32_t ws[4], wsn[4];
   uint4 xc[P == 0 ? T::PER : 1];
   uint32_t xsc[2];
   Raw8<E> xw[P == 0 ? 1 : T::PER];
   const auto load_w = [&](int s) {
-#pragma unroll
-    for (int h = 0; h < KS; h++) {
-      const int sh = min(s + h, a.steps - 1);  // (behind the last: x is zero there)
+    if constexpr (P == 0) {
+      const int at = s + 1 < a.steps ? g : g & 1;  // (an odd last step has half as many blocks; x is zero at the others)
 #pragma unroll
       for (int t = 0; t < 4; t++) {
-        wn[h * 4 + t] = *(const i4v *)(wc[t] + sh * 64);
-        wsn[h * 4 + t] = wsc[t][sh * 4];
+        const uint8_t *p = wbase[t / WF] + s * 64;
+        const uint32_t off = wrow[t % WF] * 16u + at * 32;
+        wn[t] = *(const i4v *)(p + off);
+        wn[4 + t] = *(const i4v *)(p + off + 16);
+        wsn[t] = *(const uint16_t *)(sbase[t / WF] + s * 4 + (wrow[t % WF] + at * 2));
+      }
+    } else {
+#pragma unroll
+      for (int t = 0; t < 4; t++) {
+        wn[t] = *(const i4v *)(wbase[t / WF] + s * 64 + (wrow[t % WF] * 16u + g * 16));
+        wsn[t] = sbase[t / WF][s * 4 + (wrow[t % WF] + g)];
       }
     }
   };
@@ -448,9 +457,8 @@ __global__ __launch_bounds__(256, 2) void k_mx4_tile(const Mx4Product a, const V
     if constexpr (P == 0) {
 #pragma unroll
       for (int j = 0; j < T::PER; j++) {
-        const int q = (tid + 256 * j) % U;
         xc[j] = make_uint4(0, 0, 0, 0);
-        if (xr[j] && s + (q >> 2) < a.steps) xc[j] = *(const uint4 *)((const uint8_t *)xr[j] + s * 64 + q * 16);
+        if (xr[j] && s + (q >> 2) < a.steps) xc[j] = *(const uint4 *)(xr[j] + s * 64);
       }
       xsc[0] = xsc[1] = 0;
       if (xs) {
@@ -459,16 +467,19 @@ __global__ __launch_bounds__(256, 2) void k_mx4_tile(const Mx4Product a, const V
       }
     } else {
 #pragma unroll
-      for (int j = 0; j < T::PER; j++) xw[j] = raw8<E>(a, (const E *)xr[j], s * 128 + (tid + 256 * j) % U * 8, vec.x);
+      for (int j = 0; j < T::PER; j++) {
+        const int r = r0 + 256 / U * j, src = s_src[r];
+        xw[j] = raw8<E>(a, src >= 0 ? (const E *)a.x + (int64_t)src * a.ld_x : nullptr, s * 128 + q * 8, vec.x);
+      }
     }
   };
   const auto put_x = [&](uint8_t *buf) {
 #pragma unroll
     for (int j = 0; j < T::PER; j++) {
-      const int u = tid + 256 * j, r = u / U, q = u % U;
-      if (T::UNITS % 256 && u >= T::UNITS) break;
+      const int r = r0 + 256 / U * j;
+      if (MT * U % 256 && r >= MT) break;
       if constexpr (P == 0) {
-        *(uint4 *)(buf + (q >> 2) * T::PLANE + (r >> 4) * 1024 + frag_at(r & 15, q & 3)) = xc[j];
+        *(uint4 *)(buf + (q & 1) * T::PLANE + (r >> 4) * 1024 + frag_at(r & 15, q >> 1)) = xc[j];
       } else {
         uint8_t *dst = buf + (q & 3) * T::PLANE + (r >> 4) * 1024 + frag_at(r & 15, q >> 2);
         if constexpr (P == 1) *(uint4 *)dst = xw[j].v[0];
@@ -486,11 +497,7 @@ __global__ __launch_bounds__(256, 2) void k_mx4_tile(const Mx4Product a, const V
         }
       }
     }
-    if (P == 0 && tid < MT) {
-      uint32_t *sc = (uint32_t *)(buf + T::PLANES * T::PLANE);
-      sc[tid] = xsc[0];
-      sc[MT + tid] = xsc[1];
-    }
+    if (P == 0 && tid < MT) *(uint2 *)(buf + T::PLANES * T::PLANE + tid * 8) = make_uint2(xsc[0], xsc[1]);
   };
 
   f4v acc[MF][4] = {};
@@ -502,7 +509,9 @@ __global__ __launch_bounds__(256, 2) void k_mx4_tile(const Mx4Product a, const V
     if (T::BUFS == 1) __syncthreads();  // the last iteration's reads are done
     put_x(b);
 #pragma unroll
-    for (int t = 0; t < 4 * KS; t++) { w[t] = wn[t]; ws[t] = wsn[t]; }
+    for (int t = 0; t < 4 * KS; t++) w[t] = wn[t];
+#pragma unroll
+    for (int t = 0; t < 4; t++) ws[t] = wsn[t];
     __syncthreads();
     if (s + KS < a.steps) {
       load_x(s + KS);
@@ -510,20 +519,20 @@ __global__ __launch_bounds__(256, 2) void k_mx4_tile(const Mx4Product a, const V
     }
     if constexpr (P == 0) {
 #pragma unroll
-      for (int h = 0; h < 2; h++)
+      for (int f = 0; f < MF; f++) {
+        const i4v x0 = *(const i4v *)(b + f * 1024 + frag_at(m, g)), x1 = *(const i4v *)(b + T::PLANE + f * 1024 + frag_at(m, g));
+        const int sx = *(const uint16_t *)(b + T::PLANES * T::PLANE + (f * 16 + m) * 8 + g * 2);
 #pragma unroll
-        for (int f = 0; f < MF; f++) {
-          const i4v x = *(const i4v *)(b + h * T::PLANE + f * 1024 + frag_at(m, g));
-          const int sx = b[T::PLANES * T::PLANE + (h * MT + f * 16 + m) * 4 + g];
+        for (int t = 0; t < 4; t++) acc[f][t] = mfma_mx4<0>(w[t], (int)ws[t], x0, sx, acc[f][t]);
 #pragma unroll
-          for (int t = 0; t < 4; t++) acc[f][t] = mfma_mx4(w[h * 4 + t], ws[h * 4 + t], x, sx, acc[f][t]);
-        }
+        for (int t = 0; t < 4; t++) acc[f][t] = mfma_mx4<1>(w[4 + t], (int)ws[t], x1, sx, acc[f][t]);
+      }
     } else {
 #pragma unroll
       for (int c = 0; c < 4; c++) {
         b8v v[4];
 #pragma unroll
-        for (int t = 0; t < 4; t++) v[t] = values_of((uint32_t)w[t][c], __uint_as_float((uint32_t)ws[t] << 23));
+        for (int t = 0; t < 4; t++) v[t] = values_of((uint32_t)w[t][c], __uint_as_float(ws[t] << 23));
 #pragma unroll
         for (int f = 0; f < MF; f++)
 #pragma unroll
