@@ -76,14 +76,15 @@ __device__ __forceinline__ unsigned long long wave_max_u64(unsigned long long v)
   v = max_u64_x(v, false);
   return max_u64_x(v, true);
 }
-// Inclusive running sum over the wave's lanes.
+// Inclusive running sum over the wave's lanes: within rows of sixteen lanes by shifts, then each row's last
+// lane to the next row, the second row's to the upper half.
 __device__ __forceinline__ int wave_scan(int v) {
-  const int lane = threadIdx.x & 63;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const int u = __shfl_up(v, o);
-    if (lane >= o) v += u;
-  }
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);
   return v;
 }
 // Lane i's value of lane src (src wave-uniform).
