@@ -3,6 +3,8 @@
 //
 // The layout is the matrix cores': an instruction's 128 columns of a row are 64 bytes of codes and four scale
 // bytes, of which lane group g of a wave takes the g-th 16 bytes and the g-th scale, one block of 32.
+#include <atomic>
+
 #include "dev.h"
 #include "experts.h"
 #include "rows.h"
@@ -566,11 +568,139 @@ __global__ __launch_bounds__(256, 2) void k_mx4_tile(const Mx4Product a, const V
   }
 }
 
+// ------------------------------------------------------------------ products of many 4-bit rows
+// MT rows of x against 64 rows of the matrix a wave (gated: 32 of each), 256 a workgroup, 128 columns a step. Codes and
+// scales are copied to LDS without a register, the codes a step ahead, the scales eight steps at a time: whole
+// runs of a row, as neighbouring lanes' addresses. (A wave has its rows of the matrix to itself, but loading them straight
+// into its registers has neighbouring lanes in different rows: 4096^3 66 us instead of XX.)
+// In LDS a row's four pieces of 16 bytes stand at piece ^ (row / 2 & 3), so that what eight lanes read lies in other banks.
+template <int MT>
+struct FourLds {
+  uint8_t x[2][MT * 64], w[2][256 * 64];
+  uint32_t scales[2][MT + 256][8];  // of x's rows, then the matrix's
+};
+typedef __attribute__((address_space(3))) void *lds_ptr;
+// A wave's copies from memory to LDS: 16 or 4 bytes a lane, one lane's behind the other's.
+__device__ __forceinline__ void copy16_lds(const void *from, void *to) { __builtin_amdgcn_global_load_lds(from, (lds_ptr)to, 16, 0, 0); }
+__device__ __forceinline__ void copy4_lds(const void *from, void *to) { __builtin_amdgcn_global_load_lds(from, (lds_ptr)to, 4, 0, 0); }
+
+template <int MT, bool GATED>
+__global__ __launch_bounds__(256, 2) void k_mx4_four(const Mx4Product a, const Vecs vec, int out_type, int columns) {
+  constexpr int MF = MT / 16, WF = GATED ? 2 : 4, CHUNKS = (MT + 63) / 64;  // WF: fragments of out's columns a wave
+  constexpr int SCHUNKS = (MT + 256) / 32;
+  extern __shared__ __align__(16) uint8_t lds[];
+  __shared__ int s_src[MT];
+  FourLds<MT> &b = *(FourLds<MT> *)lds;
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, m = lane & 15, g = lane >> 4;
+  Tile tile;
+  int column;
+  if (!tile_place(a, MT, columns, tile, column)) return;
+  if (tid < MT) s_src[tid] = tid < tile.count ? source_of(a, tile.row + tid) : -1;
+  __syncthreads();
+  const int n0 = (column * 4 + wave) * (16 * WF);
+  const int64_t e0 = (int64_t)tile.expert * a.n;
+  // row r of the workgroup's 256 of the matrix is row r % 64 of wave r / 64, up's after w's
+  const auto matrix_row = [&](int r, bool &up) {
+    up = GATED && (r & 32);
+    return e0 + min((column * 4 + (r >> 6)) * (16 * WF) + (GATED ? r & 31 : r & 63), a.n - 1);
+  };
+  // a lane's place in the copies: of x (a row that there is none for: some row's, which is not stored) ...
+  const int r16 = lane >> 2, piece = ((lane & 3) ^ (lane >> 3 & 3)) * 16;
+  const uint8_t *xr[CHUNKS], *wr[4];
+#pragma unroll
+  for (int j = 0; j < CHUNKS; j++) {
+    const int r = (wave + 4 * j) * 16 + r16;
+    xr[j] = (const uint8_t *)a.x + (int64_t)(r < MT ? max(s_src[r], 0) : 0) * (a.steps * 64) + piece;
+  }
+  // ... and of the matrix
+#pragma unroll
+  for (int t = 0; t < 4; t++) {
+    bool up;
+    const int64_t row = matrix_row(wave * 64 + t * 16 + r16, up);
+    wr[t] = (up ? a.up.codes : a.w.codes) + row * (a.steps * 64) + piece;
+  }
+  const auto bring = [&](int s) {
+    const int at = s & 1;
+#pragma unroll
+    for (int j = 0; j < CHUNKS; j++)
+      if (MT >= 64 || wave * 16 < MT) copy16_lds(xr[j] + s * 64, b.x[at] + (wave + 4 * j) * 1024);
+#pragma unroll
+    for (int t = 0; t < 4; t++) copy16_lds(wr[t] + s * 64, b.w[at] + wave * 4096 + t * 1024);
+  };
+  const auto bring_scales = [&](int c) {  // steps 8c .. 8c + 7 (behind the last: the last again, which nothing uses)
+    const int s = min(c * 8 + (lane & 7), a.steps - 1);
+    for (int j = wave; j < SCHUNKS * 4; j += 4) {
+      const int r = j * 8 + (lane >> 3);
+      const uint8_t *from;
+      if (j * 8 < MT) from = a.x_scales + (int64_t)max(s_src[r], 0) * (a.steps * 4);
+      else {
+        bool up;
+        const int64_t row = matrix_row(r - MT, up);
+        from = (up ? a.up.scales : a.w.scales) + row * (a.steps * 4);
+      }
+      copy4_lds(from + s * 4, b.scales[c & 1][j * 8]);
+    }
+  };
+  f4v acc[MF][4] = {};
+  const int frag = m * 64 + (g ^ (m >> 1 & 3)) * 16;
+  bring(0);
+  bring_scales(0);
+  for (int s = 0; s < a.steps; s++) {
+    // what was brought is there, and the last step's reads of the other buffer are done
+    __builtin_amdgcn_s_waitcnt(0x0f70);
+    __syncthreads();
+    if (s + 1 < a.steps) bring(s + 1);
+    if ((s & 7) == 0 && s + 8 < a.steps) bring_scales((s >> 3) + 1);
+    const uint8_t *const x = b.x[s & 1] + frag, *const w = b.w[s & 1] + wave * 4096 + frag;
+    const uint8_t *const xs = (const uint8_t *)&b.scales[s >> 3 & 1][m][s & 7] + g, *const ws = xs + (MT + wave * 64) * 32;
+    i4v wv[4];
+    int wsv[4];
+#pragma unroll
+    for (int t = 0; t < 4; t++) {
+      wv[t] = *(const i4v *)(w + t * 1024);
+      wsv[t] = ws[t * 512];
+    }
+#pragma unroll
+    for (int f = 0; f < MF; f++) {
+      const i4v xv = *(const i4v *)(x + f * 1024);
+      const int xsv = xs[f * 512];
+#pragma unroll
+      for (int t = 0; t < 4; t++) acc[f][t] = mfma_mx4<0>(wv[t], wsv[t], xv, xsv, acc[f][t]);
+    }
+  }
+#pragma unroll
+  for (int f = 0; f < MF; f++) {
+    if (s_src[f * 16 + m] < 0) continue;
+#pragma unroll
+    for (int t = 0; t < WF; t++) {
+      f4v v = acc[f][t];
+      if (GATED)
+#pragma unroll
+        for (int j = 0; j < 4; j++) v[j] = silu(v[j]) * acc[f][(t + 2) & 3][j];
+      const int c = n0 + 16 * t + 4 * g;
+      if (c < a.n) put4_by(a, out_type, tile.row + f * 16 + m, c, v, vec.out);
+    }
+  }
+}
+
 // Tiles over the launch's second and third dimension.
 static dim3 tile_grid(int64_t columns, int64_t tiles) {
   const int64_t y = tiles < 32768 ? tiles : 32768;
   return dim3((unsigned)columns, (unsigned)y, (unsigned)((tiles + y - 1) / y));
 }
+
+// The devices on which a kernel has been allowed more than 64 KB of LDS.
+struct Allowed {
+  std::atomic<uint64_t> set{0};
+  hipError_t lds(const void *kernel, unsigned bytes) {
+    int dev = 0;
+    hipError_t e = hipGetDevice(&dev);
+    if (e != hipSuccess || bytes <= 65536 || (dev < 64 && (set.load() >> dev & 1))) return e;
+    e = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+    if (e == hipSuccess && dev < 64) set |= 1ull << dev;
+    return e;
+  }
+};
 
 template <class X, int MT>
 static hipError_t tiled(const Mx4Product &a, const Vecs &vec, int out_type, hipStream_t s) {
@@ -578,6 +708,15 @@ static hipError_t tiled(const Mx4Product &a, const Vecs &vec, int out_type, hipS
   const int wide = a.up.codes ? 128 : 256, columns = (a.n + wide - 1) / wide;
   const int64_t blocks = (tiles_most(a, MT) * columns + 7) / 8 * 8, x = blocks < 1 << 20 ? blocks : 1 << 20;
   const dim3 grid((unsigned)x, (unsigned)((blocks + x - 1) / x));
+  if constexpr (T::P == 0) {
+    constexpr unsigned four = sizeof(FourLds<MT>);
+    static Allowed gated, plain;
+    const void *f = a.up.codes ? (const void *)k_mx4_four<MT, true> : (const void *)k_mx4_four<MT, false>;
+    if (const hipError_t e = (a.up.codes ? gated : plain).lds(f, four); e != hipSuccess) return e;
+    if (a.up.codes) hipLaunchKernelGGL((k_mx4_four<MT, true>), grid, dim3(256), four, s, a, vec, out_type, columns);
+    else hipLaunchKernelGGL((k_mx4_four<MT, false>), grid, dim3(256), four, s, a, vec, out_type, columns);
+    return hipGetLastError();
+  }
   constexpr unsigned bytes = T::BUFS * T::BYTES;
   if (a.up.codes) hipLaunchKernelGGL((k_mx4_tile<X, MT, true>), grid, dim3(256), bytes, s, a, vec, out_type, columns);
   else hipLaunchKernelGGL((k_mx4_tile<X, MT, false>), grid, dim3(256), bytes, s, a, vec, out_type, columns);
