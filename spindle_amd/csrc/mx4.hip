@@ -570,24 +570,34 @@ __global__ __launch_bounds__(256, 2) void k_mx4_tile(const Mx4Product a, const V
 
 // ------------------------------------------------------------------ products of many 4-bit rows
 // MT rows of x against 64 rows of the matrix a wave (gated: 32 of each), 256 a workgroup, 128 columns a step. Codes and
-// scales are copied to LDS without a register, the codes a step ahead, the scales eight steps at a time: whole
+// scales are copied to LDS without a register, the codes two steps ahead, the scales four steps at a time: whole
 // runs of a row, as neighbouring lanes' addresses. (A wave has its rows of the matrix to itself, but loading them straight
-// into its registers has neighbouring lanes in different rows: 4096^3 66 us instead of XX.)
+// into its registers has neighbouring lanes in different rows: 4096^3 66 us instead of 54.)
 // In LDS a row's four pieces of 16 bytes stand at piece ^ (row / 2 & 3), so that what eight lanes read lies in other banks.
 template <int MT>
 struct FourLds {
-  uint8_t x[2][MT * 64], w[2][256 * 64];
-  uint32_t scales[2][MT + 256][8];  // of x's rows, then the matrix's
+  uint8_t x[3][MT * 64], w[3][256 * 64];
+  uint32_t scales[MT + 256][4];  // of x's rows, then the matrix's
 };
 typedef __attribute__((address_space(3))) void *lds_ptr;
 // A wave's copies from memory to LDS: 16 or 4 bytes a lane, one lane's behind the other's.
 __device__ __forceinline__ void copy16_lds(const void *from, void *to) { __builtin_amdgcn_global_load_lds(from, (lds_ptr)to, 16, 0, 0); }
 __device__ __forceinline__ void copy4_lds(const void *from, void *to) { __builtin_amdgcn_global_load_lds(from, (lds_ptr)to, 4, 0, 0); }
 
+// Waits until at most N of the wave's copies and loads are under way and its LDS accesses are done, then for the
+// workgroup's other waves. No access to memory moves across.
+template <int N>
+__device__ __forceinline__ void wait_and_meet() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt(0x0070 | N);  // (vmcnt in the low four bits, lgkmcnt 0)
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
 template <int MT, bool GATED>
 __global__ __launch_bounds__(256, 2) void k_mx4_four(const Mx4Product a, const Vecs vec, int out_type, int columns) {
   constexpr int MF = MT / 16, WF = GATED ? 2 : 4, CHUNKS = (MT + 63) / 64;  // WF: fragments of out's columns a wave
-  constexpr int SCHUNKS = (MT + 256) / 32;
+  constexpr int COPIES = CHUNKS + 4, SCOPIES = (MT + 256) / 64;             // a wave's copies of a step's codes, of four steps' scales
   extern __shared__ __align__(16) uint8_t lds[];
   __shared__ int s_src[MT];
   FourLds<MT> &b = *(FourLds<MT> *)lds;
@@ -606,66 +616,74 @@ __global__ __launch_bounds__(256, 2) void k_mx4_four(const Mx4Product a, const V
   };
   // a lane's place in the copies: of x (a row that there is none for: some row's, which is not stored) ...
   const int r16 = lane >> 2, piece = ((lane & 3) ^ (lane >> 3 & 3)) * 16;
-  const uint8_t *xr[CHUNKS], *wr[4];
+  const int xc = MT >= 64 ? wave : wave & (MT / 16 - 1);  // (few rows: two waves copy the same)
+  const uint8_t *xr[CHUNKS], *wr[4], *sr[SCOPIES];
 #pragma unroll
-  for (int j = 0; j < CHUNKS; j++) {
-    const int r = (wave + 4 * j) * 16 + r16;
-    xr[j] = (const uint8_t *)a.x + (int64_t)(r < MT ? max(s_src[r], 0) : 0) * (a.steps * 64) + piece;
-  }
-  // ... and of the matrix
+  for (int j = 0; j < CHUNKS; j++) xr[j] = (const uint8_t *)a.x + (int64_t)max(s_src[(xc + 4 * j) * 16 + r16], 0) * (a.steps * 64) + piece;
+  // ... of the matrix ...
 #pragma unroll
   for (int t = 0; t < 4; t++) {
     bool up;
     const int64_t row = matrix_row(wave * 64 + t * 16 + r16, up);
     wr[t] = (up ? a.up.codes : a.w.codes) + row * (a.steps * 64) + piece;
   }
-  const auto bring = [&](int s) {
-    const int at = s & 1;
+  // ... and of scales: sixteen rows' four steps a copy
 #pragma unroll
-    for (int j = 0; j < CHUNKS; j++)
-      if (MT >= 64 || wave * 16 < MT) copy16_lds(xr[j] + s * 64, b.x[at] + (wave + 4 * j) * 1024);
+  for (int j = 0; j < SCOPIES; j++) {
+    const int r = (wave + 4 * j) * 16 + r16;
+    if (r < MT) sr[j] = a.x_scales + (int64_t)max(s_src[r], 0) * (a.steps * 4);
+    else {
+      bool up;
+      const int64_t row = matrix_row(r - MT, up);
+      sr[j] = (up ? a.up.scales : a.w.scales) + row * (a.steps * 4);
+    }
+  }
+  const auto bring = [&](int s, int at) {
+#pragma unroll
+    for (int j = 0; j < CHUNKS; j++) copy16_lds(xr[j] + s * 64, b.x[at] + (xc + 4 * j) * 1024);
 #pragma unroll
     for (int t = 0; t < 4; t++) copy16_lds(wr[t] + s * 64, b.w[at] + wave * 4096 + t * 1024);
   };
-  const auto bring_scales = [&](int c) {  // steps 8c .. 8c + 7 (behind the last: the last again, which nothing uses)
-    const int s = min(c * 8 + (lane & 7), a.steps - 1);
-    for (int j = wave; j < SCHUNKS * 4; j += 4) {
-      const int r = j * 8 + (lane >> 3);
-      const uint8_t *from;
-      if (j * 8 < MT) from = a.x_scales + (int64_t)max(s_src[r], 0) * (a.steps * 4);
-      else {
-        bool up;
-        const int64_t row = matrix_row(r - MT, up);
-        from = (up ? a.up.scales : a.w.scales) + row * (a.steps * 4);
-      }
-      copy4_lds(from + s * 4, b.scales[c & 1][j * 8]);
-    }
+  const auto bring_scales = [&](int s0) {  // steps s0 .. s0 + 3 (behind the last: the last again, which nothing uses)
+    const int s = min(s0 + (lane & 3), a.steps - 1);
+#pragma unroll
+    for (int j = 0; j < SCOPIES; j++) copy4_lds(sr[j] + s * 4, b.scales[(wave + 4 * j) * 16]);
   };
   f4v acc[MF][4] = {};
+  i4v xsc[MF], wsc[4];  // a row's scales of four steps
   const int frag = m * 64 + (g ^ (m >> 1 & 3)) * 16;
-  bring(0);
   bring_scales(0);
-  for (int s = 0; s < a.steps; s++) {
-    // what was brought is there, and the last step's reads of the other buffer are done
-    __builtin_amdgcn_s_waitcnt(0x0f70);
-    __syncthreads();
-    if (s + 1 < a.steps) bring(s + 1);
-    if ((s & 7) == 0 && s + 8 < a.steps) bring_scales((s >> 3) + 1);
-    const uint8_t *const x = b.x[s & 1] + frag, *const w = b.w[s & 1] + wave * 4096 + frag;
-    const uint8_t *const xs = (const uint8_t *)&b.scales[s >> 3 & 1][m][s & 7] + g, *const ws = xs + (MT + wave * 64) * 32;
-    i4v wv[4];
-    int wsv[4];
+  bring(0, 0);
+  if (a.steps > 1) bring(1, 1);
+  int at = 0;  // s % 3
+  for (int s4 = 0; s4 < a.steps; s4 += 4) {
 #pragma unroll
-    for (int t = 0; t < 4; t++) {
-      wv[t] = *(const i4v *)(w + t * 1024);
-      wsv[t] = ws[t * 512];
-    }
+    for (int i = 0; i < 4; i++) {
+      const int s = s4 + i;
+      if (s >= a.steps) break;
+      // what this step reads has been brought, by every wave, and the reads of the last one's buffers are done: of the copies
+      // only the next step's may be under way
+      if (s + 1 < a.steps) wait_and_meet<COPIES>();
+      else wait_and_meet<0>();
+      if (i == 0) {
 #pragma unroll
-    for (int f = 0; f < MF; f++) {
-      const i4v xv = *(const i4v *)(x + f * 1024);
-      const int xsv = xs[f * 512];
+        for (int f = 0; f < MF; f++) xsc[f] = *(const i4v *)b.scales[f * 16 + m];
 #pragma unroll
-      for (int t = 0; t < 4; t++) acc[f][t] = mfma_mx4<0>(wv[t], wsv[t], xv, xsv, acc[f][t]);
+        for (int t = 0; t < 4; t++) wsc[t] = *(const i4v *)b.scales[MT + wave * 64 + t * 16 + m];
+      }
+      if (i == 1 && s4 + 4 < a.steps) bring_scales(s4 + 4);
+      if (s + 2 < a.steps) bring(s + 2, at ? at - 1 : 2);
+      const uint8_t *const x = b.x[at] + frag, *const w = b.w[at] + wave * 4096 + frag;
+      i4v wv[4];
+#pragma unroll
+      for (int t = 0; t < 4; t++) wv[t] = *(const i4v *)(w + t * 1024);
+#pragma unroll
+      for (int f = 0; f < MF; f++) {
+        const i4v xv = *(const i4v *)(x + f * 1024);
+#pragma unroll
+        for (int t = 0; t < 4; t++) acc[f][t] = mfma_mx4<0>(wv[t], wsc[t][i] >> (8 * g), xv, xsc[f][i] >> (8 * g), acc[f][t]);
+      }
+      at = at == 2 ? 0 : at + 1;
     }
   }
 #pragma unroll
