@@ -231,6 +231,15 @@ __device__ __forceinline__ f4v mfma_mx4(i4v w, int ws, i4v x, int xs, f4v acc) {
   return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(A, B, acc, 4, 4, BYTE, ws, BYTE, xs);
 }
 
+typedef float f16v __attribute__((ext_vector_type(16)));
+// 32 rows of the matrix against 32 of x, 64 columns: lane l has row l % 32 of either, block l / 32, and of the products
+// those of row l % 32 of x with rows 8 (i / 4) + 4 (l / 32) + i % 4 of the matrix. (These run at 7.3 PFLOP/s here, those of
+// 16 rows and 128 columns at 4.7 to 5.9; of the bf16 ones 32 x 32 x 16 at 2.1, 16 x 16 x 32 at 1.3 to 2.0.)
+__device__ __forceinline__ f16v mfma_mx4_32(i4v w, int ws, i4v x, int xs, f16v acc) {
+  const i8v A = {w[0], w[1], w[2], w[3], 0, 0, 0, 0}, B = {x[0], x[1], x[2], x[3], 0, 0, 0, 0};
+  return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(A, B, acc, 4, 4, 0, ws, 0, xs);
+}
+
 // v over 1 + exp(-v), with the hardware's exponential and reciprocal, each good to a unit in the last place (a division and
 // an exponential rounded correctly are forty instructions: a third of a gated tile's time). Below -87, where
 // the reciprocal leaves the normal numbers, a zero is as good: it is off by 87 * 2^-126 at most.
@@ -363,11 +372,12 @@ __device__ __forceinline__ bool tile_place(const Mx4Product &a, int most, int co
       tiles += lane_i(wave_scan(c), 63);
     }
   }
-  const int64_t all = (int64_t)tiles * columns, each = (all + 7) / 8, id = blockIdx.x + (int64_t)blockIdx.y * gridDim.x;
-  const int64_t at = (id & 7) * each + (id >> 3);
+  const uint64_t all = (uint64_t)tiles * columns, each = (all + 7) / 8, id = blockIdx.x + (uint64_t)blockIdx.y * gridDim.x;
+  const uint64_t at = (id & 7) * each + (id >> 3);
   if ((id >> 3) >= each || at >= all) return false;
-  tile = tile_of(a, (int)(at / columns), most);
-  column = (int)(at % columns);
+  const uint32_t t = all >> 32 ? (uint32_t)(at / columns) : (uint32_t)at / (uint32_t)columns;  // (the wide division is slow)
+  tile = tile_of(a, (int)t, most);
+  column = (int)(at - (uint64_t)t * columns);
   return tile.count > 0;
 }
 
@@ -573,17 +583,25 @@ __global__ __launch_bounds__(256, 2) void k_mx4_tile(const Mx4Product a, const V
 // scales are copied to LDS without a register, the codes two steps ahead, the scales four steps at a time: whole
 // runs of a row, as neighbouring lanes' addresses. (A wave has its rows of the matrix to itself, but loading them straight
 // into its registers has neighbouring lanes in different rows: 4096^3 66 us instead of 54.)
-// In LDS a row's four pieces of 16 bytes stand at piece ^ (row / 2 & 3), so that what eight lanes read lies in other banks.
+// In LDS a row's four pieces of 16 bytes stand at piece ^ (row / 4 & 3), so that what sixteen lanes read at a time (0-3, 12-15
+// and 20-27 of each half) lies in other banks; with row / 2 two of them meet, at half the rate.
 template <int MT>
 struct FourLds {
   uint8_t x[3][MT * 64], w[3][256 * 64];
   uint32_t scales[MT + 256][4];  // of x's rows, then the matrix's
 };
 typedef __attribute__((address_space(3))) void *lds_ptr;
-// A wave's copies from memory to LDS: 16 or 4 bytes a lane, one lane's behind the other's.
-__device__ __forceinline__ void copy16_lds(const void *from, void *to) { __builtin_amdgcn_global_load_lds(from, (lds_ptr)to, 16, 0, 0); }
-__device__ __forceinline__ void copy4_lds(const void *from, void *to) { __builtin_amdgcn_global_load_lds(from, (lds_ptr)to, 4, 0, 0); }
-
+// A wave's copies from memory to LDS: 16 or 4 bytes a lane, one lane's behind the other's. The address is the same for all
+// lanes but for `lane`, 32 bits.
+__device__ __forceinline__ rsrc_t from_here(const void *base) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void *>(base), 0, (int)0xffffffffu, 0x00020000);
+}
+__device__ __forceinline__ void copy16_lds(rsrc_t base, uint32_t lane, int all, void *to) {
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(base, (lds_ptr)to, 16, (int)lane, all, 0, 0);
+}
+__device__ __forceinline__ void copy4_lds(rsrc_t base, uint32_t lane, int all, void *to) {
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(base, (lds_ptr)to, 4, (int)lane, all, 0, 0);
+}
 // Waits until at most N of the wave's copies and loads are under way and its LDS accesses are done, then for the
 // workgroup's other waves. No access to memory moves across.
 template <int N>
@@ -595,109 +613,109 @@ __device__ __forceinline__ void wait_and_meet() {
 }
 
 template <int MT, bool GATED>
-__global__ __launch_bounds__(256, 2) void k_mx4_four(const Mx4Product a, const Vecs vec, int out_type, int columns) {
-  constexpr int MF = MT / 16, WF = GATED ? 2 : 4, CHUNKS = (MT + 63) / 64;  // WF: fragments of out's columns a wave
-  constexpr int COPIES = CHUNKS + 4, SCOPIES = (MT + 256) / 64;             // a wave's copies of a step's codes, of four steps' scales
+__global__ __launch_bounds__(MT == 128 ? 512 : 256, MT == 128 ? 4 : 2) void k_mx4_four(const Mx4Product a, const Vecs vec, int out_type, int columns) {
+  // a wave has MF * 32 rows and COLS of out's columns; WC: its copies of the matrix's codes a step
+  constexpr int WAVES = MT == 128 ? 8 : 4, MF = MT == 32 ? 1 : 2, COLS = GATED ? 32 : 64, WC = 16 / WAVES, COPIES = WC + 1;
   extern __shared__ __align__(16) uint8_t lds[];
   __shared__ int s_src[MT];
   FourLds<MT> &b = *(FourLds<MT> *)lds;
-  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, m = lane & 15, g = lane >> 4;
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, m = lane & 31, g = lane >> 5;
+  const int wm = wave >> 2, wn = wave & 3;
   Tile tile;
   int column;
   if (!tile_place(a, MT, columns, tile, column)) return;
-  if (tid < MT) s_src[tid] = tid < tile.count ? source_of(a, tile.row + tid) : -1;
+  int src = -1;
+  if (tid < MT && tid < tile.count) src = source_of(a, tile.row + tid);
+  const int n0 = (column * 4 + wn) * COLS;
+  // the matrix from the wave's first row on
+  const int first = min(n0, a.n - 1);
+  const int64_t row0 = (int64_t)tile.expert * a.n + first;
+  const rsrc_t wcodes = from_here(a.w.codes + row0 * (a.steps * 64)), wscales = from_here(a.w.scales + row0 * (a.steps * 4));
+  const rsrc_t ucodes = GATED ? from_here(a.up.codes + row0 * (a.steps * 64)) : wcodes, uscales = GATED ? from_here(a.up.scales + row0 * (a.steps * 4)) : wscales;
+  const rsrc_t xcodes = from_here(a.x), xscales = from_here(a.x_scales);
+  // a lane's place in the copies: sixteen rows each, of the wave's 64 rows of the matrix (gated: 32 of w, 32 of up; two waves
+  // share them where there are eight) ...
+  const int r16 = lane >> 2, piece = ((lane & 3) ^ (lane >> 4)) * 16, t0 = wm * WC;
+  uint32_t wrow[WC];  // rows times steps
+#pragma unroll
+  for (int j = 0; j < WC; j++) wrow[j] = (uint32_t)(min(n0 + ((t0 + j) * 16 & (COLS - 1)) + r16, a.n - 1) - first) * (uint32_t)a.steps;
+  const auto is_up = [&](int j) { return GATED && (WC == 4 ? j >= 2 : wm != 0); };
+  const auto bring_w = [&](int s, int at) {
+#pragma unroll
+    for (int j = 0; j < WC; j++) copy16_lds(is_up(j) ? ucodes : wcodes, wrow[j] * 64u + piece, s * 64, b.w[at] + wn * 4096 + (t0 + j) * 1024);
+  };
+  bring_w(0, 0);
+  if (a.steps > 1) bring_w(1, 1);
+  if (tid < MT) s_src[tid] = src;
   __syncthreads();
-  const int n0 = (column * 4 + wave) * (16 * WF);
-  const int64_t e0 = (int64_t)tile.expert * a.n;
-  // row r of the workgroup's 256 of the matrix is row r % 64 of wave r / 64, up's after w's
-  const auto matrix_row = [&](int r, bool &up) {
-    up = GATED && (r & 32);
-    return e0 + min((column * 4 + (r >> 6)) * (16 * WF) + (GATED ? r & 31 : r & 63), a.n - 1);
-  };
-  // a lane's place in the copies: of x (a row that there is none for: some row's, which is not stored) ...
-  const int r16 = lane >> 2, piece = ((lane & 3) ^ (lane >> 3 & 3)) * 16;
-  const int xc = MT >= 64 ? wave : wave & (MT / 16 - 1);  // (few rows: two waves copy the same)
-  const uint8_t *xr[CHUNKS], *wr[4], *sr[SCOPIES];
-#pragma unroll
-  for (int j = 0; j < CHUNKS; j++) xr[j] = (const uint8_t *)a.x + (int64_t)max(s_src[(xc + 4 * j) * 16 + r16], 0) * (a.steps * 64) + piece;
-  // ... of the matrix ...
-#pragma unroll
-  for (int t = 0; t < 4; t++) {
-    bool up;
-    const int64_t row = matrix_row(wave * 64 + t * 16 + r16, up);
-    wr[t] = (up ? a.up.codes : a.w.codes) + row * (a.steps * 64) + piece;
-  }
-  // ... and of scales: sixteen rows' four steps a copy
-#pragma unroll
-  for (int j = 0; j < SCOPIES; j++) {
-    const int r = (wave + 4 * j) * 16 + r16;
-    if (r < MT) sr[j] = a.x_scales + (int64_t)max(s_src[r], 0) * (a.steps * 4);
-    else {
-      bool up;
-      const int64_t row = matrix_row(r - MT, up);
-      sr[j] = (up ? a.up.scales : a.w.scales) + row * (a.steps * 4);
-    }
-  }
-  const auto bring = [&](int s, int at) {
-#pragma unroll
-    for (int j = 0; j < CHUNKS; j++) copy16_lds(xr[j] + s * 64, b.x[at] + (xc + 4 * j) * 1024);
-#pragma unroll
-    for (int t = 0; t < 4; t++) copy16_lds(wr[t] + s * 64, b.w[at] + wave * 4096 + t * 1024);
-  };
+  // ... and of x (a row that there is none for: some row's, which is not stored; of few rows two waves copy the same)
+  const int xc = wave & (MT / 16 - 1);
+  const uint32_t xrow = (uint32_t)max(s_src[xc * 16 + r16], 0) * (uint32_t)a.steps;
+  const auto bring_x = [&](int s, int at) { copy16_lds(xcodes, xrow * 64u + piece, s * 64, b.x[at] + xc * 1024); };
   const auto bring_scales = [&](int s0) {  // steps s0 .. s0 + 3 (behind the last: the last again, which nothing uses)
-    const int s = min(s0 + (lane & 3), a.steps - 1);
+    const int s = min(s0 + (lane & 3), a.steps - 1) * 4;
 #pragma unroll
-    for (int j = 0; j < SCOPIES; j++) copy4_lds(sr[j] + s * 4, b.scales[(wave + 4 * j) * 16]);
+    for (int j = 0; j < WC; j++) copy4_lds(is_up(j) ? uscales : wscales, wrow[j] * 4u + s, 0, b.scales[MT + wn * 64 + (t0 + j) * 16]);
+    copy4_lds(xscales, xrow * 4u + s, 0, b.scales[xc * 16]);
   };
-  f4v acc[MF][4] = {};
-  i4v xsc[MF], wsc[4];  // a row's scales of four steps
-  const int frag = m * 64 + (g ^ (m >> 1 & 3)) * 16;
   bring_scales(0);
-  bring(0, 0);
-  if (a.steps > 1) bring(1, 1);
-  int at = 0;  // s % 3
+  bring_x(0, 0);
+  if (a.steps > 1) bring_x(1, 1);
+  f16v acc[MF][2] = {};
+  i4v xsc[MF], wsc[2];  // a row's scales of four steps
+  int at = 0;           // s % 3
   for (int s4 = 0; s4 < a.steps; s4 += 4) {
 #pragma unroll
     for (int i = 0; i < 4; i++) {
       const int s = s4 + i;
       if (s >= a.steps) break;
       // what this step reads has been brought, by every wave, and the reads of the last one's buffers are done: of the copies
-      // only the next step's may be under way
-      if (s + 1 < a.steps) wait_and_meet<COPIES>();
-      else wait_and_meet<0>();
+      // only the next step's may be under way (before the first only x's of the second)
+      if (s + 1 >= a.steps) wait_and_meet<0>();
+      else if (s == 0) wait_and_meet<1>();
+      else wait_and_meet<COPIES>();
       if (i == 0) {
 #pragma unroll
-        for (int f = 0; f < MF; f++) xsc[f] = *(const i4v *)b.scales[f * 16 + m];
+        for (int f = 0; f < MF; f++) xsc[f] = *(const i4v *)b.scales[wm * 64 + f * 32 + m];
 #pragma unroll
-        for (int t = 0; t < 4; t++) wsc[t] = *(const i4v *)b.scales[MT + wave * 64 + t * 16 + m];
+        for (int t = 0; t < 2; t++) wsc[t] = *(const i4v *)b.scales[MT + wn * 64 + t * 32 + m];
       }
       if (i == 1 && s4 + 4 < a.steps) bring_scales(s4 + 4);
-      if (s + 2 < a.steps) bring(s + 2, at ? at - 1 : 2);
-      const uint8_t *const x = b.x[at] + frag, *const w = b.w[at] + wave * 4096 + frag;
-      i4v wv[4];
+      if (s + 2 < a.steps) {
+        bring_w(s + 2, at ? at - 1 : 2);
+        bring_x(s + 2, at ? at - 1 : 2);
+      }
+      const uint8_t *const x = b.x[at] + wm * 4096 + m * 64, *const w = b.w[at] + wn * 4096 + m * 64;
 #pragma unroll
-      for (int t = 0; t < 4; t++) wv[t] = *(const i4v *)(w + t * 1024);
+      for (int h = 0; h < 2; h++) {  // blocks 2h and 2h + 1
+        const int u = ((2 * h + g) ^ (m >> 2 & 3)) * 16;
+        i4v wv[2];
 #pragma unroll
-      for (int f = 0; f < MF; f++) {
-        const i4v xv = *(const i4v *)(x + f * 1024);
+        for (int t = 0; t < 2; t++) wv[t] = *(const i4v *)(w + t * 2048 + u);
 #pragma unroll
-        for (int t = 0; t < 4; t++) acc[f][t] = mfma_mx4<0>(wv[t], wsc[t][i] >> (8 * g), xv, xsc[f][i] >> (8 * g), acc[f][t]);
+        for (int f = 0; f < MF; f++) {
+          const i4v xv = *(const i4v *)(x + f * 2048 + u);
+#pragma unroll
+          for (int t = 0; t < 2; t++) acc[f][t] = mfma_mx4_32(wv[t], wsc[t][i] >> (16 * h + 8 * g), xv, xsc[f][i] >> (16 * h + 8 * g), acc[f][t]);
+        }
       }
       at = at == 2 ? 0 : at + 1;
     }
   }
 #pragma unroll
   for (int f = 0; f < MF; f++) {
-    if (s_src[f * 16 + m] < 0) continue;
+    const int r = wm * 64 + f * 32 + m;
+    if (s_src[r] < 0) continue;
 #pragma unroll
-    for (int t = 0; t < WF; t++) {
-      f4v v = acc[f][t];
-      if (GATED)
+    for (int t = 0; t < (GATED ? 1 : 2); t++)
 #pragma unroll
-        for (int j = 0; j < 4; j++) v[j] = silu(v[j]) * acc[f][(t + 2) & 3][j];
-      const int c = n0 + 16 * t + 4 * g;
-      if (c < a.n) put4_by(a, out_type, tile.row + f * 16 + m, c, v, vec.out);
-    }
+      for (int i = 0; i < 4; i++) {
+        f4v v;
+#pragma unroll
+        for (int j = 0; j < 4; j++) v[j] = GATED ? silu(acc[f][0][4 * i + j]) * acc[f][1][4 * i + j] : acc[f][t][4 * i + j];
+        const int c = n0 + 32 * t + 8 * i + 4 * g;
+        if (c < a.n) put4_by(a, out_type, tile.row + r, c, v, vec.out);
+      }
   }
 }
 
@@ -731,8 +749,8 @@ static hipError_t tiled(const Mx4Product &a, const Vecs &vec, int out_type, hipS
     static Allowed gated, plain;
     const void *f = a.up.codes ? (const void *)k_mx4_four<MT, true> : (const void *)k_mx4_four<MT, false>;
     if (const hipError_t e = (a.up.codes ? gated : plain).lds(f, four); e != hipSuccess) return e;
-    if (a.up.codes) hipLaunchKernelGGL((k_mx4_four<MT, true>), grid, dim3(256), four, s, a, vec, out_type, columns);
-    else hipLaunchKernelGGL((k_mx4_four<MT, false>), grid, dim3(256), four, s, a, vec, out_type, columns);
+    if (a.up.codes) hipLaunchKernelGGL((k_mx4_four<MT, true>), grid, dim3(MT == 128 ? 512 : 256), four, s, a, vec, out_type, columns);
+    else hipLaunchKernelGGL((k_mx4_four<MT, false>), grid, dim3(MT == 128 ? 512 : 256), four, s, a, vec, out_type, columns);
     return hipGetLastError();
   }
   constexpr unsigned bytes = T::BUFS * T::BYTES;
@@ -746,7 +764,8 @@ static hipError_t product(const Mx4Product &a, int out_type, hipStream_t s) {
   constexpr int RT = 2, MOST = X::PARTS <= 1 ? 128 : 64;
   const Vecs vec = {X::PARTS == 0 || on16(a.x, a.ld_x, sizeof(typename X::R::E)),
                     (uintptr_t)a.out % (out_type == T_F32 ? 16 : 8) == 0 && a.ld_out % 4 == 0};
-  const int64_t each = a.starts ? a.rows / a.n_expert : a.rows;  // rows of a matrix, where they are even
+  int64_t each = a.starts ? a.rows / a.n_expert : a.rows;  // rows of a matrix, where they are even
+  if (X::PARTS == 0 && (int64_t)a.x_rows * a.steps * 64 > UINT32_MAX) each = 0;  // (the tiles' addresses of x have 32 bits)
   if (each > 64 && MOST == 128) return tiled<X, MOST>(a, vec, out_type, s);
   if (each > 24) return tiled<X, 64>(a, vec, out_type, s);
   if (each > 8) return tiled<X, 32>(a, vec, out_type, s);

@@ -136,7 +136,8 @@ def check(got, x, w, up, kind, dtype):
     close(np.where(over, want, got), want, tol + R.rounding(np.abs(want) + tol, dtype), (x.shape, w.shape))
 
 
-SIZES = [(1, 1, 1), (1, 2048, 33), (2, 128, 16), (3, 100, 31), (16, 129, 64), (17, 576, 65), (33, 256, 129), (64, 1000, 40), (130, 384, 200), (257, 64, 300)]
+SIZES = [(1, 1, 1), (1, 2048, 33), (2, 128, 16), (3, 100, 31), (16, 129, 64), (17, 576, 65), (33, 256, 129), (64, 1000, 40), (130, 384, 200), (257, 64, 300),
+         (12, 640, 600), (40, 128, 600), (90, 260, 600), (200, 1100, 530)]
 
 
 @pytest.mark.parametrize("kind", [F32, F16, BF16, "mx4"])
@@ -182,7 +183,8 @@ def test_strides(ctx, kind, pad, off):
     assert (into[:, :off] == 5.0).all() and (into[:, off + n:] == 5.0).all()
 
 
-GROUPS = [(1, 8, 128, 128, 40), (5, 2, 4, 100, 33), (24, 8, 32, 256, 64), (100, 4, 6, 300, 100), (90, 8, 3, 64, 130), (300, 2, 5, 160, 72)]
+GROUPS = [(1, 8, 128, 128, 40), (5, 2, 4, 100, 33), (24, 8, 32, 256, 64), (100, 4, 6, 300, 100), (90, 8, 3, 64, 130), (300, 2, 5, 160, 72),
+          (40, 2, 4, 700, 530), (100, 4, 9, 200, 300)]
 
 
 @pytest.mark.parametrize("kind", [F32, F16, BF16, "mx4"])
