@@ -579,16 +579,20 @@ __global__ __launch_bounds__(256, 2) void k_mx4_tile(const Mx4Product a, const V
 }
 
 // ------------------------------------------------------------------ products of many 4-bit rows
-// MT rows of x against 64 rows of the matrix a wave (gated: 32 of each), 256 a workgroup, 128 columns a step. Codes and
-// scales are copied to LDS without a register, the codes two steps ahead, the scales four steps at a time: whole
-// runs of a row, as neighbouring lanes' addresses. (A wave has its rows of the matrix to itself, but loading them straight
-// into its registers has neighbouring lanes in different rows: 4096^3 66 us instead of 54.)
-// In LDS a row's four pieces of 16 bytes stand at piece ^ (row / 4 & 3), so that what sixteen lanes read at a time (0-3, 12-15
-// and 20-27 of each half) lies in other banks; with row / 2 two of them meet, at half the rate.
+// MT rows of x against 64 WN rows of the matrix (gated: half of them up's), 256 columns a turn, four waves of MF * 32 rows of x
+// and 64 of the matrix each. Codes and scales are copied to LDS without a register, the codes a turn ahead, the
+// scales two turns at a time: 128 bytes of a row, a whole cache line, as neighbouring lanes' addresses. Measured on 24 KB a
+// turn from the L2, in bytes a clock and CU: 57 so, 25 by half lines (the other half is fetched again the next time), 16
+// where neighbouring lanes are in different rows, as they are when a wave loads its own rows into registers.
+// In LDS a row's eight pieces of 16 bytes stand at piece ^ (row / 2 & 7), so that what sixteen lanes read at a time (0-3, 12-15
+// and 20-27 of each half) lies in other banks.
 template <int MT>
-struct FourLds {
-  uint8_t x[3][MT * 64], w[3][256 * 64];
-  uint32_t scales[MT + 256][4];  // of x's rows, then the matrix's
+struct Four {
+  static constexpr int WM = MT == 32 ? 1 : 2, WN = 4 / WM, MF = MT / 32 / WM, ROWS = WN * 64;
+  struct Lds {
+    uint8_t x[2][MT * 128], w[2][ROWS * 128];
+    uint32_t scales[MT + ROWS][4];  // of x's rows, then the matrix's
+  };
 };
 typedef __attribute__((address_space(3))) void *lds_ptr;
 // A wave's copies from memory to LDS: 16 or 4 bytes a lane, one lane's behind the other's. The address is the same for all
@@ -602,120 +606,173 @@ __device__ __forceinline__ void copy16_lds(rsrc_t base, uint32_t lane, int all, 
 __device__ __forceinline__ void copy4_lds(rsrc_t base, uint32_t lane, int all, void *to) {
   __builtin_amdgcn_raw_ptr_buffer_load_lds(base, (lds_ptr)to, 4, (int)lane, all, 0, 0);
 }
-// Waits until at most N of the wave's copies and loads are under way and its LDS accesses are done, then for the
-// workgroup's other waves. No access to memory moves across.
-template <int N>
+// Waits until the wave's copies, loads and LDS accesses are done, then for the workgroup's other waves. No access to
+// memory moves across.
 __device__ __forceinline__ void wait_and_meet() {
   asm volatile("" ::: "memory");
-  __builtin_amdgcn_s_waitcnt(0x0070 | N);  // (vmcnt in the low four bits, lgkmcnt 0)
+  __builtin_amdgcn_s_waitcnt(0x0070);  // (vmcnt and lgkmcnt 0)
   __builtin_amdgcn_s_barrier();
   asm volatile("" ::: "memory");
 }
 
+// 32 rows of COLS neighbouring columns of out from a wave's products (or the gated ones'), through LDS of its own: a lane has
+// four neighbours of a row, 8 or 16 bytes, and stored so each store would touch 32 rows. row(r): row r's number, -1: it is not stored.
+template <int COLS, class F, class G>
+__device__ __forceinline__ void put_rows(const Mx4Product &a, int out_type, bool vec, uint8_t *lds, int c0, F row, G value) {
+  const int lane = threadIdx.x & 63, m = lane & 31, g = lane >> 5;
+  const int size = out_type == T_F32 ? 4 : 2, pitch = COLS * size + 16;
+#pragma unroll
+  for (int t = 0; t < COLS / 32; t++)
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const f4v v = value(t, i);
+      uint8_t *const to = lds + m * pitch + (32 * t + 8 * i + 4 * g) * size;
+      if (out_type == T_F32) *(f4v *)to = v;
+      else if (out_type == T_F16) {
+        alignas(8) const _Float16 e[4] = {(_Float16)v[0], (_Float16)v[1], (_Float16)v[2], (_Float16)v[3]};
+        *(uint2 *)to = *(const uint2 *)e;
+      } else {
+        alignas(8) const __bf16 e[4] = {(__bf16)v[0], (__bf16)v[1], (__bf16)v[2], (__bf16)v[3]};
+        *(uint2 *)to = *(const uint2 *)e;
+      }
+    }
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  const int pieces = COLS * size / 16, each = 16 / size;
+  for (int p = lane; p < 32 * pieces; p += 64) {
+    const int r = p / pieces, q = p & (pieces - 1), i = row(r), c = c0 + q * each;
+    if (i < 0 || c >= a.n) continue;
+    const uint4 v = *(const uint4 *)(lds + r * pitch + q * 16);
+    uint8_t *const to = (uint8_t *)a.out + ((int64_t)i * a.ld_out + c) * size;
+    if (vec && c + each <= a.n) *(uint4 *)to = v;
+    else {
+      const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        if (size == 4) {
+          if (c + j < a.n) ((uint32_t *)to)[j] = w[j];
+        } else {
+          if (c + 2 * j < a.n) ((uint16_t *)to)[2 * j] = (uint16_t)w[j];
+          if (c + 2 * j + 1 < a.n) ((uint16_t *)to)[2 * j + 1] = (uint16_t)(w[j] >> 16);
+        }
+      }
+    }
+  }
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+
 template <int MT, bool GATED>
-__global__ __launch_bounds__(MT == 128 ? 512 : 256, MT == 128 ? 4 : 2) void k_mx4_four(const Mx4Product a, const Vecs vec, int out_type, int columns) {
-  // a wave has MF * 32 rows and COLS of out's columns; WC: its copies of the matrix's codes a step
-  constexpr int WAVES = MT == 128 ? 8 : 4, MF = MT == 32 ? 1 : 2, COLS = GATED ? 32 : 64, WC = 16 / WAVES, COPIES = WC + 1;
+__global__ __launch_bounds__(256, MT == 64 ? 3 : 2) void k_mx4_four(const Mx4Product a, const Vecs vec, int out_type, int columns) {
+  typedef Four<MT> T;
+  constexpr int MF = T::MF, WN = T::WN, COLS = GATED ? 32 : 64, WC = 2 * WN, XC = MT / 32;  // WC, XC: a wave's copies a turn
   extern __shared__ __align__(16) uint8_t lds[];
   __shared__ int s_src[MT];
-  FourLds<MT> &b = *(FourLds<MT> *)lds;
+  typename T::Lds &b = *(typename T::Lds *)lds;
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, m = lane & 31, g = lane >> 5;
-  const int wm = wave >> 2, wn = wave & 3;
+  const int wm = wave / WN, wn = wave % WN;
   Tile tile;
   int column;
   if (!tile_place(a, MT, columns, tile, column)) return;
   int src = -1;
   if (tid < MT && tid < tile.count) src = source_of(a, tile.row + tid);
-  const int n0 = (column * 4 + wn) * COLS;
-  // the matrix from the wave's first row on
-  const int first = min(n0, a.n - 1);
-  const int64_t row0 = (int64_t)tile.expert * a.n + first;
+  const int col0 = column * WN * COLS;
+  // the matrix from the workgroup's first row on
+  const int64_t row0 = (int64_t)tile.expert * a.n + col0;
   const rsrc_t wcodes = from_here(a.w.codes + row0 * (a.steps * 64)), wscales = from_here(a.w.scales + row0 * (a.steps * 4));
   const rsrc_t ucodes = GATED ? from_here(a.up.codes + row0 * (a.steps * 64)) : wcodes, uscales = GATED ? from_here(a.up.scales + row0 * (a.steps * 4)) : wscales;
   const rsrc_t xcodes = from_here(a.x), xscales = from_here(a.x_scales);
-  // a lane's place in the copies: sixteen rows each, of the wave's 64 rows of the matrix (gated: 32 of w, 32 of up; two waves
-  // share them where there are eight) ...
-  const int r16 = lane >> 2, piece = ((lane & 3) ^ (lane >> 4)) * 16, t0 = wm * WC;
+  // A wave copies 8 WC rows of the matrix from row `from` on, eight at a time; row r stands for wave column r / 64, its
+  // (r % 64)-th, gated: of w the first half of these, of up the second.
+  const int from = wave * (8 * WC), r8 = lane >> 3;
   uint32_t wrow[WC];  // rows times steps
 #pragma unroll
-  for (int j = 0; j < WC; j++) wrow[j] = (uint32_t)(min(n0 + ((t0 + j) * 16 & (COLS - 1)) + r16, a.n - 1) - first) * (uint32_t)a.steps;
-  const auto is_up = [&](int j) { return GATED && (WC == 4 ? j >= 2 : wm != 0); };
+  for (int j = 0; j < WC; j++) {
+    const int r = from + 8 * j + r8;
+    wrow[j] = (uint32_t)min((r >> 6) * COLS + (r & (COLS - 1)), a.n - 1 - col0) * (uint32_t)a.steps;
+  }
+  const auto is_up = [&](int j) { return GATED && (WC == 8 ? j >= 4 : (wave & 1) != 0); };
+  // the piece of a row that a lane copies (the last turn may have half of a row: that twice, the second one unused)
+  const auto piece = [&](int j, int s) {
+    const int p = (lane & 7) ^ (((j & 1) << 2) | (lane >> 4));
+    return (uint32_t)(s + 1 < a.steps ? p : p & 3) * 16u;
+  };
   const auto bring_w = [&](int s, int at) {
 #pragma unroll
-    for (int j = 0; j < WC; j++) copy16_lds(is_up(j) ? ucodes : wcodes, wrow[j] * 64u + piece, s * 64, b.w[at] + wn * 4096 + (t0 + j) * 1024);
+    for (int j = 0; j < WC; j++) copy16_lds(is_up(j) ? ucodes : wcodes, wrow[j] * 64u + piece(j, s), s * 64, b.w[at] + (from + 8 * j) * 128);
   };
   bring_w(0, 0);
-  if (a.steps > 1) bring_w(1, 1);
   if (tid < MT) s_src[tid] = src;
   __syncthreads();
-  // ... and of x (a row that there is none for: some row's, which is not stored; of few rows two waves copy the same)
-  const int xc = wave & (MT / 16 - 1);
-  const uint32_t xrow = (uint32_t)max(s_src[xc * 16 + r16], 0) * (uint32_t)a.steps;
-  const auto bring_x = [&](int s, int at) { copy16_lds(xcodes, xrow * 64u + piece, s * 64, b.x[at] + xc * 1024); };
-  const auto bring_scales = [&](int s0) {  // steps s0 .. s0 + 3 (behind the last: the last again, which nothing uses)
-    const int s = min(s0 + (lane & 3), a.steps - 1) * 4;
+  // ... and XC times eight rows of x (one that there is none for: some row, which is not stored)
+  uint32_t xrow[XC];
 #pragma unroll
-    for (int j = 0; j < WC; j++) copy4_lds(is_up(j) ? uscales : wscales, wrow[j] * 4u + s, 0, b.scales[MT + wn * 64 + (t0 + j) * 16]);
-    copy4_lds(xscales, xrow * 4u + s, 0, b.scales[xc * 16]);
+  for (int j = 0; j < XC; j++) xrow[j] = (uint32_t)max(s_src[(wave * XC + j) * 8 + r8], 0) * (uint32_t)a.steps;
+  const auto bring_x = [&](int s, int at) {
+#pragma unroll
+    for (int j = 0; j < XC; j++) copy16_lds(xcodes, xrow[j] * 64u + piece(wave * XC + j, s), s * 64, b.x[at] + (wave * XC + j) * 1024);
+  };
+  // scales of steps s0 .. s0 + 3 (behind the last: the last again, which nothing uses), sixteen rows a copy
+  const auto bring_scales = [&](int s0) {
+    const int s = min(s0 + (lane & 3), a.steps - 1) * 4, r16 = lane >> 2;
+#pragma unroll
+    for (int j = 0; j < WC / 2; j++) {
+      const int r = from + 16 * j + r16;
+      const uint32_t row = (uint32_t)min((r >> 6) * COLS + (r & (COLS - 1)), a.n - 1 - col0) * (uint32_t)a.steps;
+      copy4_lds(is_up(2 * j) ? uscales : wscales, row * 4u + s, 0, b.scales[MT + from + 16 * j]);
+    }
+    for (int j = wave; j < MT / 16; j += 4) copy4_lds(xscales, (uint32_t)max(s_src[j * 16 + r16], 0) * (uint32_t)a.steps * 4u + s, 0, b.scales[j * 16]);
   };
   bring_scales(0);
   bring_x(0, 0);
-  if (a.steps > 1) bring_x(1, 1);
   f16v acc[MF][2] = {};
   i4v xsc[MF], wsc[2];  // a row's scales of four steps
-  int at = 0;           // s % 3
   for (int s4 = 0; s4 < a.steps; s4 += 4) {
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-      const int s = s4 + i;
+    for (int i = 0; i < 2; i++) {
+      const int s = s4 + 2 * i;
       if (s >= a.steps) break;
-      // what this step reads has been brought, by every wave, and the reads of the last one's buffers are done: of the copies
-      // only the next step's may be under way (before the first only x's of the second)
-      if (s + 1 >= a.steps) wait_and_meet<0>();
-      else if (s == 0) wait_and_meet<1>();
-      else wait_and_meet<COPIES>();
+      // what this turn reads has been brought, by every wave, and the reads of the last one's buffers are done
+      wait_and_meet();
       if (i == 0) {
 #pragma unroll
-        for (int f = 0; f < MF; f++) xsc[f] = *(const i4v *)b.scales[wm * 64 + f * 32 + m];
+        for (int f = 0; f < MF; f++) xsc[f] = *(const i4v *)b.scales[(wm * MF + f) * 32 + m];
 #pragma unroll
         for (int t = 0; t < 2; t++) wsc[t] = *(const i4v *)b.scales[MT + wn * 64 + t * 32 + m];
       }
       if (i == 1 && s4 + 4 < a.steps) bring_scales(s4 + 4);
       if (s + 2 < a.steps) {
-        bring_w(s + 2, at ? at - 1 : 2);
-        bring_x(s + 2, at ? at - 1 : 2);
+        bring_w(s + 2, i ^ 1);
+        bring_x(s + 2, i ^ 1);
       }
-      const uint8_t *const x = b.x[at] + wm * 4096 + m * 64, *const w = b.w[at] + wn * 4096 + m * 64;
+      const uint8_t *const x = b.x[i] + wm * MF * 4096 + m * 128, *const w = b.w[i] + wn * 8192 + m * 128;
 #pragma unroll
-      for (int h = 0; h < 2; h++) {  // blocks 2h and 2h + 1
-        const int u = ((2 * h + g) ^ (m >> 2 & 3)) * 16;
+      for (int h = 0; h < 4; h++) {  // blocks 2h and 2h + 1
+        if (h == 2 && s + 1 >= a.steps) break;
+        const int u = ((2 * h + g) ^ (m >> 1 & 7)) * 16, j = 2 * i + (h >> 1), shift = 16 * (h & 1) + 8 * g;
         i4v wv[2];
 #pragma unroll
-        for (int t = 0; t < 2; t++) wv[t] = *(const i4v *)(w + t * 2048 + u);
+        for (int t = 0; t < 2; t++) wv[t] = *(const i4v *)(w + t * 4096 + u);
 #pragma unroll
         for (int f = 0; f < MF; f++) {
-          const i4v xv = *(const i4v *)(x + f * 2048 + u);
+          const i4v xv = *(const i4v *)(x + f * 4096 + u);
 #pragma unroll
-          for (int t = 0; t < 2; t++) acc[f][t] = mfma_mx4_32(wv[t], wsc[t][i] >> (16 * h + 8 * g), xv, xsc[f][i] >> (16 * h + 8 * g), acc[f][t]);
+          for (int t = 0; t < 2; t++) acc[f][t] = mfma_mx4_32(wv[t], wsc[t][j] >> shift, xv, xsc[f][j] >> shift, acc[f][t]);
         }
       }
-      at = at == 2 ? 0 : at + 1;
     }
   }
+  wait_and_meet();  // (all waves' reads of LDS are done)
 #pragma unroll
   for (int f = 0; f < MF; f++) {
-    const int r = wm * 64 + f * 32 + m;
-    if (s_src[r] < 0) continue;
+    const int r0 = (wm * MF + f) * 32;
+    put_rows<COLS>(a, out_type, vec.out, lds + wave * 9216, col0 + wn * COLS, [&](int r) { return s_src[r0 + r] < 0 ? -1 : tile.row + r0 + r; },
+                   [&](int t, int i) {
+                     f4v v;
 #pragma unroll
-    for (int t = 0; t < (GATED ? 1 : 2); t++)
-#pragma unroll
-      for (int i = 0; i < 4; i++) {
-        f4v v;
-#pragma unroll
-        for (int j = 0; j < 4; j++) v[j] = GATED ? silu(acc[f][0][4 * i + j]) * acc[f][1][4 * i + j] : acc[f][t][4 * i + j];
-        const int c = n0 + 32 * t + 8 * i + 4 * g;
-        if (c < a.n) put4_by(a, out_type, tile.row + r, c, v, vec.out);
-      }
+                     for (int j = 0; j < 4; j++) v[j] = GATED ? silu(acc[f][0][4 * i + j]) * acc[f][1][4 * i + j] : acc[f][t][4 * i + j];
+                     return v;
+                   });
   }
 }
 
@@ -741,16 +798,17 @@ struct Allowed {
 template <class X, int MT>
 static hipError_t tiled(const Mx4Product &a, const Vecs &vec, int out_type, hipStream_t s) {
   typedef TileX<X, MT> T;
-  const int wide = a.up.codes ? 128 : 256, columns = (a.n + wide - 1) / wide;
+  const int wide = (T::P == 0 ? Four<MT>::ROWS : 256) / (a.up.codes ? 2 : 1), columns = (a.n + wide - 1) / wide;
   const int64_t blocks = (tiles_most(a, MT) * columns + 7) / 8 * 8, x = blocks < 1 << 20 ? blocks : 1 << 20;
   const dim3 grid((unsigned)x, (unsigned)((blocks + x - 1) / x));
   if constexpr (T::P == 0) {
-    constexpr unsigned four = sizeof(FourLds<MT>);
+    constexpr unsigned four = sizeof(typename Four<MT>::Lds);
     static Allowed gated, plain;
     const void *f = a.up.codes ? (const void *)k_mx4_four<MT, true> : (const void *)k_mx4_four<MT, false>;
     if (const hipError_t e = (a.up.codes ? gated : plain).lds(f, four); e != hipSuccess) return e;
-    if (a.up.codes) hipLaunchKernelGGL((k_mx4_four<MT, true>), grid, dim3(MT == 128 ? 512 : 256), four, s, a, vec, out_type, columns);
-    else hipLaunchKernelGGL((k_mx4_four<MT, false>), grid, dim3(MT == 128 ? 512 : 256), four, s, a, vec, out_type, columns);
+    const Vecs v16 = {1, on16(a.out, a.ld_out, out_type == T_F32 ? 4 : 2)};
+    if (a.up.codes) hipLaunchKernelGGL((k_mx4_four<MT, true>), grid, dim3(256), four, s, a, v16, out_type, columns);
+    else hipLaunchKernelGGL((k_mx4_four<MT, false>), grid, dim3(256), four, s, a, v16, out_type, columns);
     return hipGetLastError();
   }
   constexpr unsigned bytes = T::BUFS * T::BYTES;
