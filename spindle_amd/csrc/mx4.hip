@@ -4,6 +4,7 @@
 // The layout is the matrix cores': an instruction's 128 columns of a row are 64 bytes of codes and four scale
 // bytes, of which lane group g of a wave takes the g-th 16 bytes and the g-th scale, one block of 32.
 #include <atomic>
+#include <type_traits>
 
 #include "dev.h"
 #include "experts.h"
@@ -355,30 +356,65 @@ __global__ __launch_bounds__(256) void k_mx4_rows(const Mx4Product a, const Vecs
 // r and lane group g at 64 r + 16 (g ^ (r / 2 & 3)), which spreads what eight lanes read or write over the banks.
 __device__ __forceinline__ int frag_at(int r, int g) { return r * 64 + ((g ^ (r >> 1 & 3)) * 16); }
 
-// Tiles' order: those of one expert and row tile lie beside each other on one XCD (workgroups go to the eight in turn),
-// so that its L2 gives the rows of x and the matrices again. False: there is no such tile.
+// Where a workgroup works. Tiles of one expert and row tile lie beside each other on one XCD (workgroups go to the eight in
+// turn), so that its L2 gives the rows of x and the matrices again. False: there is no such tile.
 __device__ __forceinline__ bool tile_place(const Mx4Product &a, int most, int columns, Tile &tile, int &column) {
-  int tiles = 0;
-  if (!a.starts) tiles = (a.rows + most - 1) / most;
-  else {
-    const int lane = threadIdx.x & 63;
+  const int lane = threadIdx.x & 63;
+  const uint64_t id = blockIdx.x + (uint64_t)blockIdx.y * gridDim.x;
+  const auto at_of = [&](int tiles, int &t) {  // which of `tiles` tiles of rows is the workgroup's, and which column
+    const uint64_t all = (uint64_t)tiles * columns, each = (all + 7) / 8, at = (id & 7) * each + (id >> 3);
+    if ((id >> 3) >= each || at >= all) return false;
+    t = (int)(all >> 32 ? at / columns : (uint32_t)at / (uint32_t)columns);  // (the wide division is slow)
+    column = (int)(at - (uint64_t)t * columns);
+    return true;
+  };
+  int t;
+  if (!a.starts) {
+    if (!at_of((a.rows + most - 1) / most, t)) return false;
+    tile = tile_of(a, t, most);
+    return true;
+  }
+  const auto experts = [&](int b, int &lo, int &tiles) {  // a lane's expert b + lane: its first row, its tiles
+    const int e = b + lane;
+    lo = 0;
+    int hi = 0;
+    if (e < a.n_expert) {
+      lo = min(max(a.starts[e], 0), a.rows);
+      hi = min(max(a.starts[e + 1], lo), a.rows);
+    }
+    tiles = (hi - lo + most - 1) / most;
+    return hi;
+  };
+  if (a.n_expert > 256) {
+    int all = 0;
     for (int b = 0; b < a.n_expert; b += 64) {
-      const int e = b + lane;
-      int c = 0;
-      if (e < a.n_expert) {
-        const int lo = min(max(a.starts[e], 0), a.rows);
-        c = (min(max(a.starts[e + 1], lo), a.rows) - lo + most - 1) / most;
-      }
-      tiles += lane_i(wave_scan(c), 63);
+      int lo, tiles;
+      experts(b, lo, tiles);
+      all += lane_i(wave_scan(tiles), 63);
+    }
+    if (!at_of(all, t)) return false;
+    tile = tile_of(a, t, most);
+    return tile.count > 0;
+  }
+  int lo[4], hi[4], tiles[4], upto[4], all = 0;  // (all loads under way at once, each made once)
+#pragma unroll
+  for (int c = 0; c < 4; c++) hi[c] = experts(64 * c, lo[c], tiles[c]);
+#pragma unroll
+  for (int c = 0; c < 4; c++) {
+    upto[c] = all + wave_scan(tiles[c]);
+    all = lane_i(upto[c], 63);
+  }
+  if (!at_of(all, t)) return false;
+#pragma unroll
+  for (int c = 0; c < 4; c++) {
+    const unsigned long long past = __builtin_amdgcn_ballot_w64(upto[c] > t);
+    if (past) {
+      const int l = (int)__builtin_ctzll(past), r = lane_i(lo[c], l) + (t - (lane_i(upto[c], l) - lane_i(tiles[c], l))) * most;
+      tile = {64 * c + l, r, min(most, lane_i(hi[c], l) - r)};
+      return true;
     }
   }
-  const uint64_t all = (uint64_t)tiles * columns, each = (all + 7) / 8, id = blockIdx.x + (uint64_t)blockIdx.y * gridDim.x;
-  const uint64_t at = (id & 7) * each + (id >> 3);
-  if ((id >> 3) >= each || at >= all) return false;
-  const uint32_t t = all >> 32 ? (uint32_t)(at / columns) : (uint32_t)at / (uint32_t)columns;  // (the wide division is slow)
-  tile = tile_of(a, (int)t, most);
-  column = (int)(at - (uint64_t)t * columns);
-  return tile.count > 0;
+  return false;
 }
 
 // Eight columns of a row of x as they lie in memory, zeros behind the last and where there is no row.
@@ -710,7 +746,8 @@ __global__ __launch_bounds__(256, MT == 64 ? 3 : 2) void k_mx4_four(const Mx4Pro
   for (int j = 0; j < XC; j++) xrow[j] = (uint32_t)max(s_src[(wave * XC + j) * 8 + r8], 0) * (uint32_t)a.steps;
   const auto bring_x = [&](int s, int at) {
 #pragma unroll
-    for (int j = 0; j < XC; j++) copy16_lds(xcodes, xrow[j] * 64u + piece(wave * XC + j, s), s * 64, b.x[at] + (wave * XC + j) * 1024);
+    for (int j = 0; j < XC; j++)
+      if ((wave * XC + j) * 8 < tile.count) copy16_lds(xcodes, xrow[j] * 64u + piece(wave * XC + j, s), s * 64, b.x[at] + (wave * XC + j) * 1024);
   };
   // scales of steps s0 .. s0 + 3 (behind the last: the last again, which nothing uses), sixteen rows a copy
   const auto bring_scales = [&](int s0) {
@@ -727,45 +764,55 @@ __global__ __launch_bounds__(256, MT == 64 ? 3 : 2) void k_mx4_four(const Mx4Pro
   bring_x(0, 0);
   f16v acc[MF][2] = {};
   i4v xsc[MF], wsc[2];  // a row's scales of four steps
-  for (int s4 = 0; s4 < a.steps; s4 += 4) {
+  // LIVE: the wave's fragments of x that have rows (what the others hold is never stored)
+  const auto turns = [&](auto live) {
+    constexpr int LIVE = decltype(live)::value;
+    for (int s4 = 0; s4 < a.steps; s4 += 4) {
 #pragma unroll
-    for (int i = 0; i < 2; i++) {
-      const int s = s4 + 2 * i;
-      if (s >= a.steps) break;
-      // what this turn reads has been brought, by every wave, and the reads of the last one's buffers are done
-      wait_and_meet();
-      if (i == 0) {
+      for (int i = 0; i < 2; i++) {
+        const int s = s4 + 2 * i;
+        if (s >= a.steps) break;
+        // what this turn reads has been brought, by every wave, and the reads of the last one's buffers are done
+        wait_and_meet();
+        if (i == 0) {
 #pragma unroll
-        for (int f = 0; f < MF; f++) xsc[f] = *(const i4v *)b.scales[(wm * MF + f) * 32 + m];
+          for (int f = 0; f < LIVE; f++) xsc[f] = *(const i4v *)b.scales[(wm * MF + f) * 32 + m];
 #pragma unroll
-        for (int t = 0; t < 2; t++) wsc[t] = *(const i4v *)b.scales[MT + wn * 64 + t * 32 + m];
-      }
-      if (i == 1 && s4 + 4 < a.steps) bring_scales(s4 + 4);
-      if (s + 2 < a.steps) {
-        bring_w(s + 2, i ^ 1);
-        bring_x(s + 2, i ^ 1);
-      }
-      const uint8_t *const x = b.x[i] + wm * MF * 4096 + m * 128, *const w = b.w[i] + wn * 8192 + m * 128;
+          for (int t = 0; t < 2; t++) wsc[t] = *(const i4v *)b.scales[MT + wn * 64 + t * 32 + m];
+        }
+        if (i == 1 && s4 + 4 < a.steps) bring_scales(s4 + 4);
+        if (s + 2 < a.steps) {
+          bring_w(s + 2, i ^ 1);
+          bring_x(s + 2, i ^ 1);
+        }
+        if (LIVE == 0) continue;
+        const uint8_t *const x = b.x[i] + wm * MF * 4096 + m * 128, *const w = b.w[i] + wn * 8192 + m * 128;
 #pragma unroll
-      for (int h = 0; h < 4; h++) {  // blocks 2h and 2h + 1
-        if (h == 2 && s + 1 >= a.steps) break;
-        const int u = ((2 * h + g) ^ (m >> 1 & 7)) * 16, j = 2 * i + (h >> 1), shift = 16 * (h & 1) + 8 * g;
-        i4v wv[2];
+        for (int h = 0; h < 4; h++) {  // blocks 2h and 2h + 1
+          if (h == 2 && s + 1 >= a.steps) break;
+          const int u = ((2 * h + g) ^ (m >> 1 & 7)) * 16, j = 2 * i + (h >> 1), shift = 16 * (h & 1) + 8 * g;
+          i4v wv[2];
 #pragma unroll
-        for (int t = 0; t < 2; t++) wv[t] = *(const i4v *)(w + t * 4096 + u);
+          for (int t = 0; t < 2; t++) wv[t] = *(const i4v *)(w + t * 4096 + u);
 #pragma unroll
-        for (int f = 0; f < MF; f++) {
-          const i4v xv = *(const i4v *)(x + f * 4096 + u);
+          for (int f = 0; f < LIVE; f++) {
+            const i4v xv = *(const i4v *)(x + f * 4096 + u);
 #pragma unroll
-          for (int t = 0; t < 2; t++) acc[f][t] = mfma_mx4_32(wv[t], wsc[t][j] >> shift, xv, xsc[f][j] >> shift, acc[f][t]);
+            for (int t = 0; t < 2; t++) acc[f][t] = mfma_mx4_32(wv[t], wsc[t][j] >> shift, xv, xsc[f][j] >> shift, acc[f][t]);
+          }
         }
       }
     }
-  }
+  };
+  const int rows = tile.count - wm * MF * 32;
+  if (MF == 2 && rows > 32) turns(std::integral_constant<int, MF>{});
+  else if (rows > 0) turns(std::integral_constant<int, 1>{});
+  else turns(std::integral_constant<int, 0>{});
   wait_and_meet();  // (all waves' reads of LDS are done)
 #pragma unroll
   for (int f = 0; f < MF; f++) {
     const int r0 = (wm * MF + f) * 32;
+    if (r0 >= tile.count) break;
     put_rows<COLS>(a, out_type, vec.out, lds + wave * 9216, col0 + wn * COLS, [&](int r) { return s_src[r0 + r] < 0 ? -1 : tile.row + r0 + r; },
                    [&](int t, int i) {
                      f4v v;
