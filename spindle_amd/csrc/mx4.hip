@@ -349,13 +349,6 @@ __global__ __launch_bounds__(256) void k_mx4_rows(const Mx4Product a, const Vecs
   }
 }
 
-// ------------------------------------------------------------------ products of many rows
-// MT rows of x against 64 rows of the matrix a wave (gated: 32 of each), 256 a workgroup. A wave's rows of the matrix are
-// its own, so their codes come straight from memory into its registers, an iteration ahead; the rows of x are all four
-// waves' and go through LDS as the matrix instructions take them: 16 rows x 64 bytes a fragment, the 16 bytes of row
-// r and lane group g at 64 r + 16 (g ^ (r / 2 & 3)), which spreads what eight lanes read or write over the banks.
-__device__ __forceinline__ int frag_at(int r, int g) { return r * 64 + ((g ^ (r >> 1 & 3)) * 16); }
-
 // Where a workgroup works. Tiles of one expert and row tile lie beside each other on one XCD (workgroups go to the eight in
 // turn), so that its L2 gives the rows of x and the matrices again. False: there is no such tile.
 __device__ __forceinline__ bool tile_place(const Mx4Product &a, int most, int columns, Tile &tile, int &column) {
@@ -436,184 +429,6 @@ __device__ __forceinline__ Raw8<E> raw8(const Mx4Product &a, const E *row, int c
   return r;
 }
 
-template <class X, int MT>
-struct TileX {
-  static constexpr int P = X::PARTS, KS = P == 0 ? 2 : 1;              // steps of 128 columns an iteration
-  static constexpr int PLANES = P == 0 ? 2 : 4 * P;                    // fragments of 64 bytes a row
-  static constexpr int PLANE = MT * 64 + 64;                           // (planes start 16 banks apart)
-  static constexpr int U = P == 0 ? 8 : 16;                            // a row's pieces of 16 bytes, or of eight columns, an iteration
-  static constexpr int PER = (MT * U + 255) / 256;
-  static constexpr int SCALES = P == 0 ? MT * 8 : 0;
-  static constexpr int BYTES = PLANES * PLANE + SCALES;
-  static constexpr int BUFS = 2 * BYTES <= 65536 ? 2 : 1;
-};
-
-// Of an iteration's 256 columns of 4-bit rows lane group g takes blocks 2g and 2g + 1, one an instruction: 32
-// bytes of codes that lie together and two scale bytes that one load brings. Of 128 columns of others it takes block g,
-// eight columns an instruction.
-template <class X, int MT, bool GATED>
-__global__ __launch_bounds__(256, 2) void k_mx4_tile(const Mx4Product a, const Vecs vec, int out_type, int columns) {
-  typedef TileX<X, MT> T;
-  typedef typename X::R::E E;
-  constexpr int P = T::P, KS = T::KS, U = T::U, MF = MT / 16, WF = GATED ? 2 : 4;  // WF: fragments of out's columns a wave
-  extern __shared__ __align__(16) uint8_t lds[];
-  __shared__ int s_src[MT];
-  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, m = lane & 15, g = lane >> 4;
-  Tile tile;
-  int column;
-  if (!tile_place(a, MT, columns, tile, column)) return;
-  if (tid < MT) s_src[tid] = tid < tile.count ? source_of(a, tile.row + tid) : -1;
-  __syncthreads();
-  const int n0 = (column * 4 + wave) * (16 * WF);
-  // the matrix from the wave's first row on, a lane's row of each fragment
-  const int first = min(n0, a.n - 1);
-  const int64_t row0 = (int64_t)tile.expert * a.n + first;
-  const uint8_t *wbase[2] = {a.w.codes + row0 * (a.steps * 64), GATED ? a.up.codes + row0 * (a.steps * 64) : nullptr};
-  const uint8_t *sbase[2] = {a.w.scales + row0 * (a.steps * 4), GATED ? a.up.scales + row0 * (a.steps * 4) : nullptr};
-  uint32_t wrow[WF];
-#pragma unroll
-  for (int t = 0; t < WF; t++) wrow[t] = (uint32_t)(min(n0 + 16 * t + m, a.n - 1) - first) * (uint32_t)(a.steps * 4);
-  const int q = tid % U, r0 = tid / U;  // a thread's pieces of x: piece q of rows r0, r0 + 256 / U, ...
-  const uint8_t *xr[P == 0 ? T::PER : 1];
-  if constexpr (P == 0)
-#pragma unroll
-    for (int j = 0; j < T::PER; j++) {
-      const int r = r0 + 256 / U * j, src = r < MT ? s_src[r] : -1;
-      xr[j] = src >= 0 ? (const uint8_t *)a.x + (int64_t)src * (a.steps * 64) + q * 16 : nullptr;
-    }
-  const uint8_t *xs = P == 0 && tid < MT && s_src[tid] >= 0 ? a.x_scales + (int64_t)s_src[tid] * (a.steps * 4) : nullptr;
-
-  i4v w[4 * KS], wn[4 * KS];
-  uint32_t ws[4], wsn[4];
-  uint4 xc[P == 0 ? T::PER : 1];
-  uint32_t xsc[2];
-  Raw8<E> xw[P == 0 ? 1 : T::PER];
-  const auto load_w = [&](int s) {
-    if constexpr (P == 0) {
-      const int at = s + 1 < a.steps ? g : g & 1;  // (an odd last step has half as many blocks; x is zero at the others)
-#pragma unroll
-      for (int t = 0; t < 4; t++) {
-        const uint8_t *p = wbase[t / WF] + s * 64;
-        const uint32_t off = wrow[t % WF] * 16u + at * 32;
-        wn[t] = *(const i4v *)(p + off);
-        wn[4 + t] = *(const i4v *)(p + off + 16);
-        wsn[t] = *(const uint16_t *)(sbase[t / WF] + s * 4 + (wrow[t % WF] + at * 2));
-      }
-    } else {
-#pragma unroll
-      for (int t = 0; t < 4; t++) {
-        wn[t] = *(const i4v *)(wbase[t / WF] + s * 64 + (wrow[t % WF] * 16u + g * 16));
-        wsn[t] = sbase[t / WF][s * 4 + (wrow[t % WF] + g)];
-      }
-    }
-  };
-  const auto load_x = [&](int s) {
-    if constexpr (P == 0) {
-#pragma unroll
-      for (int j = 0; j < T::PER; j++) {
-        xc[j] = make_uint4(0, 0, 0, 0);
-        if (xr[j] && s + (q >> 2) < a.steps) xc[j] = *(const uint4 *)(xr[j] + s * 64);
-      }
-      xsc[0] = xsc[1] = 0;
-      if (xs) {
-        xsc[0] = *(const uint32_t *)(xs + s * 4);
-        if (s + 1 < a.steps) xsc[1] = *(const uint32_t *)(xs + s * 4 + 4);
-      }
-    } else {
-#pragma unroll
-      for (int j = 0; j < T::PER; j++) {
-        const int r = r0 + 256 / U * j, src = s_src[r];
-        xw[j] = raw8<E>(a, src >= 0 ? (const E *)a.x + (int64_t)src * a.ld_x : nullptr, s * 128 + q * 8, vec.x);
-      }
-    }
-  };
-  const auto put_x = [&](uint8_t *buf) {
-#pragma unroll
-    for (int j = 0; j < T::PER; j++) {
-      const int r = r0 + 256 / U * j;
-      if (MT * U % 256 && r >= MT) break;
-      if constexpr (P == 0) {
-        *(uint4 *)(buf + (q & 1) * T::PLANE + (r >> 4) * 1024 + frag_at(r & 15, q >> 1)) = xc[j];
-      } else {
-        uint8_t *dst = buf + (q & 3) * T::PLANE + (r >> 4) * 1024 + frag_at(r & 15, q >> 2);
-        if constexpr (P == 1) *(uint4 *)dst = xw[j].v[0];
-        else {
-          alignas(16) E e[8];
-#pragma unroll
-          for (int i = 0; i < (int)sizeof(E) / 2; i++) ((uint4 *)e)[i] = xw[j].v[i];
-          float x[8];
-#pragma unroll
-          for (int i = 0; i < 8; i++) x[i] = row_get(typename X::R{}, e[i]);
-          b8v part[P];
-          parts_of(x, part);
-#pragma unroll
-          for (int p = 0; p < P; p++) *(b8v *)(dst + p * 4 * T::PLANE) = part[p];
-        }
-      }
-    }
-    if (P == 0 && tid < MT) *(uint2 *)(buf + T::PLANES * T::PLANE + tid * 8) = make_uint2(xsc[0], xsc[1]);
-  };
-
-  f4v acc[MF][4] = {};
-  load_x(0);
-  load_w(0);
-  int buf = 0;
-  for (int s = 0; s < a.steps; s += KS) {
-    uint8_t *b = lds + buf * T::BYTES;
-    if (T::BUFS == 1) __syncthreads();  // the last iteration's reads are done
-    put_x(b);
-#pragma unroll
-    for (int t = 0; t < 4 * KS; t++) w[t] = wn[t];
-#pragma unroll
-    for (int t = 0; t < 4; t++) ws[t] = wsn[t];
-    __syncthreads();
-    if (s + KS < a.steps) {
-      load_x(s + KS);
-      load_w(s + KS);
-    }
-    if constexpr (P == 0) {
-#pragma unroll
-      for (int f = 0; f < MF; f++) {
-        const i4v x0 = *(const i4v *)(b + f * 1024 + frag_at(m, g)), x1 = *(const i4v *)(b + T::PLANE + f * 1024 + frag_at(m, g));
-        const int sx = *(const uint16_t *)(b + T::PLANES * T::PLANE + (f * 16 + m) * 8 + g * 2);
-#pragma unroll
-        for (int t = 0; t < 4; t++) acc[f][t] = mfma_mx4<0>(w[t], (int)ws[t], x0, sx, acc[f][t]);
-#pragma unroll
-        for (int t = 0; t < 4; t++) acc[f][t] = mfma_mx4<1>(w[4 + t], (int)ws[t], x1, sx, acc[f][t]);
-      }
-    } else {
-#pragma unroll
-      for (int c = 0; c < 4; c++) {
-        b8v v[4];
-#pragma unroll
-        for (int t = 0; t < 4; t++) v[t] = values_of((uint32_t)w[t][c], __uint_as_float(ws[t] << 23));
-#pragma unroll
-        for (int f = 0; f < MF; f++)
-#pragma unroll
-          for (int p = P - 1; p >= 0; p--) {
-            const b8v x = *(const b8v *)(b + (p * 4 + c) * T::PLANE + f * 1024 + frag_at(m, g));
-#pragma unroll
-            for (int t = 0; t < 4; t++) acc[f][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v[t], x, acc[f][t], 0, 0, 0);
-          }
-      }
-    }
-    if (T::BUFS == 2) buf ^= 1;
-  }
-#pragma unroll
-  for (int f = 0; f < MF; f++) {
-    if (s_src[f * 16 + m] < 0) continue;
-#pragma unroll
-    for (int t = 0; t < WF; t++) {
-      f4v v = acc[f][t];
-      if (GATED)
-#pragma unroll
-        for (int j = 0; j < 4; j++) v[j] = silu(v[j]) * acc[f][(t + 2) & 3][j];
-      const int c = n0 + 16 * t + 4 * g;
-      if (c < a.n) put4_by(a, out_type, tile.row + f * 16 + m, c, v, vec.out);
-    }
-  }
-}
-
 // ------------------------------------------------------------------ products of many 4-bit rows
 // MT rows of x against 64 WN rows of the matrix (gated: half of them up's), 256 columns a turn, four waves of MF * 32 rows of x
 // and 64 of the matrix each. Codes and scales are copied to LDS without a register, the codes a turn ahead, the
@@ -639,6 +454,7 @@ __device__ __forceinline__ rsrc_t from_here(const void *base) {
 __device__ __forceinline__ void copy16_lds(rsrc_t base, uint32_t lane, int all, void *to) {
   __builtin_amdgcn_raw_ptr_buffer_load_lds(base, (lds_ptr)to, 16, (int)lane, all, 0, 0);
 }
+__device__ __forceinline__ void copy16_lds(const void *from, void *to) { __builtin_amdgcn_global_load_lds(from, (lds_ptr)to, 16, 0, 0); }
 __device__ __forceinline__ void copy4_lds(rsrc_t base, uint32_t lane, int all, void *to) {
   __builtin_amdgcn_raw_ptr_buffer_load_lds(base, (lds_ptr)to, 4, (int)lane, all, 0, 0);
 }
@@ -823,6 +639,189 @@ __global__ __launch_bounds__(256, MT == 64 ? 3 : 2) void k_mx4_four(const Mx4Pro
   }
 }
 
+// ------------------------------------------------------------------ products of many 16- and 32-bit rows
+// The same with x as bf16 parts and the matrix's codes made values in registers, 64 columns a turn: lane half g has block g of
+// either operand, eight columns an instruction. The codes come 256 columns at a time (whole cache lines), four turns;
+// bf16 rows are copied to LDS as they lie where they can be (COPY), others go through registers, a turn ahead.
+template <class X, int MT>
+struct Wide {
+  static constexpr int P = X::PARTS, WM = MT == 32 ? 1 : 2, WN = 4 / WM, MF = MT / 32 / WM, ROWS = WN * 64;
+  static constexpr int BUFS = P == 1 || (P == 2 && MT == 64) ? 2 : 1;  // (two workgroups a CU)
+  struct Lds {
+    uint8_t x[BUFS][P][MT * 128], w[2][ROWS * 128];
+    uint32_t scales[ROWS][4];
+  };
+};
+
+template <class X, int MT, bool GATED, bool COPY>
+__global__ __launch_bounds__(256, 2) void k_mx4_wide(const Mx4Product a, const Vecs vec, int out_type, int columns) {
+  typedef Wide<X, MT> T;
+  typedef typename X::R::E E;
+  constexpr int P = T::P, MF = T::MF, WN = T::WN, BUFS = T::BUFS, COLS = GATED ? 32 : 64, WC = 2 * WN, XC = MT / 32;  // WC, XC: a wave's copies
+  extern __shared__ __align__(16) uint8_t lds[];
+  __shared__ int s_src[MT];
+  typename T::Lds &b = *(typename T::Lds *)lds;
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, m = lane & 31, g = lane >> 5;
+  const int wm = wave / WN, wn = wave % WN;
+  Tile tile;
+  int column;
+  if (!tile_place(a, MT, columns, tile, column)) return;
+  if (tid < MT) s_src[tid] = tid < tile.count ? source_of(a, tile.row + tid) : -1;
+  const int col0 = column * WN * COLS;
+  const int64_t row0 = (int64_t)tile.expert * a.n + col0;
+  const rsrc_t wcodes = from_here(a.w.codes + row0 * (a.steps * 64)), wscales = from_here(a.w.scales + row0 * (a.steps * 4));
+  const rsrc_t ucodes = GATED ? from_here(a.up.codes + row0 * (a.steps * 64)) : wcodes, uscales = GATED ? from_here(a.up.scales + row0 * (a.steps * 4)) : wscales;
+  const int from = wave * (8 * WC), r8 = lane >> 3;
+  uint32_t wrow[WC];
+#pragma unroll
+  for (int j = 0; j < WC; j++) {
+    const int r = from + 8 * j + r8;
+    wrow[j] = (uint32_t)min((r >> 6) * COLS + (r & (COLS - 1)), a.n - 1 - col0) * (uint32_t)a.steps;
+  }
+  const auto is_up = [&](int j) { return GATED && (WC == 8 ? j >= 4 : (wave & 1) != 0); };
+  const auto slot = [&](int j) { return (lane & 7) ^ (((j & 1) << 2) | (lane >> 4)); };  // the piece of a row that a lane copies
+  const auto bring_w = [&](int s, int at) {
+#pragma unroll
+    for (int j = 0; j < WC; j++) {
+      const int p = slot(j);
+      copy16_lds(is_up(j) ? ucodes : wcodes, wrow[j] * 64u + (uint32_t)(s + 1 < a.steps ? p : p & 3) * 16u, s * 64, b.w[at] + (from + 8 * j) * 128);
+    }
+  };
+  const auto bring_scales = [&](int s0) {
+    const int s = min(s0 + (lane & 3), a.steps - 1) * 4, r16 = lane >> 2;
+#pragma unroll
+    for (int j = 0; j < WC / 2; j++) {
+      const int r = from + 16 * j + r16;
+      const uint32_t row = (uint32_t)min((r >> 6) * COLS + (r & (COLS - 1)), a.n - 1 - col0) * (uint32_t)a.steps;
+      copy4_lds(is_up(2 * j) ? uscales : wscales, row * 4u + s, 0, b.scales[from + 16 * j]);
+    }
+  };
+  bring_w(0, 0);
+  bring_scales(0);
+  __syncthreads();
+  // rows of x: XC times eight of them a wave, a lane eight columns; there is none: some row, which is not stored, or zeros
+  const E *xr[XC];
+#pragma unroll
+  for (int j = 0; j < XC; j++) {
+    const int src = s_src[(wave * XC + j) * 8 + r8];
+    xr[j] = COPY || src >= 0 ? (const E *)a.x + (int64_t)max(src, 0) * a.ld_x : nullptr;
+  }
+  const auto copy_x = [&](int turn, int at) {
+#pragma unroll
+    for (int j = 0; j < XC; j++)
+      if ((wave * XC + j) * 8 < tile.count)
+        copy16_lds(xr[j] + turn * 64 + slot(wave * XC + j) * 8, b.x[at][0] + (wave * XC + j) * 1024);
+  };
+  Raw8<E> xw[COPY ? 1 : XC];
+  const auto load_x = [&](int turn) {
+#pragma unroll
+    for (int j = 0; j < XC; j++) xw[j] = raw8<E>(a, xr[j], turn * 64 + (lane & 7) * 8, vec.x);
+  };
+  const auto put_x = [&](int at) {
+#pragma unroll
+    for (int j = 0; j < XC; j++) {
+      uint8_t *const to = b.x[at][0] + (wave * XC + j) * 1024 + r8 * 128 + slot(wave * XC + j) * 16;
+      if constexpr (P == 1) *(uint4 *)to = xw[j].v[0];
+      else {
+        alignas(16) E e[8];
+#pragma unroll
+        for (int i = 0; i < (int)sizeof(E) / 2; i++) ((uint4 *)e)[i] = xw[j].v[i];
+        float x[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) x[i] = row_get(typename X::R{}, e[i]);
+        b8v part[P];
+        parts_of(x, part);
+#pragma unroll
+        for (int p = 0; p < P; p++) *(b8v *)(to + p * MT * 128) = part[p];
+      }
+    }
+  };
+  const int turns = (a.cols + 63) / 64;
+  if (COPY) copy_x(0, 0);
+  else {
+    load_x(0);
+    if (BUFS == 2) {
+      put_x(0);
+      load_x(1);
+    }
+  }
+  f16v acc[MF][2] = {};
+  i4v wsc[2];  // a row's scales of four steps
+  const auto all_turns = [&](auto live) {
+    constexpr int LIVE = decltype(live)::value;
+    for (int t4 = 0; t4 < turns; t4 += 4) {  // 256 columns of codes
+      const int at = t4 >> 2 & 1;
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        const int turn = t4 + i;
+        if (turn >= turns) break;
+        // what this turn reads has been brought, by every wave, and the reads of the last one's buffers are done
+        wait_and_meet();
+        if (i == 0 && at == 0) {
+#pragma unroll
+          for (int t = 0; t < 2; t++) wsc[t] = *(const i4v *)b.scales[wn * 64 + t * 32 + m];
+        }
+        if (i == 0 && t4 + 4 < turns) bring_w((t4 >> 1) + 2, at ^ 1);
+        if (i == 1 && at == 0 && t4 + 8 < turns) bring_scales((t4 >> 1) + 4);
+        const int xb = BUFS == 2 ? i & 1 : 0;
+        if (COPY) {
+          if (turn + 1 < turns) copy_x(turn + 1, xb ^ 1);
+        } else if (BUFS == 2) {
+          if (turn + 1 < turns) put_x(xb ^ 1);
+          if (turn + 2 < turns) load_x(turn + 2);
+        } else {
+          put_x(0);
+          __syncthreads();
+          if (turn + 1 < turns) load_x(turn + 1);
+        }
+        if (LIVE == 0) continue;
+        const uint8_t *const x = b.x[xb][0] + wm * MF * 4096 + m * 128, *const w = b.w[at] + wn * 8192 + m * 128 + ((2 * i + g) ^ (m >> 1 & 7)) * 16;
+        const int shift = 16 * (i & 1) + 8 * g;
+        i4v codes[2];
+        float scale[2];
+#pragma unroll
+        for (int t = 0; t < 2; t++) {
+          codes[t] = *(const i4v *)(w + t * 4096);
+          const int two = at ? (i < 2 ? wsc[t][2] : wsc[t][3]) : (i < 2 ? wsc[t][0] : wsc[t][1]);
+          scale[t] = __uint_as_float(((uint32_t)two >> shift & 255u) << 23);
+        }
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+          b8v v[2];
+#pragma unroll
+          for (int t = 0; t < 2; t++) v[t] = values_of((uint32_t)codes[t][j], scale[t]);
+          const int u = ((4 * g + j) ^ (m >> 1 & 7)) * 16;
+#pragma unroll
+          for (int f = 0; f < LIVE; f++)
+#pragma unroll
+            for (int p = P - 1; p >= 0; p--) {
+              const b8v xv = *(const b8v *)(x + p * MT * 128 + f * 4096 + u);
+#pragma unroll
+              for (int t = 0; t < 2; t++) acc[f][t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v[t], xv, acc[f][t], 0, 0, 0);
+            }
+        }
+      }
+    }
+  };
+  const int rows = tile.count - wm * MF * 32;
+  if (MF == 2 && rows > 32) all_turns(std::integral_constant<int, MF>{});
+  else if (rows > 0) all_turns(std::integral_constant<int, 1>{});
+  else all_turns(std::integral_constant<int, 0>{});
+  wait_and_meet();  // (all waves' reads of LDS are done)
+#pragma unroll
+  for (int f = 0; f < MF; f++) {
+    const int r0 = (wm * MF + f) * 32;
+    if (r0 >= tile.count) break;
+    put_rows<COLS>(a, out_type, vec.out, lds + wave * 9216, col0 + wn * COLS, [&](int r) { return s_src[r0 + r] < 0 ? -1 : tile.row + r0 + r; },
+                   [&](int t, int i) {
+                     f4v v;
+#pragma unroll
+                     for (int j = 0; j < 4; j++) v[j] = GATED ? silu(acc[f][0][4 * i + j]) * acc[f][1][4 * i + j] : acc[f][t][4 * i + j];
+                     return v;
+                   });
+  }
+}
+
 // Tiles over the launch's second and third dimension.
 static dim3 tile_grid(int64_t columns, int64_t tiles) {
   const int64_t y = tiles < 32768 ? tiles : 32768;
@@ -843,25 +842,27 @@ struct Allowed {
 };
 
 template <class X, int MT>
-static hipError_t tiled(const Mx4Product &a, const Vecs &vec, int out_type, hipStream_t s) {
-  typedef TileX<X, MT> T;
-  const int wide = (T::P == 0 ? Four<MT>::ROWS : 256) / (a.up.codes ? 2 : 1), columns = (a.n + wide - 1) / wide;
+static hipError_t tiled(const Mx4Product &a, const Vecs &x_vec, int out_type, hipStream_t s) {
+  constexpr int ROWS = Four<MT>::ROWS;
+  const int wide = a.up.codes ? ROWS / 2 : ROWS, columns = (a.n + wide - 1) / wide;
   const int64_t blocks = (tiles_most(a, MT) * columns + 7) / 8 * 8, x = blocks < 1 << 20 ? blocks : 1 << 20;
   const dim3 grid((unsigned)x, (unsigned)((blocks + x - 1) / x));
-  if constexpr (T::P == 0) {
-    constexpr unsigned four = sizeof(typename Four<MT>::Lds);
-    static Allowed gated, plain;
-    const void *f = a.up.codes ? (const void *)k_mx4_four<MT, true> : (const void *)k_mx4_four<MT, false>;
-    if (const hipError_t e = (a.up.codes ? gated : plain).lds(f, four); e != hipSuccess) return e;
-    const Vecs v16 = {1, on16(a.out, a.ld_out, out_type == T_F32 ? 4 : 2)};
-    if (a.up.codes) hipLaunchKernelGGL((k_mx4_four<MT, true>), grid, dim3(256), four, s, a, v16, out_type, columns);
-    else hipLaunchKernelGGL((k_mx4_four<MT, false>), grid, dim3(256), four, s, a, v16, out_type, columns);
+  const Vecs vec = {x_vec.x, on16(a.out, a.ld_out, out_type == T_F32 ? 4 : 2)};
+  static Allowed allowed[4];
+  const auto launch = [&](void (*k)(Mx4Product, Vecs, int, int), int which, unsigned bytes) {
+    if (const hipError_t e = allowed[which].lds((const void *)k, bytes); e != hipSuccess) return e;
+    hipLaunchKernelGGL(k, grid, dim3(256), bytes, s, a, vec, out_type, columns);
     return hipGetLastError();
+  };
+  if constexpr (X::PARTS == 0) {
+    constexpr unsigned bytes = sizeof(typename Four<MT>::Lds);
+    return a.up.codes ? launch(k_mx4_four<MT, true>, 0, bytes) : launch(k_mx4_four<MT, false>, 1, bytes);
+  } else {
+    constexpr unsigned bytes = sizeof(typename Wide<X, MT>::Lds);
+    if constexpr (X::PARTS == 1)
+      if (vec.x && a.cols % 64 == 0) return a.up.codes ? launch(k_mx4_wide<X, MT, true, true>, 2, bytes) : launch(k_mx4_wide<X, MT, false, true>, 3, bytes);
+    return a.up.codes ? launch(k_mx4_wide<X, MT, true, false>, 0, bytes) : launch(k_mx4_wide<X, MT, false, false>, 1, bytes);
   }
-  constexpr unsigned bytes = T::BUFS * T::BYTES;
-  if (a.up.codes) hipLaunchKernelGGL((k_mx4_tile<X, MT, true>), grid, dim3(256), bytes, s, a, vec, out_type, columns);
-  else hipLaunchKernelGGL((k_mx4_tile<X, MT, false>), grid, dim3(256), bytes, s, a, vec, out_type, columns);
-  return hipGetLastError();
 }
 
 template <class X>
