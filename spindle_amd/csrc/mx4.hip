@@ -188,22 +188,30 @@ __device__ __forceinline__ void x8(const Mx4Product &a, const typename R::E *row
     for (int j = 0; j < 8; j++) x[j] = c + j < a.cols ? row_get(R{}, row[c + j]) : 0.0f;
 }
 // A value as bf16 parts, each the upper half of what is left: 8 bits a part, and what is taken off is exact. An infinity
-// or a NaN is its first part.
+// or a NaN is its first part (rare: a way of its own, six instructions a value less).
 template <int P>
 __device__ __forceinline__ void parts_of(const float *x, b8v (&part)[P]) {
   uint32_t u[P][8];
 #pragma unroll
   for (int j = 0; j < 8; j++) {
     float r = x[j];
-    if (P == 3 && isnan(r)) r = __builtin_nanf("");  // (its upper half might be infinity's)
 #pragma unroll
     for (int p = 0; p < P; p++) {
       u[p][j] = __float_as_uint(r);
-      if (p + 1 < P) {
-        const float rest = r - __uint_as_float(u[p][j] & 0xffff0000u);
-        r = (u[p][j] & 0x7f800000u) == 0x7f800000u ? 0.0f : rest;
-      }
+      r -= __uint_as_float(u[p][j] & 0xffff0000u);
     }
+  }
+  uint32_t most = 0;
+#pragma unroll
+  for (int j = 0; j < 8; j++) most = max(most, u[0][j] & 0x7fffffffu);
+  if (__builtin_expect(most >= 0x7f800000u, 0)) {
+#pragma unroll
+    for (int j = 0; j < 8; j++)
+      if ((u[0][j] & 0x7f800000u) == 0x7f800000u) {
+        if (u[0][j] & 0x7fffffu) u[0][j] = 0x7fc00000u;  // (a NaN's upper half might be infinity's)
+#pragma unroll
+        for (int p = 1; p < P; p++) u[p][j] = 0;
+      }
   }
 #pragma unroll
   for (int p = 0; p < P; p++) {
@@ -867,7 +875,7 @@ static hipError_t tiled(const Mx4Product &a, const Vecs &x_vec, int out_type, hi
 
 template <class X>
 static hipError_t product(const Mx4Product &a, int out_type, hipStream_t s) {
-  constexpr int RT = 2, MOST = X::PARTS <= 1 ? 128 : 64;
+  constexpr int RT = 2, MOST = X::PARTS <= 2 ? 128 : 64;
   const Vecs vec = {X::PARTS == 0 || on16(a.x, a.ld_x, sizeof(typename X::R::E)),
                     (uintptr_t)a.out % (out_type == T_F32 ? 16 : 8) == 0 && a.ld_out % 4 == 0};
   int64_t each = a.starts ? a.rows / a.n_expert : a.rows;  // rows of a matrix, where they are even
