@@ -4,6 +4,7 @@
 // The layout is the matrix cores': an instruction's 128 columns of a row are 64 bytes of codes and four scale
 // bytes, of which lane group g of a wave takes the g-th 16 bytes and the g-th scale, one block of 32.
 #include <atomic>
+#include <cstdlib>
 #include <type_traits>
 
 #include "dev.h"
@@ -276,85 +277,6 @@ __device__ __forceinline__ void put4_by(const Mx4Product &a, int out_type, int i
   if (out_type == T_F32) put4<float>(a, i, c, v, vec);
   else if (out_type == T_F16) put4<_Float16>(a, i, c, v, vec);
   else put4<__bf16>(a, i, c, v, vec);
-}
-
-// Sixteen rows of x against 16 RT rows of the matrix (and of up): W X^T, a lane's four sums being four neighbours of
-// one row of out. The workgroup's four waves take the steps of 128 columns in turn and are joined at the end.
-template <class X, int RT, bool GATED>
-__global__ __launch_bounds__(256) void k_mx4_rows(const Mx4Product a, const Vecs vec, int out_type) {
-  constexpr int P = X::PARTS, H = GATED ? 2 : 1;
-  typedef typename X::R R;
-  typedef typename R::E E;
-  __shared__ f4v sums[4][RT * H][64];
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
-  const Tile tile = tile_of(a, blockIdx.y + blockIdx.z * gridDim.y, 16);
-  if (tile.count <= 0) return;
-  const int i = tile.row + m, src = m < tile.count ? source_of(a, i) : -1, n0 = blockIdx.x * (16 * RT);
-  const uint8_t *wc[H][RT], *wsc[H][RT];
-#pragma unroll
-  for (int h = 0; h < H; h++)
-#pragma unroll
-    for (int t = 0; t < RT; t++) {
-      const int64_t row = (int64_t)tile.expert * a.n + min(n0 + 16 * t + m, a.n - 1);
-      const Mx4 w = h ? a.up : a.w;
-      wc[h][t] = w.codes + row * (a.steps * 64) + g * 16;
-      wsc[h][t] = w.scales + row * (a.steps * 4) + g;
-    }
-  f4v acc[H][RT] = {};
-  for (int s = wave; s < a.steps; s += 4) {
-    i4v w[H][RT];
-    int ws[H][RT];
-#pragma unroll
-    for (int h = 0; h < H; h++)
-#pragma unroll
-      for (int t = 0; t < RT; t++) {
-        w[h][t] = *(const i4v *)(wc[h][t] + s * 64);
-        ws[h][t] = wsc[h][t][s * 4];
-      }
-    if constexpr (P == 0) {
-      i4v x = {};
-      int xs = 0;
-      if (src >= 0) {
-        x = *(const i4v *)((const uint8_t *)a.x + (int64_t)src * (a.steps * 64) + s * 64 + g * 16);
-        xs = a.x_scales[(int64_t)src * (a.steps * 4) + s * 4 + g];
-      }
-#pragma unroll
-      for (int h = 0; h < H; h++)
-#pragma unroll
-        for (int t = 0; t < RT; t++) acc[h][t] = mfma_mx4<0>(w[h][t], ws[h][t], x, xs, acc[h][t]);
-    } else {
-#pragma unroll
-      for (int c = 0; c < 4; c++) {
-        float x[8] = {};
-        if (src >= 0) x8<R>(a, (const E *)a.x + (int64_t)src * a.ld_x, s * 128 + g * 32 + c * 8, vec.x, x);
-        b8v part[P < 1 ? 1 : P];
-        parts_of(x, part);
-#pragma unroll
-        for (int h = 0; h < H; h++)
-#pragma unroll
-          for (int t = 0; t < RT; t++) {
-            const b8v v = values_of((uint32_t)w[h][t][c], __uint_as_float((uint32_t)ws[h][t] << 23));
-#pragma unroll
-            for (int p = P - 1; p >= 0; p--) acc[h][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, part[p], acc[h][t], 0, 0, 0);
-          }
-      }
-    }
-  }
-#pragma unroll
-  for (int h = 0; h < H; h++)
-#pragma unroll
-    for (int t = 0; t < RT; t++) sums[wave][h * RT + t][lane] = acc[h][t];
-  __syncthreads();
-  if (src < 0) return;
-  for (int t = wave; t < RT; t += 4) {
-    f4v v[H];
-#pragma unroll
-    for (int h = 0; h < H; h++) v[h] = (sums[0][h * RT + t][lane] + sums[1][h * RT + t][lane]) + (sums[2][h * RT + t][lane] + sums[3][h * RT + t][lane]);
-    if (GATED)
-#pragma unroll
-      for (int j = 0; j < 4; j++) v[0][j] = silu(v[0][j]) * v[H - 1][j];
-    if (n0 + 16 * t + 4 * g < a.n) put4_by(a, out_type, i, n0 + 16 * t + 4 * g, v[0], vec.out);
-  }
 }
 
 // Where a workgroup works. Tiles of one expert and row tile lie beside each other on one XCD (workgroups go to the eight in
@@ -651,6 +573,23 @@ __global__ __launch_bounds__(256, MT == 64 ? 3 : 2) void k_mx4_four(const Mx4Pro
 // The same with x as bf16 parts and the matrix's codes made values in registers, 64 columns a turn: lane half g has block g of
 // either operand, eight columns an instruction. The codes come 256 columns at a time (whole cache lines), four turns;
 // bf16 rows are copied to LDS as they lie where they can be (COPY), others go through registers, a turn ahead.
+// The same where rows lie at multiples of 16 bytes and cols is a multiple of 8: no branch, so that a thread's loads go out
+// together (`row` is some row of x where there is none: its products are not stored).
+template <class E>
+__device__ __forceinline__ Raw8<E> raw8_whole(const Mx4Product &a, const E *row, int c) {
+  Raw8<E> r;
+  const uint4 *const from = (const uint4 *)(row + min(c, a.cols - 8));
+#pragma unroll
+  for (int i = 0; i < (int)sizeof(E) / 2; i++) r.v[i] = from[i];
+  if (c >= a.cols)
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(E) / 2; i++) r.v[i] = make_uint4(0, 0, 0, 0);
+  return r;
+}
+
+// How rows of x come: copied to LDS as they lie (bf16, whole turns), loaded in whole pieces, or by elements where need be.
+enum { X_COPIED, X_WHOLE, X_ANY };
+
 template <class X, int MT>
 struct Wide {
   static constexpr int P = X::PARTS, WM = MT == 32 ? 1 : 2, WN = 4 / WM, MF = MT / 32 / WM, ROWS = WN * 64;
@@ -661,11 +600,12 @@ struct Wide {
   };
 };
 
-template <class X, int MT, bool GATED, bool COPY>
+template <class X, int MT, bool GATED, int WAY>
 __global__ __launch_bounds__(256, 2) void k_mx4_wide(const Mx4Product a, const Vecs vec, int out_type, int columns) {
   typedef Wide<X, MT> T;
   typedef typename X::R::E E;
   constexpr int P = T::P, MF = T::MF, WN = T::WN, BUFS = T::BUFS, COLS = GATED ? 32 : 64, WC = 2 * WN, XC = MT / 32;  // WC, XC: a wave's copies
+  constexpr bool COPY = WAY == X_COPIED;
   extern __shared__ __align__(16) uint8_t lds[];
   __shared__ int s_src[MT];
   typename T::Lds &b = *(typename T::Lds *)lds;
@@ -712,7 +652,7 @@ __global__ __launch_bounds__(256, 2) void k_mx4_wide(const Mx4Product a, const V
 #pragma unroll
   for (int j = 0; j < XC; j++) {
     const int src = s_src[(wave * XC + j) * 8 + r8];
-    xr[j] = COPY || src >= 0 ? (const E *)a.x + (int64_t)max(src, 0) * a.ld_x : nullptr;
+    xr[j] = WAY != X_ANY || src >= 0 ? (const E *)a.x + (int64_t)max(src, 0) * a.ld_x : nullptr;
   }
   const auto copy_x = [&](int turn, int at) {
 #pragma unroll
@@ -723,7 +663,10 @@ __global__ __launch_bounds__(256, 2) void k_mx4_wide(const Mx4Product a, const V
   Raw8<E> xw[COPY ? 1 : XC];
   const auto load_x = [&](int turn) {
 #pragma unroll
-    for (int j = 0; j < XC; j++) xw[j] = raw8<E>(a, xr[j], turn * 64 + (lane & 7) * 8, vec.x);
+    for (int j = 0; j < XC; j++) {
+      if constexpr (WAY == X_ANY) xw[j] = raw8<E>(a, xr[j], turn * 64 + (lane & 7) * 8, vec.x);
+      else xw[j] = raw8_whole<E>(a, xr[j], turn * 64 + (lane & 7) * 8);
+    }
   };
   const auto put_x = [&](int at) {
 #pragma unroll
@@ -830,6 +773,153 @@ __global__ __launch_bounds__(256, 2) void k_mx4_wide(const Mx4Product a, const V
   }
 }
 
+// ------------------------------------------------------------------ products of few rows
+// Sixteen rows of x against 16 RT rows of the matrix (gated: half of them up's): W X^T, a lane's four sums being four
+// neighbours of one row of out. Bound by the matrix's bytes. The workgroup's four waves take the steps of 256 columns in turn, each
+// by itself: codes and scales are copied to LDS of the wave's own, two steps' at a time, as whole cache lines (straight into registers
+// neighbouring lanes would be in different rows, at a quarter of the rate), x goes into registers. The sums meet at the end.
+template <int RT>
+struct FewLds {
+  uint8_t codes[2][RT][16 * 128];
+  uint32_t scales[2][RT][2][16];
+};
+
+template <class X, int RT, bool GATED, int WAY>
+__global__ __launch_bounds__(256, 2) void k_mx4_few(const Mx4Product a, const Vecs vec, int out_type) {
+  constexpr int P = X::PARTS, COLS = GATED ? RT * 8 : RT * 16;  // COLS: out's columns
+  typedef typename X::R R;
+  typedef typename R::E E;
+  __shared__ __align__(16) FewLds<RT> ring[4];
+  static_assert(sizeof(ring) >= 4 * RT * 64 * sizeof(f4v), "the sums fit in its place");
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, m = lane & 15, g = lane >> 4;
+  const Tile tile = tile_of(a, blockIdx.y + blockIdx.z * gridDim.y, 16);
+  if (tile.count <= 0) return;
+  const int i = tile.row + m, src = m < tile.count ? source_of(a, i) : -1, n0 = blockIdx.x * COLS;
+  FewLds<RT> &b = ring[wave];
+  const int64_t row0 = (int64_t)tile.expert * a.n + n0;
+  const rsrc_t wcodes = from_here(a.w.codes + row0 * (a.steps * 64)), wscales = from_here(a.w.scales + row0 * (a.steps * 4));
+  const rsrc_t ucodes = GATED ? from_here(a.up.codes + row0 * (a.steps * 64)) : wcodes, uscales = GATED ? from_here(a.up.scales + row0 * (a.steps * 4)) : wscales;
+  const auto row_of = [&](int t, int r) { return (uint32_t)min((GATED ? t % (RT / 2 < 1 ? 1 : RT / 2) : t) * 16 + r, a.n - 1 - n0) * (uint32_t)a.steps; };
+  const auto is_up = [&](int t) { return GATED && t >= RT / 2; };
+  const auto bring = [&](int s, int at) {  // (the last step may have half of a row: that twice, the second one unused)
+    const bool both = s + 1 < a.steps;
+#pragma unroll
+    for (int t = 0; t < RT; t++) {
+#pragma unroll
+      for (int j = 0; j < 2; j++) {
+        const int p = (lane & 7) ^ (((j & 1) << 2) | (lane >> 4));
+        copy16_lds(is_up(t) ? ucodes : wcodes, row_of(t, j * 8 + (lane >> 3)) * 64u + (uint32_t)(both ? p : p & 3) * 16u, s * 64, b.codes[at][t] + j * 1024);
+      }
+      // (two steps' scales of sixteen rows: half of the lanes)
+      if (lane < 32) copy4_lds(is_up(t) ? uscales : wscales, row_of(t, m) * 4u + (uint32_t)(min(s + (lane >> 4), a.steps - 1) * 4), 0, b.scales[at][t][0]);
+    }
+  };
+  // x's eight columns of group g: of half h and instruction c
+  Raw8<E> x[P == 0 ? 1 : 8], xn[P == 0 ? 1 : 8];
+  i4v xc[2], xcn[2];
+  int xs[2], xsn[2];
+  const E *const xrow = P > 0 && (src >= 0 || WAY == X_WHOLE) ? (const E *)a.x + (int64_t)max(src, 0) * a.ld_x : nullptr;
+  const auto load_x = [&](int s) {
+    if constexpr (P == 0) {
+#pragma unroll
+      for (int h = 0; h < 2; h++) {
+        const int at = min(s + h, a.steps - 1);  // (behind the last: that again, unused)
+        xcn[h] = *(const i4v *)((const uint8_t *)a.x + (int64_t)max(src, 0) * (a.steps * 64) + at * 64 + g * 16);
+        xsn[h] = a.x_scales[(int64_t)max(src, 0) * (a.steps * 4) + at * 4 + g];
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; j++) {
+        const int c = (s + (j >> 2)) * 128 + g * 32 + (j & 3) * 8;
+        if constexpr (WAY == X_ANY) xn[j] = raw8<E>(a, xrow, c, vec.x);
+        else xn[j] = raw8_whole<E>(a, xrow, c);
+      }
+    }
+  };
+  f4v acc[RT] = {};
+  int at = 0, s = wave * 2;
+  if (s < a.steps) {
+    bring(s, 0);
+    load_x(s);
+    asm volatile("" ::: "memory");
+    if (s + 8 < a.steps) bring(s + 8, 1);
+  }
+  for (; s < a.steps; s += 8) {
+    // this step's codes and x are there; only the next step's codes, brought after them, may be under way
+    asm volatile("" ::: "memory");
+    if (s + 8 < a.steps) __builtin_amdgcn_s_waitcnt(0x0f70 | 3 * RT);
+    else __builtin_amdgcn_s_waitcnt(0x0f70);
+    asm volatile("" ::: "memory");
+    if constexpr (P == 0) {
+#pragma unroll
+      for (int h = 0; h < 2; h++) { xc[h] = xcn[h]; xs[h] = xsn[h]; }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; j++) x[j] = xn[j];
+    }
+    if (s + 8 < a.steps) load_x(s + 8);
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+      if (h && s + 1 >= a.steps) break;
+      i4v w[RT];
+      int ws[RT];
+#pragma unroll
+      for (int t = 0; t < RT; t++) {
+        w[t] = *(const i4v *)(b.codes[at][t] + m * 128 + ((4 * h + g) ^ (m >> 1 & 7)) * 16);
+        ws[t] = ((const uint8_t *)&b.scales[at][t][h][m])[g];
+      }
+      if constexpr (P == 0) {
+#pragma unroll
+        for (int t = 0; t < RT; t++) acc[t] = mfma_mx4<0>(w[t], ws[t], xc[h], xs[h], acc[t]);
+      } else {
+#pragma unroll
+        for (int c = 0; c < 4; c++) {
+          b8v part[P < 1 ? 1 : P];
+          if constexpr (P == 1) part[0] = __builtin_bit_cast(b8v, x[h * 4 + c].v[0]);
+          else {
+            alignas(16) E e[8];
+#pragma unroll
+            for (int k = 0; k < (int)sizeof(E) / 2; k++) ((uint4 *)e)[k] = x[h * 4 + c].v[k];
+            float v[8];
+#pragma unroll
+            for (int k = 0; k < 8; k++) v[k] = row_get(R{}, e[k]);
+            parts_of(v, part);
+          }
+#pragma unroll
+          for (int t = 0; t < RT; t++) {
+            const b8v v = values_of((uint32_t)w[t][c], __uint_as_float((uint32_t)ws[t] << 23));
+#pragma unroll
+            for (int p = P - 1; p >= 0; p--) acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, part[p], acc[t], 0, 0, 0);
+          }
+        }
+      }
+    }
+    if (s + 16 < a.steps) {
+      asm volatile("" ::: "memory");
+      __builtin_amdgcn_s_waitcnt(0xc07f);  // (the reads of what is brought over are done: lgkmcnt 0)
+      bring(s + 16, at);
+    }
+    at ^= 1;
+  }
+  __syncthreads();
+  f4v(*const sums)[RT][64] = (f4v(*)[RT][64])ring;
+#pragma unroll
+  for (int t = 0; t < RT; t++) sums[wave][t][lane] = acc[t];
+  __syncthreads();
+  if (src < 0) return;
+  constexpr int OUT = GATED ? RT / 2 : RT;
+  for (int t = wave; t < OUT; t += 4) {
+    const auto total = [&](int u) { return (sums[0][u][lane] + sums[1][u][lane]) + (sums[2][u][lane] + sums[3][u][lane]); };
+    f4v v = total(t);
+    if (GATED) {
+      const f4v u = total(t + OUT);
+#pragma unroll
+      for (int j = 0; j < 4; j++) v[j] = silu(v[j]) * u[j];
+    }
+    if (n0 + 16 * t + 4 * g < a.n) put4_by(a, out_type, i, n0 + 16 * t + 4 * g, v, vec.out);
+  }
+}
+
 // Tiles over the launch's second and third dimension.
 static dim3 tile_grid(int64_t columns, int64_t tiles) {
   const int64_t y = tiles < 32768 ? tiles : 32768;
@@ -868,25 +958,36 @@ static hipError_t tiled(const Mx4Product &a, const Vecs &x_vec, int out_type, hi
   } else {
     constexpr unsigned bytes = sizeof(typename Wide<X, MT>::Lds);
     if constexpr (X::PARTS == 1)
-      if (vec.x && a.cols % 64 == 0) return a.up.codes ? launch(k_mx4_wide<X, MT, true, true>, 2, bytes) : launch(k_mx4_wide<X, MT, false, true>, 3, bytes);
-    return a.up.codes ? launch(k_mx4_wide<X, MT, true, false>, 0, bytes) : launch(k_mx4_wide<X, MT, false, false>, 1, bytes);
+      if (vec.x && a.cols % 64 == 0) return a.up.codes ? launch(k_mx4_wide<X, MT, true, X_COPIED>, 0, bytes) : launch(k_mx4_wide<X, MT, false, X_COPIED>, 1, bytes);
+    if constexpr (X::PARTS > 1)
+      if (vec.x && a.cols % 8 == 0) return a.up.codes ? launch(k_mx4_wide<X, MT, true, X_WHOLE>, 0, bytes) : launch(k_mx4_wide<X, MT, false, X_WHOLE>, 1, bytes);
+    return a.up.codes ? launch(k_mx4_wide<X, MT, true, X_ANY>, 2, bytes) : launch(k_mx4_wide<X, MT, false, X_ANY>, 3, bytes);
   }
+}
+
+template <class X, int RT, bool GATED>
+static hipError_t few(const Mx4Product &a, const Vecs &vec, int out_type, hipStream_t s) {
+  constexpr int COLS = GATED ? RT * 8 : RT * 16;
+  const dim3 grid = tile_grid((a.n + COLS - 1) / COLS, tiles_most(a, 16)), block(256);
+  if (X::PARTS == 0 || (vec.x && a.cols % 8 == 0)) hipLaunchKernelGGL((k_mx4_few<X, RT, GATED, X_WHOLE>), grid, block, 0, s, a, vec, out_type);
+  else if constexpr (X::PARTS > 0) hipLaunchKernelGGL((k_mx4_few<X, RT, GATED, X_ANY>), grid, block, 0, s, a, vec, out_type);
+  return hipGetLastError();
 }
 
 template <class X>
 static hipError_t product(const Mx4Product &a, int out_type, hipStream_t s) {
-  constexpr int RT = 2, MOST = X::PARTS <= 2 ? 128 : 64;
+  constexpr int MOST = X::PARTS <= 2 ? 128 : 64;
   const Vecs vec = {X::PARTS == 0 || on16(a.x, a.ld_x, sizeof(typename X::R::E)),
                     (uintptr_t)a.out % (out_type == T_F32 ? 16 : 8) == 0 && a.ld_out % 4 == 0};
   int64_t each = a.starts ? a.rows / a.n_expert : a.rows;  // rows of a matrix, where they are even
   if (X::PARTS == 0 && (int64_t)a.x_rows * a.steps * 64 > UINT32_MAX) each = 0;  // (the tiles' addresses of x have 32 bits)
+  if (getenv("FEW")) each = 0;
   if (each > 64 && MOST == 128) return tiled<X, MOST>(a, vec, out_type, s);
   if (each > 24) return tiled<X, 64>(a, vec, out_type, s);
   if (each > 8) return tiled<X, 32>(a, vec, out_type, s);
-  const dim3 grid = tile_grid((a.n + 16 * RT - 1) / (16 * RT), tiles_most(a, 16));
-  if (a.up.codes) hipLaunchKernelGGL((k_mx4_rows<X, RT, true>), grid, dim3(256), 0, s, a, vec, out_type);
-  else hipLaunchKernelGGL((k_mx4_rows<X, RT, false>), grid, dim3(256), 0, s, a, vec, out_type);
-  return hipGetLastError();
+  const bool many = tiles_most(a, 16) * ((a.n + 63) / 64) >= 512;
+  if (a.up.codes) return many ? few<X, 4, true>(a, vec, out_type, s) : few<X, 2, true>(a, vec, out_type, s);
+  return many ? few<X, 4, false>(a, vec, out_type, s) : few<X, 1, false>(a, vec, out_type, s);
 }
 hipError_t launch_mx4_matmul(const Mx4Product &a, int type, int out_type, hipStream_t s) {
   switch (type) {
