@@ -4,7 +4,6 @@
 // The layout is the matrix cores': an instruction's 128 columns of a row are 64 bytes of codes and four scale
 // bytes, of which lane group g of a wave takes the g-th 16 bytes and the g-th scale, one block of 32.
 #include <atomic>
-#include <cstdlib>
 #include <type_traits>
 
 #include "dev.h"
@@ -981,7 +980,6 @@ static hipError_t product(const Mx4Product &a, int out_type, hipStream_t s) {
                     (uintptr_t)a.out % (out_type == T_F32 ? 16 : 8) == 0 && a.ld_out % 4 == 0};
   int64_t each = a.starts ? a.rows / a.n_expert : a.rows;  // rows of a matrix, where they are even
   if (X::PARTS == 0 && (int64_t)a.x_rows * a.steps * 64 > UINT32_MAX) each = 0;  // (the tiles' addresses of x have 32 bits)
-  if (getenv("FEW")) each = 0;
   if (each > 64 && MOST == 128) return tiled<X, MOST>(a, vec, out_type, s);
   if (each > 24) return tiled<X, 64>(a, vec, out_type, s);
   if (each > 8) return tiled<X, 32>(a, vec, out_type, s);
