@@ -221,6 +221,29 @@ __device__ __forceinline__ void parts_of(const float *x, b8v (&part)[P]) {
     part[p] = __builtin_bit_cast(b8v, w);
   }
 }
+// One of the parts: off1, off2 are the masks of what the first and the second leave to it (zero where it is no later one).
+template <int P>
+__device__ __forceinline__ b8v part_at(const float *x, uint32_t off1, uint32_t off2) {
+  uint32_t u[8], most = 0;
+#pragma unroll
+  for (int j = 0; j < 8; j++) {
+    float r = x[j] - __uint_as_float(__float_as_uint(x[j]) & off1);
+    if (P > 2) r -= __uint_as_float(__float_as_uint(r) & off2);
+    u[j] = __float_as_uint(r);
+    most = max(most, __float_as_uint(x[j]) & 0x7fffffffu);
+  }
+  if (__builtin_expect(most >= 0x7f800000u, 0)) {
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+      const uint32_t v = __float_as_uint(x[j]);
+      if ((v & 0x7f800000u) == 0x7f800000u) u[j] = off1 ? 0u : v & 0x7fffffu ? 0x7fc00000u : v;
+    }
+  }
+  i4v w;
+#pragma unroll
+  for (int j = 0; j < 4; j++) w[j] = (int)__builtin_amdgcn_perm(u[2 * j + 1], u[2 * j], 0x07060302u);
+  return __builtin_bit_cast(b8v, w);
+}
 // Eight codes as values in bf16, which holds them exactly.
 __device__ __forceinline__ b8v values_of(uint32_t w, float scale) {
   b2v v[4];
@@ -793,7 +816,10 @@ __global__ __launch_bounds__(256, 2) void k_mx4_few(const Mx4Product a, const Ve
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, m = lane & 15, g = lane >> 4;
   const Tile tile = tile_of(a, blockIdx.y + blockIdx.z * gridDim.y, 16);
   if (tile.count <= 0) return;
-  const int i = tile.row + m, src = m < tile.count ? source_of(a, i) : -1, n0 = blockIdx.x * COLS;
+  // Few rows of several parts: the parts are columns of their own, one instruction for all; lane m has part m / rows of row m % rows.
+  const bool apart = P > 1 && tile.count * P <= 16;
+  const int part_of = apart ? m / tile.count : 0, r = apart ? m - part_of * tile.count : m;
+  const int i = tile.row + r, src = r < tile.count && part_of < (P > 1 ? P : 1) ? source_of(a, i) : -1, n0 = blockIdx.x * COLS;
   FewLds<RT> &b = ring[wave];
   const int64_t row0 = (int64_t)tile.expert * a.n + n0;
   const rsrc_t wcodes = from_here(a.w.codes + row0 * (a.steps * 64)), wscales = from_here(a.w.scales + row0 * (a.steps * 4));
@@ -843,72 +869,89 @@ __global__ __launch_bounds__(256, 2) void k_mx4_few(const Mx4Product a, const Ve
     asm volatile("" ::: "memory");
     if (s + 8 < a.steps) bring(s + 8, 1);
   }
-  for (; s < a.steps; s += 8) {
-    // this step's codes and x are there; only the next step's codes, brought after them, may be under way
-    asm volatile("" ::: "memory");
-    if (s + 8 < a.steps) __builtin_amdgcn_s_waitcnt(0x0f70 | 3 * RT);
-    else __builtin_amdgcn_s_waitcnt(0x0f70);
-    asm volatile("" ::: "memory");
-    if constexpr (P == 0) {
-#pragma unroll
-      for (int h = 0; h < 2; h++) { xc[h] = xcn[h]; xs[h] = xsn[h]; }
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; j++) x[j] = xn[j];
-    }
-    if (s + 8 < a.steps) load_x(s + 8);
-#pragma unroll
-    for (int h = 0; h < 2; h++) {
-      if (h && s + 1 >= a.steps) break;
-      i4v w[RT];
-      int ws[RT];
-#pragma unroll
-      for (int t = 0; t < RT; t++) {
-        w[t] = *(const i4v *)(b.codes[at][t] + m * 128 + ((4 * h + g) ^ (m >> 1 & 7)) * 16);
-        ws[t] = ((const uint8_t *)&b.scales[at][t][h][m])[g];
-      }
+  const uint32_t off1 = part_of >= 1 ? 0xffff0000u : 0u, off2 = part_of >= 2 ? 0xffff0000u : 0u;  // what a lane's part leaves out
+  const auto steps = [&](auto how) {
+    constexpr bool APART = decltype(how)::value;
+    for (; s < a.steps; s += 8) {
+      // this step's codes and x are there; only the next step's codes, brought after them, may be under way
+      asm volatile("" ::: "memory");
+      if (s + 8 < a.steps) __builtin_amdgcn_s_waitcnt(0x0f70 | 3 * RT);
+      else __builtin_amdgcn_s_waitcnt(0x0f70);
+      asm volatile("" ::: "memory");
       if constexpr (P == 0) {
 #pragma unroll
-        for (int t = 0; t < RT; t++) acc[t] = mfma_mx4<0>(w[t], ws[t], xc[h], xs[h], acc[t]);
+        for (int h = 0; h < 2; h++) { xc[h] = xcn[h]; xs[h] = xsn[h]; }
       } else {
 #pragma unroll
-        for (int c = 0; c < 4; c++) {
-          b8v part[P < 1 ? 1 : P];
-          if constexpr (P == 1) part[0] = __builtin_bit_cast(b8v, x[h * 4 + c].v[0]);
-          else {
-            alignas(16) E e[8];
+        for (int j = 0; j < 8; j++) x[j] = xn[j];
+      }
+      if (s + 8 < a.steps) load_x(s + 8);
 #pragma unroll
-            for (int k = 0; k < (int)sizeof(E) / 2; k++) ((uint4 *)e)[k] = x[h * 4 + c].v[k];
-            float v[8];
+      for (int h = 0; h < 2; h++) {
+        if (h && s + 1 >= a.steps) break;
+        i4v w[RT];
+        int ws[RT];
 #pragma unroll
-            for (int k = 0; k < 8; k++) v[k] = row_get(R{}, e[k]);
-            parts_of(v, part);
-          }
+        for (int t = 0; t < RT; t++) {
+          w[t] = *(const i4v *)(b.codes[at][t] + m * 128 + ((4 * h + g) ^ (m >> 1 & 7)) * 16);
+          ws[t] = ((const uint8_t *)&b.scales[at][t][h][m])[g];
+        }
+        if constexpr (P == 0) {
 #pragma unroll
-          for (int t = 0; t < RT; t++) {
-            const b8v v = values_of((uint32_t)w[t][c], __uint_as_float((uint32_t)ws[t] << 23));
+          for (int t = 0; t < RT; t++) acc[t] = mfma_mx4<0>(w[t], ws[t], xc[h], xs[h], acc[t]);
+        } else {
 #pragma unroll
-            for (int p = P - 1; p >= 0; p--) acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, part[p], acc[t], 0, 0, 0);
+          for (int c = 0; c < 4; c++) {
+            constexpr int PP = APART ? 1 : P;
+            b8v part[PP];
+            if constexpr (P == 1) part[0] = __builtin_bit_cast(b8v, x[h * 4 + c].v[0]);
+            else {
+              alignas(16) E e[8];
+#pragma unroll
+              for (int k = 0; k < (int)sizeof(E) / 2; k++) ((uint4 *)e)[k] = x[h * 4 + c].v[k];
+              float v[8];
+#pragma unroll
+              for (int k = 0; k < 8; k++) v[k] = row_get(R{}, e[k]);
+              if constexpr (APART) part[0] = part_at<P>(v, off1, off2);
+              else parts_of(v, part);
+            }
+#pragma unroll
+            for (int t = 0; t < RT; t++) {
+              const b8v v = values_of((uint32_t)w[t][c], __uint_as_float((uint32_t)ws[t] << 23));
+#pragma unroll
+              for (int p = PP - 1; p >= 0; p--) acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, part[p], acc[t], 0, 0, 0);
+            }
           }
         }
       }
+      if (s + 16 < a.steps) {
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_s_waitcnt(0xc07f);  // (the reads of what is brought over are done: lgkmcnt 0)
+        bring(s + 16, at);
+      }
+      at ^= 1;
     }
-    if (s + 16 < a.steps) {
-      asm volatile("" ::: "memory");
-      __builtin_amdgcn_s_waitcnt(0xc07f);  // (the reads of what is brought over are done: lgkmcnt 0)
-      bring(s + 16, at);
-    }
-    at ^= 1;
-  }
+  };
+  if constexpr (P > 1) {
+    if (apart) steps(std::true_type{});
+    else steps(std::false_type{});
+  } else steps(std::false_type{});
   __syncthreads();
   f4v(*const sums)[RT][64] = (f4v(*)[RT][64])ring;
 #pragma unroll
   for (int t = 0; t < RT; t++) sums[wave][t][lane] = acc[t];
   __syncthreads();
-  if (src < 0) return;
+  if (src < 0 || part_of > 0) return;
   constexpr int OUT = GATED ? RT / 2 : RT;
   for (int t = wave; t < OUT; t += 4) {
-    const auto total = [&](int u) { return (sums[0][u][lane] + sums[1][u][lane]) + (sums[2][u][lane] + sums[3][u][lane]); };
+    const auto total = [&](int u) {
+      f4v v = {};
+      for (int p = apart ? P - 1 : 0; p >= 0; p--) {  // (the smallest parts first)
+        const int l = lane + p * tile.count;
+        v += (sums[0][u][l] + sums[1][u][l]) + (sums[2][u][l] + sums[3][u][l]);
+      }
+      return v;
+    };
     f4v v = total(t);
     if (GATED) {
       const f4v u = total(t + OUT);
