@@ -797,22 +797,24 @@ __global__ __launch_bounds__(256, 2) void k_mx4_wide(const Mx4Product a, const V
 
 // ------------------------------------------------------------------ products of few rows
 // Sixteen rows of x against 16 RT rows of the matrix (gated: half of them up's): W X^T, a lane's four sums being four
-// neighbours of one row of out. Bound by the matrix's bytes. The workgroup's four waves take the steps of 256 columns in turn, each
-// by itself: codes and scales are copied to LDS of the wave's own, two steps' at a time, as whole cache lines (straight into registers
-// neighbouring lanes would be in different rows, at a quarter of the rate), x goes into registers. The sums meet at the end.
+// neighbours of one row of out. Bound by the matrix's bytes. The workgroup's eight waves take the steps of 256 columns in turn, each
+// by itself: codes and scales are copied to LDS of the wave's own as whole cache lines (straight into registers neighbouring
+// lanes would be in different rows, at a quarter of the rate), x goes into registers; while a wave waits, the sixteen of a CU
+// have others at work. The sums meet at the end.
+constexpr int FEW_W = 8;
 template <int RT>
 struct FewLds {
-  uint8_t codes[2][RT][16 * 128];
-  uint32_t scales[2][RT][2][16];
+  uint8_t codes[RT][16 * 128];
+  uint32_t scales[RT][2][16];
 };
 
 template <class X, int RT, bool GATED, int WAY>
-__global__ __launch_bounds__(256, 2) void k_mx4_few(const Mx4Product a, const Vecs vec, int out_type) {
+__global__ __launch_bounds__(FEW_W * 64, 4) void k_mx4_few(const Mx4Product a, const Vecs vec, int out_type) {
   constexpr int P = X::PARTS, COLS = GATED ? RT * 8 : RT * 16;  // COLS: out's columns
   typedef typename X::R R;
   typedef typename R::E E;
-  __shared__ __align__(16) FewLds<RT> ring[4];
-  static_assert(sizeof(ring) >= 4 * RT * 64 * sizeof(f4v), "the sums fit in its place");
+  __shared__ __align__(16) FewLds<RT> ring[FEW_W];
+  static_assert(sizeof(ring) >= FEW_W * RT * 64 * sizeof(f4v), "the sums fit in its place");
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, m = lane & 15, g = lane >> 4;
   const Tile tile = tile_of(a, blockIdx.y + blockIdx.z * gridDim.y, 16);
   if (tile.count <= 0) return;
@@ -826,75 +828,63 @@ __global__ __launch_bounds__(256, 2) void k_mx4_few(const Mx4Product a, const Ve
   const rsrc_t ucodes = GATED ? from_here(a.up.codes + row0 * (a.steps * 64)) : wcodes, uscales = GATED ? from_here(a.up.scales + row0 * (a.steps * 4)) : wscales;
   const auto row_of = [&](int t, int r) { return (uint32_t)min((GATED ? t % (RT / 2 < 1 ? 1 : RT / 2) : t) * 16 + r, a.n - 1 - n0) * (uint32_t)a.steps; };
   const auto is_up = [&](int t) { return GATED && t >= RT / 2; };
-  const auto bring = [&](int s, int at) {  // (the last step may have half of a row: that twice, the second one unused)
+  const auto bring = [&](int s) {  // (the last step may have half of a row: that twice, the second one unused)
     const bool both = s + 1 < a.steps;
 #pragma unroll
     for (int t = 0; t < RT; t++) {
 #pragma unroll
       for (int j = 0; j < 2; j++) {
         const int p = (lane & 7) ^ (((j & 1) << 2) | (lane >> 4));
-        copy16_lds(is_up(t) ? ucodes : wcodes, row_of(t, j * 8 + (lane >> 3)) * 64u + (uint32_t)(both ? p : p & 3) * 16u, s * 64, b.codes[at][t] + j * 1024);
+        copy16_lds(is_up(t) ? ucodes : wcodes, row_of(t, j * 8 + (lane >> 3)) * 64u + (uint32_t)(both ? p : p & 3) * 16u, s * 64, b.codes[t] + j * 1024);
       }
       // (two steps' scales of sixteen rows: half of the lanes)
-      if (lane < 32) copy4_lds(is_up(t) ? uscales : wscales, row_of(t, m) * 4u + (uint32_t)(min(s + (lane >> 4), a.steps - 1) * 4), 0, b.scales[at][t][0]);
+      if (lane < 32) copy4_lds(is_up(t) ? uscales : wscales, row_of(t, m) * 4u + (uint32_t)(min(s + (lane >> 4), a.steps - 1) * 4), 0, b.scales[t][0]);
     }
   };
-  // x's eight columns of group g: of half h and instruction c
-  Raw8<E> x[P == 0 ? 1 : 8], xn[P == 0 ? 1 : 8];
-  i4v xc[2], xcn[2];
-  int xs[2], xsn[2];
+  // x's eight columns of group g of each instruction: of 16-bit rows for the whole step, of 32-bit ones for half of it (registers
+  // for sixteen waves a CU)
+  constexpr int XN = P == 3 ? 4 : 8;
+  Raw8<E> x[P == 0 ? 1 : XN];
+  i4v xc[2];
+  int xs[2];
   const E *const xrow = P > 0 && (src >= 0 || WAY == X_WHOLE) ? (const E *)a.x + (int64_t)max(src, 0) * a.ld_x : nullptr;
-  const auto load_x = [&](int s) {
+  const auto load_x = [&](int s, int h0) {
     if constexpr (P == 0) {
 #pragma unroll
       for (int h = 0; h < 2; h++) {
         const int at = min(s + h, a.steps - 1);  // (behind the last: that again, unused)
-        xcn[h] = *(const i4v *)((const uint8_t *)a.x + (int64_t)max(src, 0) * (a.steps * 64) + at * 64 + g * 16);
-        xsn[h] = a.x_scales[(int64_t)max(src, 0) * (a.steps * 4) + at * 4 + g];
+        xc[h] = *(const i4v *)((const uint8_t *)a.x + (int64_t)max(src, 0) * (a.steps * 64) + at * 64 + g * 16);
+        xs[h] = a.x_scales[(int64_t)max(src, 0) * (a.steps * 4) + at * 4 + g];
       }
     } else {
 #pragma unroll
-      for (int j = 0; j < 8; j++) {
-        const int c = (s + (j >> 2)) * 128 + g * 32 + (j & 3) * 8;
-        if constexpr (WAY == X_ANY) xn[j] = raw8<E>(a, xrow, c, vec.x);
-        else xn[j] = raw8_whole<E>(a, xrow, c);
+      for (int j = 0; j < XN; j++) {
+        const int c = (s + h0 + (j >> 2)) * 128 + g * 32 + (j & 3) * 8;
+        if constexpr (WAY == X_ANY) x[j] = raw8<E>(a, xrow, c, vec.x);
+        else x[j] = raw8_whole<E>(a, xrow, c);
       }
     }
   };
   f4v acc[RT] = {};
-  int at = 0, s = wave * 2;
-  if (s < a.steps) {
-    bring(s, 0);
-    load_x(s);
-    asm volatile("" ::: "memory");
-    if (s + 8 < a.steps) bring(s + 8, 1);
-  }
   const uint32_t off1 = part_of >= 1 ? 0xffff0000u : 0u, off2 = part_of >= 2 ? 0xffff0000u : 0u;  // what a lane's part leaves out
   const auto steps = [&](auto how) {
     constexpr bool APART = decltype(how)::value;
-    for (; s < a.steps; s += 8) {
-      // this step's codes and x are there; only the next step's codes, brought after them, may be under way
+    for (int s = wave * 2; s < a.steps; s += 2 * FEW_W) {
+      bring(s);
+      load_x(s, 0);
       asm volatile("" ::: "memory");
-      if (s + 8 < a.steps) __builtin_amdgcn_s_waitcnt(0x0f70 | 3 * RT);
-      else __builtin_amdgcn_s_waitcnt(0x0f70);
+      __builtin_amdgcn_s_waitcnt(0x0f70);  // (vmcnt 0)
       asm volatile("" ::: "memory");
-      if constexpr (P == 0) {
-#pragma unroll
-        for (int h = 0; h < 2; h++) { xc[h] = xcn[h]; xs[h] = xsn[h]; }
-      } else {
-#pragma unroll
-        for (int j = 0; j < 8; j++) x[j] = xn[j];
-      }
-      if (s + 8 < a.steps) load_x(s + 8);
 #pragma unroll
       for (int h = 0; h < 2; h++) {
         if (h && s + 1 >= a.steps) break;
+        if (XN == 4 && h) load_x(s, 1);
         i4v w[RT];
         int ws[RT];
 #pragma unroll
         for (int t = 0; t < RT; t++) {
-          w[t] = *(const i4v *)(b.codes[at][t] + m * 128 + ((4 * h + g) ^ (m >> 1 & 7)) * 16);
-          ws[t] = ((const uint8_t *)&b.scales[at][t][h][m])[g];
+          w[t] = *(const i4v *)(b.codes[t] + m * 128 + ((4 * h + g) ^ (m >> 1 & 7)) * 16);
+          ws[t] = ((const uint8_t *)&b.scales[t][h][m])[g];
         }
         if constexpr (P == 0) {
 #pragma unroll
@@ -904,11 +894,11 @@ __global__ __launch_bounds__(256, 2) void k_mx4_few(const Mx4Product a, const Ve
           for (int c = 0; c < 4; c++) {
             constexpr int PP = APART ? 1 : P;
             b8v part[PP];
-            if constexpr (P == 1) part[0] = __builtin_bit_cast(b8v, x[h * 4 + c].v[0]);
+            if constexpr (P == 1) part[0] = __builtin_bit_cast(b8v, x[(XN == 4 ? 0 : h * 4) + c].v[0]);
             else {
               alignas(16) E e[8];
 #pragma unroll
-              for (int k = 0; k < (int)sizeof(E) / 2; k++) ((uint4 *)e)[k] = x[h * 4 + c].v[k];
+              for (int k = 0; k < (int)sizeof(E) / 2; k++) ((uint4 *)e)[k] = x[(XN == 4 ? 0 : h * 4) + c].v[k];
               float v[8];
 #pragma unroll
               for (int k = 0; k < 8; k++) v[k] = row_get(R{}, e[k]);
@@ -924,12 +914,8 @@ __global__ __launch_bounds__(256, 2) void k_mx4_few(const Mx4Product a, const Ve
           }
         }
       }
-      if (s + 16 < a.steps) {
-        asm volatile("" ::: "memory");
-        __builtin_amdgcn_s_waitcnt(0xc07f);  // (the reads of what is brought over are done: lgkmcnt 0)
-        bring(s + 16, at);
-      }
-      at ^= 1;
+      asm volatile("" ::: "memory");
+      __builtin_amdgcn_s_waitcnt(0xc07f);  // (lgkmcnt 0: the reads of what the next step is brought over)
     }
   };
   if constexpr (P > 1) {
@@ -943,12 +929,13 @@ __global__ __launch_bounds__(256, 2) void k_mx4_few(const Mx4Product a, const Ve
   __syncthreads();
   if (src < 0 || part_of > 0) return;
   constexpr int OUT = GATED ? RT / 2 : RT;
-  for (int t = wave; t < OUT; t += 4) {
+  for (int t = wave; t < OUT; t += FEW_W) {
     const auto total = [&](int u) {
       f4v v = {};
       for (int p = apart ? P - 1 : 0; p >= 0; p--) {  // (the smallest parts first)
         const int l = lane + p * tile.count;
-        v += (sums[0][u][l] + sums[1][u][l]) + (sums[2][u][l] + sums[3][u][l]);
+#pragma unroll
+        for (int w = 0; w < FEW_W; w += 4) v += (sums[w][u][l] + sums[w + 1][u][l]) + (sums[w + 2][u][l] + sums[w + 3][u][l]);
       }
       return v;
     };
@@ -1010,25 +997,43 @@ static hipError_t tiled(const Mx4Product &a, const Vecs &x_vec, int out_type, hi
 template <class X, int RT, bool GATED>
 static hipError_t few(const Mx4Product &a, const Vecs &vec, int out_type, hipStream_t s) {
   constexpr int COLS = GATED ? RT * 8 : RT * 16;
-  const dim3 grid = tile_grid((a.n + COLS - 1) / COLS, tiles_most(a, 16)), block(256);
+  const dim3 grid = tile_grid((a.n + COLS - 1) / COLS, tiles_most(a, 16)), block(FEW_W * 64);
   if (X::PARTS == 0 || (vec.x && a.cols % 8 == 0)) hipLaunchKernelGGL((k_mx4_few<X, RT, GATED, X_WHOLE>), grid, block, 0, s, a, vec, out_type);
   else if constexpr (X::PARTS > 0) hipLaunchKernelGGL((k_mx4_few<X, RT, GATED, X_ANY>), grid, block, 0, s, a, vec, out_type);
   return hipGetLastError();
 }
 
+// Which kernel: by the rows that a matrix has on average and by the workgroups that there would be. Dense products in us, from
+// a captured graph (rows of bf16, unless said otherwise; few / tiles of 64 rows):
+//   2048 columns, 4096 rows of the matrix: 16 rows 4.6 / 13, 128 rows 9.4 / 15, 256 rows 15.8 / 17.7, 384 rows 22.5 / 19
+//   4096 columns, 2048:                    64 rows 9.0 / 25, 256 rows 16 / 30, 384 rows 22.5 / 31
+//   1024 columns, 1024:                    64 rows 3.7 / 8.9, 384 rows 6.4 / 9.1
+//   2048 columns, 4096, fp32 rows:         128 rows 15 / 42, 384 rows 38 / 50
+//   2048 columns, 4096, 4-bit rows:        64 rows 5.0 / 6.4, 128 rows 7.3 / 6.6, 256 rows 11.7 / 8.6
+//   2048 columns, 151936, 9 rows:          40 / 49 (tiles of 32)
+// so the few rows' kernel has up to 16 rows, and more where the tiles would leave CUs idle: up to 128 tiles, 192 of fp32 rows,
+// 48 of 4-bit ones. By expert, 24 rows of 2048 to 8 of 128 experts take it 40 us (1.5 rows each), 216 rows 70 and in tiles of 32
+// 61 (13.5 each). Tiles of 64 and 128 rows: 4095 rows of 4096 columns 81 and 70, 512 rows of 2048 columns 21 and 24, 250 rows
+// each of 32 experts of 1024 columns 28 and 33; of 4-bit rows 4095 x 4096 35 and 28, 256 rows each of 128 experts 124 and 115.
 template <class X>
 static hipError_t product(const Mx4Product &a, int out_type, hipStream_t s) {
-  constexpr int MOST = X::PARTS <= 2 ? 128 : 64;
-  const Vecs vec = {X::PARTS == 0 || on16(a.x, a.ld_x, sizeof(typename X::R::E)),
-                    (uintptr_t)a.out % (out_type == T_F32 ? 16 : 8) == 0 && a.ld_out % 4 == 0};
-  int64_t each = a.starts ? a.rows / a.n_expert : a.rows;  // rows of a matrix, where they are even
-  if (X::PARTS == 0 && (int64_t)a.x_rows * a.steps * 64 > UINT32_MAX) each = 0;  // (the tiles' addresses of x have 32 bits)
-  if (each > 64 && MOST == 128) return tiled<X, MOST>(a, vec, out_type, s);
-  if (each > 24) return tiled<X, 64>(a, vec, out_type, s);
-  if (each > 8) return tiled<X, 32>(a, vec, out_type, s);
-  const bool many = tiles_most(a, 16) * ((a.n + 63) / 64) >= 512;
-  if (a.up.codes) return many ? few<X, 4, true>(a, vec, out_type, s) : few<X, 2, true>(a, vec, out_type, s);
-  return many ? few<X, 4, false>(a, vec, out_type, s) : few<X, 1, false>(a, vec, out_type, s);
+  constexpr int P = X::PARTS;
+  const Vecs vec = {P == 0 || on16(a.x, a.ld_x, sizeof(typename X::R::E)), (uintptr_t)a.out % (out_type == T_F32 ? 16 : 8) == 0 && a.ld_out % 4 == 0};
+  const bool gated = a.up.codes != nullptr;
+  const int64_t each = a.starts ? a.rows / a.n_expert : a.rows;
+  const int64_t tiles64 = tiles_most(a, 64) * ((a.n + (gated ? 63 : 127)) / (gated ? 64 : 128));
+  const bool far = P == 0 && (int64_t)a.x_rows * a.steps * 64 > UINT32_MAX;  // (the tiles' addresses of 4-bit rows have 32 bits)
+  if (far || each <= (a.starts ? 8 : 16) || tiles64 <= (P == 0 ? 48 : P == 3 ? 192 : 128)) {
+    // rows of the matrix a workgroup: 64 where that makes half a workgroup a CU, else 16 (gated 32): 64 rows of 2048 columns to
+    // 4096 6.3 and 10.8 us, 9 rows 5.6 and 4.1
+    const bool many = tiles_most(a, 16) * ((a.n + 63) / 64) >= 128;
+    if (gated) return many ? few<X, 4, true>(a, vec, out_type, s) : few<X, 2, true>(a, vec, out_type, s);
+    return many ? few<X, 4, false>(a, vec, out_type, s) : few<X, 1, false>(a, vec, out_type, s);
+  }
+  if (each <= 24) return tiled<X, 32>(a, vec, out_type, s);
+  if constexpr (P < 3)  // (fp32 parts of 128 rows leave LDS for one workgroup a CU: 4095 rows of 4096 columns 254 us instead of 218)
+    if (each > (P == 0 ? 64 : 512)) return tiled<X, 128>(a, vec, out_type, s);
+  return tiled<X, 64>(a, vec, out_type, s);
 }
 hipError_t launch_mx4_matmul(const Mx4Product &a, int type, int out_type, hipStream_t s) {
   switch (type) {
