@@ -183,8 +183,42 @@ def test_strides(ctx, kind, pad, off):
     assert (into[:, :off] == 5.0).all() and (into[:, off + n:] == 5.0).all()
 
 
+# Enough tiles for the kernels of many rows: of 32, 64 and 128 rows; odd columns, a part of a turn, of a step and of a block.
+TILES = [(17, 192, 24700), (24, 320, 16500), (33, 130, 24700), (60, 576, 12600), (520, 200, 2900), (600, 64, 2700), (600, 300, 2625)]
+
+
+@pytest.mark.parametrize("kind", [F32, F16, BF16, "mx4"])
+@pytest.mark.parametrize("rows,cols,n", TILES)
+@pytest.mark.parametrize("gated", [False, True])
+def test_dense_tiles(ctx, kind, rows, cols, n, gated):
+    from spindle_amd import ops
+    rng = np.random.default_rng(rows * 7 + cols + n)
+    x, xv = rows_of_x(rng, kind, rows, cols)
+    w, wv = lowered(*matrix(rng, n, cols), 2.0 ** -9)
+    up, uv = lowered(*matrix(rng, n, cols), 2.0 ** -9) if gated else (None, None)
+    dtype = BF16 if kind == "mx4" else kind
+    check(ops.mx4_matmul(ctx, x, w, up=up, dtype=dtype), xv, wv, uv, kind, dtype)
+
+
+@pytest.mark.parametrize("kind,cols", [(F32, 131), (F16, 131), (BF16, 131), (F32, 200), (BF16, 200), (BF16, 192)])
+@pytest.mark.parametrize("pad,off", [(8, 0), (3, 1), (0, 0)])
+@pytest.mark.parametrize("rows,n", [(20, 25000), (530, 2900)])
+def test_tile_strides(ctx, kind, cols, pad, off, rows, n):
+    """Tiles over rows that are apart, at odd addresses, of odd lengths; what lies between rows of out stays."""
+    from spindle_amd import ops
+    rng = np.random.default_rng(pad + cols)
+    x, xv = rows_of_x(rng, kind, rows, cols, pad, off)
+    w, wv = lowered(*matrix(rng, n, cols), 2.0 ** -9)
+    into = torch.full((rows, n + pad + off), 5.0, dtype=kind, device="cuda")
+    ops.mx4_matmul(ctx, x, w, out=into[:, off:off + n])
+    check(into[:, off:off + n], xv, wv, None, kind, kind)
+    assert (into[:, :off] == 5.0).all() and (into[:, off + n:] == 5.0).all()
+
+
 GROUPS = [(1, 8, 128, 128, 40), (5, 2, 4, 100, 33), (24, 8, 32, 256, 64), (100, 4, 6, 300, 100), (90, 8, 3, 64, 130), (300, 2, 5, 160, 72),
-          (40, 2, 4, 700, 530), (100, 4, 9, 200, 300)]
+          (40, 2, 4, 700, 530), (100, 4, 9, 200, 300),
+          # many tiles: 12, 40 and 600 rows a matrix, and more experts than a search keeps in registers
+          (300, 4, 100, 128, 300), (700, 4, 70, 200, 260), (2400, 2, 8, 100, 300), (500, 2, 300, 64, 100)]
 
 
 @pytest.mark.parametrize("kind", [F32, F16, BF16, "mx4"])
@@ -215,12 +249,12 @@ def test_by_expert(ctx, kind, rows, k, experts, cols, n, gated, sort_first, drop
 
 
 @pytest.mark.parametrize("kind", [F32, BF16, "mx4"])
-@pytest.mark.parametrize("rows", [6, 150])
-def test_rows_without_an_entry(ctx, kind, rows):
+@pytest.mark.parametrize("rows,n", [(6, 48), (150, 48), (40, 13000), (1200, 1600)])
+def test_rows_without_an_entry(ctx, kind, rows, n):
     """A row whose order names no row of x stays as it was, among rows that have one; so do rows that starts leave out."""
     from spindle_amd import ops
     rng = np.random.default_rng(rows)
-    cols, n = 128, 48
+    cols = 128
     x, xv = rows_of_x(rng, kind, rows, cols)
     w, wv = matrix(rng, 2 * n, cols)
     dtype = F32
@@ -229,12 +263,11 @@ def test_rows_without_an_entry(ctx, kind, rows):
     out = torch.full((rows, n), 7.0, dtype=dtype, device="cuda")
     cut = rows // 2
     ops.mx4_matmul(ctx, x, w, starts=ints([1, cut, rows - 1]), order=ints(order), k=2, dtype=dtype, out=out)
-    for i in range(rows):
-        if i in (0, 1, 4, rows - 1):
-            assert (out[i] == 7.0).all()
-        else:
-            at = slice(0, n) if i < cut else slice(n, 2 * n)
-            check(out[i:i + 1], xv[order[i] // 2][None], wv[at], None, kind, dtype)
+    none = [0, 1, 4, rows - 1]
+    assert (out[none] == 7.0).all()
+    for a, b, at in ((1, cut, slice(0, n)), (cut, rows - 1, slice(n, 2 * n))):
+        some = [i for i in range(a, b) if i not in none]
+        check(out[some], xv[order[some] // 2], wv[at], None, kind, dtype)
     # starts past the rows are cut there
     out.fill_(7.0)
     ops.mx4_matmul(ctx, x, w, starts=ints([-5, cut, 10 ** 6]), order=ints(order), k=2, dtype=dtype, out=out)
@@ -242,12 +275,12 @@ def test_rows_without_an_entry(ctx, kind, rows):
 
 
 @pytest.mark.parametrize("kind", [F32, F16, BF16, "mx4"])
-@pytest.mark.parametrize("rows", [3, 70, 200])
-def test_special_values(ctx, kind, rows):
+@pytest.mark.parametrize("rows,n", [(3, 36), (70, 36), (200, 36), (20, 25000), (60, 12800), (530, 2900)])
+def test_special_values(ctx, kind, rows, n):
     """NaN and infinities stay in their rows, NaN scales in their matrix's; scales to the ends of their range."""
     from spindle_amd import ops
     rng = np.random.default_rng(5)
-    cols, n = 260, 36
+    cols = 260
     w, wv = matrix(rng, n, cols)
     w.data[n * R.padded(cols) // 2 + 4 * R.padded(cols) // 32] = 255  # the first block of row 4
     if kind == "mx4":
@@ -279,12 +312,12 @@ def test_special_values(ctx, kind, rows):
     assert not np.isnan(want[np.ix_(keep, others)]).any()
 
 
-@pytest.mark.parametrize("rows", [2, 40])
-def test_wide_scales(ctx, rows):
+@pytest.mark.parametrize("rows,n", [(2, 24), (40, 24), (20, 6500), (80, 6500)])
+def test_wide_scales(ctx, rows, n):
     """Products whose scales lie far apart, each way, keep their values: x times 2^40, the matrix times 2^-60."""
     from spindle_amd import ops
     rng = np.random.default_rng(rows)
-    cols, n = 256, 24
+    cols = 256
     w, wv = lowered(*matrix(rng, n, cols, 30), 2.0 ** -60)
     m, mv = matrix(rng, rows, cols, 30)
     m.data[rows * cols // 2:] += 40
@@ -303,9 +336,9 @@ def test_no_rows(ctx):
 def test_same_bits_every_time(ctx):
     from spindle_amd import ops
     rng = np.random.default_rng(11)
-    w, _ = matrix(rng, 3 * 200, 700)
+    w, _ = matrix(rng, 3 * 3000, 700)
     for kind in (F32, BF16, "mx4"):
-        for rows in (5, 90, 400):
+        for rows in (5, 70, 90, 400, 1700):
             x, _ = rows_of_x(rng, kind, rows, 700)
             starts = ints([0, rows // 5, rows // 2, rows])
             a = ops.mx4_matmul(ctx, x, w, starts=starts, dtype=F32)
