@@ -7,7 +7,9 @@
 namespace spx {
 
 // ------------------------------------------------------------------ the router
-// A wave has a row, its lane l the logits l, l + 64, ...; NV of them.
+// A wave has a row, its lane l the logits l, l + 64, ...; NV of them. 8191 rows of 128 logits take 6.2 us, eight rounds of
+// a maximum across the wave (ten instructions that wait for each other) being most of it, the gradient 6.1; their bytes 1 and
+// 2 us. 24 rows take 3.5 us, little more than a launch.
 
 // Logits' order as numbers: larger logit, larger number; -0 as 0; NaN above all. 0: none.
 __device__ __forceinline__ uint32_t logit_key(float v) {
@@ -166,7 +168,9 @@ hipError_t launch_moe_route_grad(const RouteArgs &a, int type, hipStream_t s) {
 // A counting sort that keeps the order of equal ones. A workgroup has a run of entries, each of its waves
 // a run of those; entries of no expert are those of a last, (n_expert + 1)-th bucket. An entry's place is its
 // bucket's start, plus the bucket's entries in earlier workgroups, in the workgroup's earlier waves, earlier in the
-// wave's run and at lower lanes. Counts are sums of integers: no order of additions changes them.
+// wave's run and at lower lanes. Counts are sums of integers: no order of additions changes them. Up to 4096 entries are one
+// workgroup's (192 entries 3.9 us), more have a launch that counts before (65528 entries 4.8 + 5.7 us): both bound by launches and
+// dependent steps, not by their 0.8 MB.
 constexpr int SORT_T = 512, SORT_W = SORT_T / 64;
 constexpr int SORT_ALONE = 4096;  // so many entries are one workgroup's
 
@@ -211,7 +215,8 @@ __global__ __launch_bounds__(SORT_T) void k_moe_place(const SortArgs a, int run)
       if (gridDim.x == 1) {
         for (int w = 0; w < SORT_W; w++) all += at[w * nb + e];
       } else {
-        for (int g = 0; g < (int)gridDim.x; g++) {
+#pragma unroll 16
+        for (int g = 0; g < (int)gridDim.x; g++) {  // (sixteen loads under way: 64 workgroups 5.7 us, one by one 19)
           const int c = a.counts[(int64_t)g * nb + e];
           all += c;
           before += g < (int)blockIdx.x ? c : 0;
@@ -289,57 +294,88 @@ struct RowPiece {
     if constexpr (VEC) *(uint4 *)p = *(const uint4 *)e;
     else *p = e[0];
   }
+  // The same past the caches.
+  static __device__ __forceinline__ void put_past(E *p, const float (&x)[N]) {
+    alignas(16) E e[N];
+#pragma unroll
+    for (int i = 0; i < N; i++) e[i] = row_put(R{}, x[i]);
+    if constexpr (VEC) __builtin_nontemporal_store(*(const i4v *)e, (i4v *)p);
+    else *p = e[0];
+  }
 };
 
+// Bound by its bytes, most of them out; four rows a thread, so that their entries and then their pieces are under way
+// together, and past the caches on the way out, which leaves these to x (read k times). 8191 rows of 2048 in bf16, eight places
+// each, 302 MB: 77 us (eight rows a thread or one 84, through the caches 82), 3.9 TB/s where a copy reaches 5.1.
+constexpr int GATHER_ROWS = 4;
 template <class R, bool VEC>
 __global__ __launch_bounds__(256) void k_moe_gather(const JoinArgs a, int log_t) {
   typedef RowPiece<R, VEC> P;
   typedef typename R::E E;
-  const int i = blockIdx.x * (256 >> log_t) + (threadIdx.x >> log_t), t = threadIdx.x & ((1 << log_t) - 1);
+  const int each = 256 >> log_t, i0 = blockIdx.x * (each * GATHER_ROWS) + (threadIdx.x >> log_t), t = threadIdx.x & ((1 << log_t) - 1);
   const int n = a.rows * a.k;
-  if (i >= n) return;
-  const int entry = a.order[i];
-  const bool is = entry >= 0 && entry < n;
-  const E *src = (const E *)a.x + (int64_t)(is ? entry / a.k : 0) * a.ld_x;
-  E *dst = (E *)a.out + (int64_t)i * a.ld_out;
-  const float w = a.weights && is ? a.weights[entry] : 1.0f;
+  const E *src[GATHER_ROWS];
+  float w[GATHER_ROWS];
+  bool is[GATHER_ROWS];
+  int entry[GATHER_ROWS];
+#pragma unroll
+  for (int r = 0; r < GATHER_ROWS; r++) entry[r] = a.order[min(i0 + r * each, n - 1)];
+#pragma unroll
+  for (int r = 0; r < GATHER_ROWS; r++) {
+    is[r] = entry[r] >= 0 && entry[r] < n;
+    src[r] = (const E *)a.x + (int64_t)(is[r] ? entry[r] / a.k : 0) * a.ld_x;
+    w[r] = a.weights && is[r] ? a.weights[entry[r]] : 1.0f;
+  }
   for (int c = t; c < a.width / P::N; c += 1 << log_t) {
-    float x[P::N] = {};
-    if (is) P::get(src + c * P::N, x);
-    if (a.weights)
+    float x[GATHER_ROWS][P::N];
 #pragma unroll
-      for (int j = 0; j < P::N; j++) x[j] *= w;
-    if (!is)
+    for (int r = 0; r < GATHER_ROWS; r++) P::get(src[r] + c * P::N, x[r]);
 #pragma unroll
-      for (int j = 0; j < P::N; j++) x[j] = 0.0f;
-    P::put(dst + c * P::N, x);
+    for (int r = 0; r < GATHER_ROWS; r++) {
+      const int i = i0 + r * each;
+      if (i >= n) break;
+#pragma unroll
+      for (int j = 0; j < P::N; j++) x[r][j] = is[r] ? (a.weights ? x[r][j] * w[r] : x[r][j]) : 0.0f;
+      P::put_past((E *)a.out + (int64_t)i * a.ld_out + c * P::N, x[r]);
+    }
   }
 }
 
+// Bound by its bytes, most of them in; eight places at a time, so that their pieces are under way together. The same
+// rows, 302 MB: 56 us (four at a time 81), 5.4 TB/s.
 template <class R, bool VEC>
 __global__ __launch_bounds__(256) void k_moe_combine(const JoinArgs a, int log_t) {
   typedef RowPiece<R, VEC> P;
   typedef typename R::E E;
+  constexpr int J = 8;
   const int r = blockIdx.x * (256 >> log_t) + (threadIdx.x >> log_t), t = threadIdx.x & ((1 << log_t) - 1);
   if (r >= a.rows) return;
   const int n = a.rows * a.k;
   for (int c = t; c < a.width / P::N; c += 1 << log_t) {
     float sum[P::N] = {};
-#pragma unroll 4
-    for (int j = 0; j < a.k; j++) {
-      const int p = a.place[(int64_t)r * a.k + j];
-      const bool is = p >= 0 && p < n;
-      const float w = a.weights ? a.weights[(int64_t)r * a.k + j] : 1.0f;
-      float x[P::N];
-      P::get((const E *)a.x + (is ? p : 0) * a.ld_x + c * P::N, x);
+    for (int j0 = 0; j0 < a.k; j0 += J) {
+      int p[J];
+      float w[J], x[J][P::N];
 #pragma unroll
-      for (int i = 0; i < P::N; i++) sum[i] = is ? fmaf(w, x[i], sum[i]) : sum[i];
+      for (int j = 0; j < J; j++) {
+        p[j] = j0 + j < a.k ? a.place[(int64_t)r * a.k + j0 + j] : -1;
+        w[j] = a.weights && j0 + j < a.k ? a.weights[(int64_t)r * a.k + j0 + j] : 1.0f;
+      }
+#pragma unroll
+      for (int j = 0; j < J; j++) P::get((const E *)a.x + (p[j] >= 0 && p[j] < n ? p[j] : 0) * a.ld_x + c * P::N, x[j]);
+#pragma unroll
+      for (int j = 0; j < J; j++) {
+        const bool is = p[j] >= 0 && p[j] < n;
+#pragma unroll
+        for (int i = 0; i < P::N; i++) sum[i] = is ? fmaf(w[j], x[j][i], sum[i]) : sum[i];
+      }
     }
     P::put((E *)a.out + (int64_t)r * a.ld_out + c * P::N, sum);
   }
 }
 
-// A wave has an entry: its row's d_out against its sorted row of y.
+// A wave has an entry: its row's d_out against its sorted row of y. (4097 rows of 1024 in fp32, eight places: 49 us, 285 MB, 5.8 TB/s;
+// d_out is read eight times, seven of them from the caches.)
 template <class R, bool VEC>
 __global__ __launch_bounds__(256) void k_moe_combine_grad(const JoinArgs a) {
   typedef RowPiece<R, VEC> P;
@@ -385,7 +421,7 @@ static void join(const JoinArgs &a, int what, hipStream_t s) {
   const int pieces = vec ? a.width * size / 16 : a.width;
   int log_t = 0;
   while (log_t < 8 && (1 << log_t) < pieces) log_t++;
-  const int rows = what == 0 ? a.rows * a.k : a.rows, each = 256 >> log_t;
+  const int rows = what == 0 ? a.rows * a.k : a.rows, each = (256 >> log_t) * (what == 0 ? GATHER_ROWS : 1);
   const dim3 grid((unsigned)((rows + each - 1) / each)), block(256);
   if (what == 0) {
     if (vec) hipLaunchKernelGGL((k_moe_gather<R, true>), grid, block, 0, s, a, log_t);

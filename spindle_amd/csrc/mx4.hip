@@ -17,7 +17,9 @@ typedef __bf16 b2v __attribute__((ext_vector_type(2)));
 typedef __bf16 b8v __attribute__((ext_vector_type(8)));
 
 // ------------------------------------------------------------------ rows in and out
-// A thread has eight columns, the four threads of a quad a block, sixteen threads a step of 128 columns.
+// A thread has eight columns, the four threads of a quad a block, sixteen threads a step of 128 columns. Bound by their bytes: 8191
+// rows of 2048 in bf16 9.1 us in and 9.6 us out (42 MB each), 16384 of 1024 in fp32 13 and 14.8 us (76 MB, from and to the
+// last cache).
 struct Eight {
   int row, c8;  // columns 8 c8 ..
 };
