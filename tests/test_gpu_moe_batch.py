@@ -313,3 +313,27 @@ def test_no_rows(ctx):
     assert ops.moe_combine(ctx, x, none).shape == (0, 16)
     d_y, d_w = ops.moe_combine_grad(ctx, x, x, none.flatten(), none, torch.zeros(0, 3, device="cuda"))
     assert d_y.shape == (0, 16) and d_w.shape == (0, 3)
+
+
+def test_far_rows(ctx):
+    """Sorted rows past 2^32 bytes: gathered, joined, and the gradient, looked at in some of them."""
+    from spindle_amd import ops
+    rows, k, width, experts = 150_000, 8, 2048, 40
+    g = torch.Generator(device="cuda")
+    g.manual_seed(3)
+    ids = torch.randint(0, experts, (rows, k), generator=g, device="cuda", dtype=torch.int32)
+    o = ops.moe_sort(ctx, ids, experts)
+    x = torch.randn(rows, width, generator=g, device="cuda", dtype=BF16)
+    y = ops.moe_gather(ctx, x, o.order, k)
+    some = torch.cat([torch.arange(5, device="cuda"), torch.arange(rows * k - 5, rows * k, device="cuda"), torch.randint(0, rows * k, (50,), generator=g, device="cuda")])
+    assert torch.equal(y[some], x[o.order[some].long() // k])
+    w = torch.randint(-3, 4, (rows, k), generator=g, device="cuda").float()
+    got = ops.moe_combine(ctx, y, o.place, w)
+    want = f64(x[-50:]) * f64(w[-50:]).sum(1)[:, None]  # (every place of a row holds the row)
+    close(got[-50:], want, np.abs(f64(x[-50:])) * f64(w[-50:].abs()).sum(1)[:, None] * k * R.U + R.rounding(want * (1 + 2.0 ** -20), BF16))
+    d_y, d_w = ops.moe_combine_grad(ctx, x, y, o.order, o.place, w)
+    e = o.order[some].long()
+    want = f64(w).reshape(-1)[e.cpu().numpy()][:, None] * f64(x[e // k])
+    close(d_y[some], want, np.abs(want) * R.U + R.rounding(want * (1 + R.U), BF16))
+    sq = f64(x[-20:]) ** 2
+    close(d_w[-20:], np.repeat(sq.sum(1)[:, None], k, 1), np.repeat(sq.sum(1)[:, None], k, 1) * (width / 64 + 24) * R.U)

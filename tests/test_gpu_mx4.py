@@ -327,6 +327,53 @@ def test_wide_scales(ctx, rows, n):
     check(ops.mx4_matmul(ctx, x, w), f64(x), wv, None, F32, F32)
 
 
+@pytest.mark.parametrize("x_rows", [3_300_000, 5_000_000])
+@pytest.mark.parametrize("rows,n", [(5, 40), (80, 6500)])
+def test_far_rows_of_x(ctx, x_rows, rows, n):
+    """Rows of x whose codes lie past 2^31 and past 2^32 bytes."""
+    from spindle_amd import ops
+    rng = np.random.default_rng(rows)
+    cols = 2048
+    data = torch.zeros(ops.Mx4.nbytes(x_rows, cols), dtype=torch.uint8, device="cuda")
+    some = np.concatenate([[0, x_rows - 1], rng.integers(x_rows - 100, x_rows, rows - 2)])
+    codes, scales = rng.integers(0, 16, (100, cols)), rng.integers(121, 134, (100, cols // 32))
+    packed = torch.from_numpy(R.pack(codes, scales)).cuda()
+    end = x_rows * cols // 2
+    data[end - 100 * cols // 2:end] = packed[:100 * cols // 2]
+    data[end + (x_rows - 100) * cols // 32:] = packed[100 * cols // 2:]
+    values = R.unpack(packed.cpu().numpy(), 100, cols)
+    x = np.where((some >= x_rows - 100)[:, None], values[np.maximum(some - (x_rows - 100), 0)], 0.0)
+    w, wv = matrix(rng, n, cols)
+    got = ops.mx4_matmul(ctx, ops.Mx4(data, x_rows, cols), w, starts=ints([0, rows]), order=ints(some), dtype=F32)
+    check(got, x, wv, None, "mx4", F32)
+
+
+@pytest.mark.parametrize("kind", [BF16, "mx4"])
+@pytest.mark.parametrize("rows,n", [(3, 40), (70, 9000)])
+def test_far_matrix(ctx, kind, rows, n):
+    """The matrix of an expert past 2^32 bytes."""
+    from spindle_amd import ops
+    rng = np.random.default_rng(rows)
+    cols = 2048
+    experts = min(1024, 4_400_000 // n)
+    many = experts * n
+    if many * 1088 < 2 ** 32:
+        cols = 1 << 18 if n < 100 else cols
+    p = R.padded(cols)
+    data = torch.zeros(ops.Mx4.nbytes(many, cols), dtype=torch.uint8, device="cuda")
+    assert data.numel() > 2 ** 32
+    codes, scales = rng.integers(0, 16, (n, p)), rng.integers(112, 125, (n, p // 32))
+    packed = torch.from_numpy(R.pack(codes, scales)).cuda()
+    end = many * p // 2
+    data[end - n * p // 2:end] = packed[:n * p // 2]
+    data[end + (many - n) * p // 32:] = packed[n * p // 2:]
+    x, xv = rows_of_x(rng, kind, rows, cols)
+    starts = np.zeros(experts + 1, np.int64)
+    starts[-1] = rows
+    got = ops.mx4_matmul(ctx, x, ops.Mx4(data, many, cols), starts=ints(starts), dtype=F32)
+    check(got, xv, R.unpack(packed.cpu().numpy(), n, cols), None, kind, F32)
+
+
 def test_no_rows(ctx):
     from spindle_amd import ops
     w, _ = matrix(np.random.default_rng(1), 8, 64)
