@@ -356,7 +356,8 @@ __device__ __forceinline__ bool tile_place(const Mx4Product &a, int most, int co
   return false;
 }
 
-// Eight columns of a row of x as they lie in memory, zeros behind the last and where there is no row.
+// ------------------------------------------------------------------ rows of x
+// Eight columns of a row as they lie in memory, zeros behind the last and where there is no row.
 template <class E>
 struct Raw8 { uint4 v[sizeof(E) / 2]; };
 template <class E>
@@ -374,6 +375,23 @@ __device__ __forceinline__ Raw8<E> raw8(const Mx4Product &a, const E *row, int c
   }
   return r;
 }
+
+// The same where rows lie at multiples of 16 bytes and cols is a multiple of 8: no branch, so that a thread's loads go out
+// together (`row` is some row of x where there is none: its products are not stored).
+template <class E>
+__device__ __forceinline__ Raw8<E> raw8_whole(const Mx4Product &a, const E *row, int c) {
+  Raw8<E> r;
+  const uint4 *const from = (const uint4 *)(row + min(c, a.cols - 8));
+#pragma unroll
+  for (int i = 0; i < (int)sizeof(E) / 2; i++) r.v[i] = from[i];
+  if (c >= a.cols)
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(E) / 2; i++) r.v[i] = make_uint4(0, 0, 0, 0);
+  return r;
+}
+
+// How rows of x come: copied to LDS as they lie (bf16, whole turns), loaded in whole pieces, or by elements where need be.
+enum { X_COPIED, X_WHOLE, X_ANY };
 
 // ------------------------------------------------------------------ products of many 4-bit rows
 // MT rows of x against 64 WN rows of the matrix (gated: half of them up's), 256 columns a turn, four waves of MF * 32 rows of x
@@ -595,23 +613,6 @@ __global__ __launch_bounds__(256, MT == 64 ? 3 : 2) void k_mx4_four(const Mx4Pro
 // bf16 rows are copied to LDS as they lie where they can be, others go through registers, a turn ahead. 4095 rows of 4096 columns
 // to 2048: bf16 65-68 us (1.0 PFLOP/s, a library product of bf16 matrices of 8192 reaches 1.2), fp16 147, fp32 220 (each product
 // two and three times); 216 rows of 2048 columns to eight of 128 experts, gated: 61 us, 3.6 TB/s.
-// The same where rows lie at multiples of 16 bytes and cols is a multiple of 8: no branch, so that a thread's loads go out
-// together (`row` is some row of x where there is none: its products are not stored).
-template <class E>
-__device__ __forceinline__ Raw8<E> raw8_whole(const Mx4Product &a, const E *row, int c) {
-  Raw8<E> r;
-  const uint4 *const from = (const uint4 *)(row + min(c, a.cols - 8));
-#pragma unroll
-  for (int i = 0; i < (int)sizeof(E) / 2; i++) r.v[i] = from[i];
-  if (c >= a.cols)
-#pragma unroll
-    for (int i = 0; i < (int)sizeof(E) / 2; i++) r.v[i] = make_uint4(0, 0, 0, 0);
-  return r;
-}
-
-// How rows of x come: copied to LDS as they lie (bf16, whole turns), loaded in whole pieces, or by elements where need be.
-enum { X_COPIED, X_WHOLE, X_ANY };
-
 template <class X, int MT>
 struct Wide {
   static constexpr int P = X::PARTS, WM = MT == 32 ? 1 : 2, WN = 4 / WM, MF = MT / 32 / WM, ROWS = WN * 64;
