@@ -1,5 +1,8 @@
 // A mixture of experts over a batch: the router's choice and its gradient, rows sorted by expert, gathered,
 // joined again and that gradient (spx_moe_route .. spx_moe_combine_grad).
+#include <algorithm>
+#include <type_traits>
+
 #include "dev.h"
 #include "experts.h"
 #include "rows.h"
@@ -294,24 +297,29 @@ struct RowPiece {
     if constexpr (VEC) *(uint4 *)p = *(const uint4 *)e;
     else *p = e[0];
   }
-  // The same past the caches.
-  static __device__ __forceinline__ void put_past(E *p, const float (&x)[N]) {
-    alignas(16) E e[N];
-#pragma unroll
-    for (int i = 0; i < N; i++) e[i] = row_put(R{}, x[i]);
-    if constexpr (VEC) __builtin_nontemporal_store(*(const i4v *)e, (i4v *)p);
-    else *p = e[0];
-  }
 };
 
-// Bound by its bytes, most of them out; four rows a thread, so that their entries and then their pieces are under way
-// together, and past the caches on the way out, which leaves these to x (read k times). 8191 rows of 2048 in bf16, eight places
-// each, 302 MB: 77 us (eight rows a thread or one 84, through the caches 82), 3.9 TB/s where a copy reaches 5.1.
-constexpr int GATHER_ROWS = 4;
-template <class R, bool VEC>
+// Bound by its bytes, most of them out, which go past the caches and leave these to x (read k times); two rows a thread, so
+// that their entries and then their pieces are under way together. Without weights a piece is copied as it is. 1024 rows of 2048
+// in bf16, eight places each (38 MB): 6.9 us.
+constexpr int GATHER_ROWS = 2;
+// A piece of a row, times w where there are weights.
+template <class R, bool WEIGHTED, int N, class Piece>
+__device__ __forceinline__ Piece gathered(Piece v, float w) {
+  if constexpr (WEIGHTED) {
+    alignas(16) typename R::E e[N];
+    *(Piece *)e = v;
+#pragma unroll
+    for (int j = 0; j < N; j++) e[j] = row_put(R{}, row_get(R{}, e[j]) * w);
+    v = *(const Piece *)e;
+  }
+  return v;
+}
+template <class R, bool VEC, bool WEIGHTED>
 __global__ __launch_bounds__(256) void k_moe_gather(const JoinArgs a, int log_t) {
   typedef RowPiece<R, VEC> P;
   typedef typename R::E E;
+  typedef typename std::conditional<VEC, i4v, E>::type Piece;
   const int each = 256 >> log_t, i0 = blockIdx.x * (each * GATHER_ROWS) + (threadIdx.x >> log_t), t = threadIdx.x & ((1 << log_t) - 1);
   const int n = a.rows * a.k;
   const E *src[GATHER_ROWS];
@@ -324,19 +332,74 @@ __global__ __launch_bounds__(256) void k_moe_gather(const JoinArgs a, int log_t)
   for (int r = 0; r < GATHER_ROWS; r++) {
     is[r] = entry[r] >= 0 && entry[r] < n;
     src[r] = (const E *)a.x + (int64_t)(is[r] ? entry[r] / a.k : 0) * a.ld_x;
-    w[r] = a.weights && is[r] ? a.weights[entry[r]] : 1.0f;
+    w[r] = WEIGHTED && is[r] ? a.weights[entry[r]] : 1.0f;
   }
   for (int c = t; c < a.width / P::N; c += 1 << log_t) {
-    float x[GATHER_ROWS][P::N];
+    Piece v[GATHER_ROWS];
 #pragma unroll
-    for (int r = 0; r < GATHER_ROWS; r++) P::get(src[r] + c * P::N, x[r]);
+    for (int r = 0; r < GATHER_ROWS; r++) v[r] = *(const Piece *)(src[r] + c * P::N);
 #pragma unroll
     for (int r = 0; r < GATHER_ROWS; r++) {
       const int i = i0 + r * each;
       if (i >= n) break;
+      v[r] = is[r] ? gathered<R, WEIGHTED, P::N>(v[r], w[r]) : Piece{};
+      Piece *const to = (Piece *)((E *)a.out + (int64_t)i * a.ld_out + c * P::N);
+      if constexpr (VEC) __builtin_nontemporal_store(v[r], to);
+      else *to = v[r];
+    }
+  }
+}
+
+// The same in an order that lets a row of x come once from memory and the other times from an L2: workgroups go to the XCDs in
+// turn, and workgroup id has a slice of x's rows, about 2 MB, that is id % 8 of eight slices which are at work together. Of its
+// part of the places it picks those that are the slice's (a place of no entry is any one slice's), and its waves have four of their
+// rows each at a time. Its part is lines of 16 places from all over, the j-th turned by j times 0.618 of their number: places of
+// one slice stand together in each expert's, and even strides would give some workgroups all of them.
+// 8191 rows of 2048 in bf16, eight places each (302 MB): 57-59 us against 73 as above (four rows a thread there 75, eight 76, one 73);
+// 32768 rows 204 us against 298, 4097 of 1024 in fp32 29 against 35, 16384 of 512 in bf16 26 against 35; 2048 rows of 2048 (8 MB of x) 18 against
+// 17. Slices of 1 MB 59, of 4 MB 64; 16 places a workgroup on average 57, and 31 for the 4097 rows; a row a wave 62.
+constexpr int NEAR_LINE = 16, NEAR_RUN = 2048, NEAR_AVERAGE = 12;  // (a run is NEAR_AVERAGE places for each slice: a multiple of NEAR_LINE)
+constexpr int64_t NEAR_FROM = 12000000, NEAR_SLICE = 2200000;      // bytes of x
+template <class R, bool WEIGHTED>
+__global__ __launch_bounds__(256) void k_moe_gather_near(const JoinArgs a, int slices, int per, int run, int runs) {
+  typedef typename R::E E;
+  constexpr int N = 16 / (int)sizeof(E), U = 4;
+  __shared__ int2 list[NEAR_RUN];  // places and their entries
+  __shared__ int count;
+  const int n = a.rows * a.k, t = threadIdx.x, wave = t >> 6, lane = t & 63, at = blockIdx.x >> 3, mine = at % runs;
+  const int slice = at / runs * 8 + (blockIdx.x & 7), turn = (int)(0.618f * runs);
+  if (t == 0) count = 0;
+  __syncthreads();
+  const int lo = (int)min((int64_t)slice * per, (int64_t)a.rows) * a.k, hi = (int)min((int64_t)(slice + 1) * per, (int64_t)a.rows) * a.k;
+  for (int j = t; j < run; j += 256) {
+    const int line = j / NEAR_LINE, i = (line * runs + (int)((uint32_t)(mine + line * turn) % (uint32_t)runs)) * NEAR_LINE + j % NEAR_LINE;
+    if (i >= n) continue;
+    const int entry = a.order[i];
+    const bool is = entry >= 0 && entry < n;
+    if (is ? entry >= lo && entry < hi : i / NEAR_LINE % slices == slice) list[atomicAdd(&count, 1)] = make_int2(i, is ? entry : -1);
+  }
+  __syncthreads();
+  const int many = count, pieces = a.width / N;
+  for (int q = wave * U; q < many; q += 4 * U) {
+    const i4v *src[U];
+    i4v *to[U];
+    float w[U];
+    bool is[U];
 #pragma unroll
-      for (int j = 0; j < P::N; j++) x[r][j] = is[r] ? (a.weights ? x[r][j] * w[r] : x[r][j]) : 0.0f;
-      P::put_past((E *)a.out + (int64_t)i * a.ld_out + c * P::N, x[r]);
+    for (int u = 0; u < U; u++) {
+      const int at = min(q + u, many - 1), i = __builtin_amdgcn_readfirstlane(list[at].x), entry = __builtin_amdgcn_readfirstlane(list[at].y);
+      is[u] = entry >= 0;
+      src[u] = (const i4v *)((const E *)a.x + (int64_t)(max(entry, 0) / a.k) * a.ld_x);
+      to[u] = (i4v *)((E *)a.out + (int64_t)i * a.ld_out);
+      w[u] = WEIGHTED && is[u] ? a.weights[entry] : 1.0f;
+    }
+    for (int c = lane; c < pieces; c += 64) {
+      i4v v[U];
+#pragma unroll
+      for (int u = 0; u < U; u++) v[u] = src[u][c];
+#pragma unroll
+      for (int u = 0; u < U; u++)
+        if (q + u < many) __builtin_nontemporal_store(is[u] ? gathered<R, WEIGHTED, N>(v[u], w[u]) : i4v{}, to[u] + c);
     }
   }
 }
@@ -424,8 +487,17 @@ static void join(const JoinArgs &a, int what, hipStream_t s) {
   const int rows = what == 0 ? a.rows * a.k : a.rows, each = (256 >> log_t) * (what == 0 ? GATHER_ROWS : 1);
   const dim3 grid((unsigned)((rows + each - 1) / each)), block(256);
   if (what == 0) {
-    if (vec) hipLaunchKernelGGL((k_moe_gather<R, true>), grid, block, 0, s, a, log_t);
-    else hipLaunchKernelGGL((k_moe_gather<R, false>), grid, block, 0, s, a, log_t);
+    const int64_t bytes = (int64_t)a.rows * a.width * size;
+    if (vec && pieces >= 64 && bytes > NEAR_FROM) {
+      const int slices = 8 * (int)std::min<int64_t>((bytes + 8 * NEAR_SLICE - 1) / (8 * NEAR_SLICE), NEAR_RUN / (8 * NEAR_AVERAGE));
+      const int run = NEAR_AVERAGE * slices, runs = (rows + run - 1) / run, per = (a.rows + slices - 1) / slices;
+      const dim3 near((unsigned)(slices * runs));
+      if (a.weights) hipLaunchKernelGGL((k_moe_gather_near<R, true>), near, block, 0, s, a, slices, per, run, runs);
+      else hipLaunchKernelGGL((k_moe_gather_near<R, false>), near, block, 0, s, a, slices, per, run, runs);
+    } else if (vec && a.weights) hipLaunchKernelGGL((k_moe_gather<R, true, true>), grid, block, 0, s, a, log_t);
+    else if (vec) hipLaunchKernelGGL((k_moe_gather<R, true, false>), grid, block, 0, s, a, log_t);
+    else if (a.weights) hipLaunchKernelGGL((k_moe_gather<R, false, true>), grid, block, 0, s, a, log_t);
+    else hipLaunchKernelGGL((k_moe_gather<R, false, false>), grid, block, 0, s, a, log_t);
   } else if (what == 1) {
     if (vec) hipLaunchKernelGGL((k_moe_combine<R, true>), grid, block, 0, s, a, log_t);
     else hipLaunchKernelGGL((k_moe_combine<R, false>), grid, block, 0, s, a, log_t);

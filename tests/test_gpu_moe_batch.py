@@ -337,3 +337,32 @@ def test_far_rows(ctx):
     close(d_y[some], want, np.abs(want) * R.U + R.rounding(want * (1 + R.U), BF16))
     sq = f64(x[-20:]) ** 2
     close(d_w[-20:], np.repeat(sq.sum(1)[:, None], k, 1), np.repeat(sq.sum(1)[:, None], k, 1) * (width / 64 + 24) * R.U)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, F16, BF16])
+@pytest.mark.parametrize("rows,k,width,experts,drop", [(4097, 8, 1024, 32, 0.0), (6200, 2, 1040, 8, 0.3), (1025, 32, 8192, 128, 0.9), (12300, 1, 768, 3, 0.0), (3001, 5, 4104, 1, 1.0)])
+def test_gather_of_many_rows(ctx, dtype, rows, k, width, experts, drop):
+    """Rows past an L2's size, taken slice by slice: every place is written once, places of no expert with zeros."""
+    from spindle_amd import ops
+    g = torch.Generator(device="cuda")
+    g.manual_seed(rows)
+    ids = torch.randint(0, experts, (rows, k), generator=g, device="cuda", dtype=torch.int32)
+    ids[torch.rand(rows, k, generator=g, device="cuda") < drop] = -1
+    o = ops.moe_sort(ctx, ids, experts)
+    big = torch.randn(rows, width + 16, generator=g, device="cuda").to(dtype)
+    x = big[:, 8:8 + width]
+    some = o.order >= 0
+    e = torch.where(some, o.order, 0).long()
+    want = torch.where(some[:, None], x[e // k], torch.zeros((), dtype=dtype, device="cuda"))
+    out = torch.full((rows * k + 1, width + 8), 7.0, dtype=dtype, device="cuda")
+    ops.moe_gather(ctx, x, o.order, k, out=out[:-1, :width])
+    assert torch.equal(out[:-1, :width], want) and bool((out[:-1, width:] == 7).all()) and bool((out[-1] == 7).all())
+    w = torch.randn(rows, k, generator=g, device="cuda")
+    got = ops.moe_gather(ctx, x, o.order, k, weights=w)
+    scaled = torch.where(some[:, None], (x[e // k].float() * w.reshape(-1)[e][:, None]).to(dtype), torch.zeros((), dtype=dtype, device="cuda"))
+    assert torch.equal(got, scaled)
+    # any order that the call may be given, the same entry twice and entries out of range among them
+    other = torch.randint(-2, rows * k + 3, (rows * k,), generator=g, device="cuda", dtype=torch.int32)
+    some = (other >= 0) & (other < rows * k)
+    want = torch.where(some[:, None], x[torch.where(some, other, 0).long() // k], torch.zeros((), dtype=dtype, device="cuda"))
+    assert torch.equal(ops.moe_gather(ctx, x, other, k), want)
