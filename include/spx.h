@@ -265,7 +265,7 @@ int spx_mx4_quantize(spx_ctx *ctx, int type, const void *x, int64_t ld_x, const 
 int spx_mx4_read(spx_ctx *ctx, const spx_mx4 *m, int type, void *out, int64_t ld_out);
 
 /* Products with such matrices: out[i] = W x_i, or with `up` out[i] = silu(W x_i) * (up x_i), i < rows,
- * silu(v) = v / (1 + exp(-v)); w (and up, of one shape) holds n_expert matrices of n = w->rows / n_expert
+ * silu(v) = v / (1 + exp(-v)) (a zero where that is below 87 * 2^-126 in magnitude); w (and up, of one shape) holds n_expert matrices of n = w->rows / n_expert
  * rows one after the other, n <= 2^20, n_expert <= 1024. Without starts n_expert is 1 and order NULL. With starts
  * [n_expert + 1] (as spx_moe_sort leaves it) row i takes the matrices of the expert whose places it is among; rows behind
  * starts[n_expert] are left as they were. x_i is row order[i] / k of x, or without order row i; a row whose
