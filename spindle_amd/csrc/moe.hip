@@ -130,7 +130,7 @@ __global__ __launch_bounds__(256) void k_moe_route_grad(const RouteArgs a) {
   }
 #pragma unroll
   for (int v = 0; v < NV; v++)
-    if (lane + 64 * v < a.n_expert) out[lane + 64 * v] = row_put(R{}, bad ? __builtin_nanf("") : d[v]);
+    if (lane + 64 * v < a.n_expert) out[lane + 64 * v] = row_put(R{}, bad ? __builtin_nanf("") : m == -INFINITY ? 0.0f : d[v]);  // (-inf: whatever g is)
 }
 
 #define MOE_BY_TYPE(type, CALL)               \

@@ -366,3 +366,24 @@ def test_gather_of_many_rows(ctx, dtype, rows, k, width, experts, drop):
     some = (other >= 0) & (other < rows * k)
     want = torch.where(some[:, None], x[torch.where(some, other, 0).long() // k], torch.zeros((), dtype=dtype, device="cuda"))
     assert torch.equal(ops.moe_gather(ctx, x, other, k), want)
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("norm", [True, False])
+def test_route_grad_of_rows_of_padding(ctx, dtype, norm):
+    """A row of nothing but -inf gets zeros whatever its weights' gradient is, infinities and NaN among it; an id out of range makes
+    it NaN all the same."""
+    from spindle_amd import ops
+    rng = np.random.default_rng(4)
+    rows, n, k = 12, 40, 5
+    x = torch.from_numpy(rng.standard_normal((rows, n))).to(dtype).cuda()
+    x[1::2] = float("-inf")
+    chosen, weights = ops.moe_route(ctx, x, k, norm=norm)
+    assert not weights[1::2].any()
+    g = torch.from_numpy(rng.standard_normal((rows, k))).float().cuda()
+    g[1], g[3, 2], g[5, 0], g[7, k - 1] = float("nan"), float("inf"), float("-inf"), float("nan")
+    chosen[11, 3] = n
+    d = ops.moe_route_grad(ctx, x, chosen, g, norm=norm)
+    assert not d[1:11:2].any() and d[11].isnan().all()
+    want, tol = R.route_grad(f64(x[::2]), chosen[::2].cpu().numpy(), f64(g[::2]), norm)
+    close(d[::2], want, tol + R.rounding(want, dtype))
