@@ -267,10 +267,22 @@ __device__ __forceinline__ f16v mfma_mx4_32(i4v w, int ws, i4v x, int xs, f16v a
 }
 
 // v over 1 + exp(-v), with the hardware's exponential and reciprocal, each good to a unit in the last place (a division and
-// an exponential rounded correctly are forty instructions: a third of a gated tile's time). Below -87, where
-// the reciprocal leaves the normal numbers, a zero is as good: it is off by 87 * 2^-126 at most.
+// an exponential rounded correctly are forty instructions: a third of a gated tile's time). The exponential's argument h = -v log2(e) is
+// rounded, which moves the exponential by up to |v| 2^-24. FINE: l is what that rounding took off, and the constant's own,
+// and e (1 + l ln 2) has it back. Evaluated over -86..88 with both instructions exact, the result is then off by 4 * 2^-24 of itself at
+// most; without, by 17 * 2^-24 at -20 and 65 * 2^-24 at -80. That is a 32nd of what rounding to f16 moves it and less of bf16's, so only
+// fp32 outputs take the six instructions more (1% of an fp32 product by expert, 3 - 5% of a 16-bit one). Below -87, where the reciprocal leaves the
+// normal numbers, a zero is as good: it is off by 87 * 2^-126 at most. (There e, and of infinities l, may be no number: e stays as it is.)
+template <bool FINE>
 __device__ __forceinline__ float silu(float v) {
-  return v * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(v * -1.4426950408889634f));
+  constexpr float L = 1.4426950408889634f, L2 = (float)(1.4426950408889634 - (double)L), LN2 = 0.6931471805599453f;
+  const float h = v * -L;
+  float e = __builtin_amdgcn_exp2f(h);
+  if (FINE) {
+    const float l = fmaf(v, -L2, fmaf(v, -L, -h));
+    e = fabsf(v) < 88.0f ? fmaf(e, l * LN2, e) : e;
+  }
+  return v * __builtin_amdgcn_rcpf(1.0f + e);
 }
 
 struct Vecs { int x, out; };  // rows of x lie at multiples of 16 bytes, of out at multiples of four elements
@@ -437,17 +449,17 @@ __device__ __forceinline__ void wait_and_meet() {
 
 // 32 rows of COLS neighbouring columns of out from a wave's products (or the gated ones'), through LDS of its own: a lane has
 // four neighbours of a row, 8 or 16 bytes, and stored so each store would touch 32 rows. row(r): row r's number, -1: it is not stored.
-template <int COLS, class F, class G>
+template <int COLS, bool FP32, class F, class G>
 __device__ __forceinline__ void put_rows(const Mx4Product &a, int out_type, bool vec, uint8_t *lds, int c0, F row, G value) {
   const int lane = threadIdx.x & 63, m = lane & 31, g = lane >> 5;
-  const int size = out_type == T_F32 ? 4 : 2, pitch = COLS * size + 16;
+  constexpr int size = FP32 ? 4 : 2, pitch = COLS * size + 16;
 #pragma unroll
   for (int t = 0; t < COLS / 32; t++)
 #pragma unroll
     for (int i = 0; i < 4; i++) {
       const f4v v = value(t, i);
       uint8_t *const to = lds + m * pitch + (32 * t + 8 * i + 4 * g) * size;
-      if (out_type == T_F32) *(f4v *)to = v;
+      if constexpr (FP32) *(f4v *)to = v;
       else if (out_type == T_F16) {
         alignas(8) const _Float16 e[4] = {(_Float16)v[0], (_Float16)v[1], (_Float16)v[2], (_Float16)v[3]};
         *(uint2 *)to = *(const uint2 *)e;
@@ -458,7 +470,7 @@ __device__ __forceinline__ void put_rows(const Mx4Product &a, int out_type, bool
     }
   __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   __builtin_amdgcn_wave_barrier();
-  const int pieces = COLS * size / 16, each = 16 / size;
+  constexpr int pieces = COLS * size / 16, each = 16 / size;
   for (int p = lane; p < 32 * pieces; p += 64) {
     const int r = p / pieces, q = p & (pieces - 1), i = row(r), c = c0 + q * each;
     if (i < 0 || c >= a.n) continue;
@@ -593,18 +605,23 @@ __global__ __launch_bounds__(256, MT == 64 ? 3 : 2) void k_mx4_four(const Mx4Pro
   else if (rows > 0) turns(std::integral_constant<int, 1>{});
   else turns(std::integral_constant<int, 0>{});
   wait_and_meet();  // (all waves' reads of LDS are done)
+  const auto out = [&](auto fp32) {
+    constexpr bool FP32 = decltype(fp32)::value;
 #pragma unroll
-  for (int f = 0; f < MF; f++) {
-    const int r0 = (wm * MF + f) * 32;
-    if (r0 >= tile.count) break;
-    put_rows<COLS>(a, out_type, vec.out, lds + wave * 9216, col0 + wn * COLS, [&](int r) { return s_src[r0 + r] < 0 ? -1 : tile.row + r0 + r; },
-                   [&](int t, int i) {
-                     f4v v;
+    for (int f = 0; f < MF; f++) {
+      const int r0 = (wm * MF + f) * 32;
+      if (r0 >= tile.count) break;
+      put_rows<COLS, FP32>(a, out_type, vec.out, lds + wave * 9216, col0 + wn * COLS, [&](int r) { return s_src[r0 + r] < 0 ? -1 : tile.row + r0 + r; },
+                           [&](int t, int i) {
+                             f4v v;
 #pragma unroll
-                     for (int j = 0; j < 4; j++) v[j] = GATED ? silu(acc[f][0][4 * i + j]) * acc[f][1][4 * i + j] : acc[f][t][4 * i + j];
-                     return v;
-                   });
-  }
+                             for (int j = 0; j < 4; j++) v[j] = GATED ? silu<FP32>(acc[f][0][4 * i + j]) * acc[f][1][4 * i + j] : acc[f][t][4 * i + j];
+                             return v;
+                           });
+    }
+  };
+  if (out_type == T_F32) out(std::true_type{});
+  else out(std::false_type{});
 }
 
 // ------------------------------------------------------------------ products of many 16- and 32-bit rows
@@ -782,18 +799,23 @@ __global__ __launch_bounds__(256, 2) void k_mx4_wide(const Mx4Product a, const V
   else if (rows > 0) all_turns(std::integral_constant<int, 1>{});
   else all_turns(std::integral_constant<int, 0>{});
   wait_and_meet();  // (all waves' reads of LDS are done)
+  const auto out = [&](auto fp32) {
+    constexpr bool FP32 = decltype(fp32)::value;
 #pragma unroll
-  for (int f = 0; f < MF; f++) {
-    const int r0 = (wm * MF + f) * 32;
-    if (r0 >= tile.count) break;
-    put_rows<COLS>(a, out_type, vec.out, lds + wave * 9216, col0 + wn * COLS, [&](int r) { return s_src[r0 + r] < 0 ? -1 : tile.row + r0 + r; },
-                   [&](int t, int i) {
-                     f4v v;
+    for (int f = 0; f < MF; f++) {
+      const int r0 = (wm * MF + f) * 32;
+      if (r0 >= tile.count) break;
+      put_rows<COLS, FP32>(a, out_type, vec.out, lds + wave * 9216, col0 + wn * COLS, [&](int r) { return s_src[r0 + r] < 0 ? -1 : tile.row + r0 + r; },
+                           [&](int t, int i) {
+                             f4v v;
 #pragma unroll
-                     for (int j = 0; j < 4; j++) v[j] = GATED ? silu(acc[f][0][4 * i + j]) * acc[f][1][4 * i + j] : acc[f][t][4 * i + j];
-                     return v;
-                   });
-  }
+                             for (int j = 0; j < 4; j++) v[j] = GATED ? silu<FP32>(acc[f][0][4 * i + j]) * acc[f][1][4 * i + j] : acc[f][t][4 * i + j];
+                             return v;
+                           });
+    }
+  };
+  if (out_type == T_F32) out(std::true_type{});
+  else out(std::false_type{});
 }
 
 // ------------------------------------------------------------------ products of few rows
@@ -945,7 +967,7 @@ __global__ __launch_bounds__(FEW_W * 64, 4) void k_mx4_few(const Mx4Product a, c
     if (GATED) {
       const f4v u = total(t + OUT);
 #pragma unroll
-      for (int j = 0; j < 4; j++) v[j] = silu(v[j]) * u[j];
+      for (int j = 0; j < 4; j++) v[j] = (out_type == T_F32 ? silu<true>(v[j]) : silu<false>(v[j])) * u[j];
     }
     if (n0 + 16 * t + 4 * g < a.n) put4_by(a, out_type, i, n0 + 16 * t + 4 * g, v, vec.out);
   }

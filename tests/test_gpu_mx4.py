@@ -500,3 +500,36 @@ def test_tuning_step_in_a_graph(ctx):
             torch.cuda.synchronize()
             assert all(torch.equal(a, b) for a, b in zip(got, w))
             step()
+
+
+# ------------------------------------------------------------------------ exactness of the gate
+# few rows, and tiles of 32, 64 and 128 rows
+GATES = [(250, 40), (20, 25000), (400, 6000), (600, 2700)]
+
+
+@pytest.mark.parametrize("kind", [F32, F16, BF16, "mx4"])
+@pytest.mark.parametrize("rows,n", GATES)
+def test_gate_by_itself(ctx, kind, rows, n):
+    """silu of sums that are exact, at every magnitude that it has a value at: out is silu(v) times 1, v one of x's values.
+
+    Its error, with U = 2^-24 of a rounding: the exponential is off by a unit in the last place (2 U) and what its argument's
+    rounding takes off it is put back by a multiplication and an addition of one rounding (U), 1 + e rounds (U), the reciprocal is
+    off by a unit in the last place (2 U) and the product with v rounds (U): 7 U, and 1 U for all that is second order."""
+    from spindle_amd import ops
+    rng = np.random.default_rng(rows)
+    cols = 64
+    if kind == "mx4":  # 0.5 to 6 times 1 to 8, so up to 48
+        codes, scales = np.zeros((rows, 128), np.int64), np.full((rows, 4), 127)
+        codes[:, 0], codes[:, 32], scales[:, 0] = rng.integers(1, 8, rows) + 8 * rng.integers(0, 2, rows), 2, 127 + rng.integers(-1, 4, rows)
+        data = R.pack(codes, scales)
+        x, v = ops.Mx4(torch.from_numpy(data).cuda(), rows, cols), R.unpack(data, rows, cols)[:, 0]
+    else:
+        x = torch.zeros(rows, cols, device="cuda", dtype=kind)
+        x[:, 0] = torch.from_numpy(rng.uniform(0.01, 86.0, rows) * np.where(np.arange(rows) % 4, -1, 1)).to(kind).cuda()
+        x[:, 32] = 1.0
+        v = f64(x[:, 0])
+    one = lambda at: np.eye(1, 128, at, dtype=np.int64).repeat(n, 0) * 2  # noqa: E731 (code 2 is 1)
+    gate, up = (ops.Mx4(torch.from_numpy(R.pack(one(at), np.full((n, 4), 127))).cuda(), n, cols) for at in (0, 32))
+    got = f64(ops.mx4_matmul(ctx, x, gate, up=up, dtype=F32))
+    want = v / (1.0 + np.exp(-v))
+    close(got, np.repeat(want[:, None], n, 1), 8 * R.U * np.abs(want)[:, None])
