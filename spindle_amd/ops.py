@@ -515,17 +515,28 @@ class Mx4:
 
     @staticmethod
     def empty(rows, cols, device="cuda"):
-        return Mx4(torch.empty(Mx4.nbytes(rows, cols), dtype=torch.uint8, device=device), rows, cols)
+        """A matrix whose values are not set yet; with 0 rows that of a batch without any, which has no bytes."""
+        data = torch.empty(Mx4.nbytes(rows, cols), dtype=torch.uint8, device=device)
+        if rows == 0 and Mx4.nbytes(1, cols) > 0:
+            m = Mx4.__new__(Mx4)
+            m.data, m.rows, m.cols, m._c = data, 0, cols, _Mx4C(None, 0, cols)
+            return m
+        return Mx4(data, rows, cols)
+
+
+def _no_rows(*_):
+    """A call over a 4-bit matrix of no rows, which the C entries do not take."""
+    return 0
 
 
 def mx4_quantize(ctx, x, out=None):
-    """Rows x [rows, cols] as an Mx4 (spx_mx4_quantize)."""
+    """Rows x [rows, cols] as an Mx4 (spx_mx4_quantize); no rows as one without bytes."""
     t, ld = _row_type(x.dtype), _rows2(x, "x")
     if out is None:
         out = Mx4.empty(*x.shape, device=x.device)
     elif (out.rows, out.cols) != tuple(x.shape):
         raise ValueError(f"out must be of {tuple(x.shape)}, got {(out.rows, out.cols)}")
-    _run(ctx, (x, out.data), lib.spx_mx4_quantize, t, x.data_ptr(), ld, C.byref(out._c))
+    _run(ctx, (x, out.data), lib.spx_mx4_quantize if out.rows else _no_rows, t, x.data_ptr(), ld, C.byref(out._c))
     return out
 
 
@@ -534,7 +545,7 @@ def mx4_read(ctx, m, dtype=None, out=None):
     dtype = dtype or torch.float32
     t = _row_type(dtype)
     out, ld = _out2(out, m.data, m.rows, m.cols, dtype)
-    _run(ctx, (m.data, out), lib.spx_mx4_read, C.byref(m._c), t, out.data_ptr(), ld)
+    _run(ctx, (m.data, out), lib.spx_mx4_read if m.rows else _no_rows, C.byref(m._c), t, out.data_ptr(), ld)
     return out
 
 

@@ -533,3 +533,26 @@ def test_gate_by_itself(ctx, kind, rows, n):
     got = f64(ops.mx4_matmul(ctx, x, gate, up=up, dtype=F32))
     want = v / (1.0 + np.exp(-v))
     close(got, np.repeat(want[:, None], n, 1), 8 * R.U * np.abs(want)[:, None])
+
+
+# ----------------------------------------------------------------------------------- no rows at all
+def test_no_four_bit_rows(ctx):
+    """An empty batch in 4 bits, as in the other types: quantised, read, through a product, and a whole layer of none."""
+    from spindle_amd import ops
+    rng = np.random.default_rng(1)
+    w, _ = matrix(rng, 8, 64)
+    for dtype in (F32, BF16):
+        m = ops.mx4_quantize(ctx, torch.zeros(0, 64, device="cuda", dtype=dtype))
+        assert (m.rows, m.cols) == (0, 64)
+        assert ops.mx4_quantize(ctx, torch.zeros(0, 64, device="cuda", dtype=dtype), out=m) is m
+        v = ops.mx4_read(ctx, m, dtype)
+        assert v.shape == (0, 64) and v.dtype == dtype
+        out = ops.mx4_matmul(ctx, m, w, dtype=dtype)
+        assert out.shape == (0, 8) and out.dtype == dtype
+    into = torch.full((3, 8), 7.0, device="cuda")
+    ops.mx4_matmul(ctx, m, w, starts=ints([0, 3]), order=ints([0, 1, 2]), out=into, dtype=F32)  # (rows of an x that has none)
+    assert (into == 7.0).all()
+    experts, k, ((gate, _), (up, _), (down, _)), x, logits = layer_case(rng, 3, BF16)
+    for four in (False, True):
+        got, _ = layer(ops, ctx, x[:0], logits[:0], k, gate, up, down, experts, four)
+        assert got.shape == (0, 256) and got.dtype == BF16

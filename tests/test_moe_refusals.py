@@ -189,6 +189,20 @@ def test_python_other_devices(lib):
             f()
 
 
+def test_python_no_rows(lib):
+    """A 4-bit matrix of no rows is made by empty alone, for columns that there may be, and takes no other shape's place."""
+    from spindle_amd import ops
+    m = ops.Mx4.empty(0, 100, device="cpu")
+    assert (m.rows, m.cols, m.data.numel(), m.data.dtype) == (0, 100, 0, torch.uint8)
+    z = torch.zeros
+    for f in (lambda: ops.Mx4.empty(0, 0, device="cpu"), lambda: ops.Mx4.empty(0, (1 << 20) + 1, device="cpu"), lambda: ops.Mx4.empty(-1, 100, device="cpu"),
+              lambda: ops.Mx4.empty(0, -(1 << 40), device="cpu"), lambda: ops.mx4_quantize(Ctx, z(1, 100), out=m), lambda: ops.mx4_quantize(Ctx, z(0, 99), out=m),
+              lambda: ops.mx4_quantize(Ctx, z(0, 100).long()), lambda: ops.mx4_quantize(Ctx, z(0, 100)), lambda: ops.mx4_read(Ctx, m), lambda: ops.mx4_read(Ctx, m, torch.int32),
+              lambda: ops.mx4_read(Ctx, m, out=z(1, 100))):
+        with pytest.raises(ValueError):
+            f()
+
+
 # -------------------------------------------------------------------------- the references themselves
 def test_reference_of_the_format():
     x = np.zeros((1, 33))
