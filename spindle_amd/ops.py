@@ -496,8 +496,9 @@ class _Mx4C(C.Structure):
 
 
 class Mx4:
-    """A matrix in microscaled 4-bit floats (spx_mx4): its bytes, a uint8 tensor, and what they hold."""
-    __slots__ = ("data", "rows", "cols", "_c")
+    """A matrix in microscaled 4-bit floats (spx_mx4): its bytes, a uint8 tensor, and what they hold. data may be set to
+    another tensor that holds them; rows and cols stay."""
+    __slots__ = ("_data", "_c")
 
     def __init__(self, data, rows, cols):
         if (rows | cols) >> 31:
@@ -505,9 +506,29 @@ class Mx4:
         need = lib.spx_mx4_bytes(rows, cols)
         if need <= 0:
             raise ValueError("a 4-bit matrix has 1 or more rows, and columns in 1..2^20")
+        self._hold(data, need, rows, cols)
+
+    def _hold(self, data, need, rows, cols):
         if data.dtype is not torch.uint8 or not data.is_contiguous() or data.numel() < need:
             raise ValueError(f"the bytes must be a contiguous uint8 tensor of {need}")
-        self.data, self.rows, self.cols, self._c = data, rows, cols, _Mx4C(data.data_ptr(), rows, cols)
+        self._data, self._c = data, _Mx4C(data.data_ptr(), rows, cols)
+
+    @property
+    def rows(self):
+        return self._c.rows
+
+    @property
+    def cols(self):
+        return self._c.cols
+
+    @property
+    def data(self):
+        return self._data
+
+    @data.setter
+    def data(self, data):
+        rows, cols = self.rows, self.cols
+        self._hold(data, lib.spx_mx4_bytes(rows, cols), rows, cols)
 
     @staticmethod
     def nbytes(rows, cols):
@@ -519,7 +540,7 @@ class Mx4:
         data = torch.empty(Mx4.nbytes(rows, cols), dtype=torch.uint8, device=device)
         if rows == 0 and Mx4.nbytes(1, cols) > 0:
             m = Mx4.__new__(Mx4)
-            m.data, m.rows, m.cols, m._c = data, 0, cols, _Mx4C(None, 0, cols)
+            m._hold(data, 0, 0, cols)
             return m
         return Mx4(data, rows, cols)
 

@@ -203,6 +203,24 @@ def test_python_no_rows(lib):
             f()
 
 
+def test_python_other_bytes(lib):
+    """The calls take the bytes that a matrix has now, never those it was made with, and of the size that they were made for."""
+    from spindle_amd import ops
+    need = ops.Mx4.nbytes(8, 100)
+    a, b = torch.zeros(need, dtype=torch.uint8), torch.zeros(need + 16, dtype=torch.uint8)
+    m = ops.Mx4(a, 8, 100)
+    assert (m._c.data, m._c.rows, m._c.cols) == (a.data_ptr(), 8, 100)
+    m.data = b
+    assert m.data is b and (m._c.data, m._c.rows, m._c.cols, m.rows, m.cols) == (b.data_ptr(), 8, 100, 8, 100)
+    for bad in (torch.zeros(need - 1, dtype=torch.uint8), torch.zeros(need), b[::2]):
+        with pytest.raises(ValueError):
+            m.data = bad
+    for name in ("rows", "cols"):
+        with pytest.raises(AttributeError):
+            setattr(m, name, 9)
+    assert m.data is b and m._c.data == b.data_ptr()
+
+
 # -------------------------------------------------------------------------- the references themselves
 def test_reference_of_the_format():
     x = np.zeros((1, 33))
