@@ -648,13 +648,23 @@ __global__ __launch_bounds__(256, 2) void k_mx4_wide(const Mx4Product a, const V
   constexpr bool COPY = WAY == X_COPIED;
   extern __shared__ __align__(16) uint8_t lds[];
   __shared__ int s_src[MT];
+  // 32 rows of fp32 leave no room for it: there lane m of each wave has row m's (20 rows of 2048 columns to 151936 87 us, with one
+  // workgroup a CU 110; 216 rows to eight of 128 experts, gated, 111 and 148).
+  constexpr bool IN_LANES = 2 * (sizeof(typename T::Lds) + sizeof(s_src)) > 163840;
+  static_assert(2 * sizeof(typename T::Lds) <= 163840 && (!IN_LANES || MT == 32), "two workgroups a CU");
   typename T::Lds &b = *(typename T::Lds *)lds;
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, m = lane & 31, g = lane >> 5;
   const int wm = wave / WN, wn = wave % WN;
   Tile tile;
   int column;
   if (!tile_place(a, MT, columns, tile, column)) return;
-  if (tid < MT) s_src[tid] = tid < tile.count ? source_of(a, tile.row + tid) : -1;
+  int my_src = -1;
+  if (IN_LANES) my_src = m < tile.count ? source_of(a, tile.row + m) : -1;
+  else if (tid < MT) s_src[tid] = tid < tile.count ? source_of(a, tile.row + tid) : -1;
+  const auto src_of = [&](int r) {  // (every lane of the wave calls it)
+    if constexpr (IN_LANES) return __shfl(my_src, r);
+    else return s_src[r];
+  };
   const int col0 = column * WN * COLS;
   const int64_t row0 = (int64_t)tile.expert * a.n + col0;
   const rsrc_t wcodes = from_here(a.w.codes + row0 * (a.steps * 64)), wscales = from_here(a.w.scales + row0 * (a.steps * 4));
@@ -691,7 +701,7 @@ __global__ __launch_bounds__(256, 2) void k_mx4_wide(const Mx4Product a, const V
   const E *xr[XC];
 #pragma unroll
   for (int j = 0; j < XC; j++) {
-    const int src = s_src[(wave * XC + j) * 8 + r8];
+    const int src = src_of((wave * XC + j) * 8 + r8);
     xr[j] = WAY != X_ANY || src >= 0 ? (const E *)a.x + (int64_t)max(src, 0) * a.ld_x : nullptr;
   }
   const auto copy_x = [&](int turn, int at) {
@@ -805,7 +815,7 @@ __global__ __launch_bounds__(256, 2) void k_mx4_wide(const Mx4Product a, const V
     for (int f = 0; f < MF; f++) {
       const int r0 = (wm * MF + f) * 32;
       if (r0 >= tile.count) break;
-      put_rows<COLS, FP32>(a, out_type, vec.out, lds + wave * 9216, col0 + wn * COLS, [&](int r) { return s_src[r0 + r] < 0 ? -1 : tile.row + r0 + r; },
+      put_rows<COLS, FP32>(a, out_type, vec.out, lds + wave * 9216, col0 + wn * COLS, [&](int r) { return src_of(r0 + r) < 0 ? -1 : tile.row + r0 + r; },
                            [&](int t, int i) {
                              f4v v;
 #pragma unroll
