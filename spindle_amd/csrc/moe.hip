@@ -359,7 +359,17 @@ __global__ __launch_bounds__(256) void k_moe_gather(const JoinArgs a, int log_t)
 // 32768 rows 204 us against 298, 4097 of 1024 in fp32 29 against 35, 16384 of 512 in bf16 26 against 35; 2048 rows of 2048 (8 MB of x) 18 against
 // 17. Slices of 1 MB 59, of 4 MB 64; 16 places a workgroup on average 57, and 31 for the 4097 rows; a row a wave 62.
 constexpr int NEAR_LINE = 16, NEAR_RUN = 2048, NEAR_AVERAGE = 12;  // (a run is NEAR_AVERAGE places for each slice: a multiple of NEAR_LINE)
-constexpr int64_t NEAR_FROM = 12000000, NEAR_SLICE = 2200000;      // bytes of x
+constexpr int64_t NEAR_SLICE = 2200000;                            // bytes of x
+// Its gain is what is not read again, k - 1 of k times x, which has to be worth its searches: in us, here / as above,
+// rows of 2048 in bf16    3200: k 2 9.5 / 6.9, k 3 12.7 / 11.0;  8191: k 1 13.4 / 10.2, k 2 19.2 / 20.2, k 4 32 / 38;  16000: k 2 36.7 / 37.8, k 3 48 / 56
+// rows of 1024 in fp32    4097: k 2 10.8 / 9.5, k 3 13.1 / 14.9, k 8 29 / 36
+// rows of 512, 25 MB      k 2 12.6 / 15.2;  102 MB: k 1 34 / 31, k 2 50 / 59, k 8 161 / 228
+// With weights the waves' four rows wait for a conversion between loads and stores, the longer the rows: 8191 rows of 4 KB k 2 25.9 / 20.5, k 4 42.5 / 37.9,
+// k 6 54.9 / 55.6, k 8 69.8 / 73.5; 60000 rows of 1 KB k 2 33 / 36, k 4 51 / 71; 30000 rows of 2 KB k 2 41.7 / 37.0, k 3 51.4 / 53.0, k 8 97 / 136.
+// (What the order holds is not known here: where seven of eight places have no entry, 30000 rows of 1024 in bf16 take 96 us with k = 8, 90 as above.)
+static bool gather_near(int64_t rows, int k, int64_t row_bytes, bool weights) {
+  return rows * row_bytes * (k - 1) > 11000000ll * k && (!weights || k >= (row_bytes > 2048 ? 6 : 3));
+}
 template <class R, bool WEIGHTED>
 __global__ __launch_bounds__(256) void k_moe_gather_near(const JoinArgs a, int slices, int per, int run, int runs) {
   typedef typename R::E E;
@@ -487,8 +497,8 @@ static void join(const JoinArgs &a, int what, hipStream_t s) {
   const int rows = what == 0 ? a.rows * a.k : a.rows, each = (256 >> log_t) * (what == 0 ? GATHER_ROWS : 1);
   const dim3 grid((unsigned)((rows + each - 1) / each)), block(256);
   if (what == 0) {
-    const int64_t bytes = (int64_t)a.rows * a.width * size;
-    if (vec && pieces >= 64 && bytes > NEAR_FROM) {
+    if (vec && pieces >= 64 && gather_near(a.rows, a.k, (int64_t)a.width * size, a.weights != nullptr)) {
+      const int64_t bytes = (int64_t)a.rows * a.width * size;
       const int slices = 8 * (int)std::min<int64_t>((bytes + 8 * NEAR_SLICE - 1) / (8 * NEAR_SLICE), NEAR_RUN / (8 * NEAR_AVERAGE));
       const int run = NEAR_AVERAGE * slices, runs = (rows + run - 1) / run, per = (a.rows + slices - 1) / slices;
       const dim3 near((unsigned)(slices * runs));

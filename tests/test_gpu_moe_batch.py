@@ -387,3 +387,10 @@ def test_route_grad_of_rows_of_padding(ctx, dtype, norm):
     assert not d[1:11:2].any() and d[11].isnan().all()
     want, tol = R.route_grad(f64(x[::2]), chosen[::2].cpu().numpy(), f64(g[::2]), norm)
     close(d[::2], want, tol + R.rounding(want, dtype))
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("rows,k,width,experts,drop", [(40000, 1, 512, 16, 0.1), (33000, 2, 512, 16, 0.5), (33000, 3, 512, 40, 0.0), (9000, 4, 2056, 40, 0.1), (5003, 6, 2056, 64, 0.2)])
+def test_gather_of_many_rows_by_each_rule(ctx, dtype, rows, k, width, experts, drop):
+    """Sizes at which rows with weights and without go different ways, or the same one."""
+    test_gather_of_many_rows(ctx, dtype, rows, k, width, experts, drop)
