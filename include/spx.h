@@ -231,8 +231,9 @@ int64_t spx_moe_sort_ws(int rows, int k, int n_expert);
 int spx_moe_sort(spx_ctx *ctx, int rows, int k, int n_expert, const int32_t *chosen, int32_t *starts, int32_t *order, int32_t *place,
                  void *ws, int64_t ws_bytes);
 /* Rows in sorted order: out[i] = x[order[i] / k], times weights[order[i]] where weights [rows][k] are given;
- * i < rows * k, x [rows][width]. Zeros where order holds no entry. Its gradient is spx_moe_combine
- * (without weights: the sum over the places that a row went to). width <= 2^20. */
+ * i < rows * k, x [rows][width]. Zeros where order holds no entry. Its gradient with respect to x is spx_moe_combine
+ * of out's gradient with the same weights (without weights: the sum over the places that a row went to); with respect to the weights,
+ * x[r] . out's gradient at place[r][j], it is the d_weights of spx_moe_combine_grad with x for d_out and out's gradient for y. width <= 2^20. */
 int spx_moe_gather(spx_ctx *ctx, int type, const void *x, int64_t ld_x, int rows, int k, int width, const int32_t *order,
                    const float *weights, void *out, int64_t ld_out);
 /* Rows joined again: out[r] = sum over j of weights[r][j] * y[place[r][j]] (weights NULL: of the rows

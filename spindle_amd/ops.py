@@ -447,7 +447,8 @@ def moe_sort(ctx, chosen, n_expert, ws=None):
 
 def moe_gather(ctx, x, order, k, weights=None, out=None):
     """Rows x [rows, width] in sorted order [rows * k, width], times weights [rows, k] where given
-    (spx_moe_gather). Its gradient is moe_combine with the order's place and the same weights."""
+    (spx_moe_gather). From out's gradient d, x's is moe_combine(d, place, weights) and the weights'
+    moe_combine_grad(x, d, order, place, weights)[1]."""
     t, ld = _row_type(x.dtype), _rows2(x, "x")
     rows, width = x.shape
     if (rows | width | k | rows * k) >> 31:

@@ -394,3 +394,28 @@ def test_route_grad_of_rows_of_padding(ctx, dtype, norm):
 def test_gather_of_many_rows_by_each_rule(ctx, dtype, rows, k, width, experts, drop):
     """Sizes at which rows with weights and without go different ways, or the same one."""
     test_gather_of_many_rows(ctx, dtype, rows, k, width, experts, drop)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("drop", [False, True])
+def test_weighted_gather_gradient(ctx, dtype, drop):
+    """Both gradients of the weighted gather: of x the joining with the same weights, of the weights that of the joining's gradient with
+    x for d_out and out's gradient for y. The loss is linear in each, so over whole numbers differences are exact."""
+    from spindle_amd import ops
+    rng = np.random.default_rng(12)
+    rows, k, width = 9, 3, 24
+    o = sorted_rows(rng, ctx, rows, k, 5, drop)
+    whole = lambda *s: torch.from_numpy(rng.integers(-3, 4, s)).cuda()  # noqa: E731
+    x, w, d = whole(rows, width).to(dtype), whole(rows, k).float(), whole(rows * k, width).to(dtype)
+    loss = lambda x_, w_: float((f64(ops.moe_gather(ctx, x_, o.order, k, weights=w_)) * f64(d)).sum())  # noqa: E731
+    d_x = ops.moe_combine(ctx, d, o.place, w)
+    _, d_w = ops.moe_combine_grad(ctx, x, d, o.order, o.place, w)
+    base = loss(x, w)
+    for i in np.ndindex(rows, k):
+        w2 = w.clone()
+        w2[i] += 1
+        assert loss(x, w2) - base == float(d_w[i])
+    for i in [(0, 0), (3, 7), (4, 23), (8, 11)]:
+        x2 = x.clone()
+        x2[i] += 1
+        assert loss(x2, w) - base == float(d_x[i])
