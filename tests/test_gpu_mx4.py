@@ -556,3 +556,60 @@ def test_no_four_bit_rows(ctx):
     for four in (False, True):
         got, _ = layer(ops, ctx, x[:0], logits[:0], k, gate, up, down, experts, four)
         assert got.shape == (0, 256) and got.dtype == BF16
+
+
+# ---------------------------------------------------------------- many experts and far ones, in tiles
+# rows a matrix past what the few rows' kernel takes: tiles of 32, 64 and (16-bit rows from 512 on) 128 rows
+MANY = [(1500, 2, 300, 64, 100), (6000, 2, 300, 64, 100), (10200, 2, 257, 64, 72), (5700, 2, 1024, 64, 40)]
+
+
+@pytest.mark.parametrize("kind", [F32, F16, BF16, "mx4"])
+@pytest.mark.parametrize("rows,k,experts,cols,n", MANY)
+@pytest.mark.parametrize("gated,drop", [(True, False), (False, True)])
+def test_tiles_of_many_experts(ctx, kind, rows, k, experts, cols, n, gated, drop):
+    """More experts than a workgroup's search for its tile keeps in registers."""
+    from spindle_amd import ops
+    assert rows * k // experts > 8 and (rows * k // 64 + experts) * -(-n // 128) > 192
+    rng = np.random.default_rng(rows)
+    ids = rng.integers(0, experts, (rows, k))
+    ids[: rows // 6] = ids[0, 0]
+    ids[(ids % 7 == 3) & (ids != ids[0, 0])] = experts - 1  # experts without a row
+    if drop:
+        ids[rng.random(ids.shape) < 0.2] = -1
+    o = ops.moe_sort(ctx, ints(ids), experts)
+    starts, order = o.starts.cpu().numpy(), o.order.cpu().numpy()
+    x, xv = rows_of_x(rng, kind, rows, cols)
+    w, wv = lowered(*matrix(rng, experts * n, cols), 2.0 ** -9)
+    up, uv = lowered(*matrix(rng, experts * n, cols), 2.0 ** -9) if gated else (None, None)
+    dtype = BF16 if kind == "mx4" else kind
+    out = torch.full((rows * k, n), 123.0, dtype=dtype, device="cuda")
+    ops.mx4_matmul(ctx, x, w, up=up, starts=o.starts, order=o.order, k=k, dtype=dtype, out=out)
+    assert (out[starts[-1]:] == 123.0).all()
+    for e in range(experts):
+        a, b = starts[e], starts[e + 1]
+        if a < b:
+            at = slice(e * n, (e + 1) * n)
+            check(out[a:b], xv[order[a:b] // k], wv[at], uv[at] if gated else None, kind, dtype)
+
+
+@pytest.mark.parametrize("kind", [F32, BF16, "mx4"])
+@pytest.mark.parametrize("rows", [80, 240, 560])
+def test_far_matrix_in_tiles(ctx, kind, rows):
+    """The last columns of the last of eight experts, past 2^32 bytes, in tiles of 32, 64 and (4-bit rows) 128 rows."""
+    from spindle_amd import ops
+    rng = np.random.default_rng(rows)
+    experts, n, cols, some = 8, 1 << 19, 2304, 200
+    many = experts * n
+    data = torch.zeros(ops.Mx4.nbytes(many, cols), dtype=torch.uint8, device="cuda")
+    end = many * cols // 2
+    assert end - some * cols // 2 > 2 ** 32 and rows // experts > 8
+    codes, scales = rng.integers(0, 16, (some, cols)), rng.integers(112, 125, (some, cols // 32))
+    packed = torch.from_numpy(R.pack(codes, scales)).cuda()
+    data[end - some * cols // 2:end] = packed[:some * cols // 2]
+    data[end + (many - some) * cols // 32:] = packed[some * cols // 2:]
+    x, xv = rows_of_x(rng, kind, rows, cols)
+    starts = np.zeros(experts + 1, np.int64)
+    starts[-1] = rows
+    out = ops.mx4_matmul(ctx, x, ops.Mx4(data, many, cols), starts=ints(starts), dtype=BF16 if kind == "mx4" else None)
+    assert not out[:, :n - some].any()
+    check(out[:, n - some:], xv, R.unpack(packed.cpu().numpy(), some, cols), None, kind, out.dtype)
