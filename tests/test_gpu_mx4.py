@@ -613,3 +613,30 @@ def test_far_matrix_in_tiles(ctx, kind, rows):
     out = ops.mx4_matmul(ctx, x, ops.Mx4(data, many, cols), starts=ints(starts), dtype=BF16 if kind == "mx4" else None)
     assert not out[:, :n - some].any()
     check(out[:, n - some:], xv, R.unpack(packed.cpu().numpy(), some, cols), None, kind, out.dtype)
+
+
+# --------------------------------------------------------------------------- every bit of a value
+@pytest.mark.parametrize("kind", [F32, F16])
+@pytest.mark.parametrize("rows,cols,n", [(1, 2048, 48), (5, 4096, 48), (40, 2048, 48), (20, 2048, 12500), (130, 4096, 9000), (600, 2048, 2700)])
+def test_last_bits_of_long_rows(ctx, kind, rows, cols, n):
+    """Long rows whose last bits make the whole sum: pairs of neighbours, a number plus some last bits and its negative, times
+    equal weights. (fp32: 1 + 2^-8, whose parts are a bit each, so that the last bits are a third one's; fp16: 1.)
+
+    A pair is in one instruction, whose sum is off by at most 2 U of what it adds up and of the sum so far. The latter is at
+    most that of the last bits (the rest cancels in each), so the bound does not grow with the columns' square as it does
+    for any order of any values; a part that was left out would be off by more (asserted)."""
+    from spindle_amd import ops
+    rng = np.random.default_rng(cols + n)
+    first, low, step = (1.0 + 2.0 ** -8, 2.0 ** -15, 2.0 ** -23) if kind == F32 else (1.0, 2.0 ** -7, 2.0 ** -10)
+    last = (np.floor(rng.uniform(0.5, 1.0, (rows, cols // 2)) * low / step)) * step
+    v = np.stack([first + last, np.full_like(last, -first)], -1).reshape(rows, cols)
+    x = torch.from_numpy(v).to(kind).cuda()
+    assert np.array_equal(f64(x), v)
+    codes = np.repeat(rng.integers(1, 8, (n, cols // 2)), 2, 1)
+    data = R.pack(codes, rng.integers(124, 128, (n, cols // 32)))
+    w, wv = ops.Mx4(torch.from_numpy(data).cuda(), n, cols), R.unpack(data, n, cols)
+    got = f64(ops.mx4_matmul(ctx, x, w, dtype=F32))
+    want, mag = v @ wv.T, np.abs(v) @ wv.T
+    tol = 2 * R.U * (PARTS[kind] * (cols / 16 + 8) * want + mag) + np.abs(want) * R.U
+    assert (tol < want / 4).all()
+    close(got, want, tol)
