@@ -640,3 +640,69 @@ def test_last_bits_of_long_rows(ctx, kind, rows, cols, n):
     tol = 2 * R.U * (PARTS[kind] * (cols / 16 + 8) * want + mag) + np.abs(want) * R.U
     assert (tol < want / 4).all()
     close(got, want, tol)
+
+
+# ------------------------------------------------------------------------------ ends of the scales
+def ends_case(rng, kind, rows, cols, n, w_bytes, x_power):
+    """A matrix with scales of these bytes, x of about 2^x_power."""
+    from spindle_amd import ops
+    p = R.padded(cols)
+    codes = rng.integers(0, 16, (n, p))
+    codes[:, cols:] = 0
+    data = R.pack(codes, rng.choice(w_bytes, (n, p // 32)))
+    w = ops.Mx4(torch.from_numpy(data).cuda(), n, cols)
+    if kind == "mx4":
+        codes = rng.integers(0, 16, (rows, p))
+        codes[:, cols:] = 0
+        xd = R.pack(codes, 127 + x_power + rng.integers(-2, 3, (rows, p // 32)))
+        return w, R.unpack(data, n, cols), ops.Mx4(torch.from_numpy(xd).cuda(), rows, cols), R.unpack(xd, rows, cols)
+    x = torch.from_numpy(rng.standard_normal((rows, cols)) * 2.0 ** x_power).to(kind).cuda()
+    return w, R.unpack(data, n, cols), x, f64(x)
+
+
+ENDS = [(3, 40), (70, 40), (20, 25000), (60, 12800), (530, 2900)]
+
+
+@pytest.mark.parametrize("kind", [F32, F16, BF16, "mx4"])
+@pytest.mark.parametrize("rows,n", ENDS)
+@pytest.mark.parametrize("low", [True, False])
+def test_smallest_and_largest_scales(ctx, kind, rows, n, low):
+    """Matrices of the smallest scales (2^-127, whose values lie below the normal numbers, to 2^-124) against large x, and of the
+    largest whose every value is a number (2^123 to 2^125) against small x."""
+    rng = np.random.default_rng(rows)
+    power = {F16: (12, -14)}.get(kind, (100, -110))[0 if low else 1]
+    w, wv, x, xv = ends_case(rng, kind, rows, 260, n, [0, 1, 2, 3] if low else [250, 251, 252], power)
+    from spindle_amd import ops
+    check(ops.mx4_matmul(ctx, x, w, dtype=F32), xv, wv, None, kind, F32)
+
+
+@pytest.mark.parametrize("kind", [F32, BF16])
+@pytest.mark.parametrize("rows,n", ENDS)
+def test_rows_below_the_normal_numbers(ctx, kind, rows, n):
+    """x of 2^-133 to 2^-124 against large scales: what is at least 2^-133 counts."""
+    from spindle_amd import ops
+    rng = np.random.default_rng(rows + 1)
+    w, wv, x, xv = ends_case(rng, kind, rows, 260, n, [224, 225, 226, 227], -127)
+    x = torch.where(torch.rand(x.shape, device="cuda") < 0.5, x, x / 16)
+    xv = f64(x)
+    assert (np.abs(xv) < 2.0 ** -126).mean() > 0.5
+    check(ops.mx4_matmul(ctx, x, w, dtype=F32), xv, wv, None, kind, F32)
+
+
+@pytest.mark.parametrize("kind", [F32, F16, BF16, "mx4"])
+@pytest.mark.parametrize("rows,n", ENDS)
+def test_scales_past_the_range(ctx, kind, rows, n):
+    """Rows of the matrix with scales 2^126 and 2^127 may overflow, and do so in their own column of out; what does not is right."""
+    from spindle_amd import ops
+    rng = np.random.default_rng(rows + 2)
+    w, wv, x, xv = ends_case(rng, kind, rows, 260, n, [125, 126, 127, 128], {F16: -10}.get(kind, -20))
+    at, big = n * R.padded(260) // 2, [3, n // 2, n - 1]
+    for i in big:
+        w.data[at + i * 12 + 1] = 253 + (i & 1)
+    wv = R.unpack(w.data.cpu().numpy(), n, 260)
+    got = f64(ops.mx4_matmul(ctx, x, w, dtype=F32))
+    want, tol = R.product(xv, wv, None, PARTS[kind])
+    rest = np.setdiff1d(np.arange(n), big)
+    close(got[:, rest], want[:, rest], (tol + R.rounding(np.abs(want) + tol, F32))[:, rest])
+    fine = np.isfinite(got[:, big])
+    close(np.where(fine, got[:, big], 0.0), np.where(fine, want[:, big], 0.0), (tol + R.rounding(np.abs(want) + tol, F32))[:, big])
