@@ -205,7 +205,9 @@ int spx_logprobs(spx_ctx *ctx, int type, const void *logits, int64_t ld, int row
  * the host and has neither sort, format nor gradient. What the batch operators above promise holds
  * here too: nothing is allocated, waited for or copied to the host, scratch is the caller's, types are
  * SPX_F32, SPX_F16 and SPX_BF16, roundings to 16 bits are to nearest even, addresses are multiples of their
- * elements' size. Outputs are memory of their own. A call's outputs have the same bits every time. */
+ * elements' size. Outputs are memory of their own. A call's outputs have the same bits every time. The gradients are those that
+ * tuning a router over fixed experts takes: of the joining and of the router. None goes back through the products, so what
+ * spx_moe_combine_grad leaves in d_y is for a caller that has products of its own. */
 
 /* The k experts of each row of router logits [rows][n_expert]: chosen [rows][k] gets the ids of the
  * largest logits, larger first, equal ones by ascending id, weights [rows][k] their softmax
@@ -254,7 +256,7 @@ int spx_moe_combine_grad(spx_ctx *ctx, int type, const void *d_out, int64_t ld_d
  * Layout, with cols padded by zeros to a multiple of 128 (P): codes [rows][P / 2], two a byte, the lower
  * column in the low half, the sign above the code; then scale bytes [rows][P / 32]: E + 127, 255 for NaN. The
  * products take any bytes: 255 is NaN, 253 and 254 may overflow; padding columns hold codes 0 and scales other than 255. */
-enum { SPX_MX4 = 39 };
+enum { SPX_MX4 = 39 }; /* (GGML's number for this format; its files hold blocks of 17 bytes, scale first, in another order of columns: not these bytes) */
 typedef struct {
   void *data;  /* spx_mx4_bytes bytes, a multiple of 16 in address */
   int rows, cols;
@@ -274,7 +276,9 @@ int spx_mx4_read(spx_ctx *ctx, const spx_mx4 *m, int type, void *out, int64_t ld
  * ld_x apart of type SPX_F32, SPX_F16 or SPX_BF16, or SPX_MX4: x is an spx_mx4's data of x_rows rows (ld_x is not used).
  * out: rows ld_out apart, of out_type (SPX_F32, SPX_F16, SPX_BF16), rounded once. Sums are held in 32
  * bits; every value of x meets the matrices with all its bits (an fp32 value as three bf16 parts, an f16 value as two;
- * what is below 2^-133 in magnitude is lost). rows <= 2^23, x_rows <= 2^23. */
+ * what is below 2^-133 in magnitude is lost). rows <= 2^23, x_rows <= 2^23. The kernel is chosen by rows / n_expert, so by all of order, also what
+ * stands for no row here (it costs up to 1.6 times the call with the rows that are here alone); 4-bit rows whose codes take
+ * 4 GB or more all go through the one made for few rows. */
 int spx_mx4_matmul(spx_ctx *ctx, int type, const void *x, int64_t ld_x, int x_rows, const spx_mx4 *w, const spx_mx4 *up, int n_expert,
                    const int32_t *starts, const int32_t *order, int k, int rows, int out_type, void *out, int64_t ld_out);
 

@@ -270,8 +270,8 @@ __device__ __forceinline__ f16v mfma_mx4_32(i4v w, int ws, i4v x, int xs, f16v a
 // an exponential rounded correctly are forty instructions: a third of a gated tile's time). The exponential's argument h = -v log2(e) is
 // rounded, which moves the exponential by up to |v| 2^-24. FINE: l is what that rounding took off, and the constant's own,
 // and e (1 + l ln 2) has it back. Evaluated over -86..88 with both instructions exact, the result is then off by 4 * 2^-24 of itself at
-// most; without, by 17 * 2^-24 at -20 and 65 * 2^-24 at -80. That is a 32nd of what rounding to f16 moves it and less of bf16's, so only
-// fp32 outputs take the six instructions more (1% of an fp32 product by expert, 3 - 5% of a 16-bit one). Below -87, where the reciprocal leaves the
+// most; without, by 17 * 2^-24 at -20 and 65 * 2^-24 at -80. That is a hundredth of what rounding to f16 moves it and less of bf16's, so
+// only fp32 outputs take the six instructions more (1% of an fp32 product by expert, 3 - 5% of a 16-bit one). Below -87, where the reciprocal leaves the
 // normal numbers, a zero is as good: it is off by 87 * 2^-126 at most. (There e, and of infinities l, may be no number: e stays as it is.)
 template <bool FINE>
 __device__ __forceinline__ float silu(float v) {
@@ -413,7 +413,7 @@ enum { X_COPIED, X_WHOLE, X_ANY };
 // where neighbouring lanes are in different rows, as they are when a wave loads its own rows into registers.
 // In LDS a row's eight pieces of 16 bytes stand at piece ^ (row / 2 & 7), so that what sixteen lanes read at a time (0-3, 12-15
 // and 20-27 of each half) lies in other banks.
-// 4095 rows of 2048 columns to eight of 128 experts each, gated, 768 columns out: 112-116 us, 1.8 PFLOP/s; 4096 x 4096 to 4096 55 us,
+// 4095 rows of 2048 columns to eight of 128 experts each, gated, 768 columns out: 108-116 us, 1.8 PFLOP/s; 4096 x 4096 to 4096 55 us,
 // 2.5. Of a turn's 1900 clocks 1000 are the matrix instructions of the CU's two workgroups; the copies' way into LDS takes as
 // long, and the clock falls to 1.5 - 1.6 GHz under the load. A workgroup's search and first copies (6000 clocks) and its way out
 // (4000) are hidden by the other's turns in part.
@@ -628,8 +628,8 @@ __global__ __launch_bounds__(256, MT == 64 ? 3 : 2) void k_mx4_four(const Mx4Pro
 // The same with x as bf16 parts and the matrix's codes made values in registers, 64 columns a turn: lane half g has block g of
 // either operand, eight columns an instruction. The codes come 256 columns at a time (whole cache lines), four turns;
 // bf16 rows are copied to LDS as they lie where they can be, others go through registers, a turn ahead. 4095 rows of 4096 columns
-// to 2048: bf16 65-68 us (1.0 PFLOP/s, a library product of bf16 matrices of 8192 reaches 1.2), fp16 147, fp32 220 (each product
-// two and three times); 216 rows of 2048 columns to eight of 128 experts, gated: 61 us, 3.6 TB/s.
+// to 2048: bf16 63-68 us (1.0 PFLOP/s, a library product of bf16 matrices of 8192 reaches 1.2), fp16 153, fp32 224 (each product
+// two and three times); 216 rows of 2048 columns to eight of 128 experts, gated: 60-61 us, 3.6 TB/s, fp16 93, fp32 110.
 template <class X, int MT>
 struct Wide {
   static constexpr int P = X::PARTS, WM = MT == 32 ? 1 : 2, WN = 4 / WM, MF = MT / 32 / WM, ROWS = WN * 64;

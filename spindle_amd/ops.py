@@ -374,7 +374,8 @@ def logprobs(ctx, logits, targets=None, top=0, logit_scale=1.0, ws=None):
 # ------------------------------------------------------------------ experts over a batch
 # A step of a mixture of experts over a batch's rows: moe_route, moe_sort, mx4_matmul over the sorted rows
 # (gated, then down), moe_combine. As above: on the context's stream in order with torch's, nothing waits on
-# the host, everything can be captured.
+# the host, everything can be captured. Results carry no autograd history: a program that tunes a router calls moe_combine_grad
+# and moe_route_grad (in its autograd.Function's backward, where it has one).
 def _rows2(t, name, width=None):
     """The distance between the rows of a [rows, width] tensor whose rows are dense."""
     if t.dim() != 2 or (width is not None and t.shape[1] != width) or (t.stride(1) != 1 and t.shape[1] > 1):
