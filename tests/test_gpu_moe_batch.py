@@ -419,3 +419,47 @@ def test_weighted_gather_gradient(ctx, dtype, drop):
         x2 = x.clone()
         x2[i] += 1
         assert loss(x2, w) - base == float(d_x[i])
+
+
+def test_sort_and_route_at_their_limits(ctx):
+    """As many rows, experts and choices as there may be: 2^18 rows, 1024 experts, 32 of them a row."""
+    from spindle_amd import ops
+    rows, n, k = 1 << 18, 1024, 32
+    g = torch.Generator(device="cuda")
+    g.manual_seed(7)
+    # distinct logits in each row, so that the choice does not hang on ties: a permutation's values
+    x = torch.rand(rows, n, generator=g, device="cuda").argsort(1).float() / 64
+    chosen, weights = ops.moe_route(ctx, x, k)
+    values, ids = x.topk(k, 1)
+    assert torch.equal(chosen.long(), ids)
+    # (64 bits; logits apart by less than 16 and exact, a few roundings each: 64 * 2^-24)
+    assert (weights.double() - torch.softmax(values.double(), 1)).abs().max() <= 64 * R.U
+    o = ops.moe_sort(ctx, chosen, n)
+    sorted_ids, order = torch.sort(chosen.flatten(), stable=True)
+    assert torch.equal(o.order.long(), order)
+    assert torch.equal(o.starts.long(), torch.searchsorted(sorted_ids, torch.arange(n + 1, device="cuda", dtype=torch.int32)))
+    assert torch.equal(o.place.flatten()[order].long(), torch.arange(rows * k, device="cuda"))
+    one = torch.arange(rows, device="cuda", dtype=torch.float32).view(rows, 1)
+    assert torch.equal(ops.moe_gather(ctx, one, o.order, k).view(-1).long(), order // k)
+    assert torch.equal(ops.moe_combine(ctx, (order // k).float().view(-1, 1), o.place), one * k)  # (whole numbers below 2^24)
+
+
+def test_two_contexts_at_once(ctx):
+    """Layers' sorts and gathers on two contexts' streams at the same time keep to themselves."""
+    from spindle_amd import ops
+    other = ops.Context(0)
+    g = torch.Generator(device="cuda")
+    g.manual_seed(8)
+    rows, k, n = 9000, 4, 40
+    ids = [torch.randint(0, n, (rows, k), generator=g, device="cuda", dtype=torch.int32) for _ in range(2)]
+    x = [torch.randn(rows, 256, generator=g, device="cuda") for _ in range(2)]
+    want = [x[i][torch.sort(ids[i].flatten(), stable=True).indices // k] for i in range(2)]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(10):
+        for i, c in enumerate((ctx, other)):
+            with torch.cuda.stream(c.torch_stream()):
+                got[i].append(ops.moe_gather(c, x[i], ops.moe_sort(c, ids[i], n).order, k))
+    torch.cuda.synchronize()
+    assert all(torch.equal(v, want[i]) for i in range(2) for v in got[i])
+    other.close()

@@ -706,3 +706,31 @@ def test_scales_past_the_range(ctx, kind, rows, n):
     close(got[:, rest], want[:, rest], (tol + R.rounding(np.abs(want) + tol, F32))[:, rest])
     fine = np.isfinite(got[:, big])
     close(np.where(fine, got[:, big], 0.0), np.where(fine, want[:, big], 0.0), (tol + R.rounding(np.abs(want) + tol, F32))[:, big])
+
+
+@pytest.mark.parametrize("kind", [F32, F16, BF16, "mx4"])
+def test_as_many_rows_as_there_may_be(ctx, kind):
+    """2^23 rows, dense and by 1024 experts, looked at in some of them: whole numbers, so without rounding."""
+    from spindle_amd import ops
+    rows, cols, n = 1 << 23, 8, 5
+    rng = np.random.default_rng(3)
+    experts = 1024
+    codes = np.zeros((experts * n, 128), np.int64)
+    codes[:, :cols] = rng.choice([0, 2, 4, 5, 6, 7, 10, 12], (experts * n, cols))  # 0, 1, 2, 3, 4, 6, -1, -2
+    data = R.pack(codes, np.full((experts * n, 4), 127))
+    w, wv = ops.Mx4(torch.from_numpy(data).cuda(), experts * n, cols), R.unpack(data, experts * n, cols)
+    g = torch.Generator(device="cuda")
+    g.manual_seed(4)
+    v = torch.randint(-4, 5, (rows, cols), generator=g, device="cuda", dtype=torch.float32)
+    v[:, 0] = 4.0  # (the block's scale is 1: every value is a code)
+    x = ops.mx4_quantize(ctx, v) if kind == "mx4" else v.to(kind)
+    some = torch.cat([torch.arange(3, device="cuda"), torch.randint(0, rows, (200,), generator=g, device="cuda"), torch.arange(rows - 3, rows, device="cuda")])
+    xv = f64(v[some])
+    got = ops.mx4_matmul(ctx, x, ops.Mx4(torch.from_numpy(R.pack(codes[:n], np.full((n, 4), 127))).cuda(), n, cols), dtype=F32)
+    assert np.array_equal(f64(got[some]), xv @ wv[:n].T)
+    starts = torch.sort(torch.randint(0, rows, (experts + 1,), generator=g, device="cuda", dtype=torch.int32)).values
+    starts[0], starts[-1] = 0, rows
+    got = ops.mx4_matmul(ctx, x, w, starts=starts, dtype=F32)
+    e = torch.searchsorted(starts[1:].contiguous(), some.int(), right=True).cpu().numpy()
+    want = np.stack([xv[i] @ wv[e[i] * n:(e[i] + 1) * n].T for i in range(len(e))])
+    assert np.array_equal(f64(got[some]), want)
